@@ -557,7 +557,7 @@ LaunchFn pick(int epi, int ot, bool bias) {
 
 }  // namespace
 
-// Macros (those of h3metal/ops.py:161-164): WFMT (1 q8, 4 f16, 5 bf16, 6 h8), EPI (0 or 1), OUT_T (half | bfloat |
+// Macros (those of h3metal/ops.py:161-164): WFMT (1 q8, 4 f16, 5 bf16, 6 h8; 9 f8 is this build's, gemm_f8.hip), EPI (0 or 1), OUT_T (half | bfloat |
 // float; float for EPI 1), HAS_BIAS. The reference's tile and layout choices TM, TN, NSG, G, SWZ, FAST_LAYOUT
 // are accepted and unused (this kernel's tiles are its own); LORA must be 0. TILE (this build's, default 0: what is
 // estimated fastest) names the tiles at every size: 1 to 4 the 32 x 32, 64 x 64, 96 x 64 and (16-bit activations)
@@ -584,8 +584,8 @@ bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string
       return false;
     }
   }
-  if (wfmt != 1 && wfmt != 4 && wfmt != 5 && wfmt != 6) {
-    *err = "weight format " + std::to_string(wfmt) + " not built (WFMT 1 q8, 4 f16, 5 bf16, 6 h8)";
+  if (wfmt != 1 && wfmt != 4 && wfmt != 5 && wfmt != 6 && wfmt != 9) {
+    *err = "weight format " + std::to_string(wfmt) + " not built (WFMT 1 q8, 4 f16, 5 bf16, 6 h8, 9 f8)";
     return false;
   }
   if (lora) {
@@ -596,14 +596,15 @@ bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string
     *err = "EPI must be 0 or 1";
     return false;
   }
-  if (tile < 0 || tile > TILE_256 || (wfmt == 1 && tile == TILE_KSPLIT + KSPLIT_96x128)) {
-    *err = "TILE must be 0 to 6, and not 4 (96 x 128) with int8 activations";
-    return false;
-  }
   const std::string t = macro_str(m, "OUT_T", epi ? "float" : "half");
   int ot = t == "bfloat" || t == "bf16" ? T_BF16 : t == "half" || t == "f16" ? T_F16 : t == "float" || t == "f32" ? T_F32 : -1;
   if (ot < 0 || (epi == 1 && ot != T_F32)) {
     *err = "OUT_T must be half|bfloat|float (float with EPI 1)";
+    return false;
+  }
+  if (wfmt == 9) return make_gemm_f8(epi, ot, hb != 0, tile, pl, err);
+  if (tile < 0 || tile > TILE_256 || (wfmt == 1 && tile == TILE_KSPLIT + KSPLIT_96x128)) {
+    *err = "TILE must be 0 to 6, and not 4 (96 x 128) with int8 activations";
     return false;
   }
   pl->launch = wfmt == 1 ? pick<1>(epi, ot, hb != 0)

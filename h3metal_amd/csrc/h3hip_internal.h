@@ -6,6 +6,7 @@
 //   QkRopeParams <- kernels/ops.metal:344-349, packed by h3metal/ops.py:237 ("8ifi")
 //   RotQParams   <- kernels/params.h:25-29, packed by h3metal/ops.py:221 ("4i")
 //   GemmParams   <- kernels/params.h:7-16, packed by h3metal/ops.py:165-166 ("8i")
+// NormQ8Params ("6ifi") and SwigluF8Params ("4i") have no counterpart there.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -57,6 +58,22 @@ struct GemmParams {
 };
 static_assert(sizeof(GemmParams) == 32, "GemmParams must match struct.pack('<8i')");
 
+struct NormQ8Params {
+  int M, D;                           // rows, columns
+  int x_stride, r_stride, ro_stride;  // elements between rows of the input, the residual, the residual's sum
+  int o_stride;                       // elements between rows of codes
+  float eps;
+  int norm;                           // 0: the rows without the norm
+};
+static_assert(sizeof(NormQ8Params) == 32, "NormQ8Params must match struct.pack('<6ifi')");
+
+struct SwigluF8Params {
+  int M, D;      // rows, columns of the result
+  int x_stride;  // elements between rows of [value | gate]
+  int o_stride;  // elements between rows of codes
+};
+static_assert(sizeof(SwigluF8Params) == 16, "SwigluF8Params must match struct.pack('<4i')");
+
 using Macros = std::map<std::string, std::string>;
 
 // One bound buffer argument as the launchers see it: a device address and the
@@ -94,7 +111,9 @@ struct Pipeline {
 bool make_attention(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
 bool make_ops(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
 bool make_rot_q8(const Macros &m, Pipeline *pl, std::string *err);  // module "ops", function "rot_q8"
+bool make_rows_q8(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);  // rms_norm_q8, swiglu_f8
 bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
+bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err);  // weight format f8
 
 // Wave64 lane exchanges inside a 32-lane half wave, shared by the row kernels: the value of lane (lane ^ S).
 // DPP for S = 1, 2 (quad_perm) and 8 (row_ror:8, a 16-lane rotation by 8), ds_swizzle's xor mode (no LDS

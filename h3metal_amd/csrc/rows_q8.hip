@@ -1,0 +1,413 @@
+// Row kernels that make the 8-bit inputs of the matrix products, for gfx950:
+//
+//  rms_norm_q8: h = res + x, rounded once to the residual's type and stored (or h = x without a residual);
+//    v = h / sqrt(mean(h^2) + eps) * w (v = h * w without the norm), and v in 8 bits:
+//    * e4m3 codes with a float scale for each row and block of 128 columns (the last one may be short):
+//      s = amax|v| / 448 (1 where amax is 0), code = e4m3(v / s), round to nearest even;
+//    * or int8 codes with one scale a row: s = amax|v| / 127, code = rint(v / s).
+//  swiglu_f8: v = value * gate / (1 + exp(-gate)) in e4m3, value in columns 0 .. D-1 and gate in D .. 2D-1 of a row (as
+//    rot_q8's mode 1).
+//
+// amax passes over NaN; the code of NaN is NaN (e4m3) or 0 (int8). A block that holds an infinity has an infinite scale
+// and NaN at the infinity. Sums, maxima and products are float.
+//
+// The row's root mean square R scales every value of a block and its amax alike, so v / s = (h w) 448 / amax|h w| does
+// not need it: the codes of a block are written at once and only the scales wait for the row's sum. So a row takes one
+// pass, is never held (e4m3), and may have any length.
+#include "h3hip_internal.h"
+
+#include <cmath>
+#include <cstring>
+
+namespace h3 {
+namespace {
+
+enum { T_NONE = 0, T_BF16 = 1, T_F16 = 2, T_F32 = 3 };
+
+template <int T> struct Elem;
+template <> struct Elem<T_BF16> { using type = __bf16; };
+template <> struct Elem<T_F16> { using type = _Float16; };
+template <> struct Elem<T_F32> { using type = float; };
+template <> struct Elem<T_NONE> { using type = float; };
+
+constexpr int FB = 128;  // columns of a block
+constexpr int PL = 8;    // columns of a lane: 16 lanes hold a block
+constexpr float F8_MAX = 448.0f;
+
+// 8 values from p, which is aligned to its element only (gfx950 loads 16 bytes from any address); those from column n
+// on are 0
+template <typename E>
+__device__ __forceinline__ void load8(float (&v)[PL], const E *p, int n) {
+  typedef E V __attribute__((ext_vector_type(PL), aligned(sizeof(E))));
+  if (n >= PL) {
+    const V x = *(const V *)p;
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] = (float)x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] = i < n ? (float)p[i] : 0.0f;
+  }
+}
+template <typename E>
+__device__ __forceinline__ void store8(E *p, const E (&v)[PL], int n) {
+  typedef E V __attribute__((ext_vector_type(PL), aligned(sizeof(E))));
+  if (n >= PL) {
+    V x;
+#pragma unroll
+    for (int i = 0; i < PL; i++) x[i] = v[i];
+    *(V *)p = x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PL; i++)
+      if (i < n) p[i] = v[i];
+  }
+}
+
+// The largest of 16 neighbouring lanes' values, in each of them
+__device__ __forceinline__ float max16(float m) {
+  m = fmaxf(m, xshfl<8>(m));
+  m = fmaxf(m, xshfl<4>(m));
+  m = fmaxf(m, xshfl<2>(m));
+  return fmaxf(m, xshfl<1>(m));
+}
+
+// The e4m3 codes of 8 values whose block's largest magnitude is m. Blocks below 2^-100 are scaled up first: 448 / m
+// would overflow there.
+__device__ __forceinline__ uint2 codes_f8(const float (&t)[PL], float m) {
+  const float up = m < 0x1p-100f ? 0x1p64f : 1.0f;
+  const float rs = m > 0.0f ? F8_MAX / (m * up) : 1.0f;
+  float y[PL];
+#pragma unroll
+  for (int i = 0; i < PL; i++) y[i] = t[i] * up * rs;
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
+  return make_uint2((unsigned)lo, (unsigned)hi);
+}
+
+__device__ __forceinline__ void store_codes(unsigned char *p, uint2 c, int n) {
+  typedef unsigned V __attribute__((ext_vector_type(2), aligned(1)));
+  if (n >= PL) {
+    V x = {c.x, c.y};
+    *(V *)p = x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < PL; i++)
+      if (i < n) p[i] = (unsigned char)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+  }
+}
+
+struct NormArgs {
+  const char *x, *res;
+  const float *w;
+  unsigned char *out;
+  float *scale;
+  char *res_out;
+};
+
+// One workgroup of 256 threads per row.
+template <int XT, int RT, bool I8>
+__global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Params p) {
+  using XE = typename Elem<XT>::type;
+  using RE = typename Elem<RT>::type;
+  extern __shared__ float top[];  // e4m3: the blocks' largest magnitudes
+  __shared__ float red[8];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const size_t m = blockIdx.x;
+  const int nb = (p.D + FB - 1) / FB;
+  const XE *xr = (const XE *)a.x + m * p.x_stride;
+  const RE *rr = (const RE *)a.res + m * p.r_stride;
+  RE *ro = (RE *)a.res_out + m * p.ro_stride;
+  unsigned char *out = a.out + m * p.o_stride;
+
+  auto load = [&](int c, float (&h)[PL]) __attribute__((always_inline)) {
+    const int n = p.D - c;
+    load8(h, xr + c, n);
+    if constexpr (RT != T_NONE) {
+      float r[PL];
+      load8(r, rr + c, n);
+      RE s[PL];
+#pragma unroll
+      for (int i = 0; i < PL; i++) {
+        s[i] = (RE)(r[i] + h[i]);
+        h[i] = (float)s[i];
+      }
+      store8(ro + c, s, n);
+    }
+  };
+  auto weigh = [&](int c, float (&h)[PL]) __attribute__((always_inline)) {
+    if (!a.w) return;
+    float g[PL];
+    load8(g, a.w + c, p.D - c);
+#pragma unroll
+    for (int i = 0; i < PL; i++) h[i] *= g[i];
+  };
+  auto wave_sum = [](float v) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+    return v;
+  };
+
+  float sq = 0.0f, rowmax = 0.0f;
+  for (int c = tid * PL; c < (p.D + FB - 1) / FB * FB; c += 256 * PL) {
+    float h[PL];
+    load(c, h);
+#pragma unroll
+    for (int i = 0; i < PL; i++) sq = __builtin_fmaf(h[i], h[i], sq);
+    weigh(c, h);
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PL; i++) mx = fmaxf(mx, fabsf(h[i]));
+    if constexpr (!I8) {
+      mx = max16(mx);
+      store_codes(out + c, codes_f8(h, mx), p.D - c);
+      if ((lane & 15) == 0) top[c / FB] = mx;
+    }
+    rowmax = fmaxf(rowmax, mx);
+  }
+  sq = wave_sum(sq);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) rowmax = fmaxf(rowmax, __shfl_xor(rowmax, s));
+  if (lane == 0) red[w] = sq, red[4 + w] = rowmax;
+  __syncthreads();
+  sq = (red[0] + red[1]) + (red[2] + red[3]);
+  const float r = p.norm ? 1.0f / sqrtf(sq / (float)p.D + p.eps) : 1.0f;
+  if constexpr (!I8) {
+    for (int b = tid; b < nb; b += 256) a.scale[m * nb + b] = top[b] > 0.0f ? top[b] * r / F8_MAX : 1.0f;
+  } else {
+    rowmax = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+    const float up = rowmax < 0x1p-100f ? 0x1p64f : 1.0f;
+    const float rs = rowmax > 0.0f ? 127.0f / (rowmax * up) : 1.0f;
+    for (int c = tid * PL; c < p.D; c += 256 * PL) {
+      float h[PL];
+      if constexpr (RT != T_NONE) load8(h, (const RE *)ro + c, p.D - c);
+      else load8(h, xr + c, p.D - c);
+      weigh(c, h);
+      unsigned char q[PL];
+#pragma unroll
+      for (int i = 0; i < PL; i++) q[i] = (unsigned char)(int)rintf(h[i] * up * rs);
+      store8(out + c, q, p.D - c);
+    }
+    if (tid == 0) a.scale[m] = rowmax > 0.0f ? rowmax * r / 127.0f : 1.0f;
+  }
+}
+
+// value * gate / (1 + exp(-gate)) from e = exp(-|gate|) <= 1, which does not overflow: gate / (1 + e), or gate e / (1 + e)
+// for negative gates. The exponent |gate| log2(e) is taken with its rounding error and the constant's second part, put
+// back to first order. Gates below GATE_MIN, where e leaves the normal floats, are left to gated_low.
+constexpr float GATE_MIN = -86.0f;
+__device__ __forceinline__ float gated(float v, float g) {
+  constexpr float L = 1.44269504088896340736f, L2 = 1.92596303e-8f, LN2 = 0.693147180559945309417f;
+  const float n = fabsf(g), t = n * -L;
+  const float lo = __builtin_fmaf(n, -L2, __builtin_fmaf(n, -L, -t));
+  const float e0 = __builtin_amdgcn_exp2f(t);
+  const float e = n < 200.0f ? __builtin_fmaf(e0, lo * LN2, e0) : 0.0f;
+  return v * ((g < 0.0f ? g * e : g) * __builtin_amdgcn_rcpf(1.0f + e));
+}
+// The same below GATE_MIN, where 1 + exp(gate) is 1: value gate exp(gate), from 2^64 exp(gate), a normal float down to
+// gates whose result no float holds.
+__device__ __forceinline__ float gated_low(float v, float g) {
+  constexpr float L = 1.44269504088896340736f, L2 = 1.92596303e-8f, LN2 = 0.693147180559945309417f;
+  const float t = g * L;
+  const float lo = __builtin_fmaf(g, L2, __builtin_fmaf(g, L, -t));
+  const float e0 = __builtin_amdgcn_exp2f(t + 64.0f);
+  const float e = g > -200.0f ? __builtin_fmaf(e0, lo * LN2, e0) : 0.0f;
+  return v * g * e * 0x1p-64f;
+}
+
+// 16 lanes per block of 128 columns, blocks in row order
+template <int XT>
+__global__ __launch_bounds__(256) void swiglu_f8_kernel(const char *x, unsigned char *out, float *scale, SwigluF8Params p) {
+  using XE = typename Elem<XT>::type;
+  const unsigned nb = (unsigned)(p.D + FB - 1) / FB;
+  const size_t b = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const size_t m = b / nb;
+  if (m >= (size_t)p.M) return;
+  const int c = (int)(b - m * nb) * FB + (threadIdx.x & 15) * PL, n = p.D - c;
+  const XE *row = (const XE *)x + m * p.x_stride;
+  float v[PL], g[PL];
+  load8(v, row + c, n);
+  load8(g, row + p.D + c, n);
+  float mx = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PL; i++) {
+    v[i] = g[i] < GATE_MIN ? gated_low(v[i], g[i]) : gated(v[i], g[i]);
+    mx = fmaxf(mx, fabsf(v[i]));
+  }
+  mx = max16(mx);
+  store_codes(out + m * p.o_stride + c, codes_f8(v, mx), n);
+  if ((threadIdx.x & 15) == 0) scale[b] = mx > 0.0f ? mx / F8_MAX : 1.0f;
+}
+
+int esize(int t) { return t == T_F32 ? 4 : 2; }
+
+// the bytes of M rows of `cols` elements, `stride` apart
+uint64_t extent(int M, int stride, int cols, int size) { return ((uint64_t)(M - 1) * stride + cols) * size; }
+
+bool fits(const Arg *a, int i, uint64_t bytes, int align, const char *what, std::string *err) {
+  if (!a[i].ptr) {
+    *err = std::string(what) + " is not bound";
+    return false;
+  }
+  if (bytes > a[i].avail) {
+    *err = std::string(what) + " needs " + std::to_string(bytes) + " bytes, its buffer holds " + std::to_string(a[i].avail);
+    return false;
+  }
+  if ((uintptr_t)a[i].ptr % align) {
+    *err = std::string(what) + " must be aligned to its " + std::to_string(align) + "-byte elements";
+    return false;
+  }
+  return true;
+}
+
+bool overlap(const char *p, uint64_t n, const char *q, uint64_t k) { return p < q + k && q < p + n; }
+
+template <int XT, int RT, bool I8>
+int launch_norm(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const void *params, uint32_t params_len,
+                std::string *err) {
+  (void)pl;
+  if (params_len != sizeof(NormQ8Params)) {
+    *err = "parameter block of " + std::to_string(params_len) + " bytes, expected " + std::to_string(sizeof(NormQ8Params));
+    return -1;
+  }
+  NormQ8Params p;
+  memcpy(&p, params, sizeof p);
+  const bool has_res = RT != T_NONE;
+  if (p.M < 0 || p.D < 1 || p.D > (1 << 20) || p.x_stride < p.D || p.o_stride < p.D ||
+      (has_res && (p.r_stride < p.D || p.ro_stride < p.D)) || !(p.eps >= 0.0f)) {
+    *err = "bad shape: M " + std::to_string(p.M) + " D " + std::to_string(p.D) + " (1 to 2^20) x_stride " +
+           std::to_string(p.x_stride) + " res_stride " + std::to_string(p.r_stride) + ", " + std::to_string(p.ro_stride) +
+           " o_stride " + std::to_string(p.o_stride) + " eps " + std::to_string(p.eps);
+    return -1;
+  }
+  if (nargs < 6) {
+    *err = "expected buffers x, res, w, out, scale, res_out";
+    return -1;
+  }
+  if (p.M == 0) return 0;
+  if (p.M >= 1 << 24) {  // a grid holds less than 2^32 threads
+    *err = "over 2^24 - 1 rows";
+    return -1;
+  }
+  const int nb = (p.D + FB - 1) / FB;
+  const uint64_t xb = extent(p.M, p.x_stride, p.D, esize(XT)), ob = extent(p.M, p.o_stride, p.D, 1);
+  const uint64_t rb = extent(p.M, p.r_stride, p.D, esize(RT)), wb = extent(p.M, p.ro_stride, p.D, esize(RT));
+  const uint64_t sb = (uint64_t)p.M * (I8 ? 1 : nb) * 4;
+  if (!fits(a, 0, xb, esize(XT), "x", err) || (has_res && !fits(a, 1, rb, esize(RT), "res", err)) ||
+      (a[2].ptr && !fits(a, 2, (uint64_t)p.D * 4, 4, "w", err)) || !fits(a, 3, ob, 1, "out", err) ||
+      !fits(a, 4, sb, 4, "scale", err) || (has_res && !fits(a, 5, wb, esize(RT), "res_out", err)))
+    return -1;
+  // Rows are worked on in any order and a value is read before its own place is written: the sum may take its residual's
+  // (or x's) own place, nothing else may share memory with an output.
+  struct Range { const char *p; uint64_t n; int stride, size; const char *name; };
+  const Range in[] = {{a[0].ptr, xb, p.x_stride, esize(XT), "x"},
+                      {has_res ? a[1].ptr : nullptr, rb, p.r_stride, esize(RT), "res"},
+                      {a[2].ptr, (uint64_t)p.D * 4, 0, 4, "w"}};
+  const Range to[] = {{a[3].ptr, ob, 0, 1, "out"}, {a[4].ptr, sb, 0, 4, "scale"},
+                      {has_res ? a[5].ptr : nullptr, wb, p.ro_stride, esize(RT), "res_out"}};
+  for (int i = 0; i < 3; i++) {
+    if (!to[i].p) continue;
+    for (const Range &q : in)
+      if (q.p && overlap(to[i].p, to[i].n, q.p, q.n) &&
+          !(i == 2 && to[i].p == q.p && to[i].stride == q.stride && to[i].size == q.size)) {
+        *err = std::string(to[i].name) + " shares memory with " + q.name;
+        return -1;
+      }
+    for (int k = 0; k < i; k++)
+      if (overlap(to[i].p, to[i].n, to[k].p, to[k].n)) {
+        *err = std::string(to[i].name) + " shares memory with " + to[k].name;
+        return -1;
+      }
+  }
+  const NormArgs g{a[0].ptr, has_res ? a[1].ptr : nullptr, (const float *)a[2].ptr, (unsigned char *)a[3].ptr,
+                   (float *)a[4].ptr, has_res ? a[5].ptr : nullptr};
+  hipLaunchKernelGGL((rms_norm_q8_kernel<XT, RT, I8>), dim3((unsigned)p.M), dim3(256), I8 ? 0 : nb * 4, ex.stream, g, p);
+  return 0;
+}
+
+template <int XT>
+int launch_swiglu(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const void *params, uint32_t params_len,
+                  std::string *err) {
+  (void)pl;
+  if (params_len != sizeof(SwigluF8Params)) {
+    *err = "parameter block of " + std::to_string(params_len) + " bytes, expected " + std::to_string(sizeof(SwigluF8Params));
+    return -1;
+  }
+  SwigluF8Params p;
+  memcpy(&p, params, sizeof p);
+  if (p.M < 0 || p.D < 1 || p.D > (1 << 20) || p.x_stride < 2 * p.D || p.o_stride < p.D) {
+    *err = "bad shape: M " + std::to_string(p.M) + " D " + std::to_string(p.D) + " (1 to 2^20) x_stride " +
+           std::to_string(p.x_stride) + " o_stride " + std::to_string(p.o_stride);
+    return -1;
+  }
+  if (nargs < 3) {
+    *err = "expected buffers x, out, scale";
+    return -1;
+  }
+  if (p.M == 0) return 0;
+  const int nb = (p.D + FB - 1) / FB;
+  const uint64_t xb = extent(p.M, p.x_stride, 2 * p.D, esize(XT)), ob = extent(p.M, p.o_stride, p.D, 1);
+  const uint64_t blocks = (uint64_t)p.M * nb, sb = blocks * 4;
+  if (!fits(a, 0, xb, esize(XT), "x", err) || !fits(a, 1, ob, 1, "out", err) || !fits(a, 2, sb, 4, "scale", err)) return -1;
+  if (overlap(a[0].ptr, xb, a[1].ptr, ob) || overlap(a[0].ptr, xb, a[2].ptr, sb) || overlap(a[1].ptr, ob, a[2].ptr, sb)) {
+    *err = "x, out and scale share memory";
+    return -1;
+  }
+  if (blocks >= (1ull << 28)) {  // 16 threads each, and a grid holds less than 2^32
+    *err = "over 2^28 - 1 blocks of 128 columns";
+    return -1;
+  }
+  hipLaunchKernelGGL((swiglu_f8_kernel<XT>), dim3((unsigned)((blocks + 15) / 16)), dim3(256), 0, ex.stream, a[0].ptr,
+                     (unsigned char *)a[1].ptr, (float *)a[2].ptr, p);
+  return 0;
+}
+
+template <int XT, int RT>
+LaunchFn pick_out(bool i8) {
+  return i8 ? launch_norm<XT, RT, true> : launch_norm<XT, RT, false>;
+}
+template <int XT>
+LaunchFn pick_res(int rt, bool i8) {
+  return rt == T_NONE   ? pick_out<XT, T_NONE>(i8)
+         : rt == T_BF16 ? pick_out<XT, T_BF16>(i8)
+         : rt == T_F16  ? pick_out<XT, T_F16>(i8)
+                        : pick_out<XT, T_F32>(i8);
+}
+
+int type_of(const std::string &s) {
+  if (s == "bfloat" || s == "bf16") return T_BF16;
+  if (s == "half" || s == "f16") return T_F16;
+  if (s == "float" || s == "f32") return T_F32;
+  if (s == "none") return T_NONE;
+  return -1;
+}
+
+}  // namespace
+
+// Macros: IN_T (half | bfloat | float), and for rms_norm_q8 RES_T (the residual's type, none without one) and OUT_T (f8 |
+// i8).
+bool make_rows_q8(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err) {
+  const bool norm = fn == "rms_norm_q8";
+  for (auto &kv : m)
+    if (kv.first != "IN_T" && !(norm && (kv.first == "RES_T" || kv.first == "OUT_T"))) {
+      *err = "unknown macro " + kv.first;
+      return false;
+    }
+  const int xt = type_of(macro_str(m, "IN_T", "bfloat")), rt = type_of(macro_str(m, "RES_T", "none"));
+  const std::string ot = macro_str(m, "OUT_T", "f8");
+  if (xt <= 0 || rt < 0 || (ot != "f8" && ot != "i8")) {
+    *err = "IN_T must be half|bfloat|float, RES_T that or none, OUT_T f8|i8";
+    return false;
+  }
+  const bool i8 = ot == "i8";
+  if (norm)
+    pl->launch = xt == T_BF16 ? pick_res<T_BF16>(rt, i8) : xt == T_F16 ? pick_res<T_F16>(rt, i8) : pick_res<T_F32>(rt, i8);
+  else
+    pl->launch = xt == T_BF16 ? launch_swiglu<T_BF16> : xt == T_F16 ? launch_swiglu<T_F16> : launch_swiglu<T_F32>;
+  pl->threads = 256;
+  return true;
+}
+
+}  // namespace h3

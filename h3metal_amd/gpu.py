@@ -93,10 +93,11 @@ def _call(name: str, *args, fails=lambda r: r != 0):
 
 _NULL = lambda r: not r  # noqa: E731 -- handle-returning calls fail with NULL
 
-# element type name -> (numpy dtype of its raw bytes, bytes per element); "bf16" travels as uint16 bit patterns
+# element type name -> (numpy dtype of its raw bytes, bytes per element); "bf16" travels as uint16 bit patterns, "f8"
+# (e4m3: 4 exponent and 3 mantissa bits, no infinities, largest value 448) as uint8 ones
 _DT = {"f32": (np.float32, 4), "f16": (np.float16, 2), "bf16": (np.uint16, 2), "i8": (np.int8, 1),
        "u8": (np.uint8, 1), "i32": (np.int32, 4), "u32": (np.uint32, 4), "i16": (np.int16, 2),
-       "u16": (np.uint16, 2)}
+       "u16": (np.uint16, 2), "f8": (np.uint8, 1)}
 _BY_NUMPY = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int8): "i8",
              np.dtype(np.uint8): "u8", np.dtype(np.int32): "i32", np.dtype(np.uint32): "u32",
              np.dtype(np.uint16): "bf16", np.dtype(np.int16): "i16"}

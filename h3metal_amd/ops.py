@@ -8,8 +8,12 @@ return value (None; results are valid after `gpu.wait()`):
   qk_norm_rope  <- h3metal/ops.py:225-239
   rot_q8        <- h3metal/ops.py:214-222 (the consumer of the attention output, h3metal/dit.py:209)
   QWeight, gemm <- h3metal/ops.py:19-34, 124-174 (the projections around attention; weight formats q8, h8,
-                   f16, bf16)
+                   f16, bf16 and f8)
   pad_rows      <- h3metal/ops.py:116-117
+
+and, without a counterpart there, the 8-bit feed-forward path: rms_norm_q8 (RMS norm with the residual's addition and an
+8-bit output), swiglu_f8 (the gated unit with an 8-bit output) and gemm's weight format f8 (e4m3 operands with a scale for
+each block of 128).
 
 Element types come from the tensors, as in the reference (`OUT_DT`,
 ops.py:17). The gfx950 kernels additionally accept bf16 Q/K/V (the reference's
@@ -24,8 +28,9 @@ from dataclasses import dataclass, replace
 from .gpu import Gpu, Tensor, pack
 
 OUT_DT = {"f16": "half", "bf16": "bfloat", "f32": "float"}
-FMT_ID = {"q8": 1, "q4": 2, "q4g": 3, "f16": 4, "bf16": 5, "h8": 6, "h4": 7, "h4g": 8}  # h3metal/ops.py:15
-GEMM_ACT = {"q8": "i8", "h8": "f16", "f16": "f16", "bf16": "bf16"}  # the formats built here and their activations
+FMT_ID = {"q8": 1, "q4": 2, "q4g": 3, "f16": 4, "bf16": 5, "h8": 6, "h4": 7, "h4g": 8,  # h3metal/ops.py:15
+          "f8": 9}
+GEMM_ACT = {"q8": "i8", "h8": "f16", "f16": "f16", "bf16": "bf16", "f8": "f8"}  # the formats built here and their activations
 LOG2E = 1.4426950408889634
 
 
@@ -124,11 +129,61 @@ def rot_q8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor | None, M: int, D: int, 
     gpu.launch(k, None, None, [x, out, sa], params)
 
 
+def rms_norm_q8(gpu: Gpu, x: Tensor, w: Tensor | None, out: Tensor, scale: Tensor, M: int, D: int, *, eps: float,
+                res: Tensor | None = None, res_out: Tensor | None = None, norm: bool = True,
+                x_stride: int | None = None, res_stride: int | None = None, res_out_stride: int | None = None,
+                o_stride: int | None = None):
+    """The residual's addition, the RMS norm of its rows and their rounding to 8 bits, in front of a projection:
+
+      h = res + x, rounded to res's type and written to res_out (default: res itself); h = x without res
+      v = h / sqrt(mean(h^2) + eps) * w (without w: no gain; with norm=False: v = h * w)
+      out f8: codes e4m3(v / s) with a scale for each row and block of 128 columns (the last may be short),
+              s = amax|v| / 448, or 1 where amax is 0; scale [M][ceil(D / 128)] f32: what gemm takes with format f8
+      out i8: codes rint(v / s), s = amax|v| / 127, or 1; scale [M] f32: what gemm takes with format q8
+
+    x [M][x_stride], res [M][res_stride], res_out [M][res_out_stride] f16 / bf16 / f32 (res_out as res), w [D] f32, out
+    [M][o_stride] f8 / i8; any D up to 2^20, any stride from D. The sum may take the place of res, or of x if that has its
+    type and stride. amax passes over NaN, whose code is NaN (f8) or 0 (i8)."""
+    if out.dtype not in ("f8", "i8") or scale.dtype != "f32":
+        raise ValueError(f"rms_norm_q8: out must be f8 or i8 and scale f32, got {out.dtype}, {scale.dtype}")
+    if w is not None and w.dtype != "f32":
+        raise ValueError(f"rms_norm_q8: w must be f32, got {w.dtype}")
+    if res is None:
+        if res_out is not None:
+            raise ValueError("rms_norm_q8: res_out needs res")
+    elif res_out is None:
+        res_out, res_out_stride = res, res_out_stride or res_stride
+    elif res_out.dtype != res.dtype:
+        raise ValueError(f"rms_norm_q8: res_out must be {res.dtype} as res, got {res_out.dtype}")
+    if x.dtype not in OUT_DT or (res is not None and res.dtype not in OUT_DT):
+        raise ValueError(f"rms_norm_q8: x and res must be f16, bf16 or f32, got {x.dtype}"
+                         + (f", {res.dtype}" if res is not None else ""))
+    k = gpu.kernel("ops", "rms_norm_q8", IN_T=OUT_DT[x.dtype], RES_T="none" if res is None else OUT_DT[res.dtype],
+                   OUT_T=out.dtype)
+    params = pack("6ifi", M, D, x_stride or D, res_stride or D, res_out_stride or D, o_stride or D, eps, int(norm))
+    gpu.launch(k, None, None, [x, res, w, out, scale, res_out], params)
+
+
+def swiglu_f8(gpu: Gpu, x: Tensor, out: Tensor, scale: Tensor, M: int, D: int, *, x_stride: int | None = None,
+              o_stride: int | None = None):
+    """value * silu(gate), value in columns 0..D-1 and gate in D..2D-1 of x, as e4m3 codes with a scale for each row and
+    block of 128 columns (the last may be short): s = amax / 448, or 1 where amax is 0, codes e4m3(v / s).
+    x [M][x_stride] f16 / bf16 / f32, out [M][o_stride] f8, scale [M][ceil(D / 128)] f32; any D up to 2^20. The
+    rotated int8 form with one scale a row is rot_q8(swiglu=True)."""
+    if x.dtype not in OUT_DT or out.dtype != "f8" or scale.dtype != "f32":
+        raise ValueError(f"swiglu_f8: x must be f16, bf16 or f32, out f8 and scale f32, got {x.dtype}, {out.dtype}, "
+                         f"{scale.dtype}")
+    k = gpu.kernel("ops", "swiglu_f8", IN_T=OUT_DT[x.dtype])
+    gpu.launch(k, None, None, [x, out, scale], pack("4i", M, D, x_stride or 2 * D, o_stride or D))
+
+
 @dataclass
 class QWeight:
     """A linear layer's weight on the GPU: W[N][K] in one of the reference's formats (h3metal/ops.py:19-34).
     This build runs "q8" and "h8" (int8 codes W[N][K] row-major, one float scale per output row sw[N]; int8 or
-    half activations) and "f16" / "bf16" (W[N][K] half / bfloat, no scales)."""
+    half activations), "f16" / "bf16" (W[N][K] half / bfloat, no scales) and, of its own, "f8" (e4m3 codes
+    W[N][K] row-major, one float scale per 128 x 128 block, sw[ceil(N / 128)][ceil(K / 128)]; e4m3 activations;
+    f8.block_codes makes both)."""
     fmt: str
     w: Tensor
     sw: Tensor | None
@@ -152,6 +207,9 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
       q8:  A int8 [M][K] with row scales sa, W int8 codes, v = sa[m] * sw[n] * (a_m . w_n)
       h8:  A half, W int8 codes, v = sw[n] * (a_m . w_n)
       f16 / bf16: A and W half / bfloat, v = a_m . w_n
+      f8:  A e4m3 [M][K] with scales sa[M][ceil(K / 128)], W e4m3, v = the sum over blocks b of 128 of K of
+           sa[m][b] * sw[n / 128][b] * (a_m . w_n over b). K a multiple of 16, any N; exactly M rows of A are read and
+           of out written (the other formats take rows padded to tile[0])
 
     ksplit: accumulate over that many consecutive slices of K in separate dispatches (epi 1 only), as the
     reference does. tile / swz are the Metal kernel's tile choices: checked as the reference checks them (the
@@ -160,7 +218,7 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
     no_alloc: dispatch through the allocation-free entry point (h3_dispatch_static); the h8 format's widened
     weights then live in its fixed scratch array."""
     if wt.fmt not in GEMM_ACT:
-        raise NotImplementedError(f"gemm: weight format {wt.fmt!r} is not built (q8, h8, f16, bf16)")
+        raise NotImplementedError(f"gemm: weight format {wt.fmt!r} is not built (q8, h8, f16, bf16, f8)")
     if a.dtype != GEMM_ACT[wt.fmt]:
         raise ValueError(f"gemm: format {wt.fmt} takes {GEMM_ACT[wt.fmt]} activations, got {a.dtype}")
     if wt.low is not None or _low is not None:
@@ -177,17 +235,22 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
                  no_alloc=no_alloc, **variant)
         return
     tm, tn, nsg = tile
-    if wt.N % tn:
+    f8 = wt.fmt == "f8"
+    if wt.N % tn and not f8:
         raise ValueError(f"gemm tile {tile}: {tn} columns do not divide the product's {wt.N}")
     if wt.fmt == "q8" and sa is None:
         raise ValueError("gemm: int8 activations need their row scales sa")
+    if f8:
+        if sa is None or wt.sw is None or wt.G != 128:
+            raise ValueError("gemm: e4m3 operands need their scales sa and sw, for blocks of 128")
+        tm = 1
     out_t = OUT_DT[out.dtype] if epi == 0 else "float"
     k = gpu.kernel("gemm", "gemm", WFMT=FMT_ID[wt.fmt], EPI=epi, OUT_T=out_t, TM=tm, TN=tn, NSG=nsg, G=wt.G,
                    HAS_BIAS=int(wt.bias is not None), SWZ=swz, **variant)
     if wt.fmt == "h8":
         gpu.reserve_workspace(wt.N * wt.K * 2)  # the widened weights; grows (and waits) only the first time
     m_pad = (M + tm - 1) // tm * tm
-    params = pack("8i", m_pad, wt.N, wt.K, a_stride or wt.K, c_stride or wt.N, wt.w_stride, wt.K // wt.G,
-                  g_stride or wt.N)
+    params = pack("8i", m_pad, wt.N, wt.K, a_stride or wt.K, c_stride or wt.N, wt.w_stride,
+                  (wt.K + 127) // 128 if f8 else wt.K // wt.G, g_stride or wt.N)
     gpu.launch(k, None, None, [a, wt.w, wt.sw, sa, out, wt.bias, rtype, gate], params, params_index=8,
                no_alloc=no_alloc)
