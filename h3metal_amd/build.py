@@ -34,7 +34,7 @@ PER_FILE = {
     "rot_q8.hip": ["-ffp-contract=off"],
     "gemm.hip": ["-ffp-contract=off"],
     "gemm_ksplit.hip": ["-ffp-contract=off"],
-    "gemm_f8.hip": ["-ffp-contract=off"],
+    "gemm_f8.hip": ["-ffp-contract=off", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "rows_q8.hip": ["-ffp-contract=off"],
     # score MFMAs with VGPR results (the softmax reads them), P V accumulators in AGPRs (inline assembly)
     "attention_wave.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
