@@ -62,20 +62,23 @@ __device__ __forceinline__ Operand<MODE> operand(const Codes &c) {
 // sees would make it wait for all of them.
 typedef const __attribute__((address_space(4))) float *Scalars;
 
-// The 32 x 32 sums of a block's products: element e is that of W row 8 (e / 4) + 4 (lane / 32) + e % 4 and A row lane % 32
-__device__ __forceinline__ f32x16 block_sums(const Codes &w, const Codes &a) {
-  f32x16 t = {};
-#pragma unroll
-  for (int c = 0; c < 4; c += 2)
-    t = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-        __builtin_shufflevector(w.d[c], w.d[c + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-        __builtin_shufflevector(a.d[c], a.d[c + 1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0, 0, 0, 0, 0, 0);
-  return t;
+// The 32 x 32 sums of a block's products, one matrix instruction of MMAS after the other: element e is that of W row
+// 8 (e / 4) + 4 (lane / 32) + e % 4 and A row lane % 32
+template <int MODE>
+constexpr int MMAS = MODE == HALF ? 8 : 2;
+__device__ __forceinline__ f32x16 mma(int c, const Codes &w, const Codes &a, f32x16 t) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+      __builtin_shufflevector(w.d[2 * c], w.d[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7),
+      __builtin_shufflevector(a.d[2 * c], a.d[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0, 0, 0, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 block_sums(const Halves &w, const Halves &a) {
+__device__ __forceinline__ f32x16 mma(int c, const Halves &w, const Halves &a, f32x16 t) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(w.d[c], a.d[c], t, 0, 0, 0);
+}
+template <int MODE>
+__device__ __forceinline__ f32x16 block_sums(const Operand<MODE> &w, const Operand<MODE> &a) {
   f32x16 t = {};
 #pragma unroll
-  for (int d = 0; d < 8; d++) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(w.d[d], a.d[d], t, 0, 0, 0);
+  for (int c = 0; c < MMAS<MODE>; c++) t = mma(c, w, a, t);
   return t;
 }
 
@@ -160,28 +163,61 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *p, size_t 
                                            __builtin_amdgcn_readfirstlane(max(0, rows) * str), 0x00020000);
 }
 
-// ---- large products: 8 waves on a TM x TN tile -----------------------------------------------------------------------
+// ---- large products: 8 waves on TM x TN tiles -------------------------------------------------------------------------
+
+// 16 x 16 sums of a block: lane l holds row l % 16's pieces 2 (l / 16) and 2 (l / 16) + 1; element e is that of W row
+// 4 (l / 16) + e and A row l % 16
+struct Codes16 {
+  i32x4 d[2];
+};
+struct Halves16 {
+  f16x8 d[4];
+};
+template <int MODE>
+using Operand16 = typename std::conditional<MODE == HALF, Halves16, Codes16>::type;
+
+template <int MODE>
+__device__ __forceinline__ Operand16<MODE> operand16(const Codes16 &c) {
+  if constexpr (MODE == E4M3) return c;
+  else {
+    Halves16 h;
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+      h.d[2 * d] = widen(c.d[d][0], c.d[d][1]);
+      h.d[2 * d + 1] = widen(c.d[d][2], c.d[d][3]);
+    }
+    return h;
+  }
+}
+template <int MODE>
+constexpr int MMAS16 = MODE == HALF ? 4 : 1;
+__device__ __forceinline__ f32x4 mma16(int, const Codes16 &w, const Codes16 &a, f32x4 t) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(w.d[0], w.d[1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                          __builtin_shufflevector(a.d[0], a.d[1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0,
+                                                          0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(int c, const Halves16 &w, const Halves16 &a, f32x4 t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(w.d[c], a.d[c], t, 0, 0, 0);
+}
 
 template <int MODE_, int TM_, int TN_>
 struct Tile {
   static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NW = 8, WGM = 4, WGN = 2;
-  static constexpr int WTM = TM / WGM, WTN = TN / WGN, MI = WTM / 32, NJ = WTN / 32;
-  static constexpr int NST = 2;                               // stages
-  static constexpr int STAGE = (TM + TN) * KB;                // LDS bytes of a block's rows
-  static constexpr int NQA = TM / 8 / NW, NQW = TN / 8 / NW;   // loads of A and W per wave and stage
-  static constexpr int SCALES = TM * 16;                      // LDS bytes of 4 blocks' scales
-  static constexpr int RS = TN * 4 + 16;                      // bytes of a row of results
-  static constexpr int PR = TM * RS <= 160 * 1024 ? TM : TM / 2;  // rows of results at a time
-  static constexpr int LDS = NST * STAGE + 2 * SCALES > PR * RS ? NST * STAGE + 2 * SCALES : PR * RS;
-  static_assert(LDS <= 160 * 1024 && PR % WTM == 0, "LDS");
+  static constexpr int WTM = TM / WGM, WTN = TN / WGN, MI = WTM / 16, NJ = WTN / 16;
+  static constexpr int STAGE = (TM + TN) * KB;                // LDS bytes of a block's rows; two stages
+  static constexpr int NQA = TM / 8 / NW, NQW = TN / 8 / NW;  // loads of A and W per wave and stage
+  static constexpr int SCALES = TM * 16;                      // LDS bytes of 4 blocks' scales; two of them
+  static constexpr int RS = 128 + 16, OUT = 16 * RS;          // LDS bytes of a row of results, of a wave's 16 rows
+  static constexpr int LDS = 2 * STAGE + 2 * SCALES + NW * OUT;
+  static_assert(LDS <= 160 * 1024 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
 };
 
 template <class C>
 __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_f8_tile(GemmArgs g, GemmParams p,
                                                                                                    int ntm, int ntn, int ot, int epi) {
-  constexpr int TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4;
+  constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4, MH = MI / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / C::WGN, wn = w % C::WGN;
   // bands of SW row tiles
   const int lid = xcd_order(blockIdx.x, gridDim.x), band = lid / (SW * ntn), in_band = lid - band * SW * ntn;
@@ -194,106 +230,202 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
   const __amdgpu_buffer_rsrc_t rs = rows_of(g.sa, m0, min(TM, p.M - m0), p.groups * 4);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
   // a stage: TM rows of A, then TN of W, 8 rows a load; wave w takes the loads NQA w .. of A and NQW w .. of W
-  int offa[C::NQA], offw[C::NQW];
-#pragma unroll
-  for (int q = 0; q < C::NQA; q++) offa[q] = (8 * (C::NQA * w + q) + (lane >> 3)) * p.a_stride + fetch_piece(C::NQA * w + q, lane) * 16;
-#pragma unroll
-  for (int q = 0; q < C::NQW; q++) offw[q] = (8 * (C::NQW * w + q) + (lane >> 3)) * p.w_stride + fetch_piece(C::NQW * w + q, lane) * 16;
-  auto dma = [&](int kt) __attribute__((always_inline)) {
+  const int fetch[2] = {fetch_piece(0, lane) * 16, fetch_piece(1, lane) * 16};
+  const int offa = (8 * C::NQA * w + (lane >> 3)) * p.a_stride, offw = (8 * C::NQW * w + (lane >> 3)) * p.w_stride;
+  auto dma = [&](int q, int kt) __attribute__((always_inline)) {
     const unsigned st = lds0 + (kt & 1) * C::STAGE;
-    const int left = p.K - kt * KB;
-    if (left >= KB) {
-#pragma unroll
-      for (int q = 0; q < C::NQA; q++) dma16(st + (C::NQA * w + q) * 1024, (unsigned)(offa[q] + kt * KB), ra);
-#pragma unroll
-      for (int q = 0; q < C::NQW; q++) dma16(st + TM * KB + (C::NQW * w + q) * 1024, (unsigned)(offw[q] + kt * KB), rw);
-    } else {  // pieces past K read as zero
-#pragma unroll
-      for (int q = 0; q < C::NQA; q++)
-        dma16(st + (C::NQA * w + q) * 1024,
-              fetch_piece(C::NQA * w + q, lane) * 16 < left ? (unsigned)(offa[q] + kt * KB) : 0x80000000u, ra);
-#pragma unroll
-      for (int q = 0; q < C::NQW; q++)
-        dma16(st + TM * KB + (C::NQW * w + q) * 1024,
-              fetch_piece(C::NQW * w + q, lane) * 16 < left ? (unsigned)(offw[q] + kt * KB) : 0x80000000u, rw);
+    const int left = p.K - kt * KB;  // pieces past K (all of them in blocks past the last) read as zero
+    if (q < C::NQA) {
+      const int f = fetch[(C::NQA % 2 ? w * C::NQA + q : q) & 1];
+      dma16(st + (C::NQA * w + q) * 1024, f < left ? (unsigned)(offa + 8 * q * p.a_stride + f + kt * KB) : 0x80000000u, ra);
+    } else {
+      const int r = q - C::NQA, f = fetch[(C::NQW % 2 ? w * C::NQW + r : r) & 1];
+      dma16(st + TM * KB + (C::NQW * w + r) * 1024, f < left ? (unsigned)(offw + 8 * r * p.w_stride + f + kt * KB) : 0x80000000u,
+            rw);
     }
   };
+  constexpr int NQ = C::NQA + C::NQW;
   // 4 blocks' scales of the tile's rows, [row][4]: blocks first .. first + 3; the last four where there are no more
   auto first = [&](int c) { return min(4 * c, nb - 4); };
   auto dma_scales = [&](int c) __attribute__((always_inline)) {
     if (w < TM / 64)
-      dma16(lds0 + C::NST * C::STAGE + (c & 1) * C::SCALES + w * 1024, (unsigned)((64 * w + lane) * p.groups + first(c)) * 4, rs);
+      dma16(lds0 + 2 * C::STAGE + (c & 1) * C::SCALES + w * 1024, (unsigned)((64 * w + lane) * p.groups + first(c)) * 4, rs);
   };
-  float *scales = (float *)(smem + C::NST * C::STAGE);
+  float *scales = (float *)(smem + 2 * C::STAGE);
   const Scalars sw = (Scalars)(g.sw + (size_t)min((n0 + WTN * wn) / KB, (p.N - 1) / KB) * p.groups);
 
-  f32x16 acc[MI][NJ];
+  f32x4 acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) acc[i][j] = f32x16{};
+    for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{};
 
-  dma(0);
+  // (16 rows further the swizzle is the same)
+  int pa[2], pw[2];
+#pragma unroll
+  for (int d = 0; d < 2; d++) {
+    pa[d] = slot(WTM * wm + l16, 2 * lg + d);
+    pw[d] = TM * KB + slot(WTN * wn + l16, 2 * lg + d);
+  }
+  auto read = [&](const int (&at)[2], int t, int kt) __attribute__((always_inline)) {
+    Codes16 c;
+#pragma unroll
+    for (int d = 0; d < 2; d++) c.d[d] = *(const i32x4 *)(smem + (at[d] + (kt & 1) * C::STAGE) + 16 * t * KB);
+    return c;
+  };
+  auto read_scale = [&](int i, int kt) __attribute__((always_inline)) {
+    const int r = WTM * wm + 16 * i + l16, c = kt >> 2, at = nb >= 4 ? kt - first(c) : kt;
+    return scales[(c & 1) * (C::SCALES / 4) + 4 * r + at];
+  };
+
+#pragma unroll
+  for (int q = 0; q < NQ; q++) dma(q, 0);
   if (nb >= 4) {
     dma_scales(0);
   } else if (tid < TM) {
     for (int b = 0; b < nb; b++) scales[4 * tid + b] = g.sa[(size_t)min(m0 + tid, p.M - 1) * p.groups + b];
   }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NQ; q++) dma(q, 1);
+
+  // Step kt multiplies A's rows of a block (held for the whole step) by W's, 16 at a time. All of stage kt has been read when
+  // W's last 32 rows are still to be multiplied: there the waves meet, stage kt + 2 takes its place, and beside the last
+  // multiplications the first operands of step kt + 1 are read (half of A's rows into registers of their own, the others
+  // into those that the last multiplications free).
+  // The order is kept as written (sched_barrier): each matrix instruction is followed by the fused adds of the sums MI
+  // instructions before it. One wave then keeps the matrix unit busy; sums multiplied and added by turns left it idle for
+  // the adds (16 x 16 tiles: 135 cycles for what takes the matrix unit 128, 32 x 32 ones 148 to 200).
+  Codes16 a[MI], an[MH], wb[2], wl;
+  float sc[MI], fs[MI];
+  f32x4 t[MI];
+#pragma unroll
+  for (int i = 0; i < MI; i++) {
+    a[i] = read(pa, i, 0);
+    sc[i] = read_scale(i, 0);
+    t[i] = f32x4{};
+    fs[i] = 0.0f;
+  }
+  wb[0] = read(pw, 0, 0);
+  float s = sw[0];
   for (int kt = 0; kt < nb; kt++) {
-    // stage kt has landed, and every wave has read stage kt - 1
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kt + 1 < nb) dma(kt + 1);
-    if ((kt & 3) == 0 && kt + 4 < nb) dma_scales(kt / 4 + 1);
-    const char *sA = smem + (kt & 1) * C::STAGE, *sW = sA + TM * KB;
-    const float s = sw[kt];
-    const int c = kt >> 2, at = nb >= 4 ? kt - first(c) : kt;
-    Operand<C::MODE> a[MI];
-    float sc[MI];
-#pragma unroll
-    for (int i = 0; i < MI; i++) {
-      const int r = WTM * wm + 32 * i + l32;
-      a[i] = operand<C::MODE>(read_codes(sA, r, hl));
-      sc[i] = scales[(c & 1) * (C::SCALES / 4) + 4 * r + at] * s;
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const Operand<C::MODE> b = operand<C::MODE>(read_codes(sW, WTN * wn + 32 * j + l32, hl));
+    const int nx = min(kt + 1, nb - 1);
+    const float snext = sw[nx];
+    Operand16<MODE> ao[MI];
+    // sums (i, j) for every i; `with(n)` goes behind the n-th of them
+    auto row = [&](int j, const Codes16 &wc, auto with) __attribute__((always_inline)) {
+      constexpr int NM = MMAS16<MODE>;
+      const Operand16<MODE> b = operand16<MODE>(wc);
+      f32x4 u[MI];
 #pragma unroll
       for (int i = 0; i < MI; i++) {
-        const f32x16 t = block_sums(b, a[i]);
+        if (j == 0) ao[i] = operand16<MODE>(a[i]);
+        u[i] = f32x4{};
 #pragma unroll
-        for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(t[e], sc[i], acc[i][j][e]);
+        for (int c = 0; c < NM; c++) u[i] = mma16(c, b, ao[i], u[i]);
+        __builtin_amdgcn_sched_barrier(0);
+        const int pj = (j + NJ - 1) % NJ;
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
+        asm volatile("" : "+v"(acc[i][pj]));
+        if (j == 0) fs[i] = sc[i] * s;
+        with(i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
+#pragma unroll
+      for (int i = 0; i < MI; i++) t[i] = u[i];
+    };
+#pragma unroll
+    for (int j = 0; j < NJ - 2; j++)
+      row(j, wb[j & 1], [&](int i) __attribute__((always_inline)) {
+        if (i == 0) wb[(j + 1) & 1] = read(pw, j + 1, kt);
+        if (i == 1 && j == NJ - 3) wl = read(pw, NJ - 1, kt);
+      });
+    // stage kt + 1 has landed, and every wave has read stage kt
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    if ((kt & 3) == 0 && kt + 4 < nb) dma_scales(kt / 4 + 1);
+    row(NJ - 2, wb[0], [&](int i) __attribute__((always_inline)) {
+      if (i < MH) {
+        an[i] = read(pa, i, nx);
+      } else {
+#pragma unroll
+        for (int q = (i - MH) * NQ / (2 * MH); q < (i - MH + 1) * NQ / (2 * MH); q++) dma(q, kt + 2);
+      }
+    });
+    wb[0] = read(pw, 0, nx);
+    row(NJ - 1, wl, [&](int i) __attribute__((always_inline)) {
+      sc[i] = read_scale(i, nx);
+      if (i >= MH) a[i] = read(pa, i, nx);
+#pragma unroll
+      for (int q = NQ / 2 + i * (NQ - NQ / 2) / MI; q < NQ / 2 + (i + 1) * (NQ - NQ / 2) / MI; q++) dma(q, kt + 2);
+    });
+#pragma unroll
+    for (int i = 0; i < MH; i++) a[i] = an[i];
+    s = snext;
   }
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[i][NJ - 1][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][NJ - 1][e]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-  // results through LDS, PR rows at a time, then 8 columns a thread
-  constexpr int PPR = TN / 8;
+  // Results leave through a wave's own 16 rows of LDS, 128 bytes of each at a time, so no wave waits for another.
+  char *own = smem + 2 * C::STAGE + 2 * C::SCALES + w * C::OUT;
+  const int mw = m0 + WTM * wm, nw = n0 + WTN * wn;
+  if (ot == T_F32) {
 #pragma unroll
-  for (int ps = 0; ps < TM / C::PR; ps++) {
-    __syncthreads();
-    if (WTM * wm / C::PR == ps) {
+    for (int i = 0; i < MI; i++)
 #pragma unroll
-      for (int i = 0; i < MI; i++)
+      for (int j = 0; j < NJ; j += 2) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-          for (int q = 0; q < 4; q++)
-            *(f32x4 *)(smem + (WTM * wm + 32 * i + l32 - C::PR * ps) * C::RS + (WTN * wn + 32 * j + 8 * q + 4 * hl) * 4) =
-                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    }
-    __syncthreads();
-    const int nl = 8 * (tid % PPR), n = n0 + nl;
-    if (n < p.N) {
-#pragma unroll 2
-      for (int ml = tid / PPR; ml < C::PR; ml += C::NW * 64 / PPR) {
-        const int m = m0 + C::PR * ps + ml;
-        if (m >= p.M) break;
+        for (int h = 0; h < 2; h++) *(f32x4 *)(own + l16 * C::RS + h * 64 + lg * 16) = acc[i][j + h];
+        const int r = lane >> 2, m = mw + 16 * i + r, n = nw + 16 * j + (lane & 3) * 8;
         float v[8];
-        *(f32x4 *)v = *(const f32x4 *)(smem + ml * C::RS + nl * 4);
-        *(f32x4 *)(v + 4) = *(const f32x4 *)(smem + ml * C::RS + nl * 4 + 16);
-        finish(g, p, ot, epi, m, n, g.vec, v);
+        *(f32x4 *)v = *(const f32x4 *)(own + r * C::RS + (lane & 3) * 32);
+        *(f32x4 *)(v + 4) = *(const f32x4 *)(own + r * C::RS + (lane & 3) * 32 + 16);
+        if (m < p.M && n < p.N) finish(g, p, ot, epi, m, n, g.vec, v);
+      }
+  } else {
+    const bool all = g.vec;
+#pragma unroll
+    for (int j = 0; j < NJ; j += 4) {
+      f32x4 bias[4] = {};
+      if (g.bias)
+#pragma unroll
+        for (int h = 0; h < 4; h++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) bias[h][e] = g.bias[min(nw + 16 * (j + h) + 4 * lg + e, p.N - 1)];
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+          typedef unsigned short h4 __attribute__((ext_vector_type(4)));
+          h4 o;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float v = g.bias ? acc[i][j + h][e] + bias[h][e] : acc[i][j + h][e];
+            o[e] = ot == T_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v) : __builtin_bit_cast(unsigned short, (_Float16)v);
+          }
+          *(h4 *)(own + l16 * C::RS + h * 32 + lg * 8) = o;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int r = 8 * h + (lane >> 3), m = mw + 16 * i + r, n = nw + 16 * j + (lane & 7) * 8;
+          const uint4 d = *(const uint4 *)(own + r * C::RS + (lane & 7) * 16);
+          if (m < p.M && n < p.N) {
+            unsigned short *dst = (unsigned short *)g.out + (size_t)m * p.c_stride + n;
+            if (all) {
+              *(uint4 *)dst = d;
+            } else {
+              const unsigned short *hs = (const unsigned short *)&d;
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (n + e < p.N) dst[e] = hs[e];
+            }
+          }
+        }
       }
     }
   }
@@ -383,7 +515,7 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
       const float sc = cur.sa[i] * swk;
 #pragma unroll
       for (int j = 0; j < NJ; j++) {
-        const f32x16 t = block_sums(b[j], a);
+        const f32x16 t = block_sums<C::MODE>(b[j], a);
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(t[e], sc, acc[i][j][e]);
       }
