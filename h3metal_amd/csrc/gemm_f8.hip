@@ -209,171 +209,15 @@ struct Tile {
   static constexpr int SCALES = TM * 16;                      // LDS bytes of 4 blocks' scales; two of them
   static constexpr int RS = 128 + 16, OUT = 16 * RS;          // LDS bytes of a row of results, of a wave's 16 rows
   static constexpr int LDS = 2 * STAGE + 2 * SCALES + NW * OUT;
-  static_assert(LDS <= 160 * 1024 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
+  static_assert(LDS <= 160 * 1024 && NQA % 2 == 0 && NQW % 2 == 0 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
 };
 
+// The sums of a wave's rows mw .. and columns nw ..: they leave through a wave's own 16 rows of LDS, 128 bytes of each at a time, so no wave waits for another.
 template <class C>
-__global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_f8_tile(GemmArgs g, GemmParams p,
-                                                                                                   int ntm, int ntn, int ot, int epi) {
-  constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4, MH = MI / 2;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / C::WGN, wn = w % C::WGN;
-  // bands of SW row tiles
-  const int lid = xcd_order(blockIdx.x, gridDim.x), band = lid / (SW * ntn), in_band = lid - band * SW * ntn;
-  const int rows_in_band = min(SW, ntm - band * SW);
-  const int m0 = (band * SW + in_band % rows_in_band) * TM, n0 = in_band / rows_in_band * TN;
-  const int nb = (p.K + KB - 1) / KB;
-
-  const __amdgpu_buffer_rsrc_t ra = rows_of(g.a, m0, min(TM, p.M - m0), p.a_stride);
-  const __amdgpu_buffer_rsrc_t rw = rows_of(g.w, n0, min(TN, p.N - n0), p.w_stride);
-  const __amdgpu_buffer_rsrc_t rs = rows_of(g.sa, m0, min(TM, p.M - m0), p.groups * 4);
-  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
-  // a stage: TM rows of A, then TN of W, 8 rows a load; wave w takes the loads NQA w .. of A and NQW w .. of W
-  const int fetch[2] = {fetch_piece(0, lane) * 16, fetch_piece(1, lane) * 16};
-  const int offa = (8 * C::NQA * w + (lane >> 3)) * p.a_stride, offw = (8 * C::NQW * w + (lane >> 3)) * p.w_stride;
-  auto dma = [&](int q, int kt) __attribute__((always_inline)) {
-    const unsigned st = lds0 + (kt & 1) * C::STAGE;
-    const int left = p.K - kt * KB;  // pieces past K (all of them in blocks past the last) read as zero
-    if (q < C::NQA) {
-      const int f = fetch[(C::NQA % 2 ? w * C::NQA + q : q) & 1];
-      dma16(st + (C::NQA * w + q) * 1024, f < left ? (unsigned)(offa + 8 * q * p.a_stride + f + kt * KB) : 0x80000000u, ra);
-    } else {
-      const int r = q - C::NQA, f = fetch[(C::NQW % 2 ? w * C::NQW + r : r) & 1];
-      dma16(st + TM * KB + (C::NQW * w + r) * 1024, f < left ? (unsigned)(offw + 8 * r * p.w_stride + f + kt * KB) : 0x80000000u,
-            rw);
-    }
-  };
-  constexpr int NQ = C::NQA + C::NQW;
-  // 4 blocks' scales of the tile's rows, [row][4]: blocks first .. first + 3; the last four where there are no more
-  auto first = [&](int c) { return min(4 * c, nb - 4); };
-  auto dma_scales = [&](int c) __attribute__((always_inline)) {
-    if (w < TM / 64)
-      dma16(lds0 + 2 * C::STAGE + (c & 1) * C::SCALES + w * 1024, (unsigned)((64 * w + lane) * p.groups + first(c)) * 4, rs);
-  };
-  float *scales = (float *)(smem + 2 * C::STAGE);
-  const Scalars sw = (Scalars)(g.sw + (size_t)min((n0 + WTN * wn) / KB, (p.N - 1) / KB) * p.groups);
-
-  f32x4 acc[MI][NJ];
-#pragma unroll
-  for (int i = 0; i < MI; i++)
-#pragma unroll
-    for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{};
-
-  // (16 rows further the swizzle is the same)
-  int pa[2], pw[2];
-#pragma unroll
-  for (int d = 0; d < 2; d++) {
-    pa[d] = slot(WTM * wm + l16, 2 * lg + d);
-    pw[d] = TM * KB + slot(WTN * wn + l16, 2 * lg + d);
-  }
-  auto read = [&](const int (&at)[2], int t, int kt) __attribute__((always_inline)) {
-    Codes16 c;
-#pragma unroll
-    for (int d = 0; d < 2; d++) c.d[d] = *(const i32x4 *)(smem + (at[d] + (kt & 1) * C::STAGE) + 16 * t * KB);
-    return c;
-  };
-  auto read_scale = [&](int i, int kt) __attribute__((always_inline)) {
-    const int r = WTM * wm + 16 * i + l16, c = kt >> 2, at = nb >= 4 ? kt - first(c) : kt;
-    return scales[(c & 1) * (C::SCALES / 4) + 4 * r + at];
-  };
-
-#pragma unroll
-  for (int q = 0; q < NQ; q++) dma(q, 0);
-  if (nb >= 4) {
-    dma_scales(0);
-  } else if (tid < TM) {
-    for (int b = 0; b < nb; b++) scales[4 * tid + b] = g.sa[(size_t)min(m0 + tid, p.M - 1) * p.groups + b];
-  }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < NQ; q++) dma(q, 1);
-
-  // Step kt multiplies A's rows of a block (held for the whole step) by W's, 16 at a time. All of stage kt has been read when
-  // W's last 32 rows are still to be multiplied: there the waves meet, stage kt + 2 takes its place, and beside the last
-  // multiplications the first operands of step kt + 1 are read (half of A's rows into registers of their own, the others
-  // into those that the last multiplications free).
-  // The order is kept as written (sched_barrier): each matrix instruction is followed by the fused adds of the sums MI
-  // instructions before it. One wave then keeps the matrix unit busy; sums multiplied and added by turns left it idle for
-  // the adds (16 x 16 tiles: 135 cycles for what takes the matrix unit 128, 32 x 32 ones 148 to 200).
-  Codes16 a[MI], an[MH], wb[2], wl;
-  float sc[MI], fs[MI];
-  f32x4 t[MI];
-#pragma unroll
-  for (int i = 0; i < MI; i++) {
-    a[i] = read(pa, i, 0);
-    sc[i] = read_scale(i, 0);
-    t[i] = f32x4{};
-    fs[i] = 0.0f;
-  }
-  wb[0] = read(pw, 0, 0);
-  float s = sw[0];
-  for (int kt = 0; kt < nb; kt++) {
-    const int nx = min(kt + 1, nb - 1);
-    const float snext = sw[nx];
-    Operand16<MODE> ao[MI];
-    // sums (i, j) for every i; `with(n)` goes behind the n-th of them
-    auto row = [&](int j, const Codes16 &wc, auto with) __attribute__((always_inline)) {
-      constexpr int NM = MMAS16<MODE>;
-      const Operand16<MODE> b = operand16<MODE>(wc);
-      f32x4 u[MI];
-#pragma unroll
-      for (int i = 0; i < MI; i++) {
-        if (j == 0) ao[i] = operand16<MODE>(a[i]);
-        u[i] = f32x4{};
-#pragma unroll
-        for (int c = 0; c < NM; c++) u[i] = mma16(c, b, ao[i], u[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        const int pj = (j + NJ - 1) % NJ;
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
-        asm volatile("" : "+v"(acc[i][pj]));
-        if (j == 0) fs[i] = sc[i] * s;
-        with(i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int i = 0; i < MI; i++) t[i] = u[i];
-    };
-#pragma unroll
-    for (int j = 0; j < NJ - 2; j++)
-      row(j, wb[j & 1], [&](int i) __attribute__((always_inline)) {
-        if (i == 0) wb[(j + 1) & 1] = read(pw, j + 1, kt);
-        if (i == 1 && j == NJ - 3) wl = read(pw, NJ - 1, kt);
-      });
-    // stage kt + 1 has landed, and every wave has read stage kt
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __syncthreads();
-    if ((kt & 3) == 0 && kt + 4 < nb) dma_scales(kt / 4 + 1);
-    row(NJ - 2, wb[0], [&](int i) __attribute__((always_inline)) {
-      if (i < MH) {
-        an[i] = read(pa, i, nx);
-      } else {
-#pragma unroll
-        for (int q = (i - MH) * NQ / (2 * MH); q < (i - MH + 1) * NQ / (2 * MH); q++) dma(q, kt + 2);
-      }
-    });
-    wb[0] = read(pw, 0, nx);
-    row(NJ - 1, wl, [&](int i) __attribute__((always_inline)) {
-      sc[i] = read_scale(i, nx);
-      if (i >= MH) a[i] = read(pa, i, nx);
-#pragma unroll
-      for (int q = NQ / 2 + i * (NQ - NQ / 2) / MI; q < NQ / 2 + (i + 1) * (NQ - NQ / 2) / MI; q++) dma(q, kt + 2);
-    });
-#pragma unroll
-    for (int i = 0; i < MH; i++) a[i] = an[i];
-    s = snext;
-  }
-#pragma unroll
-  for (int i = 0; i < MI; i++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[i][NJ - 1][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][NJ - 1][e]);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-
-  // Results leave through a wave's own 16 rows of LDS, 128 bytes of each at a time, so no wave waits for another.
-  char *own = smem + 2 * C::STAGE + 2 * C::SCALES + w * C::OUT;
-  const int mw = m0 + WTM * wm, nw = n0 + WTN * wn;
+__device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, int mw, int nw, int lane,
+                                           char *own, const f32x4 (&acc)[C::MI][C::NJ]) {
+  constexpr int MI = C::MI, NJ = C::NJ;
+  const int l16 = lane & 15, lg = lane >> 4;
   if (ot == T_F32) {
 #pragma unroll
     for (int i = 0; i < MI; i++)
@@ -429,6 +273,211 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
       }
     }
   }
+}
+
+template <class C>
+__global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_f8_tile(GemmArgs g, GemmParams p,
+                                                                                                   int ntm, int ntn, int ot, int epi) {
+  constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4;
+  constexpr int MH = 1;  // operands of the next step in registers of their own
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / C::WGN, wn = w % C::WGN;
+  // A workgroup takes several tiles: those of its XCD (workgroup b runs on XCD b % 8), which are consecutive ones in bands of
+  // SW row tiles, by turns with the others there.
+  const int nt = ntm * ntn, xcd = blockIdx.x & 7, per = nt >> 3, rem = nt & 7;
+  const int tend = xcd * per + min(xcd, rem) + per + (xcd < rem), tstep = ((int)gridDim.x - xcd + 7) >> 3;
+  int tile = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
+  if (tile >= tend) return;
+  const int nb = (p.K + KB - 1) / KB, ns = max(nb, 2);  // blocks, steps (a step past the blocks adds nothing)
+
+  struct At {
+    int m0, n0;
+    __amdgpu_buffer_rsrc_t ra, rw, rs;
+  };
+  auto at_tile = [&](int t) __attribute__((always_inline)) {  // t past the end: no rows, every load reads zero
+    At x;
+    const int band = t / (SW * ntn), in_band = t - band * SW * ntn, rows_in_band = max(1, min(SW, ntm - band * SW));
+    x.m0 = (band * SW + in_band % rows_in_band) * TM, x.n0 = in_band / rows_in_band * TN;
+    const int mr = t < tend ? min(TM, p.M - x.m0) : 0, nr = t < tend ? min(TN, p.N - x.n0) : 0;
+    const size_t m = mr ? x.m0 : 0, n = nr ? x.n0 : 0;
+    x.ra = rows_of(g.a, m, mr, p.a_stride);
+    x.rw = rows_of(g.w, n, nr, p.w_stride);
+    x.rs = rows_of(g.sa, m, mr, p.groups * 4);
+    return x;
+  };
+  At ld = at_tile(tile);  // the tile whose rows are being loaded: two steps ahead of the multiplications
+  int m0 = ld.m0, n0 = ld.n0;
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem;
+  // a stage: TM rows of A, then TN of W, 8 rows a load; wave w takes the loads NQA w .. of A and NQW w .. of W
+  const int fetch = fetch_piece(0, lane) * 16;  // of even loads; ^ 64 for odd ones
+  const int offa = (8 * C::NQA * w + (lane >> 3)) * p.a_stride, offw = (8 * C::NQW * w + (lane >> 3)) * p.w_stride;
+  int phase = 0;  // step kt's stage is (kt + phase) & 1, chunk c of its scales in buffer (c + sphase) & 1
+  int sphase = 0;
+  auto dma = [&](int q, int kt, int stage) __attribute__((always_inline)) {
+    const unsigned st = lds0 + stage * C::STAGE;
+    const int left = p.K - kt * KB;  // pieces past K (all of them in blocks past the last) read as zero
+    const int r = q < C::NQA ? q : q - C::NQA, f = r & 1 ? fetch ^ 64 : fetch;
+    if (q < C::NQA)
+      dma16(st + (C::NQA * w + r) * 1024, f < left ? (unsigned)(offa + 8 * r * p.a_stride + f + kt * KB) : 0x80000000u, ld.ra);
+    else
+      dma16(st + TM * KB + (C::NQW * w + r) * 1024, f < left ? (unsigned)(offw + 8 * r * p.w_stride + f + kt * KB) : 0x80000000u,
+            ld.rw);
+  };
+  constexpr int NQ = C::NQA + C::NQW;
+  // 4 blocks' scales of the tile's rows, [row][4]: blocks first .. first + 3; the last four where there are no more
+  auto first = [&](int c) { return min(4 * c, nb - 4); };
+  const int nc = (ns + 3) >> 2;
+  auto dma_scales = [&](int c, int buf) __attribute__((always_inline)) {
+    if (w < TM / 64)
+      dma16(lds0 + 2 * C::STAGE + buf * C::SCALES + w * 1024, (unsigned)((64 * w + lane) * p.groups + first(c)) * 4, ld.rs);
+  };
+  float *scales = (float *)(smem + 2 * C::STAGE);
+  // few blocks: read straight from memory, by every thread a row
+  auto load_scales = [&](int buf) __attribute__((always_inline)) {
+    if (tid < TM)
+      for (int b = 0; b < ns; b++)
+        scales[buf * (C::SCALES / 4) + 4 * tid + b] = g.sa[(size_t)min(m0 + tid, p.M - 1) * p.groups + min(b, nb - 1)];
+  };
+  auto scales_of = [&](int n) { return (Scalars)(g.sw + (size_t)min((n + WTN * wn) / KB, (p.N - 1) / KB) * p.groups); };
+
+  f32x4 acc[MI][NJ];
+
+  // (16 rows further the swizzle is the same)
+  const int at[2] = {slot(l16, 2 * lg), slot(l16, 2 * lg + 1)}, pa = WTM * wm * KB, pw = (TM + WTN * wn) * KB;
+  auto read = [&](int rows, int t, int stage) __attribute__((always_inline)) {
+    Codes16 c;
+#pragma unroll
+    for (int d = 0; d < 2; d++) c.d[d] = *(const i32x4 *)(smem + (at[d] + (rows + stage * C::STAGE)) + 16 * t * KB);
+    return c;
+  };
+  // of block kt from buffer buf
+  auto read_scale = [&](int i, int kt, int buf) __attribute__((always_inline)) {
+    const int r = WTM * wm + 16 * i + l16, at = nb >= 4 ? kt - first(kt >> 2) : kt;
+    return scales[buf * (C::SCALES / 4) + 4 * r + at];
+  };
+
+#pragma unroll
+  for (int q = 0; q < NQ; q++) dma(q, 0, 0);
+  if (nb >= 4) dma_scales(0, 0);
+  else load_scales(0);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NQ; q++) dma(q, 1, 1);
+
+  // Step kt multiplies A's rows of a block (held for the whole step) by W's, 16 at a time. All of stage kt has been read when
+  // W's last 32 rows are still to be multiplied: there the waves meet, stage kt + 2 takes its place, and beside the last
+  // multiplications the first operands of step kt + 1 are read (A's first 16 rows into registers of their own, the others
+  // into those that the last multiplications free).
+  // The order is kept as written (sched_barrier): each matrix instruction is followed by the fused adds of the sums MI
+  // instructions before it. One wave then keeps the matrix unit busy; sums multiplied and added by turns left it idle for
+  // the adds (16 x 16 tiles: 135 cycles for what takes the matrix unit 128, 32 x 32 ones 148 to 200).
+  Codes16 a[MI], an[MH], wb[2], wl;
+  float sc[MI], fs[MI];
+  f32x4 t[MI];
+#pragma unroll
+  for (int i = 0; i < MI; i++) {
+    a[i] = read(pa, i, 0);
+    sc[i] = read_scale(i, 0, 0);
+  }
+  wb[0] = read(pw, 0, 0);
+  Scalars sw = scales_of(n0), swn = sw;
+  float s = sw[0];
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
+#pragma unroll
+      for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{};
+      t[i] = f32x4{};
+      fs[i] = 0.0f;
+    }
+    for (int kt = 0; kt < ns; kt++) {
+      const bool last = kt + 1 == ns;
+      const int nx = last ? 0 : kt + 1, stage = (kt + phase) & 1;  // the next step: of the next tile behind the last
+      const int nbuf = last ? (nc + sphase) & 1 : ((nx >> 2) + sphase) & 1;
+      Operand16<MODE> ao[MI];
+      // sums (i, j) for every i; `with(n)` goes behind the n-th of them
+      auto row = [&](int j, const Codes16 &wc, auto with) __attribute__((always_inline)) {
+        constexpr int NM = MMAS16<MODE>;
+        const Operand16<MODE> b = operand16<MODE>(wc);
+        f32x4 u[MI];
+#pragma unroll
+        for (int i = 0; i < MI; i++) {
+          if (j == 0) ao[i] = operand16<MODE>(a[i]);
+          u[i] = f32x4{};
+#pragma unroll
+          for (int c = 0; c < NM; c++) u[i] = mma16(c, b, ao[i], u[i]);
+          __builtin_amdgcn_sched_barrier(0);
+          const int pj = (j + NJ - 1) % NJ;
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
+          asm volatile("" : "+v"(acc[i][pj]));
+          if (j == 0) fs[i] = sc[i] * s;
+          with(i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < MI; i++) t[i] = u[i];
+      };
+#pragma unroll
+      for (int j = 0; j < NJ - 2; j++)
+        row(j, wb[j & 1], [&](int i) __attribute__((always_inline)) {
+          if (i == 0) wb[(j + 1) & 1] = read(pw, j + 1, stage);
+          if (i == 1 && j == NJ - 3) wl = read(pw, NJ - 1, stage);
+        });
+      // the next stage has landed, and every wave has read this one
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+      int kl = kt + 2;  // the step to load; behind the last one the next tile's
+      if (kl == ns) {
+        ld = at_tile(tile + tstep);
+        swn = scales_of(ld.n0);
+        if (nb >= 4) dma_scales(0, (nc + sphase) & 1);
+      } else if ((kt & 3) == 0 && kt + 4 < nb) {
+        dma_scales((kt >> 2) + 1, ((kt >> 2) + 1 + sphase) & 1);
+      }
+      kl = kl >= ns ? kl - ns : kl;
+      const float snext = last ? swn[0] : sw[min(nx, nb - 1)];
+      row(NJ - 2, wb[0], [&](int i) __attribute__((always_inline)) {
+        if (i < MH) {
+          an[i] = read(pa, i, stage ^ 1);
+        } else {
+#pragma unroll
+          for (int q = (i - MH) * (NQ / 2) / (MI - MH); q < (i - MH + 1) * (NQ / 2) / (MI - MH); q++) dma(q, kl, stage);
+        }
+      });
+      wb[0] = read(pw, 0, stage ^ 1);
+      row(NJ - 1, wl, [&](int i) __attribute__((always_inline)) {
+        sc[i] = read_scale(i, nx, nbuf);
+        if (i >= MH) a[i] = read(pa, i, stage ^ 1);
+#pragma unroll
+        for (int q = NQ / 2 + i * (NQ - NQ / 2) / MI; q < NQ / 2 + (i + 1) * (NQ - NQ / 2) / MI; q++) dma(q, kl, stage);
+      });
+#pragma unroll
+      for (int i = 0; i < MH; i++) a[i] = an[i];
+      s = snext;
+    }
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[i][NJ - 1][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][NJ - 1][e]);
+    store_tile<C>(g, p, ot, epi, m0 + WTM * wm, n0 + WTN * wn, lane, smem + 2 * C::STAGE + 2 * C::SCALES + w * C::OUT, acc);
+    tile += tstep;
+    if (tile >= tend) break;
+    phase = (phase + ns) & 1;
+    sphase = (sphase + nc) & 1;
+    m0 = ld.m0, n0 = ld.n0;
+    sw = swn;
+    if (nb < 4) {
+      __syncthreads();  // every wave has read its last scales
+      load_scales(sphase);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MI; i++) sc[i] = read_scale(i, 0, sphase);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // ---- few tiles: the waves of a workgroup split K ----------------------------------------------------------------------
@@ -646,7 +695,8 @@ int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_
   if (!set && set_lds(kern, C::LDS, err)) return -1;
   set = true;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(ntm * ntn)), dim3(C::NW * 64), C::LDS, stream, g, p, ntm, ntn, ot, epi);
+  const int cus = cu_count(), slots = cus > 0 ? cus * (160 * 1024 / C::LDS) : 256;
+  hipLaunchKernelGGL(kern, dim3((unsigned)std::min(ntm * ntn, slots)), dim3(C::NW * 64), C::LDS, stream, g, p, ntm, ntn, ot, epi);
   return 0;
 }
 
