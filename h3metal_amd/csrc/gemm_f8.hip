@@ -171,7 +171,7 @@ struct Codes16 {
   i32x4 d[2];
 };
 struct Halves16 {
-  f16x8 d[4];
+  i32x4 d[4];  // 8 halves each
 };
 template <int MODE>
 using Operand16 = typename std::conditional<MODE == HALF, Halves16, Codes16>::type;
@@ -183,12 +183,22 @@ __device__ __forceinline__ Operand16<MODE> operand16(const Codes16 &c) {
     Halves16 h;
 #pragma unroll
     for (int d = 0; d < 2; d++) {
-      h.d[2 * d] = widen(c.d[d][0], c.d[d][1]);
-      h.d[2 * d + 1] = widen(c.d[d][2], c.d[d][3]);
+      h.d[2 * d] = __builtin_bit_cast(i32x4, widen(c.d[d][0], c.d[d][1]));
+      h.d[2 * d + 1] = __builtin_bit_cast(i32x4, widen(c.d[d][2], c.d[d][3]));
     }
     return h;
   }
 }
+// the k-th two of the 32 values that operand16 makes, here and not where they are used
+__device__ __forceinline__ void widen_two(Halves16 &h, const Codes16 &c, int k) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const int v = c.d[k >> 3][(k >> 1) & 3];
+  const h2 x = k & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false);
+  int y = __builtin_bit_cast(int, x);
+  asm volatile("" : "+v"(y));
+  h.d[k >> 2][k & 3] = y;
+}
+
 template <int MODE>
 constexpr int MMAS16 = MODE == HALF ? 4 : 1;
 __device__ __forceinline__ f32x4 mma16(int, const Codes16 &w, const Codes16 &a, f32x4 t) {
@@ -197,7 +207,7 @@ __device__ __forceinline__ f32x4 mma16(int, const Codes16 &w, const Codes16 &a, 
                                                           0, 0, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mma16(int c, const Halves16 &w, const Halves16 &a, f32x4 t) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(w.d[c], a.d[c], t, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.d[c]), __builtin_bit_cast(f16x8, a.d[c]), t, 0, 0, 0);
 }
 
 template <int MODE_, int TM_, int TN_>
@@ -209,13 +219,15 @@ struct Tile {
   static constexpr int SCALES = TM * 16;                      // LDS bytes of 4 blocks' scales; two of them
   static constexpr int RS = 128 + 16, OUT = 16 * RS;          // LDS bytes of a row of results, of a wave's 16 rows
   static constexpr int LDS = 2 * STAGE + 2 * SCALES + NW * OUT;
+  static constexpr int STORES = MI * NJ / 2;                  // a wave's stores of a whole tile of 16-bit values
+  static constexpr int NQ = NQA + NQW;
   static_assert(LDS <= 160 * 1024 && NQA % 2 == 0 && NQW % 2 == 0 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
 };
 
 // The sums of a wave's rows mw .. and columns nw ..: they leave through a wave's own 16 rows of LDS, 128 bytes of each at a time, so no wave waits for another.
 template <class C>
 __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, int mw, int nw, int lane,
-                                           char *own, const f32x4 (&acc)[C::MI][C::NJ]) {
+                                           char *own, bool full, const f32x4 (&acc)[C::MI][C::NJ]) {
   constexpr int MI = C::MI, NJ = C::NJ;
   const int l16 = lane & 15, lg = lane >> 4;
   if (ot == T_F32) {
@@ -231,12 +243,15 @@ __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &
         *(f32x4 *)(v + 4) = *(const f32x4 *)(own + r * C::RS + (lane & 3) * 32 + 16);
         if (m < p.M && n < p.N) finish(g, p, ot, epi, m, n, g.vec, v);
       }
-  } else {
-    const bool all = g.vec;
+    return;
+  }
+  // 16-bit values: rounded (with the bias, if there is one) on their way to LDS
+  auto halves = [&](auto bias_c, auto round) __attribute__((always_inline)) {
+    constexpr bool BIAS = decltype(bias_c)::value;
 #pragma unroll
     for (int j = 0; j < NJ; j += 4) {
-      f32x4 bias[4] = {};
-      if (g.bias)
+      f32x4 bias[4];
+      if constexpr (BIAS)
 #pragma unroll
         for (int h = 0; h < 4; h++)
 #pragma unroll
@@ -248,38 +263,38 @@ __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &
           typedef unsigned short h4 __attribute__((ext_vector_type(4)));
           h4 o;
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float v = g.bias ? acc[i][j + h][e] + bias[h][e] : acc[i][j + h][e];
-            o[e] = ot == T_BF16 ? __builtin_bit_cast(unsigned short, (__bf16)v) : __builtin_bit_cast(unsigned short, (_Float16)v);
-          }
+          for (int e = 0; e < 4; e++) o[e] = round(BIAS ? acc[i][j + h][e] + bias[h][e] : acc[i][j + h][e]);
           *(h4 *)(own + l16 * C::RS + h * 32 + lg * 8) = o;
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           const int r = 8 * h + (lane >> 3), m = mw + 16 * i + r, n = nw + 16 * j + (lane & 7) * 8;
           const uint4 d = *(const uint4 *)(own + r * C::RS + (lane & 7) * 16);
-          if (m < p.M && n < p.N) {
-            unsigned short *dst = (unsigned short *)g.out + (size_t)m * p.c_stride + n;
-            if (all) {
-              *(uint4 *)dst = d;
-            } else {
-              const unsigned short *hs = (const unsigned short *)&d;
+          unsigned short *dst = (unsigned short *)g.out + (size_t)m * p.c_stride + n;
+          if (full) {
+            __builtin_nontemporal_store(__builtin_bit_cast(i32x4, d), (i32x4 *)dst);  // nothing here reads it again
+          } else if (m < p.M && n < p.N) {
+            const unsigned short *hs = (const unsigned short *)&d;
 #pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (n + e < p.N) dst[e] = hs[e];
-            }
+            for (int e = 0; e < 8; e++)
+              if (n + e < p.N) dst[e] = hs[e];
           }
         }
       }
     }
-  }
+  };
+  auto with_bias = [&](auto round) __attribute__((always_inline)) {
+    if (g.bias) halves(std::true_type{}, round);
+    else halves(std::false_type{}, round);
+  };
+  if (ot == T_BF16) with_bias([](float v) { return __builtin_bit_cast(unsigned short, (__bf16)v); });
+  else with_bias([](float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); });
 }
 
 template <class C>
 __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_f8_tile(GemmArgs g, GemmParams p,
                                                                                                    int ntm, int ntn, int ot, int epi) {
   constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4;
-  constexpr int MH = 1;  // operands of the next step in registers of their own
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / C::WGN, wn = w % C::WGN;
@@ -312,6 +327,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
   // a stage: TM rows of A, then TN of W, 8 rows a load; wave w takes the loads NQA w .. of A and NQW w .. of W
   const int fetch = fetch_piece(0, lane) * 16;  // of even loads; ^ 64 for odd ones
   const int offa = (8 * C::NQA * w + (lane >> 3)) * p.a_stride, offw = (8 * C::NQW * w + (lane >> 3)) * p.w_stride;
+  int a8 = 8 * p.a_stride, w8 = 8 * p.w_stride;
   int phase = 0;  // step kt's stage is (kt + phase) & 1, chunk c of its scales in buffer (c + sphase) & 1
   int sphase = 0;
   auto dma = [&](int q, int kt, int stage) __attribute__((always_inline)) {
@@ -319,12 +335,12 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
     const int left = p.K - kt * KB;  // pieces past K (all of them in blocks past the last) read as zero
     const int r = q < C::NQA ? q : q - C::NQA, f = r & 1 ? fetch ^ 64 : fetch;
     if (q < C::NQA)
-      dma16(st + (C::NQA * w + r) * 1024, f < left ? (unsigned)(offa + 8 * r * p.a_stride + f + kt * KB) : 0x80000000u, ld.ra);
+      dma16(st + (C::NQA * w + r) * 1024, f < left ? (unsigned)(offa + r * a8 + f + kt * KB) : 0x80000000u, ld.ra);
     else
-      dma16(st + TM * KB + (C::NQW * w + r) * 1024, f < left ? (unsigned)(offw + 8 * r * p.w_stride + f + kt * KB) : 0x80000000u,
+      dma16(st + TM * KB + (C::NQW * w + r) * 1024, f < left ? (unsigned)(offw + r * w8 + f + kt * KB) : 0x80000000u,
             ld.rw);
   };
-  constexpr int NQ = C::NQA + C::NQW;
+  constexpr int NQ = C::NQ;
   // 4 blocks' scales of the tile's rows, [row][4]: blocks first .. first + 3; the last four where there are no more
   auto first = [&](int c) { return min(4 * c, nb - 4); };
   const int nc = (ns + 3) >> 2;
@@ -348,7 +364,10 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
   auto read = [&](int rows, int t, int stage) __attribute__((always_inline)) {
     Codes16 c;
 #pragma unroll
-    for (int d = 0; d < 2; d++) c.d[d] = *(const i32x4 *)(smem + (at[d] + (rows + stage * C::STAGE)) + 16 * t * KB);
+    for (int d = 0; d < 2; d++) {
+      const char *q = smem + (at[d] + (rows + stage * C::STAGE));
+      c.d[d] = *(const i32x4 *)(q + 16 * t * KB);
+    }
     return c;
   };
   // of block kt from buffer buf
@@ -373,7 +392,8 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
   // The order is kept as written (sched_barrier): each matrix instruction is followed by the fused adds of the sums MI
   // instructions before it. One wave then keeps the matrix unit busy; sums multiplied and added by turns left it idle for
   // the adds (16 x 16 tiles: 135 cycles for what takes the matrix unit 128, 32 x 32 ones 148 to 200).
-  Codes16 a[MI], an[MH], wb[2], wl;
+  Codes16 a[MI], an[1], wb[2], wl;
+  Operand16<MODE> ao[MI], b;  // HALF: the widened rows
   float sc[MI], fs[MI];
   f32x4 t[MI];
 #pragma unroll
@@ -382,8 +402,15 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
     sc[i] = read_scale(i, 0, 0);
   }
   wb[0] = read(pw, 0, 0);
+  if constexpr (MODE == HALF) {
+    wb[1] = read(pw, 1, 0);
+#pragma unroll
+    for (int i = 0; i < 2; i++) ao[i] = operand16<MODE>(a[i]);
+    b = operand16<MODE>(wb[0]);
+  }
   Scalars sw = scales_of(n0), swn = sw;
   float s = sw[0];
+  bool stored = false;
   for (;;) {
 #pragma unroll
     for (int i = 0; i < MI; i++) {
@@ -392,80 +419,144 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
       t[i] = f32x4{};
       fs[i] = 0.0f;
     }
+#pragma nounroll
     for (int kt = 0; kt < ns; kt++) {
+      // the loads' offsets are made of these where they are issued, not held in a register for each load
+      asm volatile("" : "+s"(a8), "+s"(w8));
       const bool last = kt + 1 == ns;
       const int nx = last ? 0 : kt + 1, stage = (kt + phase) & 1;  // the next step: of the next tile behind the last
       const int nbuf = last ? (nc + sphase) & 1 : ((nx >> 2) + sphase) & 1;
-      Operand16<MODE> ao[MI];
-      // sums (i, j) for every i; `with(n)` goes behind the n-th of them
-      auto row = [&](int j, const Codes16 &wc, auto with) __attribute__((always_inline)) {
-        constexpr int NM = MMAS16<MODE>;
-        const Operand16<MODE> b = operand16<MODE>(wc);
-        f32x4 u[MI];
-#pragma unroll
-        for (int i = 0; i < MI; i++) {
-          if (j == 0) ao[i] = operand16<MODE>(a[i]);
-          u[i] = f32x4{};
-#pragma unroll
-          for (int c = 0; c < NM; c++) u[i] = mma16(c, b, ao[i], u[i]);
-          __builtin_amdgcn_sched_barrier(0);
-          const int pj = (j + NJ - 1) % NJ;
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
-          asm volatile("" : "+v"(acc[i][pj]));
-          if (j == 0) fs[i] = sc[i] * s;
-          with(i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int i = 0; i < MI; i++) t[i] = u[i];
-      };
-#pragma unroll
-      for (int j = 0; j < NJ - 2; j++)
-        row(j, wb[j & 1], [&](int i) __attribute__((always_inline)) {
-          if (i == 0) wb[(j + 1) & 1] = read(pw, j + 1, stage);
-          if (i == 1 && j == NJ - 3) wl = read(pw, NJ - 1, stage);
-        });
-      // the next stage has landed, and every wave has read this one
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __syncthreads();
       int kl = kt + 2;  // the step to load; behind the last one the next tile's
-      if (kl == ns) {
-        ld = at_tile(tile + tstep);
-        swn = scales_of(ld.n0);
-        if (nb >= 4) dma_scales(0, (nc + sphase) & 1);
-      } else if ((kt & 3) == 0 && kt + 4 < nb) {
-        dma_scales((kt >> 2) + 1, ((kt >> 2) + 1 + sphase) & 1);
-      }
-      kl = kl >= ns ? kl - ns : kl;
-      const float snext = last ? swn[0] : sw[min(nx, nb - 1)];
-      row(NJ - 2, wb[0], [&](int i) __attribute__((always_inline)) {
-        if (i < MH) {
-          an[i] = read(pa, i, stage ^ 1);
-        } else {
-#pragma unroll
-          for (int q = (i - MH) * (NQ / 2) / (MI - MH); q < (i - MH + 1) * (NQ / 2) / (MI - MH); q++) dma(q, kl, stage);
+      float snext;
+      // The next stage has landed, and every wave has read this one (in a tile's first step the stores of the tile before it
+      // may still be under way: they were issued after the loads).
+      auto meet = [&]() __attribute__((always_inline)) {
+        if (kt == 0 && stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(C::STORES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (kl == ns) {
+          ld = at_tile(tile + tstep);
+          swn = scales_of(ld.n0);
+          if (nb >= 4) dma_scales(0, (nc + sphase) & 1);
+        } else if ((kt & 3) == 0 && kt + 4 < nb) {
+          dma_scales((kt >> 2) + 1, ((kt >> 2) + 1 + sphase) & 1);
         }
-      });
-      wb[0] = read(pw, 0, stage ^ 1);
-      row(NJ - 1, wl, [&](int i) __attribute__((always_inline)) {
-        sc[i] = read_scale(i, nx, nbuf);
-        if (i >= MH) a[i] = read(pa, i, stage ^ 1);
+        kl = kl >= ns ? kl - ns : kl;
+        snext = last ? swn[0] : sw[min(nx, nb - 1)];
+      };
+      // slot n of the 2 MI NM behind the meeting: its share of the loads
+      auto load_some = [&](int n) __attribute__((always_inline)) {
+        constexpr int SL = 2 * MI * MMAS16<MODE>;
 #pragma unroll
-        for (int q = NQ / 2 + i * (NQ - NQ / 2) / MI; q < NQ / 2 + (i + 1) * (NQ - NQ / 2) / MI; q++) dma(q, kl, stage);
-      });
+        for (int q = n * NQ / SL; q < (n + 1) * NQ / SL; q++) dma(q, kl, stage);
+      };
+      if constexpr (MODE == E4M3) {
+        // sums (i, j) for every i; `with(n)` goes behind the n-th of them
+        auto row = [&](int j, const Codes16 &b, auto with) __attribute__((always_inline)) {
+          const int pj = (j + NJ - 1) % NJ;
+          f32x4 u[MI];
 #pragma unroll
-      for (int i = 0; i < MH; i++) a[i] = an[i];
+          for (int i = 0; i < MI; i++) {
+            u[i] = mma16(0, b, a[i], f32x4{});
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
+            asm volatile("" : "+v"(acc[i][pj]));
+            if (j == 0) fs[i] = sc[i] * s;
+            with(i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int i = 0; i < MI; i++) t[i] = u[i];
+        };
+#pragma unroll
+        for (int j = 0; j < NJ - 2; j++)
+          row(j, wb[j & 1], [&](int i) __attribute__((always_inline)) {
+            if (i == 0) wb[(j + 1) & 1] = read(pw, j + 1, stage);
+            if (i == 1 && j == NJ - 3) wl = read(pw, NJ - 1, stage);
+          });
+        meet();
+        row(NJ - 2, wb[0], [&](int i) __attribute__((always_inline)) {
+          if (i == 0) an[0] = read(pa, 0, stage ^ 1);
+          load_some(i);
+        });
+        wb[0] = read(pw, 0, stage ^ 1);
+        row(NJ - 1, wl, [&](int i) __attribute__((always_inline)) {
+          sc[i] = read_scale(i, nx, nbuf);
+          if (i > 0) a[i] = read(pa, i, stage ^ 1);
+          load_some(MI + i);
+        });
+        a[0] = an[0];
+      } else {
+        // A sum is four matrix instructions that depend on each other, so two sums are made at a time. `with(n)` goes behind
+        // the n-th of the row's 4 MI instructions. Between them W's next 16 rows (read two rows ahead) are widened, and A's
+        // for the next step: its first 32 rows in the second half of a step's last row, the others in the next step's first.
+        auto row = [&](int j, auto with) __attribute__((always_inline)) {
+          const int pj = (j + NJ - 1) % NJ;
+          Halves16 bn;
+          f32x4 u[MI];
+#pragma unroll
+          for (int h = 0; h < MI; h += 2)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = h; i < h + 2; i++) {
+                const int n = 4 * h + 2 * c + i - h;
+                u[i] = mma16(c, b, ao[i], c ? u[i] : f32x4{});
+                __builtin_amdgcn_sched_barrier(0);
+                acc[i][pj][c] = __builtin_fmaf(t[i][c], fs[i], acc[i][pj][c]);
+                if (c == 3) asm volatile("" : "+v"(acc[i][pj]));
+                if (c == 3 && j == 0) fs[i] = sc[i] * s;
+#pragma unroll
+                for (int k = 16 * n / (4 * MI); k < 16 * (n + 1) / (4 * MI); k++) widen_two(bn, wb[(j + 1) & 1], k);
+                if (MI == 4 && h == 0 && j == 0)
+#pragma unroll
+                  for (int k = 4 * n; k < 4 * (n + 1); k++) widen_two(ao[MI - 2 + k / 16], a[MI - 2 + k / 16], k % 16);
+                if (MI == 4 && h == 2 && j == NJ - 1)
+#pragma unroll
+                  for (int k = 4 * (n - 8); k < 4 * (n - 7); k++) widen_two(ao[k / 16], a[k / 16], k % 16);
+                with(n);
+                __builtin_amdgcn_sched_barrier(0);
+              }
+#pragma unroll
+          for (int i = 0; i < MI; i++) t[i] = u[i];
+          b = bn;
+        };
+        if (MI == 2)
+#pragma unroll
+          for (int i = 0; i < MI; i++) ao[i] = operand16<MODE>(a[i]);
+#pragma unroll
+        for (int j = 0; j < NJ - 2; j++)
+          row(j, [&](int n) __attribute__((always_inline)) {
+            if (n == 4 * MI - 1) wb[j & 1] = read(pw, j + 2, stage);
+          });
+        meet();
+        row(NJ - 2, [&](int n) __attribute__((always_inline)) {
+          if (n == 4 * MI - 1) wb[0] = read(pw, 0, stage ^ 1);
+          if (n < 2) a[n] = read(pa, n, stage ^ 1);
+          load_some(n);
+        });
+        row(NJ - 1, [&](int n) __attribute__((always_inline)) {
+          if (n == 4 * MI - 1) wb[1] = read(pw, 1, stage ^ 1);
+          if (n < MI) sc[n] = read_scale(n, nx, nbuf);
+          if (n > 1 && n < MI) a[n] = read(pa, n, stage ^ 1);
+          load_some(4 * MI + n);
+        });
+      }
       s = snext;
     }
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[i][NJ - 1][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][NJ - 1][e]);
-    store_tile<C>(g, p, ot, epi, m0 + WTM * wm, n0 + WTN * wn, lane, smem + 2 * C::STAGE + 2 * C::SCALES + w * C::OUT, acc);
+    phase = (phase + ns) & 1;
+    const bool full = g.vec && m0 + TM <= p.M && n0 + TN <= p.N;
+    int le = lane;
+    asm volatile("" : "+v"(le));  // what the stores need of it is made here, not held through the multiplications
+    store_tile<C>(g, p, ot, epi, m0 + WTM * wm, n0 + WTN * wn, le, smem + 2 * C::STAGE + 2 * C::SCALES + w * C::OUT, full, acc);
+    stored = full && ot != T_F32;
     tile += tstep;
     if (tile >= tend) break;
-    phase = (phase + ns) & 1;
     sphase = (sphase + nc) & 1;
     m0 = ld.m0, n0 = ld.n0;
     sw = swn;
