@@ -217,69 +217,88 @@ struct Tile {
   static constexpr int STAGE = (TM + TN) * KB;                // LDS bytes of a block's rows; two stages
   static constexpr int NQA = TM / 8 / NW, NQW = TN / 8 / NW;  // loads of A and W per wave and stage
   static constexpr int SCALES = TM * 16;                      // LDS bytes of 4 blocks' scales; two of them
-  static constexpr int RS = 128 + 16, OUT = 16 * RS;          // LDS bytes of a row of results, of a wave's 16 rows
+  // results: RB bytes of 16 rows of a wave at a time (64 for the small tile: two workgroups then fit a compute unit)
+  static constexpr int RB = TM * TN > 128 * 128 ? 128 : 64, RS = RB + 16, OUT = 16 * RS;
   static constexpr int LDS = 2 * STAGE + 2 * SCALES + NW * OUT;
   static constexpr int STORES = MI * NJ / 2;                  // a wave's stores of a whole tile of 16-bit values
   static constexpr int NQ = NQA + NQW;
   static_assert(LDS <= 160 * 1024 && NQA % 2 == 0 && NQW % 2 == 0 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
 };
 
-// The sums of a wave's rows mw .. and columns nw ..: they leave through a wave's own 16 rows of LDS, 128 bytes of each at a time, so no wave waits for another.
+// Between a wave's writes to LDS and its reads of what its other lanes wrote, and before the next writes: the LDS keeps a
+// wave's order, the compiler only at such a point (it split lanes that take a branch from those that do not, and let one half
+// write before the other had read).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The sums of a wave's rows mw .. and columns nw ..: they leave through its own 16 rows of LDS, RB bytes of each at a time,
+// so no wave waits for another. `full`: the whole tile is there and 16-byte accesses are aligned.
 template <class C>
 __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, int mw, int nw, int lane,
                                            char *own, bool full, const f32x4 (&acc)[C::MI][C::NJ]) {
-  constexpr int MI = C::MI, NJ = C::NJ;
+  constexpr int MI = C::MI, NJ = C::NJ, RB = C::RB, RS = C::RS;
   const int l16 = lane & 15, lg = lane >> 4;
   if (ot == T_F32) {
+    constexpr int JS = RB / 64, LR = RB / 32, RP = 64 / LR;  // 16-column groups, lanes of 8 columns a row, rows a pass
 #pragma unroll
-    for (int i = 0; i < MI; i++)
+    for (int j = 0; j < NJ; j += JS)
 #pragma unroll
-      for (int j = 0; j < NJ; j += 2) {
+      for (int i = 0; i < MI; i++) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) *(f32x4 *)(own + l16 * C::RS + h * 64 + lg * 16) = acc[i][j + h];
-        const int r = lane >> 2, m = mw + 16 * i + r, n = nw + 16 * j + (lane & 3) * 8;
-        float v[8];
-        *(f32x4 *)v = *(const f32x4 *)(own + r * C::RS + (lane & 3) * 32);
-        *(f32x4 *)(v + 4) = *(const f32x4 *)(own + r * C::RS + (lane & 3) * 32 + 16);
-        if (m < p.M && n < p.N) finish(g, p, ot, epi, m, n, g.vec, v);
+        for (int h = 0; h < JS; h++) *(f32x4 *)(own + l16 * RS + h * 64 + lg * 16) = acc[i][j + h];
+        wave_sync();
+        const int r = lane / LR, m = mw + 16 * i + r, n = nw + 16 * j + lane % LR * 8;
+        if (RP <= 16 || r < 16) {
+          float v[8];
+          *(f32x4 *)v = *(const f32x4 *)(own + r * RS + lane % LR * 32);
+          *(f32x4 *)(v + 4) = *(const f32x4 *)(own + r * RS + lane % LR * 32 + 16);
+          if (m < p.M && n < p.N) finish(g, p, ot, epi, m, n, g.vec, v);
+        }
+        wave_sync();
       }
     return;
   }
   // 16-bit values: rounded (with the bias, if there is one) on their way to LDS
   auto halves = [&](auto bias_c, auto round) __attribute__((always_inline)) {
     constexpr bool BIAS = decltype(bias_c)::value;
+    constexpr int JS = RB / 32, LR = RB / 16, RP = 64 / LR;  // 16-column groups, lanes of 8 columns a row, rows a pass
 #pragma unroll
-    for (int j = 0; j < NJ; j += 4) {
-      f32x4 bias[4];
+    for (int j = 0; j < NJ; j += JS) {
+      f32x4 bias[JS];
       if constexpr (BIAS)
 #pragma unroll
-        for (int h = 0; h < 4; h++)
+        for (int h = 0; h < JS; h++)
 #pragma unroll
           for (int e = 0; e < 4; e++) bias[h][e] = g.bias[min(nw + 16 * (j + h) + 4 * lg + e, p.N - 1)];
 #pragma unroll
       for (int i = 0; i < MI; i++) {
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
+        for (int h = 0; h < JS; h++) {
           typedef unsigned short h4 __attribute__((ext_vector_type(4)));
           h4 o;
 #pragma unroll
           for (int e = 0; e < 4; e++) o[e] = round(BIAS ? acc[i][j + h][e] + bias[h][e] : acc[i][j + h][e]);
-          *(h4 *)(own + l16 * C::RS + h * 32 + lg * 8) = o;
+          *(h4 *)(own + l16 * RS + h * 32 + lg * 8) = o;
         }
+        wave_sync();
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int r = 8 * h + (lane >> 3), m = mw + 16 * i + r, n = nw + 16 * j + (lane & 7) * 8;
-          const uint4 d = *(const uint4 *)(own + r * C::RS + (lane & 7) * 16);
+        for (int h = 0; h < 16 / RP; h++) {
+          const int r = RP * h + lane / LR, m = mw + 16 * i + r, n = nw + 16 * j + lane % LR * 8;
+          const i32x4 d = *(const i32x4 *)(own + r * RS + lane % LR * 16);
           unsigned short *dst = (unsigned short *)g.out + (size_t)m * p.c_stride + n;
           if (full) {
-            __builtin_nontemporal_store(__builtin_bit_cast(i32x4, d), (i32x4 *)dst);  // nothing here reads it again
+            __builtin_nontemporal_store(d, (i32x4 *)dst);  // past the caches: nothing here reads it again
           } else if (m < p.M && n < p.N) {
-            const unsigned short *hs = (const unsigned short *)&d;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-              if (n + e < p.N) dst[e] = hs[e];
+            for (int e = 0; e < 8; e++) {
+              const int x = d[e / 2];
+              if (n + e < p.N) dst[e] = (unsigned short)(e & 1 ? x >> 16 : x);
+            }
           }
         }
+        wave_sync();
       }
     }
   };
@@ -758,7 +777,8 @@ __global__ __launch_bounds__(RW * 64) void gemm_f8_rows(GemmArgs g, GemmParams p
 
 // ---- the launch ---------------------------------------------------------------------------------------------------
 
-enum { TILE_ROWS = 1, TILE_32, TILE_64, TILE_128, TILE_256, TILE_LAST = TILE_256 };  // values of the macro TILE, 0 the plan's
+// values of the macro TILE, 0 the plan's choice
+enum { TILE_ROWS = 1, TILE_32, TILE_64, TILE_128, TILE_256x128, TILE_256, TILE_LAST = TILE_256 };
 
 template <class K>
 int set_lds(K kern, int bytes, std::string *err) {
@@ -882,6 +902,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
     case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, ex.stream, err);
     case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 4, 2>>(g, p, ot, epi, ex.stream, err);
     case TILE_128: return run_tile<Tile<E4M3, 128, 128>>(g, p, ot, epi, ex.stream, err);
+    case TILE_256x128: return run_tile<Tile<E4M3, 256, 128>>(g, p, ot, epi, ex.stream, err);
     default: return run_tile<Tile<E4M3, 256, 256>>(g, p, ot, epi, ex.stream, err);
   }
 }
@@ -890,7 +911,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
 
 bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err) {
   if (tile < 0 || tile > TILE_LAST) {
-    *err = "TILE must be 0 to 5 with format f8";
+    *err = "TILE must be 0 to 6 with format f8";
     return false;
   }
   pl->launch = launch_f8;

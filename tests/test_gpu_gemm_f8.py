@@ -20,9 +20,9 @@ from oracle.bf16 import from_bf16, to_bf16
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
-# the plan's own choice, 32 x 32 and 64 x 64 tiles whose waves split K, 128 x 128 and 256-row tiles; up to 16 rows have a
-# kernel of their own
-TILES = pytest.mark.parametrize("TILE", [0, 1, 2, 3, 4, 5], ids=["plan", "rows", "32", "64", "128", "256"])
+# the plan's own choice, the kernel of up to 16 rows, 32 x 32 and 64 x 64 tiles whose waves split K, 128 x 128, 256 x 128 and
+# 256 x 256 tiles (256 x 128 again for float outputs)
+TILES = pytest.mark.parametrize("TILE", [0, 1, 2, 3, 4, 5, 6], ids=["plan", "rows", "32", "64", "128", "256x128", "256"])
 
 
 def bound(mag, K, *values):
