@@ -222,7 +222,8 @@ struct Tile {
   static constexpr int LDS = 2 * STAGE + 2 * SCALES + NW * OUT;
   static constexpr int STORES = MI * NJ / 2;                  // a wave's stores of a whole tile of 16-bit values
   static constexpr int NQ = NQA + NQW;
-  static_assert(LDS <= 160 * 1024 && NQA % 2 == 0 && NQW % 2 == 0 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
+  static constexpr int PER_CU = MODE == E4M3 && TM * TN <= 128 * 128 ? 2 : 1;  // workgroups that a compute unit holds
+  static_assert(PER_CU * LDS <= 160 * 1024 && NQA % 2 == 0 && NQW % 2 == 0 && MI % 2 == 0 && NJ % 2 == 0, "tile configuration");
 };
 
 // Between a wave's writes to LDS and its reads of what its other lanes wrote, and before the next writes: the LDS keeps a
@@ -291,10 +292,14 @@ __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &
           if (full) {
             __builtin_nontemporal_store(d, (i32x4 *)dst);  // past the caches: nothing here reads it again
           } else if (m < p.M && n < p.N) {
+            if (g.vec) {
+              *(i32x4 *)dst = d;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const int x = d[e / 2];
-              if (n + e < p.N) dst[e] = (unsigned short)(e & 1 ? x >> 16 : x);
+              for (int e = 0; e < 8; e++) {
+                const int x = d[e / 2];
+                if (n + e < p.N) dst[e] = (unsigned short)(e & 1 ? x >> 16 : x);
+              }
             }
           }
         }
@@ -311,7 +316,7 @@ __device__ __forceinline__ void store_tile(const GemmArgs &g, const GemmParams &
 }
 
 template <class C>
-__global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_f8_tile(GemmArgs g, GemmParams p,
+__global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * C::PER_CU))) void gemm_f8_tile(GemmArgs g, GemmParams p,
                                                                                                    int ntm, int ntn, int ot, int epi) {
   constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, WTM = C::WTM, WTN = C::WTN, SW = 4;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -718,67 +723,10 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
   }
 }
 
-// ---- up to 16 rows: 16 columns a workgroup, operands straight from memory ---------------------------------------------
-
-constexpr int RW = 8;  // waves
-constexpr int RU = 4;  // blocks whose loads are in flight
-
-__global__ __launch_bounds__(RW * 64) void gemm_f8_rows(GemmArgs g, GemmParams p, int ot, int epi) {
-  __shared__ float part[RW][16][20];  // [wave][row of A][column]
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, gr = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = xcd_order(blockIdx.x, gridDim.x) * 16, nb = (p.K + KB - 1) / KB;
-  const bool aok = l16 < p.M, wok = n0 + l16 < p.N;
-  const char *ar = g.a + (size_t)(aok ? l16 : 0) * p.a_stride, *wr = g.w + (size_t)(wok ? n0 + l16 : 0) * p.w_stride;
-  const float *sa = g.sa + (size_t)(aok ? l16 : 0) * p.groups, *sw = g.sw + (size_t)(n0 / KB) * p.groups;
-  const i32x4 z = {0, 0, 0, 0};
-  f32x4 acc = {0, 0, 0, 0};
-  for (int b0 = w; b0 < nb; b0 += RW * RU) {
-    i32x4 a[RU][2], x[RU][2];
-    float s[RU];
-#pragma unroll
-    for (int u = 0; u < RU; u++) {
-      const int b = b0 + u * RW;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int k = b * KB + gr * 32 + h * 16;
-        x[u][h] = wok && k < p.K ? *(const i32x4 *)(wr + k) : z;
-        a[u][h] = aok && k < p.K ? *(const i32x4 *)(ar + k) : z;
-      }
-      s[u] = b < nb ? sa[b] * sw[b] : 0.0f;
-    }
-#pragma unroll
-    for (int u = 0; u < RU; u++) {
-      f32x4 t = {0, 0, 0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int c = 0; c < 4; c += 2)
-          t = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(x[u][h][c], x[u][h][c + 1]), widen(a[u][h][c], a[u][h][c + 1]), t, 0,
-                                                     0, 0);
-#pragma unroll
-      for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(t[e], s[u], acc[e]);
-    }
-  }
-  // element e is column 4 gr + e of row l16
-  *(f32x4 *)&part[w][l16][4 * gr] = acc;
-  __syncthreads();
-  const int m = tid / 4, nl = 4 * (tid % 4), n = n0 + nl;
-  if (m >= p.M || m >= 16 || n >= p.N) return;
-  float v[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int u = 0; u < RW; u++) {
-    const f32x4 d = *(const f32x4 *)&part[u][m][nl];
-#pragma unroll
-    for (int r = 0; r < 4; r++) v[r] += d[r];
-  }
-  finish(g, p, ot, epi, m, n, g.vec, v);
-}
-
 // ---- the launch ---------------------------------------------------------------------------------------------------
 
 // values of the macro TILE, 0 the plan's choice
-enum { TILE_ROWS = 1, TILE_32, TILE_64, TILE_128, TILE_256x128, TILE_256, TILE_LAST = TILE_256 };
+enum { TILE_32 = 1, TILE_64, TILE_128, TILE_256x128, TILE_256, TILE_LAST = TILE_256 };
 
 template <class K>
 int set_lds(K kern, int bytes, std::string *err) {
@@ -806,16 +754,78 @@ int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_
   if (!set && set_lds(kern, C::LDS, err)) return -1;
   set = true;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
-  const int cus = cu_count(), slots = cus > 0 ? cus * (160 * 1024 / C::LDS) : 256;
+  const int cus = cu_count(), slots = (cus > 0 ? cus : 256) * C::PER_CU;
   hipLaunchKernelGGL(kern, dim3((unsigned)std::min(ntm * ntn, slots)), dim3(C::NW * 64), C::LDS, stream, g, p, ntm, ntn, ot, epi);
   return 0;
 }
 
-int plan_of(const GemmParams &p) {
-  if (p.M <= 16) return TILE_ROWS;
-  const long n32 = (long)((p.M + 31) / 32) * ((p.N + 31) / 32), n64 = (long)((p.M + 63) / 64) * ((p.N + 63) / 64);
-  const long n128 = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  return n128 > 512 ? TILE_256 : n128 > 200 ? TILE_128 : n64 > 256 ? TILE_64 : n32 > 512 ? TILE_64 : TILE_32;
+// What a launch of each kind of tile takes: rounds (tiles over compute units, rounded up) of fixed + per_block * blocks of K
+// microseconds, or, where the card's power bounds it, the operations over `rate` (in 10^6 a microsecond) if that is longer.
+struct Cost {
+  int tm, tn;
+  double fixed, per_block, rate;
+};
+constexpr Cost E4M3_COST[] = {{}, {32, 32, 2.35, 0.093, 1e9}, {64, 64, 3.95, 0.184, 1e9}, {128, 128, 3.5, 0.65, 1540},
+                              {256, 128, 4.5, 0.92, 1800}, {256, 256, 6.5, 1.35, 2200}};
+constexpr Cost HALF_COST[] = {{}, {32, 32, 2.34, 0.102, 1e9}, {64, 64, 3.94, 0.257, 1e9}, {128, 128, 4.81, 1.074, 870},
+                              {256, 128, 7.6, 1.6, 1070}, {256, 128, 7.6, 1.6, 1070}};
+
+// The tiles of a product, and of its last rows where those take others (`rows`: those of `tile`).
+struct Plan {
+  int tile, rows, tail;
+};
+
+Plan make_plan(const GemmParams &p, bool half) {
+  const int cus = cu_count() > 0 ? cu_count() : 256;
+  const Cost *cost = half ? HALF_COST : E4M3_COST;
+  const double nb = (p.K + KB - 1) / KB;
+  auto tiles = [&](int t, long rows) { return ((rows + cost[t].tm - 1) / cost[t].tm) * (((long)p.N + cost[t].tn - 1) / cost[t].tn); };
+  auto time = [&](int t, long rows) {
+    const double rounds = (double)((tiles(t, rows) + cus - 1) / cus);
+    return std::max(rounds * (cost[t].fixed + cost[t].per_block * nb), 2e-6 * rows * p.N * p.K / cost[t].rate);
+  };
+  Plan best{TILE_32, p.M, 0};
+  double least = time(TILE_32, p.M);
+  for (int t = TILE_64; t <= TILE_LAST; t++) {
+    const double us = time(t, p.M);
+    if (us < least) least = us, best = {t, p.M, 0};
+  }
+  // whole rounds of large tiles, and the rows of what is left of a round on smaller ones
+  for (int t = TILE_128; t <= TILE_LAST; t++) {
+    const long ntn = ((long)p.N + cost[t].tn - 1) / cost[t].tn;
+    const long rows = tiles(t, p.M) / cus * cus / ntn * cost[t].tm;
+    if (rows <= 0 || rows >= p.M) continue;
+    for (int u = TILE_32; u < t; u++) {
+      const double us = time(t, rows) + time(u, p.M - rows) + 3.0;
+      if (us < 0.97 * least) least = us, best = {t, (int)rows, u};
+    }
+  }
+  return best;
+}
+
+// One launch on the product's rows from row0
+int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, int rows, int ot, int epi, hipStream_t stream,
+              std::string *err) {
+  GemmArgs g = all;
+  GemmParams p = whole;
+  g.a += (size_t)row0 * p.a_stride;
+  g.sa += (size_t)row0 * p.groups;
+  g.out += (size_t)row0 * p.c_stride * (ot == T_F32 ? 4 : 2);
+  if (epi) g.rtype += row0;
+  p.M = rows;
+  if (ot == T_F32) switch (tile) {
+      case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
+      case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
+      case TILE_128: return run_tile<Tile<HALF, 128, 128>>(g, p, ot, epi, stream, err);
+      default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, stream, err);
+    }
+  switch (tile) {
+    case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
+    case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
+    case TILE_128: return run_tile<Tile<E4M3, 128, 128>>(g, p, ot, epi, stream, err);
+    case TILE_256x128: return run_tile<Tile<E4M3, 256, 128>>(g, p, ot, epi, stream, err);
+    default: return run_tile<Tile<E4M3, 256, 256>>(g, p, ot, epi, stream, err);
+  }
 }
 
 int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const void *params, uint32_t params_len,
@@ -878,40 +888,21 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
   const GemmArgs g{a[0].ptr, a[1].ptr, (const float *)a[2].ptr, (const float *)a[3].ptr, a[4].ptr,
                    has_bias ? (const float *)a[5].ptr : nullptr, epi ? (const unsigned char *)a[6].ptr : nullptr,
                    epi ? (const float *)a[7].ptr : nullptr, ntypes, vec};
-  const int tile = pl.ival[0] ? pl.ival[0] : plan_of(p);
-  if (tile == TILE_ROWS) {
-    if (p.M > 16) {
-      *err = "TILE 1 is for up to 16 rows";
-      return -1;
-    }
-    hipLaunchKernelGGL(gemm_f8_rows, dim3((unsigned)((p.N + 15) / 16)), dim3(RW * 64), 0, ex.stream, g, p, ot, epi);
-    return 0;
-  }
-  const long side = tile <= TILE_32 ? 32 : tile == TILE_64 ? 64 : 128;
-  if (((p.M + side - 1) / side) * ((p.N + side - 1) / side) * 512 >= (1ll << 32)) {
+  const Plan plan = pl.ival[0] ? Plan{pl.ival[0], p.M, 0} : make_plan(p, ot == T_F32);
+  const long side = plan.tile == TILE_32 ? 32 : plan.tile == TILE_64 ? 64 : 128;
+  if (((p.M + side - 1) / side) * ((p.N + side - 1) / side) * 512 >= (1ll << 32)) {  // a grid holds less than 2^32 threads
     *err = "too many tiles: M " + std::to_string(p.M) + " N " + std::to_string(p.N);
     return -1;
   }
-  if (ot == T_F32) switch (tile) {
-      case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, ex.stream, err);
-      case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 4, 2>>(g, p, ot, epi, ex.stream, err);
-      case TILE_128: return run_tile<Tile<HALF, 128, 128>>(g, p, ot, epi, ex.stream, err);
-      default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, ex.stream, err);
-    }
-  switch (tile) {
-    case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, ex.stream, err);
-    case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 4, 2>>(g, p, ot, epi, ex.stream, err);
-    case TILE_128: return run_tile<Tile<E4M3, 128, 128>>(g, p, ot, epi, ex.stream, err);
-    case TILE_256x128: return run_tile<Tile<E4M3, 256, 128>>(g, p, ot, epi, ex.stream, err);
-    default: return run_tile<Tile<E4M3, 256, 256>>(g, p, ot, epi, ex.stream, err);
-  }
+  if (run_tiles(plan.tile, g, p, 0, plan.rows, ot, epi, ex.stream, err)) return -1;
+  return plan.tail ? run_tiles(plan.tail, g, p, plan.rows, p.M - plan.rows, ot, epi, ex.stream, err) : 0;
 }
 
 }  // namespace
 
 bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err) {
   if (tile < 0 || tile > TILE_LAST) {
-    *err = "TILE must be 0 to 6 with format f8";
+    *err = "TILE must be 0 to 5 with format f8";
     return false;
   }
   pl->launch = launch_f8;

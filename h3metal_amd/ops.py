@@ -245,7 +245,8 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
             raise ValueError("gemm: e4m3 operands need their scales sa and sw, for blocks of 128")
         tm = 1
     out_t = OUT_DT[out.dtype] if epi == 0 else "float"
-    k = gpu.kernel("gemm", "gemm", WFMT=FMT_ID[wt.fmt], EPI=epi, OUT_T=out_t, TM=tm, TN=tn, NSG=nsg, G=wt.G,
+    k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=out_t, HAS_BIAS=int(wt.bias is not None), **variant) if f8 else \
+        gpu.kernel("gemm", "gemm", WFMT=FMT_ID[wt.fmt], EPI=epi, OUT_T=out_t, TM=tm, TN=tn, NSG=nsg, G=wt.G,
                    HAS_BIAS=int(wt.bias is not None), SWZ=swz, **variant)
     if wt.fmt == "h8":
         gpu.reserve_workspace(wt.N * wt.K * 2)  # the widened weights; grows (and waits) only the first time

@@ -20,9 +20,9 @@ from oracle.bf16 import from_bf16, to_bf16
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
-# the plan's own choice, the kernel of up to 16 rows, 32 x 32 and 64 x 64 tiles whose waves split K, 128 x 128, 256 x 128 and
-# 256 x 256 tiles (256 x 128 again for float outputs)
-TILES = pytest.mark.parametrize("TILE", [0, 1, 2, 3, 4, 5, 6], ids=["plan", "rows", "32", "64", "128", "256x128", "256"])
+# the plan's own choice, 32 x 32 and 64 x 64 tiles whose waves split K, 128 x 128, 256 x 128 and 256 x 256 tiles (256 x 128
+# again for float outputs)
+TILES = pytest.mark.parametrize("TILE", [0, 1, 2, 3, 4, 5], ids=["plan", "32", "64", "128", "256x128", "256"])
 
 
 def bound(mag, K, *values):
@@ -36,11 +36,6 @@ def aligned(a, sa, w, sw):
         x = np.pad(x, ((0, 0), (0, -x.shape[1] % 8)))
         return x.reshape(x.shape[0], -1, 8).max(-1)
     return 7 * 2.0 ** -13 * (top(orq.dequantised(a, sa)) @ top(orq.dequantised(w, sw, 128)).T)
-
-
-def needs_rows(TILE, M):
-    if TILE == 1 and M > 16:
-        pytest.skip("the kernel of up to 16 rows")
 
 
 def operands(rng, M, N, K):
@@ -110,7 +105,6 @@ SIZES = [(1, 1, 16), (1, 5, 128), (1, 4096, 512), (2, 130, 144), (3, 33, 2000), 
 @TILES
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_sizes(gpu, M, N, K, TILE):
-    needs_rows(TILE, M)
     rng = np.random.default_rng(M * 3 + N * 5 + K)
     ops4 = operands(rng, M, N, K)
     for out in ("f32", "bf16"):
@@ -121,7 +115,6 @@ def test_sizes(gpu, M, N, K, TILE):
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("M,N,K,pads", [(7, 264, 384, (0, 0, 0)), (70, 261, 336, (16, 48, 3)), (300, 512, 256, (128, 0, 8))])
 def test_outputs_bias_strides(gpu, M, N, K, pads, out, TILE):
-    needs_rows(TILE, M)
     rng = np.random.default_rng(M + N)
     ops4 = operands(rng, M, N, K)
     bias = rng.standard_normal(N).astype(np.float32)
@@ -133,7 +126,6 @@ def test_outputs_bias_strides(gpu, M, N, K, pads, out, TILE):
                                         (520, 640, 384, True)])
 def test_residual_form(gpu, M, N, K, bias, TILE):
     """X += gate[rtype] * (v + bias); a row type past the gate table's rows takes its last."""
-    needs_rows(TILE, M)
     rng = np.random.default_rng(M + K)
     a, sa, w, sw = operands(rng, M, N, K)
     b = rng.standard_normal(N).astype(np.float32) if bias else None
@@ -159,7 +151,6 @@ def test_residual_form(gpu, M, N, K, bias, TILE):
 @pytest.mark.parametrize("M", [13, 130])
 def test_scales_of_every_block_are_its_own(gpu, M, TILE):
     """Codes 1 and scales from 2^-3 to 2^3: v is a sum of powers of two, exact in float."""
-    needs_rows(TILE, M)
     N, K = 300, 656
     rng = np.random.default_rng(4)
     one = f8.to_f8(np.float32([1]))[0]
@@ -174,7 +165,6 @@ def test_scales_of_every_block_are_its_own(gpu, M, TILE):
 @TILES
 @pytest.mark.parametrize("M,out", [(15, "f32"), (40, "f32"), (40, "bf16")])
 def test_nan_stays_in_its_row(gpu, M, out, TILE):
-    needs_rows(TILE, M)
     rng = np.random.default_rng(5)
     a, sa, w, sw = operands(rng, M, 140, 400)
     clean = run(gpu, a, sa, w, sw, out=out, TILE=TILE)
@@ -191,19 +181,24 @@ def test_nan_stays_in_its_row(gpu, M, out, TILE):
 def test_same_call_same_bits(gpu, TILE):
     """Two calls, and the allocation-free entry point, give the same bits: sums have a fixed order."""
     rng = np.random.default_rng(6)
-    ops4 = operands(rng, 16 if TILE == 1 else 150, 384, 1536)
+    ops4 = operands(rng, 150, 384, 1536)
     first = run(gpu, *ops4, TILE=TILE)
     assert np.array_equal(run(gpu, *ops4, TILE=TILE), first)
     assert np.array_equal(run(gpu, *ops4, TILE=TILE, no_alloc=True), first)
 
 
-def test_large_product_on_sampled_rows(gpu):
-    rng = np.random.default_rng(7)
-    M, N, K = 4700, 4224, 1296
+@pytest.mark.parametrize("TILE", [0, 3, 4, 5], ids=["plan", "128", "256x128", "256"])
+@pytest.mark.parametrize("M,N,K,out", [(4700, 4224, 1296, "bf16"), (2500, 4100, 400, "f32"), (5000, 2056, 128, "f16"),
+                                       (4400, 2304, 272, "f32"), (4607, 4096, 640, "bf16")])
+def test_large_products_on_sampled_rows(gpu, M, N, K, out, TILE):
+    """More tiles than compute units: workgroups take several, and a last, partly filled round's rows may run on smaller
+    tiles. One, two, three and more blocks of K."""
+    rng = np.random.default_rng(M)
     a, sa, w, sw = operands(rng, M, N, K)
-    got = run(gpu, a, sa, w, sw, out="bf16")
-    rows = np.r_[0:3, 255:258, 2300, 4095:4100, M - 2:M]
-    check(got[rows], a[rows], sa[rows], w, sw, "bf16")
+    got = run(gpu, a, sa, w, sw, out=out, TILE=TILE)
+    rows = np.r_[0:3, 255:258, 2047:2050, 2300, 4095:4100, M - 300:M - 295, M - 2:M]
+    rows = rows[rows < M]
+    check(got[rows], a[rows], sa[rows], w, sw, out)
 
 
 def test_output_past_32_bit_offsets(gpu):
