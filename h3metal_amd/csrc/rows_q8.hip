@@ -71,20 +71,60 @@ __device__ __forceinline__ float max16(float m) {
   return fmaxf(m, xshfl<1>(m));
 }
 
-// The e4m3 codes of 8 values whose block's largest magnitude is m. Blocks below 2^-100 are scaled up first: 448 / m
-// would overflow there.
-__device__ __forceinline__ uint2 codes_f8(const float (&t)[PL], float m) {
-  const float up = m < 0x1p-100f ? 0x1p64f : 1.0f;
-  const float rs = m > 0.0f ? F8_MAX / (m * up) : 1.0f;
-  float y[PL];
-#pragma unroll
-  for (int i = 0; i < PL; i++) y[i] = t[i] * up * rs;
+// The largest of LPR neighbouring lanes' values (LPR at most 64), in each of them
+template <int LPR>
+__device__ __forceinline__ float max_of(float m) {
+  if constexpr (LPR > 32) m = fmaxf(m, __shfl_xor(m, 32));
+  if constexpr (LPR > 16) m = fmaxf(m, xshfl<16>(m));
+  return max16(m);
+}
+template <int LPR>
+__device__ __forceinline__ float sum_of(float m) {
+  if constexpr (LPR > 32) m += __shfl_xor(m, 32);
+  m += xshfl<16>(m);
+  m += xshfl<8>(m);
+  m += xshfl<4>(m);
+  m += xshfl<2>(m);
+  return m + xshfl<1>(m);
+}
+
+// The scale s = m / most of values whose largest magnitude is m (1 where m is 0), and 1 / (s up): values below 2^-100 are
+// scaled by `up` before their product with it, which would overflow.
+struct Scale {
+  float s, inv, up;
+};
+template <int MOST>
+__device__ __forceinline__ Scale scale_of(float m) {
+  const float up = m < 0x1p-100f && m > 0.0f ? 0x1p64f : 1.0f;
+  const float s = m > 0.0f ? m * up * (1.0f / MOST) : 1.0f;  // a normal float, and so is its reciprocal
+  const float r = __builtin_amdgcn_rcpf(s);
+  // one Newton step; infinity's 0 stays
+  return {m > 0.0f ? m * (1.0f / MOST) : 1.0f, __builtin_amdgcn_div_fixupf(__builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r), s, 1.0f), up};
+}
+
+__device__ __forceinline__ uint2 pack_f8(const float (&y)[PL]) {
   int lo = 0, hi = 0;
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], lo, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], hi, false);
   hi = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], hi, true);
   return make_uint2((unsigned)lo, (unsigned)hi);
+}
+
+// Whether y, a quotient within 8 * 2^-24, may round to another e4m3 value than the exact one: its 20 dropped mantissa bits
+// are near one half, or it is a subnormal code's (whose dropped bits are more).
+__device__ __forceinline__ bool near_tie(float y) {
+  const unsigned u = __builtin_bit_cast(unsigned, y) & 0x7fffffffu;
+  return ((u + 8 - 0x80000u) & 0xfffffu) <= 16 || u - 1 < 0x3c800000u - 1;
+}
+
+// x in float, rounded to odd: a further rounding to few bits then gives what rounding x itself gives
+__device__ __forceinline__ float to_odd(double x) {
+  const float f = (float)x;
+  if ((double)f == x || x != x) return f;
+  unsigned u = __builtin_bit_cast(unsigned, f);
+  if (fabs((double)f) > fabs(x)) u--;
+  return __builtin_bit_cast(float, u | 1);
 }
 
 __device__ __forceinline__ void store_codes(unsigned char *p, uint2 c, int n) {
@@ -107,21 +147,28 @@ struct NormArgs {
   char *res_out;
 };
 
-// One workgroup of 256 threads per row.
-template <int XT, int RT, bool I8>
+// LPR lanes a row: 256 / LPR rows a workgroup. The e4m3 codes are the exactly rounded ones: where a float quotient is near a
+// tie (about one in a hundred of the waves' steps), its products and the largest of them are taken again in double.
+template <int XT, int RT, bool I8, int LPR>
 __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Params p) {
   using XE = typename Elem<XT>::type;
   using RE = typename Elem<RT>::type;
-  extern __shared__ float top[];  // e4m3: the blocks' largest magnitudes
+  constexpr int STEP = LPR * PL, HELD = I8 ? 4 : 1;  // int8: this many steps of a row stay in registers until its amax is known
+    extern __shared__ float tops[];  // e4m3: the blocks' largest magnitudes
   __shared__ float red[8];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const size_t m = blockIdx.x;
-  const int nb = (p.D + FB - 1) / FB;
+  const int tid = threadIdx.x, lane = tid % LPR, wave = tid >> 6;
+  const int nb = (p.D + FB - 1) / FB, end = nb * FB;
+  size_t m = (size_t)blockIdx.x * (256 / LPR) + tid / LPR;
+  const bool there = m < (size_t)p.M;
+  if (LPR > 64 && !there) return;
+  m = there ? m : p.M - 1;  // (lanes past the last row go along with it and write nothing)
   const XE *xr = (const XE *)a.x + m * p.x_stride;
   const RE *rr = (const RE *)a.res + m * p.r_stride;
   RE *ro = (RE *)a.res_out + m * p.ro_stride;
   unsigned char *out = a.out + m * p.o_stride;
+  float *top = tops + tid / LPR * nb;
 
+  // h of 8 columns; the first time the sum is made and stored
   auto load = [&](int c, float (&h)[PL]) __attribute__((always_inline)) {
     const int n = p.D - c;
     load8(h, xr + c, n);
@@ -134,77 +181,124 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
         s[i] = (RE)(r[i] + h[i]);
         h[i] = (float)s[i];
       }
-      store8(ro + c, s, n);
+      if (there) store8(ro + c, s, n);
     }
   };
-  auto weigh = [&](int c, float (&h)[PL]) __attribute__((always_inline)) {
-    if (!a.w) return;
-    float g[PL];
-    load8(g, a.w + c, p.D - c);
-#pragma unroll
-    for (int i = 0; i < PL; i++) h[i] *= g[i];
+  auto reload = [&](int c, float (&h)[PL]) __attribute__((always_inline)) {
+    if constexpr (RT != T_NONE) load8(h, (const RE *)ro + c, p.D - c);
+    else load8(h, xr + c, p.D - c);
   };
-  auto wave_sum = [](float v) {
+  auto gain = [&](int c, float (&g)[PL]) __attribute__((always_inline)) {
+    if (a.w) {
+      load8(g, a.w + c, p.D - c);
+    } else {
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
-    return v;
+      for (int i = 0; i < PL; i++) g[i] = 1.0f;
+    }
   };
 
-  float sq = 0.0f, rowmax = 0.0f;
-  for (int c = tid * PL; c < (p.D + FB - 1) / FB * FB; c += 256 * PL) {
-    float h[PL];
+  float sq = 0.0f, rowmax = 0.0f, held[HELD][PL];
+  auto step = [&](int c, float (&t)[PL]) __attribute__((always_inline)) {
+    float h[PL], g[PL];
     load(c, h);
-#pragma unroll
-    for (int i = 0; i < PL; i++) sq = __builtin_fmaf(h[i], h[i], sq);
-    weigh(c, h);
+    gain(c, g);
     float mx = 0.0f;
 #pragma unroll
-    for (int i = 0; i < PL; i++) mx = fmaxf(mx, fabsf(h[i]));
+    for (int i = 0; i < PL; i++) {
+      sq = __builtin_fmaf(h[i], h[i], sq);
+      t[i] = h[i] * g[i];
+      mx = fmaxf(mx, fabsf(t[i]));
+    }
     if constexpr (!I8) {
       mx = max16(mx);
-      store_codes(out + c, codes_f8(h, mx), p.D - c);
+      const Scale v = scale_of<448>(mx);
+      float y[PL];
+      bool tie = v.up != 1.0f;
+#pragma unroll
+      for (int i = 0; i < PL; i++) {
+        y[i] = t[i] * v.inv;
+        tie |= near_tie(y[i]);
+      }
+      if (__any(tie)) {
+        double d[PL], dm = 0.0;
+#pragma unroll
+        for (int i = 0; i < PL; i++) {
+          d[i] = (double)h[i] * g[i];
+          dm = fmax(dm, fabs(d[i]));
+        }
+#pragma unroll
+        for (int k = 8; k > 0; k >>= 1) dm = fmax(dm, __shfl_xor(dm, k));
+        if (dm > 0.0 && dm < (double)INFINITY)  // (float quotients of NaN and infinities are as they should be)
+#pragma unroll
+          for (int i = 0; i < PL; i++) y[i] = to_odd(d[i] * (double)F8_MAX / dm);
+      }
+      if (there) store_codes(out + c, pack_f8(y), p.D - c);
       if ((lane & 15) == 0) top[c / FB] = mx;
     }
     rowmax = fmaxf(rowmax, mx);
-  }
-  sq = wave_sum(sq);
+  };
+  int c = lane * PL;
+  if constexpr (I8) {
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) rowmax = fmaxf(rowmax, __shfl_xor(rowmax, s));
-  if (lane == 0) red[w] = sq, red[4 + w] = rowmax;
-  __syncthreads();
-  sq = (red[0] + red[1]) + (red[2] + red[3]);
+    for (int k = 0; k < HELD; k++)
+      if (c + k * STEP < end) step(c + k * STEP, held[k]);
+    c += HELD * STEP;
+  }
+  for (; c < end; c += STEP) {
+    float t[PL];
+    step(c, t);
+  }
+  sq = sum_of<LPR < 64 ? LPR : 64>(sq);
+  if constexpr (I8) rowmax = max_of<LPR < 64 ? LPR : 64>(rowmax);
+  if constexpr (LPR > 64) {
+    if ((tid & 63) == 0) red[wave] = sq, red[4 + wave] = rowmax;
+    __syncthreads();
+    sq = (red[0] + red[1]) + (red[2] + red[3]);
+    rowmax = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+  } else {
+    __syncthreads();  // the blocks' largest magnitudes are there
+  }
   const float r = p.norm ? 1.0f / sqrtf(sq / (float)p.D + p.eps) : 1.0f;
   if constexpr (!I8) {
-    for (int b = tid; b < nb; b += 256) a.scale[m * nb + b] = top[b] > 0.0f ? top[b] * r / F8_MAX : 1.0f;
+    if (there)
+      for (int b = lane; b < nb; b += LPR) a.scale[m * nb + b] = top[b] > 0.0f ? top[b] * r / F8_MAX : 1.0f;
   } else {
-    rowmax = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-    const float up = rowmax < 0x1p-100f ? 0x1p64f : 1.0f;
-    const float rs = rowmax > 0.0f ? 127.0f / (rowmax * up) : 1.0f;
-    for (int c = tid * PL; c < p.D; c += 256 * PL) {
-      float h[PL];
-      if constexpr (RT != T_NONE) load8(h, (const RE *)ro + c, p.D - c);
-      else load8(h, xr + c, p.D - c);
-      weigh(c, h);
+    const Scale v = scale_of<127>(rowmax);
+    auto codes = [&](int c, const float (&t)[PL]) __attribute__((always_inline)) {
       unsigned char q[PL];
 #pragma unroll
-      for (int i = 0; i < PL; i++) q[i] = (unsigned char)(int)rintf(h[i] * up * rs);
-      store8(out + c, q, p.D - c);
+      for (int i = 0; i < PL; i++) q[i] = (unsigned char)(int)rintf(t[i] * v.up * v.inv);
+      if (there) store8(out + c, q, p.D - c);
+    };
+    c = lane * PL;
+#pragma unroll
+    for (int k = 0; k < HELD; k++)
+      if (c + k * STEP < end) codes(c + k * STEP, held[k]);
+    for (c += HELD * STEP; c < end; c += STEP) {
+      float h[PL], g[PL];
+      reload(c, h);
+      gain(c, g);
+#pragma unroll
+      for (int i = 0; i < PL; i++) h[i] *= g[i];
+      codes(c, h);
     }
-    if (tid == 0) a.scale[m] = rowmax > 0.0f ? rowmax * r / 127.0f : 1.0f;
+    if (lane == 0 && there) a.scale[m] = rowmax > 0.0f ? rowmax * r / 127.0f : 1.0f;
   }
 }
 
-// value * gate / (1 + exp(-gate)) from e = exp(-|gate|) <= 1, which does not overflow: gate / (1 + e), or gate e / (1 + e)
-// for negative gates. The exponent |gate| log2(e) is taken with its rounding error and the constant's second part, put
-// back to first order. Gates below GATE_MIN, where e leaves the normal floats, are left to gated_low.
+// value * gate / (1 + exp(-gate)) for gates from GATE_MIN, where 1 + exp(-gate) and its reciprocal are normal floats. The
+// exponent -gate log2(e) is taken with its rounding error and the constant's second part, put back to first order; the
+// hardware reciprocal gets one Newton step (14 instructions a value; 25 from exp(-|gate|) and a corrected division: 16896 x
+// 10240 values 187 us then, 145 now with the block's division below as a product).
 constexpr float GATE_MIN = -86.0f;
 __device__ __forceinline__ float gated(float v, float g) {
   constexpr float L = 1.44269504088896340736f, L2 = 1.92596303e-8f, LN2 = 0.693147180559945309417f;
-  const float n = fabsf(g), t = n * -L;
+  const float n = fminf(g, 100.0f), t = n * -L;  // exp(-100) is nothing beside 1
   const float lo = __builtin_fmaf(n, -L2, __builtin_fmaf(n, -L, -t));
   const float e0 = __builtin_amdgcn_exp2f(t);
-  const float e = n < 200.0f ? __builtin_fmaf(e0, lo * LN2, e0) : 0.0f;
-  return v * ((g < 0.0f ? g * e : g) * __builtin_amdgcn_rcpf(1.0f + e));
+  const float d = 1.0f + __builtin_fmaf(e0, lo * LN2, e0);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return v * (g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r));
 }
 // The same below GATE_MIN, where 1 + exp(gate) is 1: value gate exp(gate), from 2^64 exp(gate), a normal float down to
 // gates whose result no float holds.
@@ -217,28 +311,43 @@ __device__ __forceinline__ float gated_low(float v, float g) {
   return v * g * e * 0x1p-64f;
 }
 
+// b / nb for b < 2^28 as a product: magic = ceil(2^(32 + shift) / nb), 2^shift the power of two from nb / 16 on (nb = 1: b)
+struct Divide {
+  unsigned nb, magic, shift;
+};
+
 // 16 lanes per block of 128 columns, blocks in row order
 template <int XT>
-__global__ __launch_bounds__(256) void swiglu_f8_kernel(const char *x, unsigned char *out, float *scale, SwigluF8Params p) {
+__global__ __launch_bounds__(256) void swiglu_f8_kernel(const char *x, unsigned char *out, float *scale, SwigluF8Params p, Divide d) {
   using XE = typename Elem<XT>::type;
-  const unsigned nb = (unsigned)(p.D + FB - 1) / FB;
-  const size_t b = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
-  const size_t m = b / nb;
-  if (m >= (size_t)p.M) return;
-  const int c = (int)(b - m * nb) * FB + (threadIdx.x & 15) * PL, n = p.D - c;
-  const XE *row = (const XE *)x + m * p.x_stride;
+  const unsigned b = blockIdx.x * 16 + threadIdx.x / 16, m = d.nb == 1 ? b : __umulhi(b, d.magic) >> d.shift;
+  if (m >= (unsigned)p.M) return;
+  const int c = (int)(b - m * d.nb) * FB + (threadIdx.x & 15) * PL, n = p.D - c;
+  const XE *row = (const XE *)x + (size_t)m * p.x_stride;
   float v[PL], g[PL];
   load8(v, row + c, n);
   load8(g, row + p.D + c, n);
-  float mx = 0.0f;
+  float low = g[0], mx = 0.0f;
 #pragma unroll
-  for (int i = 0; i < PL; i++) {
-    v[i] = g[i] < GATE_MIN ? gated_low(v[i], g[i]) : gated(v[i], g[i]);
-    mx = fmaxf(mx, fabsf(v[i]));
+  for (int i = 1; i < PL; i++) low = fminf(low, g[i]);
+  if (__builtin_expect(__any(low < GATE_MIN), 0)) {
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] = g[i] < GATE_MIN ? gated_low(v[i], g[i]) : gated(v[i], g[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] = gated(v[i], g[i]);
   }
+#pragma unroll
+  for (int i = 0; i < PL; i++) mx = fmaxf(mx, fabsf(v[i]));
   mx = max16(mx);
-  store_codes(out + m * p.o_stride + c, codes_f8(v, mx), n);
-  if ((threadIdx.x & 15) == 0) scale[b] = mx > 0.0f ? mx / F8_MAX : 1.0f;
+  const Scale s = scale_of<448>(mx);
+  if (__builtin_expect(__any(s.up != 1.0f), 0))
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] *= s.up;
+#pragma unroll
+  for (int i = 0; i < PL; i++) v[i] *= s.inv;
+  store_codes(out + (size_t)m * p.o_stride + c, pack_f8(v), n);
+  if ((threadIdx.x & 15) == 0) scale[b] = s.s;
 }
 
 int esize(int t) { return t == T_F32 ? 4 : 2; }
@@ -323,7 +432,17 @@ int launch_norm(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, con
   }
   const NormArgs g{a[0].ptr, has_res ? a[1].ptr : nullptr, (const float *)a[2].ptr, (unsigned char *)a[3].ptr,
                    (float *)a[4].ptr, has_res ? a[5].ptr : nullptr};
-  hipLaunchKernelGGL((rms_norm_q8_kernel<XT, RT, I8>), dim3((unsigned)p.M), dim3(256), I8 ? 0 : nb * 4, ex.stream, g, p);
+  // Lanes a row. Short rows share a workgroup: bf16 rows and residual, 16896 of 256 columns 7.8 us with 32 lanes (64: 10.6,
+  // 256: 22.3), of 1024 columns 20 with 64 (256: 29), of 2048 columns 35 with 64 (256: 38), of 4096 columns 91 with 256 (64:
+  // 98; 300 rows 6.0, 64: 12.7).
+  auto go = [&](auto lpr) {
+    constexpr int LPR = decltype(lpr)::value, ROWS = 256 / LPR;
+    hipLaunchKernelGGL((rms_norm_q8_kernel<XT, RT, I8, LPR>), dim3((unsigned)((p.M + ROWS - 1) / ROWS)), dim3(256),
+                       I8 ? 0 : ROWS * nb * 4, ex.stream, g, p);
+  };
+  if (p.D <= 32 * PL) go(std::integral_constant<int, 32>{});
+  else if (p.D <= 256 * PL) go(std::integral_constant<int, 64>{});
+  else go(std::integral_constant<int, 256>{});
   return 0;
 }
 
@@ -359,8 +478,11 @@ int launch_swiglu(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, c
     *err = "over 2^28 - 1 blocks of 128 columns";
     return -1;
   }
+  Divide d{(unsigned)nb, 0, 0};
+  while (nb > 16 << d.shift) d.shift++;
+  if (nb > 1) d.magic = (unsigned)(((1ull << (32 + d.shift)) + nb - 1) / nb);
   hipLaunchKernelGGL((swiglu_f8_kernel<XT>), dim3((unsigned)((blocks + 15) / 16)), dim3(256), 0, ex.stream, a[0].ptr,
-                     (unsigned char *)a[1].ptr, (float *)a[2].ptr, p);
+                     (unsigned char *)a[1].ptr, (float *)a[2].ptr, p, d);
   return 0;
 }
 

@@ -2,8 +2,9 @@
 roundings, at lengths from one column, odd strides and offsets, all type pairs; rows of zeros, tiny and huge values, NaN
 and infinities; what lies behind the rows stays; refusals.
 
-Bounds. A code is right if it is the rounding of some value within 5 * 2^-24 of v / s: h w, 448 / amax (two roundings with
-amax's own), the product, and for the gated unit its value's own error, given apart. A scale is amax times the reciprocal
+Bounds. rms_norm_q8's e4m3 codes are the rounded exact quotients (EXACT: what the oracle's own float64 steps may be off). An
+int8 code is right if it is the rounding of some value within 5 * 2^-24 of v / s: h w, 127 / amax (two roundings with amax's
+own) and the product; a gated unit's code likewise, its value's own error given apart. A scale is amax times the reciprocal
 root over 448: 6 roundings, and half the relative error of the sum of squares, whose positive terms are added on at least 16
 lanes (D / 16 additions in a row and 12 across lanes and waves, at most)."""
 
@@ -18,6 +19,7 @@ from oracle.bf16 import from_bf16, to_bf16
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24  # half a step of float, relative to the value
+EXACT = 2.0 ** -49
 
 
 def as_type(x, t):
@@ -101,7 +103,7 @@ def check_norm(h, codes, scale, w, D, out, eps=1e-6, norm=True):
     tol = (6 + 0.5 * (D / 16 + 12)) * U
     assert np.all(np.abs(scale - ws) <= tol * ws), np.max(np.abs(scale - ws) / ws)
     if out == "f8":
-        check_codes(codes, v / orq.per_column(ws, D), 5 * U)
+        check_codes(codes, v / orq.per_column(ws, D), EXACT)
     else:
         q = v / ws
         lo, hi = np.rint(q - np.abs(q) * 5 * U), np.rint(q + np.abs(q) * 5 * U)
@@ -135,6 +137,16 @@ def test_norm_types(gpu, xt, rt, out):
         check_norm(h, c, s, None, D, out)
 
 
+def test_many_rows_have_exact_codes(gpu):
+    """Half a million values, of which about ten have a float quotient beyond a tie from the exact one."""
+    rng = np.random.default_rng(14)
+    M, D = 128, 4096
+    x = rng.standard_normal((M, D))
+    w = (1 + 0.1 * rng.standard_normal(D)).astype(np.float32)
+    h, c, s = norm_case(gpu, x, "f32", None, None, w, D)
+    check_norm(h, c, s, w, D, "f8")
+
+
 @pytest.mark.parametrize("out", ["f8", "i8"])
 def test_norm_options(gpu, out):
     """Without the norm (plain rounding to 8 bits), with a gain or none, and a large eps."""
@@ -160,7 +172,7 @@ def test_extreme_magnitudes(gpu, mag, out):
     ws = orq.block_scales(v) if out == "f8" else orq.row_scales(v)[:, None]
     assert np.all(np.abs(s - ws) <= 3 * U * ws + 2.0 ** -149)
     if out == "f8":
-        check_codes(c, v / orq.per_column(ws, D), 5 * U)
+        check_codes(c, v / orq.per_column(ws, D), EXACT)
     else:
         q = v / ws
         assert np.all((c >= np.rint(q - np.abs(q) * 5 * U)) & (c <= np.rint(q + np.abs(q) * 5 * U)))
@@ -197,7 +209,7 @@ def test_nan_and_infinity(gpu):
     at = np.repeat(ok, 128, 1)[:, :D].copy()
     at[1, 5] = False
     q = clean / orq.per_column(ws, D)
-    check_codes(c[at], q[at], 5 * U)
+    check_codes(c[at], q[at], EXACT)
     rest = c[2, 128:256].copy()
     rest[200 - 128] = 0
     assert not (rest & 0x7F).any()
