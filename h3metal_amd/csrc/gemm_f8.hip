@@ -3,14 +3,21 @@
 // A [M][K] and W [N][K] e4m3, row-major in k, sa a scale for each row and block of 128 columns, sw one for each 128 x 128
 // block of W (the last blocks of K and of N may be short). The epilogues are gemm.hip's: C[m][n] = OUT_T(v + bias[n]), or
 // X[m][n] += gate[rtype[m]][n] * (v + bias[n]) with X float.
-// A block's 128 products are summed by the matrix unit in float; each block's sum enters the float accumulator in one fused
-// step with the product of its two scales. The codes are widened to half (exact) and multiplied as halves: the matrix unit
-// aligns the 8 products of a group of 8-bit operands to the largest and keeps 13 bits below it (sums of 128 are 1.5e-5 off
-// in the mean; 1.5e-8 with halves).
+// Each block's sum enters the float accumulator in one fused step with the product of its two scales.
 //
-// One wave per 32 x 32 tile, operands straight from memory.
+// Precision. The 8-bit matrix instruction aligns the 8 products of a group (8 neighbours in K) to the largest and keeps 13
+// bits below its exponent; sums of such groups are float. Random sums of 128 products are then 1.5e-5 off (2-norm), where
+// codes widened to half (exact: a half holds every e4m3 value) and the half instruction give 1.5e-8. 16-bit outputs, whose own
+// rounding is 1.7e-3 (bf16) or 2.1e-4 (f16), take the 8-bit instruction; float outputs, the residual's among them, the half
+// one, at half its rate.
+//
+// What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 747 to 797 us by box, 2.1 to 2.3 PFLOP/s at
+// 1.6 GHz with the matrix unit busy 56% of the time; all-zero operands 604 us; the instruction loop alone, operands in
+// registers, 3.5 PFLOP/s), for float outputs the vector instructions as well (2 conversions and an add for each matrix
+// instruction). Few tiles: the L2 -> LDS stream of the operands and the start and end of the launch.
 #include "gemm_common.h"
 
+#include <algorithm>
 #include <cstring>
 
 namespace h3 {
@@ -29,17 +36,16 @@ __device__ __forceinline__ f16x8 widen(int lo, int hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// What a block's products are multiplied as. E4M3: the 8-bit matrix instruction, for 16-bit outputs; HALF: codes widened to
-// half, for float outputs and where the reading of the operands bounds the time anyway.
+// What a block's products are multiplied as (16-bit outputs, float outputs)
 enum { E4M3 = 0, HALF = 1 };
 
-// A lane's codes of a block: the 16-byte pieces 2 d + hl (d = 0..3) of its row's 128. Any order of K that both operands
-// share will do.
+// 16 x 16 sums of a block: lane l holds row l % 16's pieces 2 (l / 16) and 2 (l / 16) + 1; element e is that of W row
+// 4 (l / 16) + e and A row l % 16
 struct Codes {
-  i32x4 d[4];
+  i32x4 d[2];
 };
 struct Halves {
-  f16x8 d[8];
+  i32x4 d[4];  // 8 halves each
 };
 template <int MODE>
 using Operand = typename std::conditional<MODE == HALF, Halves, Codes>::type;
@@ -50,49 +56,42 @@ __device__ __forceinline__ Operand<MODE> operand(const Codes &c) {
   else {
     Halves h;
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
-      h.d[2 * d] = widen(c.d[d][0], c.d[d][1]);
-      h.d[2 * d + 1] = widen(c.d[d][2], c.d[d][3]);
+    for (int d = 0; d < 2; d++) {
+      h.d[2 * d] = __builtin_bit_cast(i32x4, widen(c.d[d][0], c.d[d][1]));
+      h.d[2 * d + 1] = __builtin_bit_cast(i32x4, widen(c.d[d][2], c.d[d][3]));
     }
     return h;
   }
+}
+// the k-th two of the 32 values that operand makes, here and not where they are used
+__device__ __forceinline__ void widen_two(Halves &h, const Codes &c, int k) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const int v = c.d[k >> 3][(k >> 1) & 3];
+  const h2 x = k & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false);
+  int y = __builtin_bit_cast(int, x);
+  asm volatile("" : "+v"(y));
+  h.d[k >> 2][k & 3] = y;
+}
+
+template <int MODE>
+constexpr int MMAS = MODE == HALF ? 4 : 1;
+__device__ __forceinline__ f32x4 mma(int, const Codes &w, const Codes &a, f32x4 t) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(w.d[0], w.d[1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                          __builtin_shufflevector(a.d[0], a.d[1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0,
+                                                          0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(int c, const Halves &w, const Halves &a, f32x4 t) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.d[c]), __builtin_bit_cast(f16x8, a.d[c]), t, 0, 0, 0);
 }
 
 // The weight's scales are read through the scalar unit: the loop counts its vector loads itself, and one that the compiler
 // sees would make it wait for all of them.
 typedef const __attribute__((address_space(4))) float *Scalars;
 
-// The 32 x 32 sums of a block's products, one matrix instruction of MMAS after the other: element e is that of W row
-// 8 (e / 4) + 4 (lane / 32) + e % 4 and A row lane % 32
-template <int MODE>
-constexpr int MMAS = MODE == HALF ? 8 : 2;
-__device__ __forceinline__ f32x16 mma(int c, const Codes &w, const Codes &a, f32x16 t) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-      __builtin_shufflevector(w.d[2 * c], w.d[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-      __builtin_shufflevector(a.d[2 * c], a.d[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0, 0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mma(int c, const Halves &w, const Halves &a, f32x16 t) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(w.d[c], a.d[c], t, 0, 0, 0);
-}
-template <int MODE>
-__device__ __forceinline__ f32x16 block_sums(const Operand<MODE> &w, const Operand<MODE> &a) {
-  f32x16 t = {};
-#pragma unroll
-  for (int c = 0; c < MMAS<MODE>; c++) t = mma(c, w, a, t);
-  return t;
-}
-
 // 16-byte piece p of an LDS row of 128 bytes sits at slot p ^ ((row / 2) % 8): the 16 rows of a pass of a 16-byte read then
 // cover all banks. A 1 KB LDS-direct load fills 8 rows; lane l fills slot l % 8 of row l / 8.
 __device__ __forceinline__ int slot(int row, int piece) { return row * KB + ((piece ^ ((row >> 1) & 7)) << 4); }
 __device__ __forceinline__ int fetch_piece(int q, int lane) { return (lane & 7) ^ ((4 * q + (lane >> 4)) & 7); }
-
-__device__ __forceinline__ Codes read_codes(const char *rows, int row, int hl) {
-  Codes c;
-#pragma unroll
-  for (int d = 0; d < 4; d++) c.d[d] = *(const i32x4 *)(rows + slot(row, 2 * d + hl));
-  return c;
-}
 
 // The epilogue on V consecutive columns n .. of row m, of which v holds the products' sums; `all`: every column is there
 // and 16-byte accesses are aligned
@@ -165,51 +164,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *p, size_t 
 
 // ---- large products: 8 waves on TM x TN tiles -------------------------------------------------------------------------
 
-// 16 x 16 sums of a block: lane l holds row l % 16's pieces 2 (l / 16) and 2 (l / 16) + 1; element e is that of W row
-// 4 (l / 16) + e and A row l % 16
-struct Codes16 {
-  i32x4 d[2];
-};
-struct Halves16 {
-  i32x4 d[4];  // 8 halves each
-};
-template <int MODE>
-using Operand16 = typename std::conditional<MODE == HALF, Halves16, Codes16>::type;
-
-template <int MODE>
-__device__ __forceinline__ Operand16<MODE> operand16(const Codes16 &c) {
-  if constexpr (MODE == E4M3) return c;
-  else {
-    Halves16 h;
-#pragma unroll
-    for (int d = 0; d < 2; d++) {
-      h.d[2 * d] = __builtin_bit_cast(i32x4, widen(c.d[d][0], c.d[d][1]));
-      h.d[2 * d + 1] = __builtin_bit_cast(i32x4, widen(c.d[d][2], c.d[d][3]));
-    }
-    return h;
-  }
-}
-// the k-th two of the 32 values that operand16 makes, here and not where they are used
-__device__ __forceinline__ void widen_two(Halves16 &h, const Codes16 &c, int k) {
-  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-  const int v = c.d[k >> 3][(k >> 1) & 3];
-  const h2 x = k & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false);
-  int y = __builtin_bit_cast(int, x);
-  asm volatile("" : "+v"(y));
-  h.d[k >> 2][k & 3] = y;
-}
-
-template <int MODE>
-constexpr int MMAS16 = MODE == HALF ? 4 : 1;
-__device__ __forceinline__ f32x4 mma16(int, const Codes16 &w, const Codes16 &a, f32x4 t) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(w.d[0], w.d[1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                                          __builtin_shufflevector(a.d[0], a.d[1], 0, 1, 2, 3, 4, 5, 6, 7), t, 0,
-                                                          0, 0, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma16(int c, const Halves16 &w, const Halves16 &a, f32x4 t) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.d[c]), __builtin_bit_cast(f16x8, a.d[c]), t, 0, 0, 0);
-}
-
+// Rows of a block (128 bytes) go to LDS through LDS-direct loads, two stages of TM + TN rows; a wave owns TM / 4 rows x TN / 2
+// columns. What it measured at 16896 x 12288 x 4096 (us): 32 x 32 instructions, their sums added after each pair 872; 16 x 16
+// ones with the adds of earlier sums between them 828; a workgroup on several tiles, the next one's loads issued before the
+// results leave 793; results stored past the caches 750. Tried and not kept: the loads spread over the whole step (their
+// latency shows; 2% slower), a second meeting of the waves a step for it (2% faster with zero operands, nothing under power).
 template <int MODE_, int TM_, int TN_>
 struct Tile {
   static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NW = 8, WGM = 4, WGN = 2;
@@ -386,7 +345,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
   // (16 rows further the swizzle is the same)
   const int at[2] = {slot(l16, 2 * lg), slot(l16, 2 * lg + 1)}, pa = WTM * wm * KB, pw = (TM + WTN * wn) * KB;
   auto read = [&](int rows, int t, int stage) __attribute__((always_inline)) {
-    Codes16 c;
+    Codes c;
 #pragma unroll
     for (int d = 0; d < 2; d++) {
       const char *q = smem + (at[d] + (rows + stage * C::STAGE));
@@ -416,8 +375,8 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
   // The order is kept as written (sched_barrier): each matrix instruction is followed by the fused adds of the sums MI
   // instructions before it. One wave then keeps the matrix unit busy; sums multiplied and added by turns left it idle for
   // the adds (16 x 16 tiles: 135 cycles for what takes the matrix unit 128, 32 x 32 ones 148 to 200).
-  Codes16 a[MI], an[1], wb[2], wl;
-  Operand16<MODE> ao[MI], b;  // HALF: the widened rows
+  Codes a[MI], an[1], wb[2], wl;
+  Operand<MODE> ao[MI], b;  // HALF: the widened rows
   float sc[MI], fs[MI];
   f32x4 t[MI];
 #pragma unroll
@@ -429,8 +388,8 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
   if constexpr (MODE == HALF) {
     wb[1] = read(pw, 1, 0);
 #pragma unroll
-    for (int i = 0; i < 2; i++) ao[i] = operand16<MODE>(a[i]);
-    b = operand16<MODE>(wb[0]);
+    for (int i = 0; i < 2; i++) ao[i] = operand<MODE>(a[i]);
+    b = operand<MODE>(wb[0]);
   }
   Scalars sw = scales_of(n0), swn = sw;
   float s = sw[0];
@@ -470,18 +429,18 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
       };
       // slot n of the 2 MI NM behind the meeting: its share of the loads
       auto load_some = [&](int n) __attribute__((always_inline)) {
-        constexpr int SL = 2 * MI * MMAS16<MODE>;
+        constexpr int SL = 2 * MI * MMAS<MODE>;
 #pragma unroll
         for (int q = n * NQ / SL; q < (n + 1) * NQ / SL; q++) dma(q, kl, stage);
       };
       if constexpr (MODE == E4M3) {
         // sums (i, j) for every i; `with(n)` goes behind the n-th of them
-        auto row = [&](int j, const Codes16 &b, auto with) __attribute__((always_inline)) {
+        auto row = [&](int j, const Codes &b, auto with) __attribute__((always_inline)) {
           const int pj = (j + NJ - 1) % NJ;
           f32x4 u[MI];
 #pragma unroll
           for (int i = 0; i < MI; i++) {
-            u[i] = mma16(0, b, a[i], f32x4{});
+            u[i] = mma(0, b, a[i], f32x4{});
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[i][pj][e] = __builtin_fmaf(t[i][e], fs[i], acc[i][pj][e]);
@@ -517,7 +476,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
         // for the next step: its first 32 rows in the second half of a step's last row, the others in the next step's first.
         auto row = [&](int j, auto with) __attribute__((always_inline)) {
           const int pj = (j + NJ - 1) % NJ;
-          Halves16 bn;
+          Halves bn;
           f32x4 u[MI];
 #pragma unroll
           for (int h = 0; h < MI; h += 2)
@@ -526,7 +485,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
 #pragma unroll
               for (int i = h; i < h + 2; i++) {
                 const int n = 4 * h + 2 * c + i - h;
-                u[i] = mma16(c, b, ao[i], c ? u[i] : f32x4{});
+                u[i] = mma(c, b, ao[i], c ? u[i] : f32x4{});
                 __builtin_amdgcn_sched_barrier(0);
                 acc[i][pj][c] = __builtin_fmaf(t[i][c], fs[i], acc[i][pj][c]);
                 if (c == 3) asm volatile("" : "+v"(acc[i][pj]));
@@ -548,7 +507,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
         };
         if (MI == 2)
 #pragma unroll
-          for (int i = 0; i < MI; i++) ao[i] = operand16<MODE>(a[i]);
+          for (int i = 0; i < MI; i++) ao[i] = operand<MODE>(a[i]);
 #pragma unroll
         for (int j = 0; j < NJ - 2; j++)
           row(j, [&](int n) __attribute__((always_inline)) {
@@ -598,22 +557,24 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
 // ---- few tiles: the waves of a workgroup split K ----------------------------------------------------------------------
 
 // Wave w multiplies the whole TM x TN tile over blocks w, w + NWK, ... from LDS slots of its own, filled NST blocks ahead; no
-// wave waits for another before the end, where the partial tiles meet in LDS and are added in the order of the waves.
+// wave waits for another before the end, where the partial tiles meet in LDS and are added in the order of the waves. Heights
+// from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 18.4 us in 64 rows, 13.1 in 80).
 template <int MODE_, int TM_, int TN_, int NWK_, int NST_>
 struct KTile {
-  static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NWK = NWK_, NST = NST_, MI = TM / 32, NJ = TN / 32;
-  static constexpr int SLOT = (TM + TN) * KB + 256;           // a block's rows of A and W, and the A rows' scales
-  static constexpr int LPS = (TM + TN) / 8 + 1;               // loads per slot
+  static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NWK = NWK_, NST = NST_, MI = TM / 16, NJ = TN / 16;
+  static constexpr int NS = (TM + 63) / 64;                   // loads of the A rows' scales
+  static constexpr int SLOT = (TM + TN) * KB + NS * 256;      // a block's rows of A and W, and the scales
+  static constexpr int LPS = (TM + TN) / 8 + NS;              // loads per slot
   static constexpr int RS = TN * 4 + 16;
   static constexpr int LDS = NWK * (NST * SLOT > TM * RS ? NST * SLOT : TM * RS);
-  static_assert(TM <= 64 && KB % TN == 0 && LDS <= 160 * 1024 && (NST - 1) * LPS <= 63, "tile configuration");
+  static_assert(KB % TN == 0 && LDS <= 160 * 1024 && (NST - 1) * LPS <= 63, "tile configuration");
 };
 
 template <class C>
 __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmParams p, int ntm, int ot, int epi) {
-  constexpr int TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, NST = C::NST, NWK = C::NWK;
+  constexpr int MODE = C::MODE, TM = C::TM, TN = C::TN, MI = C::MI, NJ = C::NJ, NST = C::NST, NWK = C::NWK;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lid = xcd_order(blockIdx.x, gridDim.x), nt = lid / ntm, mt = lid - nt * ntm;
   const int m0 = mt * TM, n0 = nt * TN;
@@ -624,65 +585,79 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
   const __amdgpu_buffer_rsrc_t rs = rows_of(g.sa, m0, min(TM, p.M - m0), p.groups * 4);
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem + w * (NST * C::SLOT);
   const char *own = smem + w * (NST * C::SLOT);
-  int offa[TM / 8], offw[TN / 8];
-#pragma unroll
-  for (int q = 0; q < TM / 8; q++) offa[q] = (8 * q + (lane >> 3)) * p.a_stride + fetch_piece(q, lane) * 16;
-#pragma unroll
-  for (int q = 0; q < TN / 8; q++) offw[q] = (8 * q + (lane >> 3)) * p.w_stride + fetch_piece(q, lane) * 16;
+  const int fetch = fetch_piece(0, lane) * 16;  // of even loads; ^ 64 for odd ones
+  const int offa = (lane >> 3) * p.a_stride, offw = (lane >> 3) * p.w_stride;
   auto dma = [&](int s) __attribute__((always_inline)) {
     const unsigned st = lds0 + ((unsigned)s % NST) * C::SLOT;
     const int kt = s * NWK + w, left = p.K - kt * KB;  // pieces and blocks past K read as zero
+    const int f[2] = {fetch, fetch ^ 64};
+    const bool in[2] = {f[0] < left, f[1] < left};
 #pragma unroll
     for (int q = 0; q < TM / 8; q++)
-      dma16(st + q * 1024, fetch_piece(q, lane) * 16 < left ? (unsigned)(offa[q] + kt * KB) : 0x80000000u, ra);
+      dma16(st + q * 1024, in[q & 1] ? (unsigned)(offa + 8 * q * p.a_stride + f[q & 1] + kt * KB) : 0x80000000u, ra);
 #pragma unroll
     for (int q = 0; q < TN / 8; q++)
-      dma16(st + TM * KB + q * 1024, fetch_piece(q, lane) * 16 < left ? (unsigned)(offw[q] + kt * KB) : 0x80000000u, rw);
-    dma4(st + (TM + TN) * KB, lane < TM && left > 0 ? (unsigned)(lane * p.groups + kt) * 4 : 0x80000000u, rs);
+      dma16(st + TM * KB + q * 1024, in[q & 1] ? (unsigned)(offw + 8 * q * p.w_stride + f[q & 1] + kt * KB) : 0x80000000u, rw);
+#pragma unroll
+    for (int q = 0; q < C::NS; q++)
+      dma4(st + (TM + TN) * KB + q * 256,
+           64 * q + lane < TM && left > 0 ? (unsigned)((64 * q + lane) * p.groups + kt) * 4 : 0x80000000u, rs);
   };
   const Scalars sw = (Scalars)(g.sw + (size_t)(n0 / KB) * p.groups);
 
-  f32x16 acc[MI][NJ];
+  f32x4 acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) acc[i][j] = f32x16{};
+    for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{};
 
   struct Ops {
     Codes a[MI], w[NJ];
     float sa[MI];
   };
+  // (16 rows further the swizzle is the same)
+  const int at[2] = {slot(l16, 2 * lg), slot(l16, 2 * lg + 1)};
   auto read_ops = [&](Ops &o, int s) __attribute__((always_inline)) {
     const char *st = own + ((unsigned)s % NST) * C::SLOT;
 #pragma unroll
-    for (int i = 0; i < MI; i++) {
-      o.a[i] = read_codes(st, 32 * i + l32, hl);
-      o.sa[i] = *(const float *)(st + (TM + TN) * KB + (32 * i + l32) * 4);
-    }
+    for (int d = 0; d < 2; d++) {
+      const char *q = st + at[d];
 #pragma unroll
-    for (int j = 0; j < NJ; j++) o.w[j] = read_codes(st + TM * KB, 32 * j + l32, hl);
+      for (int i = 0; i < MI; i++) o.a[i].d[d] = *(const i32x4 *)(q + 16 * i * KB);
+#pragma unroll
+      for (int j = 0; j < NJ; j++) o.w[j].d[d] = *(const i32x4 *)(q + (TM + 16 * j) * KB);
+    }
+    const char *q = st + (TM + TN) * KB + l16 * 4;
+#pragma unroll
+    for (int i = 0; i < MI; i++) o.sa[i] = *(const float *)(q + 64 * i);
   };
   // Step s: its operands are in registers (cur), so its slot is free and takes step s + NST; the reads of step s + 1 (once
-  // landed) run beside the MFMAs of step s.
+  // landed) run beside the matrix instructions of step s.
   auto step = [&](int s, const Ops &cur, Ops &nxt) __attribute__((always_inline)) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const float swk = sw[min(s * NWK + w, nb - 1)];
     dma(s + NST);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
     read_ops(nxt, s + 1);
-    Operand<C::MODE> b[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; j++) b[j] = operand<C::MODE>(cur.w[j]);
+    Operand<MODE> a[MI];
+    float sc[MI];
 #pragma unroll
     for (int i = 0; i < MI; i++) {
-      const Operand<C::MODE> a = operand<C::MODE>(cur.a[i]);
-      const float sc = cur.sa[i] * swk;
+      a[i] = operand<MODE>(cur.a[i]);
+      sc[i] = cur.sa[i] * swk;
+    }
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const f32x16 t = block_sums<C::MODE>(b[j], a);
+    for (int j = 0; j < NJ; j++) {
+      const Operand<MODE> b = operand<MODE>(cur.w[j]);
+      f32x4 t[MI];
 #pragma unroll
-        for (int e = 0; e < 16; e++) acc[i][j][e] = __builtin_fmaf(t[e], sc, acc[i][j][e]);
-      }
+      for (int c = 0; c < MMAS<MODE>; c++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) t[i] = mma(c, b, a[i], c ? t[i] : f32x4{});
+#pragma unroll
+      for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(t[i][e], sc[i], acc[i][j][e]);
     }
   };
 #pragma unroll
@@ -699,11 +674,7 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
 #pragma unroll
   for (int i = 0; i < MI; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++)
-#pragma unroll
-      for (int q = 0; q < 4; q++)
-        *(f32x4 *)(smem + (w * TM + 32 * i + l32) * C::RS + (32 * j + 8 * q + 4 * hl) * 4) =
-            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    for (int j = 0; j < NJ; j++) *(f32x4 *)(smem + (w * TM + 16 * i + l16) * C::RS + (16 * j + 4 * lg) * 4) = acc[i][j];
   __syncthreads();
   constexpr int PPR = TN / 4;
   const int nl = 4 * (tid % PPR), n = n0 + nl;
@@ -726,22 +697,28 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
 // ---- the launch ---------------------------------------------------------------------------------------------------
 
 // values of the macro TILE, 0 the plan's choice
-enum { TILE_32 = 1, TILE_64, TILE_128, TILE_256x128, TILE_256, TILE_LAST = TILE_256 };
+enum { TILE_16 = 1, TILE_32, TILE_48, TILE_64, TILE_80, TILE_128, TILE_256x128, TILE_256, TILE_LAST = TILE_256 };
 
+// Once for each kernel and device: its workgroups may have `bytes` of LDS
 template <class K>
-int set_lds(K kern, int bytes, std::string *err) {
-  hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) return 0;
-  *err = std::string("hipFuncSetAttribute: ") + hipGetErrorString(e);
-  return -1;
+int set_lds(K kern, int bytes, uint64_t *done, std::string *err) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e == hipSuccess && dev < 64 && *done >> dev & 1) return 0;
+  if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    *err = std::string("hipFuncSetAttribute: ") + hipGetErrorString(e);
+    return -1;
+  }
+  if (dev < 64) *done |= 1ull << dev;
+  return 0;
 }
 
 template <class C>
 int run_ksplit(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_t stream, std::string *err) {
   auto kern = gemm_f8_ksplit<C>;
-  static bool set = false;
-  if (!set && set_lds(kern, C::LDS, err)) return -1;
-  set = true;
+  static uint64_t done = 0;
+  if (set_lds(kern, C::LDS, &done, err)) return -1;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
   hipLaunchKernelGGL(kern, dim3((unsigned)(ntm * ntn)), dim3(C::NWK * 64), C::LDS, stream, g, p, ntm, ot, epi);
   return 0;
@@ -750,25 +727,29 @@ int run_ksplit(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStrea
 template <class C>
 int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_t stream, std::string *err) {
   auto kern = gemm_f8_tile<C>;
-  static bool set = false;
-  if (!set && set_lds(kern, C::LDS, err)) return -1;
-  set = true;
+  static uint64_t done = 0;
+  if (set_lds(kern, C::LDS, &done, err)) return -1;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
   const int cus = cu_count(), slots = (cus > 0 ? cus : 256) * C::PER_CU;
   hipLaunchKernelGGL(kern, dim3((unsigned)std::min(ntm * ntn, slots)), dim3(C::NW * 64), C::LDS, stream, g, p, ntm, ntn, ot, epi);
   return 0;
 }
 
-// What a launch of each kind of tile takes: rounds (tiles over compute units, rounded up) of fixed + per_block * blocks of K
-// microseconds, or, where the card's power bounds it, the operations over `rate` (in 10^6 a microsecond) if that is longer.
+// What a launch of each kind of tile takes, in microseconds: launch + rounds (tiles over compute units, rounded up) of fixed +
+// per_block * blocks of K; or, where the card's power bounds it, the operations over `rate` (in 10^6 a microsecond) if that is
+// longer. pair: per block for two tiles at a time on a compute unit, where it holds two. Fitted to 13 row counts (1 to 4608) x
+// 4 N (128 to 12288) x 4 K (256 to 10240) for 16-bit and for float outputs; the plan's tiles were the fastest ones or within
+// 10% of them there, split rounds up to 30% faster than any one kind (4608 x 4096 x 10240 263 -> 197 us).
 struct Cost {
   int tm, tn;
-  double fixed, per_block, rate;
+  double launch, fixed, per_block, pair, rate;
 };
-constexpr Cost E4M3_COST[] = {{}, {32, 32, 2.35, 0.093, 1e9}, {64, 64, 3.95, 0.184, 1e9}, {128, 128, 3.5, 0.65, 1540},
-                              {256, 128, 4.5, 0.92, 1800}, {256, 256, 6.5, 1.35, 2200}};
-constexpr Cost HALF_COST[] = {{}, {32, 32, 2.34, 0.102, 1e9}, {64, 64, 3.94, 0.257, 1e9}, {128, 128, 4.81, 1.074, 870},
-                              {256, 128, 7.6, 1.6, 1070}, {256, 128, 7.6, 1.6, 1070}};
+constexpr Cost E4M3_COST[] = {{}, {16, 32, 2.0, 1.66, 0.0646, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
+                              {48, 64, 0.3, 3.21, 0.157, 0, 1e9}, {64, 64, 0.0, 3.8, 0.188, 0, 1e9}, {80, 64, 0.0, 4.6, 0.225, 0, 1e9},
+                              {128, 128, 2.7, 1.35, 0.8, 1.3, 1540}, {256, 128, 1.4, 3.48, 0.936, 0, 1800}, {256, 256, 0.0, 6.6, 1.33, 0, 2200}};
+constexpr Cost HALF_COST[] = {{}, {16, 32, 1.7, 1.77, 0.0697, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
+                              {48, 64, 0.6, 3.22, 0.215, 0, 1e9}, {64, 64, 0.4, 4.04, 0.279, 0, 1e9}, {80, 64, 0.8, 4.84, 0.315, 0, 1e9},
+                              {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
 
 // The tiles of a product, and of its last rows where those take others (`rows`: those of `tile`).
 struct Plan {
@@ -781,12 +762,15 @@ Plan make_plan(const GemmParams &p, bool half) {
   const double nb = (p.K + KB - 1) / KB;
   auto tiles = [&](int t, long rows) { return ((rows + cost[t].tm - 1) / cost[t].tm) * (((long)p.N + cost[t].tn - 1) / cost[t].tn); };
   auto time = [&](int t, long rows) {
-    const double rounds = (double)((tiles(t, rows) + cus - 1) / cus);
-    return std::max(rounds * (cost[t].fixed + cost[t].per_block * nb), 2e-6 * rows * p.N * p.K / cost[t].rate);
+    const Cost &c = cost[t];
+    const long n = tiles(t, rows), rounds = (n + cus - 1) / cus;
+    const double us = c.pair == 0 ? rounds * (c.fixed + c.per_block * nb)
+                                  : (rounds / 2) * (2 * c.fixed + c.pair * nb) + (rounds % 2) * (c.fixed + c.per_block * nb);
+    return c.launch + std::max(us, 2e-6 * rows * p.N * p.K / c.rate);
   };
-  Plan best{TILE_32, p.M, 0};
-  double least = time(TILE_32, p.M);
-  for (int t = TILE_64; t <= TILE_LAST; t++) {
+  Plan best{TILE_16, p.M, 0};
+  double least = time(TILE_16, p.M);
+  for (int t = TILE_32; t <= TILE_LAST; t++) {
     const double us = time(t, p.M);
     if (us < least) least = us, best = {t, p.M, 0};
   }
@@ -795,8 +779,8 @@ Plan make_plan(const GemmParams &p, bool half) {
     const long ntn = ((long)p.N + cost[t].tn - 1) / cost[t].tn;
     const long rows = tiles(t, p.M) / cus * cus / ntn * cost[t].tm;
     if (rows <= 0 || rows >= p.M) continue;
-    for (int u = TILE_32; u < t; u++) {
-      const double us = time(t, rows) + time(u, p.M - rows) + 3.0;
+    for (int u = TILE_16; u < t; u++) {
+      const double us = time(t, rows) + time(u, p.M - rows) + 2.0;
       if (us < 0.97 * least) least = us, best = {t, (int)rows, u};
     }
   }
@@ -814,14 +798,20 @@ int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, 
   if (epi) g.rtype += row0;
   p.M = rows;
   if (ot == T_F32) switch (tile) {
+      case TILE_16: return run_ksplit<KTile<HALF, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
+      case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 4, 2>>(g, p, ot, epi, stream, err);
       case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
+      case TILE_80: return run_ksplit<KTile<HALF, 80, 64, 4, 2>>(g, p, ot, epi, stream, err);
       case TILE_128: return run_tile<Tile<HALF, 128, 128>>(g, p, ot, epi, stream, err);
       default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, stream, err);
     }
   switch (tile) {
+    case TILE_16: return run_ksplit<KTile<E4M3, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
+    case TILE_48: return run_ksplit<KTile<E4M3, 48, 64, 4, 2>>(g, p, ot, epi, stream, err);
     case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
+    case TILE_80: return run_ksplit<KTile<E4M3, 80, 64, 4, 2>>(g, p, ot, epi, stream, err);
     case TILE_128: return run_tile<Tile<E4M3, 128, 128>>(g, p, ot, epi, stream, err);
     case TILE_256x128: return run_tile<Tile<E4M3, 256, 128>>(g, p, ot, epi, stream, err);
     default: return run_tile<Tile<E4M3, 256, 256>>(g, p, ot, epi, stream, err);
@@ -840,7 +830,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
   constexpr int MAX_STRIDE = 1 << 22;  // 256 rows of a tile then lie within 2^30 bytes
   const int nb = p.K > 0 ? (p.K - 1) / KB + 1 : 0;
   if (p.M < 0 || p.N < 1 || p.K < 16 || p.K % 16 || p.a_stride < p.K || p.w_stride < p.K || p.c_stride < p.N ||
-      p.a_stride % 16 || p.w_stride % 16 || p.a_stride > MAX_STRIDE || p.w_stride > MAX_STRIDE || p.groups < nb) {
+      p.a_stride % 16 || p.w_stride % 16 || p.a_stride > MAX_STRIDE || p.w_stride > MAX_STRIDE || p.groups < nb || p.groups > MAX_STRIDE / 4) {
     *err = "bad shape: M " + std::to_string(p.M) + " N " + std::to_string(p.N) + " K " + std::to_string(p.K) +
            " (a multiple of 16) a_stride " + std::to_string(p.a_stride) + " w_stride " + std::to_string(p.w_stride) +
            " (multiples of 16 up to 2^22) c_stride " + std::to_string(p.c_stride) + " scales a row " +
@@ -889,7 +879,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
                    has_bias ? (const float *)a[5].ptr : nullptr, epi ? (const unsigned char *)a[6].ptr : nullptr,
                    epi ? (const float *)a[7].ptr : nullptr, ntypes, vec};
   const Plan plan = pl.ival[0] ? Plan{pl.ival[0], p.M, 0} : make_plan(p, ot == T_F32);
-  const long side = plan.tile == TILE_32 ? 32 : plan.tile == TILE_64 ? 64 : 128;
+  const long side = plan.tile == TILE_16 ? 16 : plan.tile < TILE_128 ? 32 : 128;
   if (((p.M + side - 1) / side) * ((p.N + side - 1) / side) * 512 >= (1ll << 32)) {  // a grid holds less than 2^32 threads
     *err = "too many tiles: M " + std::to_string(p.M) + " N " + std::to_string(p.N);
     return -1;
@@ -900,9 +890,11 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
 
 }  // namespace
 
+// TILE (0: the plan's choice) names the tiles: 1 to 5 the 16 x 32, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 ones whose waves split
+// K, 6 to 8 128 x 128, 256 x 128 and 256 x 256 (256 x 128 again for float outputs).
 bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err) {
   if (tile < 0 || tile > TILE_LAST) {
-    *err = "TILE must be 0 to 5 with format f8";
+    *err = "TILE must be 0 to 8 with format f8";
     return false;
   }
   pl->launch = launch_f8;

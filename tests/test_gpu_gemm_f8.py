@@ -20,9 +20,9 @@ from oracle.bf16 import from_bf16, to_bf16
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
-# the plan's own choice, 32 x 32 and 64 x 64 tiles whose waves split K, 128 x 128, 256 x 128 and 256 x 256 tiles (256 x 128
-# again for float outputs)
-TILES = pytest.mark.parametrize("TILE", [0, 1, 2, 3, 4, 5], ids=["plan", "32", "64", "128", "256x128", "256"])
+# the plan's own choice; 16 x 32, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 tiles whose waves split K; 128 x 128, 256 x 128 and
+# 256 x 256 tiles (256 x 128 again for float outputs)
+TILES = pytest.mark.parametrize("TILE", range(9), ids=["plan", "16", "32", "48", "64", "80", "128", "256x128", "256"])
 
 
 def bound(mag, K, *values):
@@ -187,7 +187,7 @@ def test_same_call_same_bits(gpu, TILE):
     assert np.array_equal(run(gpu, *ops4, TILE=TILE, no_alloc=True), first)
 
 
-@pytest.mark.parametrize("TILE", [0, 3, 4, 5], ids=["plan", "128", "256x128", "256"])
+@pytest.mark.parametrize("TILE", [0, 6, 7, 8], ids=["plan", "128", "256x128", "256"])
 @pytest.mark.parametrize("M,N,K,out", [(4700, 4224, 1296, "bf16"), (2500, 4100, 400, "f32"), (5000, 2056, 128, "f16"),
                                        (4400, 2304, 272, "f32"), (4607, 4096, 640, "bf16")])
 def test_large_products_on_sampled_rows(gpu, M, N, K, out, TILE):
