@@ -9,7 +9,7 @@
 //    rot_q8's mode 1).
 //
 // amax passes over NaN; the code of NaN is NaN (e4m3) or 0 (int8). A block that holds an infinity has an infinite scale
-// and NaN at the infinity. Sums, maxima and products are float.
+// and NaN at the infinity; with the norm, whose root is then infinite, its scale is NaN and the row's other scales are 0. Sums, maxima and products are float.
 //
 // The row's root mean square R scales every value of a block and its amax alike, so v / s = (h w) 448 / amax|h w| does
 // not need it: the codes of a block are written at once and only the scales wait for the row's sum. So a row takes one
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
   using XE = typename Elem<XT>::type;
   using RE = typename Elem<RT>::type;
   constexpr int STEP = LPR * PL, HELD = I8 ? 4 : 1;  // int8: this many steps of a row stay in registers until its amax is known
-    extern __shared__ float tops[];  // e4m3: the blocks' largest magnitudes
+  extern __shared__ float tops[];  // e4m3: the blocks' largest magnitudes
   __shared__ float red[8];
   const int tid = threadIdx.x, lane = tid % LPR, wave = tid >> 6;
   const int nb = (p.D + FB - 1) / FB, end = nb * FB;
@@ -300,15 +300,16 @@ __device__ __forceinline__ float gated(float v, float g) {
   const float r = __builtin_amdgcn_rcpf(d);
   return v * (g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r));
 }
-// The same below GATE_MIN, where 1 + exp(gate) is 1: value gate exp(gate), from 2^64 exp(gate), a normal float down to
-// gates whose result no float holds.
+// The same below GATE_MIN, where 1 + exp(gate) is 1: value gate exp(gate), the exponential as the square of
+// 2^-64 (2^64 exp(gate / 2)), whose factors go to the value and the gate so that neither product leaves the normal floats
+// while the result is one, for values up to the largest.
 __device__ __forceinline__ float gated_low(float v, float g) {
   constexpr float L = 1.44269504088896340736f, L2 = 1.92596303e-8f, LN2 = 0.693147180559945309417f;
   const float t = g * L;
   const float lo = __builtin_fmaf(g, L2, __builtin_fmaf(g, L, -t));
-  const float e0 = __builtin_amdgcn_exp2f(t + 64.0f);
-  const float e = g > -200.0f ? __builtin_fmaf(e0, lo * LN2, e0) : 0.0f;
-  return v * g * e * 0x1p-64f;
+  const float h = __builtin_amdgcn_exp2f(fmaxf(t, -500.0f) * 0.5f + 64.0f);  // 0 from gates whose result no float holds
+  const float e = g > -300.0f ? __builtin_fmaf(lo, LN2, 1.0f) : 1.0f;
+  return v * 0x1p-90f * h * (g * h * 0x1p-38f) * e;
 }
 
 // b / nb for b < 2^28 as a product: magic = ceil(2^(32 + shift) / nb), 2^shift the power of two from nb / 16 on (nb = 1: b)

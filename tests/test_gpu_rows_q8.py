@@ -215,6 +215,9 @@ def test_nan_and_infinity(gpu):
     assert not (rest & 0x7F).any()
     h, c, s = norm_case(gpu, x, "f32", None, None, None, D, out="i8", norm=False)
     assert c[1, 5] == 0 and np.isinf(s[2, 0]) and np.isfinite(s[:2]).all()
+    h, c, s = norm_case(gpu, x, "f32", None, None, None, D)  # with the norm: the NaN's row, the infinity's
+    check_norm(x[:1], c[:1], s[:1], None, D, "f8")
+    assert np.isnan(s[1]).all() and np.array_equal(s[2, [0, 2]], [0, 0]) and np.isnan(s[2, 1])
 
 
 def test_no_rows(gpu):
@@ -307,6 +310,20 @@ def test_gate_ranges(gpu, lo, hi):
     x = np.concatenate([rng.uniform(0.1, 1, (M, D)) * 1e6, rng.uniform(lo, hi, (M, D))], 1)
     xf, c, s = gated_case(gpu, x, "f32", D)
     check_gated(xf, c, s, D)
+
+
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+@pytest.mark.parametrize("lo,hi", [(-90, -86), (-130, -90), (-170, -130)])
+def test_low_gates_of_huge_values(gpu, lo, hi, xt):
+    """value * gate alone passes the largest float, the exponential alone the smallest one."""
+    rng = np.random.default_rng(15)
+    M, D = 3, 384
+    x = np.concatenate([rng.uniform(0.1, 1, (M, D)) * 3.3e38, rng.uniform(lo, hi, (M, D))], 1)
+    xf, c, s = gated_case(gpu, x, xt, D)
+    check_gated(xf, c, s, D)
+    x[:, D:] = rng.uniform(-1000, -250, (M, D))  # no float holds these products: zeros
+    xf, c, s = gated_case(gpu, x, xt, D)
+    assert not (c & 0x7F).any() and np.all(s == 1)
 
 
 def test_gated_zero_nan_infinity(gpu):
