@@ -18,6 +18,7 @@
 #include "gemm_common.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 
 namespace h3 {
@@ -287,7 +288,8 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
   const int tend = xcd * per + min(xcd, rem) + per + (xcd < rem), tstep = ((int)gridDim.x - xcd + 7) >> 3;
   int tile = xcd * per + min(xcd, rem) + (blockIdx.x >> 3);
   if (tile >= tend) return;
-  const int nb = (p.K + KB - 1) / KB, ns = max(nb, 2);  // blocks, steps (a step past the blocks adds nothing)
+  const int nb = (p.K + KB - 1) / KB, ns = max(nb, 2);  // blocks, steps (a step past the blocks adds nothing: its scales are 0,
+  // whatever the last block's are)
 
   struct At {
     int m0, n0;
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
   auto load_scales = [&](int buf) __attribute__((always_inline)) {
     if (tid < TM)
       for (int b = 0; b < ns; b++)
-        scales[buf * (C::SCALES / 4) + 4 * tid + b] = g.sa[(size_t)min(m0 + tid, p.M - 1) * p.groups + min(b, nb - 1)];
+        scales[buf * (C::SCALES / 4) + 4 * tid + b] = b < nb ? g.sa[(size_t)min(m0 + tid, p.M - 1) * p.groups + b] : 0.0f;
   };
   auto scales_of = [&](int n) { return (Scalars)(g.sw + (size_t)min((n + WTN * wn) / KB, (p.N - 1) / KB) * p.groups); };
 
@@ -425,7 +427,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
           dma_scales((kt >> 2) + 1, ((kt >> 2) + 1 + sphase) & 1);
         }
         kl = kl >= ns ? kl - ns : kl;
-        snext = last ? swn[0] : sw[min(nx, nb - 1)];
+        snext = last ? swn[0] : nx < nb ? sw[nx] : 0.0f;
       };
       // slot n of the 2 MI NM behind the meeting: its share of the loads
       auto load_some = [&](int n) __attribute__((always_inline)) {
@@ -635,7 +637,7 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
   // landed) run beside the matrix instructions of step s.
   auto step = [&](int s, const Ops &cur, Ops &nxt) __attribute__((always_inline)) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const float swk = sw[min(s * NWK + w, nb - 1)];
+    const float swk = s * NWK + w < nb ? sw[s * NWK + w] : 0.0f;  // (a block past K adds nothing)
     dma(s + NST);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
     read_ops(nxt, s + 1);
@@ -701,24 +703,24 @@ enum { TILE_16 = 1, TILE_32, TILE_48, TILE_64, TILE_80, TILE_128, TILE_256x128, 
 
 // Once for each kernel and device: its workgroups may have `bytes` of LDS
 template <class K>
-int set_lds(K kern, int bytes, uint64_t *done, std::string *err) {
+int set_lds(K kern, int bytes, std::atomic<uint64_t> &done, std::string *err) {
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
-  if (e == hipSuccess && dev < 64 && *done >> dev & 1) return 0;
+  if (e == hipSuccess && dev < 64 && done >> dev & 1) return 0;
   if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) {
     *err = std::string("hipFuncSetAttribute: ") + hipGetErrorString(e);
     return -1;
   }
-  if (dev < 64) *done |= 1ull << dev;
+  if (dev < 64) done |= 1ull << dev;
   return 0;
 }
 
 template <class C>
 int run_ksplit(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_t stream, std::string *err) {
   auto kern = gemm_f8_ksplit<C>;
-  static uint64_t done = 0;
-  if (set_lds(kern, C::LDS, &done, err)) return -1;
+  static std::atomic<uint64_t> done{0};
+  if (set_lds(kern, C::LDS, done, err)) return -1;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
   hipLaunchKernelGGL(kern, dim3((unsigned)(ntm * ntn)), dim3(C::NWK * 64), C::LDS, stream, g, p, ntm, ot, epi);
   return 0;
@@ -727,8 +729,8 @@ int run_ksplit(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStrea
 template <class C>
 int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_t stream, std::string *err) {
   auto kern = gemm_f8_tile<C>;
-  static uint64_t done = 0;
-  if (set_lds(kern, C::LDS, &done, err)) return -1;
+  static std::atomic<uint64_t> done{0};
+  if (set_lds(kern, C::LDS, done, err)) return -1;
   const int ntm = (p.M + C::TM - 1) / C::TM, ntn = (p.N + C::TN - 1) / C::TN;
   const int cus = cu_count(), slots = (cus > 0 ? cus : 256) * C::PER_CU;
   hipLaunchKernelGGL(kern, dim3((unsigned)std::min(ntm * ntn, slots)), dim3(C::NW * 64), C::LDS, stream, g, p, ntm, ntn, ot, epi);
@@ -751,6 +753,12 @@ constexpr Cost HALF_COST[] = {{}, {16, 32, 1.7, 1.77, 0.0697, 0, 1e9}, {32, 32, 
                               {48, 64, 0.6, 3.22, 0.215, 0, 1e9}, {64, 64, 0.4, 4.04, 0.279, 0, 1e9}, {80, 64, 0.8, 4.84, 0.315, 0, 1e9},
                               {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
 
+// the tiles that cover a product of `rows` rows and N columns
+long tiles_of(const Cost &c, long rows, long N) { return ((rows + c.tm - 1) / c.tm) * ((N + c.tn - 1) / c.tn); }
+
+// a grid holds less than 2^32 threads
+bool grid_fits(const Cost &c, long rows, long N) { return tiles_of(c, rows, N) < (1l << 32) / 512; }
+
 // The tiles of a product, and of its last rows where those take others (`rows`: those of `tile`).
 struct Plan {
   int tile, rows, tail;
@@ -760,10 +768,10 @@ Plan make_plan(const GemmParams &p, bool half) {
   const int cus = cu_count() > 0 ? cu_count() : 256;
   const Cost *cost = half ? HALF_COST : E4M3_COST;
   const double nb = (p.K + KB - 1) / KB;
-  auto tiles = [&](int t, long rows) { return ((rows + cost[t].tm - 1) / cost[t].tm) * (((long)p.N + cost[t].tn - 1) / cost[t].tn); };
   auto time = [&](int t, long rows) {
     const Cost &c = cost[t];
-    const long n = tiles(t, rows), rounds = (n + cus - 1) / cus;
+    if (!grid_fits(c, rows, p.N)) return 1e30;
+    const long n = tiles_of(c, rows, p.N), rounds = (n + cus - 1) / cus;
     const double us = c.pair == 0 ? rounds * (c.fixed + c.per_block * nb)
                                   : (rounds / 2) * (2 * c.fixed + c.pair * nb) + (rounds % 2) * (c.fixed + c.per_block * nb);
     return c.launch + std::max(us, 2e-6 * rows * p.N * p.K / c.rate);
@@ -777,7 +785,7 @@ Plan make_plan(const GemmParams &p, bool half) {
   // whole rounds of large tiles, and the rows of what is left of a round on smaller ones
   for (int t = TILE_128; t <= TILE_LAST; t++) {
     const long ntn = ((long)p.N + cost[t].tn - 1) / cost[t].tn;
-    const long rows = tiles(t, p.M) / cus * cus / ntn * cost[t].tm;
+    const long rows = tiles_of(cost[t], p.M, p.N) / cus * cus / ntn * cost[t].tm;
     if (rows <= 0 || rows >= p.M) continue;
     for (int u = TILE_16; u < t; u++) {
       const double us = time(t, rows) + time(u, p.M - rows) + 2.0;
@@ -829,7 +837,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
   memcpy(&p, params, sizeof p);
   constexpr int MAX_STRIDE = 1 << 22;  // 256 rows of a tile then lie within 2^30 bytes
   const int nb = p.K > 0 ? (p.K - 1) / KB + 1 : 0;
-  if (p.M < 0 || p.N < 1 || p.K < 16 || p.K % 16 || p.a_stride < p.K || p.w_stride < p.K || p.c_stride < p.N ||
+  if (p.M < 0 || p.M > (1 << 30) || p.N < 1 || p.N > (1 << 30) || p.K < 16 || p.K % 16 || p.a_stride < p.K || p.w_stride < p.K || p.c_stride < p.N ||
       p.a_stride % 16 || p.w_stride % 16 || p.a_stride > MAX_STRIDE || p.w_stride > MAX_STRIDE || p.groups < nb || p.groups > MAX_STRIDE / 4) {
     *err = "bad shape: M " + std::to_string(p.M) + " N " + std::to_string(p.N) + " K " + std::to_string(p.K) +
            " (a multiple of 16) a_stride " + std::to_string(p.a_stride) + " w_stride " + std::to_string(p.w_stride) +
@@ -872,15 +880,26 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
     }
     ntypes = (int)std::min<uint64_t>(256, (a[7].avail / 4 - N) / p.g_stride + 1);
   }
-  // 16-byte accesses to whole groups of 8 columns of the output, the residual's gates and the bias
+  // one workgroup reads what another writes, so the output shares no memory with the inputs (of the gates, whose rows
+  // the types choose, the first row is looked at)
+  struct Range { int i; uint64_t bytes; const char *what; };
+  const uint64_t out_bytes = ((M - 1) * p.c_stride + N) * osz;
+  for (const Range &r : {Range{0, (M - 1) * p.a_stride + p.K, "a"}, {1, (N - 1) * p.w_stride + p.K, "w"},
+                         {2, ((NB - 1) * p.groups + nb) * 4, "sw"}, {3, ((M - 1) * p.groups + nb) * 4, "sa"},
+                         {5, has_bias ? N * 4 : 0, "bias"}, {6, epi ? M : 0, "rtype"}, {7, epi ? N * 4 : 0, "gate"}})
+    if (r.bytes && a[r.i].ptr < a[4].ptr + out_bytes && a[4].ptr < a[r.i].ptr + r.bytes) {
+      *err = std::string("out shares memory with ") + r.what;
+      return -1;
+    }
+  // 16-byte accesses to whole groups of 8 columns of the output and the residual's gates
   auto al16 = [](const void *q) { return (uintptr_t)q % 16 == 0; };
   const bool vec = al16(a[4].ptr) && p.c_stride * osz % 16 == 0 && p.N % 8 == 0 && (!epi || (al16(a[7].ptr) && p.g_stride % 4 == 0));
   const GemmArgs g{a[0].ptr, a[1].ptr, (const float *)a[2].ptr, (const float *)a[3].ptr, a[4].ptr,
                    has_bias ? (const float *)a[5].ptr : nullptr, epi ? (const unsigned char *)a[6].ptr : nullptr,
                    epi ? (const float *)a[7].ptr : nullptr, ntypes, vec};
   const Plan plan = pl.ival[0] ? Plan{pl.ival[0], p.M, 0} : make_plan(p, ot == T_F32);
-  const long side = plan.tile == TILE_16 ? 16 : plan.tile < TILE_128 ? 32 : 128;
-  if (((p.M + side - 1) / side) * ((p.N + side - 1) / side) * 512 >= (1ll << 32)) {  // a grid holds less than 2^32 threads
+  const Cost *cost = ot == T_F32 ? HALF_COST : E4M3_COST;
+  if (!grid_fits(cost[plan.tile], plan.rows, p.N)) {
     *err = "too many tiles: M " + std::to_string(p.M) + " N " + std::to_string(p.N);
     return -1;
   }

@@ -241,8 +241,10 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
     if wt.fmt == "q8" and sa is None:
         raise ValueError("gemm: int8 activations need their row scales sa")
     if f8:
-        if sa is None or wt.sw is None or wt.G != 128:
-            raise ValueError("gemm: e4m3 operands need their scales sa and sw, for blocks of 128")
+        if sa is None or wt.sw is None or wt.G != 128 or (sa.dtype, wt.sw.dtype, wt.w.dtype) != ("f32", "f32", "f8"):
+            raise ValueError("gemm: e4m3 operands need their f32 scales sa and sw, for blocks of 128")
+        if epi and out.dtype != "f32":
+            raise ValueError(f"gemm: the residual must be f32, got {out.dtype}")
         tm = 1
     out_t = OUT_DT[out.dtype] if epi == 0 else "float"
     k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=out_t, HAS_BIAS=int(wt.bias is not None), **variant) if f8 else \

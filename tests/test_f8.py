@@ -129,8 +129,10 @@ def test_gemm_launcher_f8():
     assert pi == 8 and args == [a, wt.w, wt.sw, sa, out, None, None, None]
     assert struct.unpack("<8i", params) == (9, 1001, 2000, 2000, 1001, 2000, 16, 1001)
     for bad in (dict(a=T((9, 2000), "i8")), dict(sa=None), dict(wt=ops.QWeight("f8", wt.w, None, 1001, 2000)),
-                dict(wt=ops.QWeight("f8", wt.w, wt.sw, 1001, 2000, G=64)), dict(ksplit=2)):
-        k = dict(a=a, sa=sa, wt=wt, ksplit=1) | bad
+                dict(wt=ops.QWeight("f8", wt.w, wt.sw, 1001, 2000, G=64)), dict(ksplit=2), dict(sa=T((9, 16), "f16")),
+                dict(wt=ops.QWeight("f8", T((1001, 2000), "i8"), wt.sw, 1001, 2000)), dict(epi=1, out=T((9, 1001), "bf16")),
+                dict(wt=ops.QWeight("f8", wt.w, T((8, 16), "bf16"), 1001, 2000))):
+        k = dict(a=a, sa=sa, wt=wt, ksplit=1, epi=0, out=out) | bad
         with pytest.raises(ValueError, match="gemm|split"):
-            ops.gemm(g, k["a"], k["wt"], out, 9, sa=k["sa"], ksplit=k["ksplit"])
+            ops.gemm(g, k["a"], k["wt"], k["out"], 9, sa=k["sa"], ksplit=k["ksplit"], epi=k["epi"])
     assert len(g.launches) == 1

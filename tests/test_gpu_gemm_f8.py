@@ -178,6 +178,26 @@ def test_nan_stays_in_its_row(gpu, M, out, TILE):
 
 
 @TILES
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [96, 128, 400, 1040])
+def test_infinite_last_scales(gpu, K, out, TILE):
+    """An infinite scale of K's last block gives infinities of the block sum's sign, not NaN, in its row and its columns."""
+    rng = np.random.default_rng(16)
+    M, N = 21, 140
+    a, sa, w, sw = operands(rng, M, N, K)
+    a[:, -1], w[:, -1] = 0x38, 0x38
+    block = orq.product(a[:, (K - 1) // 128 * 128:], np.ones((M, 1)), w[:, (K - 1) // 128 * 128:], np.ones((2, 1)))[0]
+    clean = run(gpu, a, sa, w, sw, out=out, TILE=TILE)
+    sa[3, -1] = sw[1, -1] = np.inf
+    got = run(gpu, a, sa, w, sw, out=out, TILE=TILE)
+    far = np.abs(block) > 0.1  # (the sums' own error is far smaller)
+    hit = np.zeros((M, N), bool)
+    hit[3], hit[:, 128:] = True, True
+    assert np.array_equal(got[hit & far], np.copysign(np.inf, block)[hit & far])
+    assert np.array_equal(got[~hit], clean[~hit])
+
+
+@TILES
 def test_same_call_same_bits(gpu, TILE):
     """Two calls, and the allocation-free entry point, give the same bits: sums have a fixed order."""
     rng = np.random.default_rng(6)
@@ -289,6 +309,8 @@ def test_refusals(gpu):
                       (dict(M=7, a=gpu.empty((M * K,), "f8").view((7, K), offset_elems=8)), "aligned"),
                       (dict(o=x, epi=1), "rtype"), (dict(o=x, epi=1, rtype=rt), "gate"),
                       (dict(o=x, epi=1, rtype=gpu.empty((M - 1,), "u8"), gate=gate), "rtype needs"),
-                      (dict(o=x, epi=1, rtype=rt, gate=gate, g_stride=128), "g_stride"), (dict(TILE=9), "TILE")):
+                      (dict(o=x, epi=1, rtype=rt, gate=gate, g_stride=128), "g_stride"), (dict(TILE=9), "TILE"),
+                      (dict(o=a.view((4, N), "bf16"), M=4), "shares memory"), (dict(o=w.view((M, N), "bf16")), "shares memory"),
+                      (dict(o=x, epi=1, rtype=rt, gate=x.view((1, N))), "shares memory")):
         with pytest.raises(GpuError, match=what):
             call(**bad)
