@@ -557,8 +557,8 @@ LaunchFn pick(int epi, int ot, bool bias) {
 
 }  // namespace
 
-// Macros (those of h3metal/ops.py:161-164): WFMT (1 q8, 4 f16, 5 bf16, 6 h8; 9 f8 is this build's, gemm_f8.hip), EPI (0 or 1), OUT_T (half | bfloat |
-// float; float for EPI 1), HAS_BIAS. The reference's tile and layout choices TM, TN, NSG, G, SWZ, FAST_LAYOUT
+// Macros (those of h3metal/ops.py:161-164): WFMT (1 q8, 4 f16, 5 bf16, 6 h8; and 9 f8, which has no counterpart there:
+// gemm_f8.hip), EPI (0 or 1), OUT_T (half | bfloat | float; float for EPI 1), HAS_BIAS. The reference's tile and layout choices TM, TN, NSG, G, SWZ, FAST_LAYOUT
 // are accepted and unused (this kernel's tiles are its own); LORA must be 0. TILE (this build's, default 0: what is
 // estimated fastest) names the tiles at every size: 1 to 4 the 32 x 32, 64 x 64, 96 x 64 and (16-bit activations)
 // 96 x 128 tiles whose waves split K, 5 128 x 128, 6 256 x 256 and their tail launch.

@@ -132,7 +132,7 @@ def rot_q8(gpu: Gpu, x: Tensor, out: Tensor, sa: Tensor | None, M: int, D: int, 
 def rms_norm_q8(gpu: Gpu, x: Tensor, w: Tensor | None, out: Tensor, scale: Tensor, M: int, D: int, *, eps: float,
                 res: Tensor | None = None, res_out: Tensor | None = None, norm: bool = True,
                 x_stride: int | None = None, res_stride: int | None = None, res_out_stride: int | None = None,
-                o_stride: int | None = None):
+                o_stride: int | None = None, no_alloc: bool = False):
     """The residual's addition, the RMS norm of its rows and their rounding to 8 bits, in front of a projection:
 
       h = res + x, rounded to res's type and written to res_out (default: res itself); h = x without res
@@ -143,7 +143,8 @@ def rms_norm_q8(gpu: Gpu, x: Tensor, w: Tensor | None, out: Tensor, scale: Tenso
 
     x [M][x_stride], res [M][res_stride], res_out [M][res_out_stride] f16 / bf16 / f32 (res_out as res), w [D] f32, out
     [M][o_stride] f8 / i8; any D up to 2^20, any stride from D. The sum may take the place of res, or of x if that has its
-    type and stride. amax passes over NaN, whose code is NaN (f8) or 0 (i8)."""
+    type and stride; out, scale and res_out share memory with nothing else. amax passes over NaN, whose code is NaN (f8) or 0
+    (i8). no_alloc: dispatch through the allocation-free entry point (h3_dispatch_static)."""
     if out.dtype not in ("f8", "i8") or scale.dtype != "f32":
         raise ValueError(f"rms_norm_q8: out must be f8 or i8 and scale f32, got {out.dtype}, {scale.dtype}")
     if w is not None and w.dtype != "f32":
@@ -161,20 +162,20 @@ def rms_norm_q8(gpu: Gpu, x: Tensor, w: Tensor | None, out: Tensor, scale: Tenso
     k = gpu.kernel("ops", "rms_norm_q8", IN_T=OUT_DT[x.dtype], RES_T="none" if res is None else OUT_DT[res.dtype],
                    OUT_T=out.dtype)
     params = pack("6ifi", M, D, x_stride or D, res_stride or D, res_out_stride or D, o_stride or D, eps, int(norm))
-    gpu.launch(k, None, None, [x, res, w, out, scale, res_out], params)
+    gpu.launch(k, None, None, [x, res, w, out, scale, res_out], params, no_alloc=no_alloc)
 
 
 def swiglu_f8(gpu: Gpu, x: Tensor, out: Tensor, scale: Tensor, M: int, D: int, *, x_stride: int | None = None,
-              o_stride: int | None = None):
+              o_stride: int | None = None, no_alloc: bool = False):
     """value * silu(gate), value in columns 0..D-1 and gate in D..2D-1 of x, as e4m3 codes with a scale for each row and
     block of 128 columns (the last may be short): s = amax / 448, or 1 where amax is 0, codes e4m3(v / s).
     x [M][x_stride] f16 / bf16 / f32, out [M][o_stride] f8, scale [M][ceil(D / 128)] f32; any D up to 2^20. The
-    rotated int8 form with one scale a row is rot_q8(swiglu=True)."""
+    rotated int8 form with one scale a row is rot_q8(swiglu=True). no_alloc: as rms_norm_q8's."""
     if x.dtype not in OUT_DT or out.dtype != "f8" or scale.dtype != "f32":
         raise ValueError(f"swiglu_f8: x must be f16, bf16 or f32, out f8 and scale f32, got {x.dtype}, {out.dtype}, "
                          f"{scale.dtype}")
     k = gpu.kernel("ops", "swiglu_f8", IN_T=OUT_DT[x.dtype])
-    gpu.launch(k, None, None, [x, out, scale], pack("4i", M, D, x_stride or 2 * D, o_stride or D))
+    gpu.launch(k, None, None, [x, out, scale], pack("4i", M, D, x_stride or 2 * D, o_stride or D), no_alloc=no_alloc)
 
 
 @dataclass
@@ -209,12 +210,14 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
       f16 / bf16: A and W half / bfloat, v = a_m . w_n
       f8:  A e4m3 [M][K] with scales sa[M][ceil(K / 128)], W e4m3, v = the sum over blocks b of 128 of K of
            sa[m][b] * sw[n / 128][b] * (a_m . w_n over b). K a multiple of 16, any N; exactly M rows of A are read and
-           of out written (the other formats take rows padded to tile[0])
+           of out written (the other formats take rows padded to tile[0]), and out shares memory with no input.
+           Float outputs are float sums of exact products; 16-bit ones take the 8-bit matrix instruction, whose sums of
+           128 products are off by about 1.5e-5
 
     ksplit: accumulate over that many consecutive slices of K in separate dispatches (epi 1 only), as the
     reference does. tile / swz are the Metal kernel's tile choices: checked as the reference checks them (the
     tile width must divide N) and otherwise unused (the gfx950 kernels have tiles of their own, chosen by the size, and
-    cover any N). variant: TILE names those tiles (csrc/gemm.hip: make_gemm).
+    cover any N). variant: TILE names those tiles (csrc/gemm.hip: make_gemm; csrc/gemm_f8.hip: make_gemm_f8).
     no_alloc: dispatch through the allocation-free entry point (h3_dispatch_static); the h8 format's widened
     weights then live in its fixed scratch array."""
     if wt.fmt not in GEMM_ACT:

@@ -13,7 +13,7 @@ import numpy as np
 import pytest
 
 from h3metal_amd import f8, ops
-from h3metal_amd.gpu import GpuError
+from h3metal_amd.gpu import Gpu, GpuError
 from oracle import rows_q8 as orq
 from oracle.bf16 import from_bf16, to_bf16
 
@@ -269,6 +269,47 @@ def test_feed_forward(gpu, M, D, F):
     p, mag = orq.product(b, sb, w2, s2)
     want = h + gate[rt].astype(np.float64) * p
     assert np.all(np.abs(Y.numpy() - want) <= bound(mag, F) + 2 * U * (np.abs(p) + np.abs(want)))
+
+
+def test_run_in_two_contexts_at_once(gpu):
+    """Norm, product, gated unit and product queued on two contexts' streams, one of them through the allocation-free entry
+    point, three times in turn: the bits of a run alone."""
+    rng = np.random.default_rng(17)
+    M, D, F = 300, 512, 640
+    print(f"[feed-forward] two contexts M={M} D={D} F={F}", flush=True)
+    x = to_bf16(rng.standard_normal((M, D)).astype(np.float32))
+    w1, s1 = f8.block_codes((rng.standard_normal((2 * F, D)) / np.sqrt(D)).astype(np.float32))
+    w2, s2 = f8.block_codes((rng.standard_normal((D, F)) / np.sqrt(F)).astype(np.float32))
+
+    def state(g):
+        return dict(x=g.upload(x, "bf16"), a=g.empty((M, D), "f8"), sa=g.empty((M, 4), "f32"), w1=weight(g, w1, s1),
+                    h=g.empty((M, 2 * F), "bf16"), b=g.empty((M, F), "f8"), sb=g.empty((M, 5), "f32"), w2=weight(g, w2, s2),
+                    o=g.empty((M, D), "f32"))
+
+    def queue(g, t, no_alloc):
+        ops.rms_norm_q8(g, t["x"], None, t["a"], t["sa"], M, D, eps=1e-6, no_alloc=no_alloc)
+        ops.gemm(g, t["a"], t["w1"], t["h"], M, sa=t["sa"], no_alloc=no_alloc)
+        ops.swiglu_f8(g, t["h"], t["b"], t["sb"], M, F, no_alloc=no_alloc)
+        ops.gemm(g, t["b"], t["w2"], t["o"], M, sa=t["sb"], no_alloc=no_alloc)
+
+    first = state(gpu)
+    queue(gpu, first, False)
+    gpu.wait()
+    want = first["o"].numpy()
+    other = Gpu()
+    second = state(other)
+    try:
+        for _ in range(3):
+            first["o"].write(np.zeros((M, D), np.float32))
+            second["o"].write(np.zeros((M, D), np.float32))
+            queue(gpu, first, False)
+            queue(other, second, True)
+            gpu.wait()
+            other.wait()
+            assert np.array_equal(first["o"].numpy(), want) and np.array_equal(second["o"].numpy(), want)
+    finally:
+        second.clear()  # its buffers are freed before their context
+        other.close()
 
 
 def test_int8_rows_feed_the_int8_product(gpu):
