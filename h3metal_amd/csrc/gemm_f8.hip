@@ -785,14 +785,15 @@ Plan make_plan(const GemmParams &p, bool half) {
     const double us = time(t, p.M);
     if (us < least) least = us, best = {t, p.M, 0};
   }
-  // whole rounds of large tiles, and the rows of what is left of a round on smaller ones
+  // whole rounds of large tiles, and the rows of what is left of a round on smaller ones, where that gains over 3%
+  least *= 0.97;
   for (int t = TILE_128; t <= TILE_LAST; t++) {
     const long ntn = ((long)p.N + cost[t].tn - 1) / cost[t].tn;
     const long rows = tiles_of(cost[t], p.M, p.N) / cus * cus / ntn * cost[t].tm;
     if (rows <= 0 || rows >= p.M) continue;
     for (int u = TILE_16; u < t; u++) {
       const double us = time(t, rows) + time(u, p.M - rows) + 2.0;
-      if (us < 0.97 * least) least = us, best = {t, (int)rows, u};
+      if (us < least) least = us, best = {t, (int)rows, u};
     }
   }
   return best;
