@@ -11,8 +11,8 @@
 // rounding is 1.7e-3 (bf16) or 2.1e-4 (f16), take the 8-bit instruction; float outputs, the residual's among them, the half
 // one, at half its rate.
 //
-// What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 747 to 797 us by box, 2.1 to 2.3 PFLOP/s at
-// 1.6 GHz with the matrix unit busy 56% of the time; all-zero operands 604 us; the instruction loop alone, operands in
+// What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 750 to 790 us by card, 2.2 PFLOP/s at
+// 1.6 to 1.8 GHz with the matrix unit busy 55% of the time; all-zero operands 604 us; the instruction loop alone, operands in
 // registers, 3.5 PFLOP/s), for float outputs the vector instructions as well (2 conversions and an add for each matrix
 // instruction). Few tiles: the L2 -> LDS stream of the operands and the start and end of the launch.
 #include "gemm_common.h"
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
 
 // Wave w multiplies the whole TM x TN tile over blocks w, w + NWK, ... from LDS slots of its own, filled NST blocks ahead; no
 // wave waits for another before the end, where the partial tiles meet in LDS and are added in the order of the waves. Heights
-// from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 18.4 us in 64 rows, 13.1 in 80).
+// from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 18.4 us in 64 rows, 12.9 in 80).
 template <int MODE_, int TM_, int TN_, int NWK_, int NST_>
 struct KTile {
   static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NWK = NWK_, NST = NST_, MI = TM / 16, NJ = TN / 16;

@@ -221,6 +221,28 @@ def test_large_products_on_sampled_rows(gpu, M, N, K, out, TILE):
     check(got[rows], a[rows], sa[rows], w, sw, out)
 
 
+@pytest.mark.parametrize("TILE", [0, 6, 7], ids=["plan", "128", "256x128"])
+def test_large_residual_form_on_sampled_rows(gpu, TILE):
+    """The last rows, on smaller tiles in the plan's choice, take their own row types and rows of X."""
+    rng = np.random.default_rng(18)
+    M, N, K = 4607, 4096, 1040
+    a, sa, w, sw = operands(rng, M, N, K)
+    x, gate = rng.standard_normal((M, N)).astype(np.float32), rng.standard_normal((3, N)).astype(np.float32)
+    rt = rng.integers(0, 3, M).astype(np.uint8)
+    X = gpu.upload(x)
+    print(f"[gemm f8] residual M={M} N={N} K={K} TILE={TILE}", flush=True)
+    ops.gemm(gpu, gpu.upload(a, "f8"), weight(gpu, w, sw), X, M, sa=gpu.upload(sa), epi=1, rtype=gpu.upload(rt),
+             gate=gpu.upload(gate), **(dict(TILE=TILE) if TILE else {}))
+    gpu.wait()
+    rows = np.r_[0:3, 255:258, 2047:2050, 4090:4100, M - 130:M - 125, M - 2:M]
+    v, mag = orq.product(a[rows], sa[rows], w, sw)
+    g = gate[rt[rows]].astype(np.float64)
+    want = x[rows] + g * v
+    tol = np.abs(g) * bound(mag, K) + 2 * U * (np.abs(g * v) + np.abs(want))
+    got = X.numpy()[rows]
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
 def test_output_past_32_bit_offsets(gpu):
     """Output rows whose element offsets pass 2^31."""
     rng = np.random.default_rng(8)
