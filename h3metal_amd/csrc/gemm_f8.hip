@@ -563,15 +563,16 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
 
 // Wave w multiplies the whole TM x TN tile over blocks w, w + NWK, ... from LDS slots of its own, filled NST blocks ahead; no
 // wave waits for another before the end, where the partial tiles meet in LDS and are added in the order of the waves. Heights
-// from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 18.4 us in 64 rows, 12.9 in 80).
+// from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 17.0 us in 64 rows, 11.6 in 80).
+// The tiles of 48 rows and more have one slot for each of 8 waves, two on a SIMD: while one waits for its loads and reads the
+// other multiplies (4 waves of two slots: the same 300 rows 12.5 us, to float 17.8 instead of 14.9).
 template <int MODE_, int TM_, int TN_, int NWK_, int NST_>
 struct KTile {
   static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NWK = NWK_, NST = NST_, MI = TM / 16, NJ = TN / 16;
   static constexpr int NS = (TM + 63) / 64;                   // loads of the A rows' scales
   static constexpr int SLOT = (TM + TN) * KB + NS * 256;      // a block's rows of A and W, and the scales
   static constexpr int LPS = (TM + TN) / 8 + NS;              // loads per slot
-  static constexpr int RS = TN * 4 + 16;
-  static constexpr int LDS = NWK * (NST * SLOT > TM * RS ? NST * SLOT : TM * RS);
+  static constexpr int LDS = NWK * (NST * SLOT > TM * TN * 4 ? NST * SLOT : TM * TN * 4);
   static_assert(KB % TN == 0 && LDS <= 160 * 1024 && (NST - 1) * LPS <= 63, "tile configuration");
 };
 
@@ -636,14 +637,7 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
 #pragma unroll
     for (int i = 0; i < MI; i++) o.sa[i] = *(const float *)(q + 64 * i);
   };
-  // Step s: its operands are in registers (cur), so its slot is free and takes step s + NST; the reads of step s + 1 (once
-  // landed) run beside the matrix instructions of step s.
-  auto step = [&](int s, const Ops &cur, Ops &nxt) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const float swk = s * NWK + w < nb ? sw[s * NWK + w] : 0.0f;  // (a block past K adds nothing)
-    dma(s + NST);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
-    read_ops(nxt, s + 1);
+  auto multiply = [&](const Ops &cur, float swk) __attribute__((always_inline)) {
     Operand<MODE> a[MI];
     float sc[MI];
 #pragma unroll
@@ -665,23 +659,49 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
         for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(t[i][e], sc[i], acc[i][j][e]);
     }
   };
+  auto weight_scale = [&](int s) { return s * NWK + w < nb ? sw[s * NWK + w] : 0.0f; };  // (a block past K adds nothing)
+  // Step s: its operands are in registers (cur), so its slot is free and takes step s + NST; the reads of step s + 1 (once
+  // landed) run beside the matrix instructions of step s.
+  auto step = [&](int s, const Ops &cur, Ops &nxt) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const float swk = weight_scale(s);
+    dma(s + NST);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
+    read_ops(nxt, s + 1);
+    multiply(cur, swk);
+  };
 #pragma unroll
   for (int s = 0; s < NST; s++) dma(s);
-  Ops o0, o1;
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
-  read_ops(o0, 0);
-  for (int s = 0; s < steps; s += 2) {
-    step(s, o0, o1);
-    if (s + 1 < steps) step(s + 1, o1, o0);
+  if constexpr (NST == 1) {
+    // one slot a wave and two waves a SIMD: a wave's loads and reads run beside the other's multiplications
+    for (int s = 0; s < steps; s++) {
+      Ops o;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      read_ops(o, s);
+      const float swk = weight_scale(s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      dma(s + 1);
+      multiply(o, swk);
+    }
+  } else {
+    Ops o0, o1;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * C::LPS) : "memory");
+    read_ops(o0, 0);
+    for (int s = 0; s < steps; s += 2) {
+      step(s, o0, o1);
+      if (s + 1 < steps) step(s + 1, o1, o0);
+    }
   }
+  // 16-byte piece c of row r of a partial tile: 16 rows' writes of one piece, and reads of a row, cover all banks
+  constexpr int PPR = TN / 4;
+  auto sum_at = [](int r, int c) { return (r * PPR + (c ^ (r * TN / 64 & (PPR - 1)))) * 16; };
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < MI; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) *(f32x4 *)(smem + (w * TM + 16 * i + l16) * C::RS + (16 * j + 4 * lg) * 4) = acc[i][j];
+    for (int j = 0; j < NJ; j++) *(f32x4 *)(smem + w * (TM * TN * 4) + sum_at(16 * i + l16, 4 * j + lg)) = acc[i][j];
   __syncthreads();
-  constexpr int PPR = TN / 4;
   const int nl = 4 * (tid % PPR), n = n0 + nl;
   if (n >= p.N) return;
 #pragma unroll 1
@@ -691,7 +711,7 @@ __global__ __launch_bounds__(C::NWK * 64) void gemm_f8_ksplit(GemmArgs g, GemmPa
     float v[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int u = 0; u < NWK; u++) {
-      const f32x4 d = *(const f32x4 *)(smem + (u * TM + ml) * C::RS + nl * 4);
+      const f32x4 d = *(const f32x4 *)(smem + u * (TM * TN * 4) + sum_at(ml, nl / 4));
 #pragma unroll
       for (int r = 0; r < 4; r++) v[r] += d[r];
     }
@@ -744,16 +764,16 @@ int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_
 // per_block * blocks of K; or, where the card's power bounds it, the operations over `rate` (in 10^6 a microsecond) if that is
 // longer. pair: per block for two tiles at a time on a compute unit, where it holds two. Fitted to 13 row counts (1 to 4608) x
 // 4 N (128 to 12288) x 4 K (256 to 10240) for 16-bit and for float outputs; the plan's tiles were the fastest ones or within
-// 10% of them there, split rounds up to 30% faster than any one kind (4608 x 4096 x 10240 263 -> 197 us).
+// 10% of them there, split rounds up to 30% faster than any one kind (4608 x 4096 x 10240 254 -> 188 us).
 struct Cost {
   int tm, tn;
   double launch, fixed, per_block, pair, rate;
 };
 constexpr Cost E4M3_COST[] = {{}, {16, 32, 2.0, 1.66, 0.0646, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
-                              {48, 64, 0.3, 3.21, 0.157, 0, 1e9}, {64, 64, 0.0, 3.8, 0.188, 0, 1e9}, {80, 64, 0.0, 4.6, 0.225, 0, 1e9},
+                              {48, 64, 0.3, 3.1, 0.157, 0, 1e9}, {64, 64, 0.0, 3.8, 0.186, 0, 1e9}, {80, 64, 0.0, 4.3, 0.22, 0, 1e9},
                               {128, 128, 2.7, 1.35, 0.8, 1.3, 1540}, {256, 128, 1.4, 3.48, 0.936, 0, 1800}, {256, 256, 0.0, 6.6, 1.33, 0, 2200}};
 constexpr Cost HALF_COST[] = {{}, {16, 32, 1.7, 1.77, 0.0697, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
-                              {48, 64, 0.6, 3.22, 0.215, 0, 1e9}, {64, 64, 0.4, 4.04, 0.279, 0, 1e9}, {80, 64, 0.8, 4.84, 0.315, 0, 1e9},
+                              {48, 64, 0.6, 3.2, 0.195, 0, 1e9}, {64, 64, 0.4, 4.04, 0.25, 0, 1e9}, {80, 64, 0.4, 4.7, 0.3, 0, 1e9},
                               {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
 
 // the tiles that cover a product of `rows` rows and N columns
@@ -812,18 +832,18 @@ int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, 
   if (ot == T_F32) switch (tile) {
       case TILE_16: return run_ksplit<KTile<HALF, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
-      case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 4, 2>>(g, p, ot, epi, stream, err);
-      case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
-      case TILE_80: return run_ksplit<KTile<HALF, 80, 64, 4, 2>>(g, p, ot, epi, stream, err);
+      case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
+      case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 8, 1>>(g, p, ot, epi, stream, err);
+      case TILE_80: return run_ksplit<KTile<HALF, 80, 64, 8, 1>>(g, p, ot, epi, stream, err);
       case TILE_128: return run_tile<Tile<HALF, 128, 128>>(g, p, ot, epi, stream, err);
       default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, stream, err);
     }
   switch (tile) {
     case TILE_16: return run_ksplit<KTile<E4M3, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
-    case TILE_48: return run_ksplit<KTile<E4M3, 48, 64, 4, 2>>(g, p, ot, epi, stream, err);
-    case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 4, 2>>(g, p, ot, epi, stream, err);
-    case TILE_80: return run_ksplit<KTile<E4M3, 80, 64, 4, 2>>(g, p, ot, epi, stream, err);
+    case TILE_48: return run_ksplit<KTile<E4M3, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
+    case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 8, 1>>(g, p, ot, epi, stream, err);
+    case TILE_80: return run_ksplit<KTile<E4M3, 80, 64, 8, 1>>(g, p, ot, epi, stream, err);
     case TILE_128: return run_tile<Tile<E4M3, 128, 128>>(g, p, ot, epi, stream, err);
     case TILE_256x128: return run_tile<Tile<E4M3, 256, 128>>(g, p, ot, epi, stream, err);
     default: return run_tile<Tile<E4M3, 256, 256>>(g, p, ot, epi, stream, err);
