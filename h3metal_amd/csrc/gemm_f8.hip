@@ -564,8 +564,9 @@ __global__ __launch_bounds__(C::NW * 64) __attribute__((amdgpu_waves_per_eu(2 * 
 // Wave w multiplies the whole TM x TN tile over blocks w, w + NWK, ... from LDS slots of its own, filled NST blocks ahead; no
 // wave waits for another before the end, where the partial tiles meet in LDS and are added in the order of the waves. Heights
 // from 16 to 80 rows, so that few rows fill a round of the compute units (300 x 4096 x 4096: 17.0 us in 64 rows, 11.6 in 80).
+// The lowest tile has 16 columns, so that more compute units load the weight (1 x 20480 x 4096: 16.0 us, 17.3 with 32 columns).
 // The tiles of 48 rows and more have one slot for each of 8 waves, two on a SIMD: while one waits for its loads and reads the
-// other multiplies (4 waves of two slots: the same 300 rows 12.5 us, to float 17.8 instead of 14.9).
+// other multiplies (4 waves of two slots: 300 x 4096 x 4096 12.5 us instead of 11.6, to float 17.8 instead of 14.9).
 template <int MODE_, int TM_, int TN_, int NWK_, int NST_>
 struct KTile {
   static constexpr int MODE = MODE_, TM = TM_, TN = TN_, NWK = NWK_, NST = NST_, MI = TM / 16, NJ = TN / 16;
@@ -769,10 +770,10 @@ struct Cost {
   int tm, tn;
   double launch, fixed, per_block, pair, rate;
 };
-constexpr Cost E4M3_COST[] = {{}, {16, 32, 2.0, 1.66, 0.0646, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
+constexpr Cost E4M3_COST[] = {{}, {16, 16, 3.0, 0.6, 0.0625, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
                               {48, 64, 0.3, 3.1, 0.157, 0, 1e9}, {64, 64, 0.0, 3.8, 0.186, 0, 1e9}, {80, 64, 0.0, 4.3, 0.22, 0, 1e9},
                               {128, 128, 2.7, 1.35, 0.8, 1.3, 1540}, {256, 128, 1.4, 3.48, 0.936, 0, 1800}, {256, 256, 0.0, 6.6, 1.33, 0, 2200}};
-constexpr Cost HALF_COST[] = {{}, {16, 32, 1.7, 1.77, 0.0697, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
+constexpr Cost HALF_COST[] = {{}, {16, 16, 2.9, 0.4, 0.069, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
                               {48, 64, 0.6, 3.2, 0.195, 0, 1e9}, {64, 64, 0.4, 4.04, 0.25, 0, 1e9}, {80, 64, 0.4, 4.7, 0.3, 0, 1e9},
                               {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
 
@@ -830,7 +831,7 @@ int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, 
   if (epi) g.rtype += row0;
   p.M = rows;
   if (ot == T_F32) switch (tile) {
-      case TILE_16: return run_ksplit<KTile<HALF, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
+      case TILE_16: return run_ksplit<KTile<HALF, 16, 16, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
       case TILE_64: return run_ksplit<KTile<HALF, 64, 64, 8, 1>>(g, p, ot, epi, stream, err);
@@ -839,7 +840,7 @@ int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, 
       default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, stream, err);
     }
   switch (tile) {
-    case TILE_16: return run_ksplit<KTile<E4M3, 16, 32, 8, 2>>(g, p, ot, epi, stream, err);
+    case TILE_16: return run_ksplit<KTile<E4M3, 16, 16, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_48: return run_ksplit<KTile<E4M3, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
     case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 8, 1>>(g, p, ot, epi, stream, err);
@@ -933,7 +934,7 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
 
 }  // namespace
 
-// TILE (0: the plan's choice) names the tiles: 1 to 5 the 16 x 32, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 ones whose waves split
+// TILE (0: the plan's choice) names the tiles: 1 to 5 the 16 x 16, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 ones whose waves split
 // K, 6 to 8 128 x 128, 256 x 128 and 256 x 256 (256 x 128 again for float outputs).
 bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err) {
   if (tile < 0 || tile > TILE_LAST) {

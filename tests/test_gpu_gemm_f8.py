@@ -20,7 +20,7 @@ from oracle.bf16 import from_bf16, to_bf16
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
-# the plan's own choice; 16 x 32, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 tiles whose waves split K; 128 x 128, 256 x 128 and
+# the plan's own choice; 16 x 16, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 tiles whose waves split K; 128 x 128, 256 x 128 and
 # 256 x 256 tiles (256 x 128 again for float outputs)
 TILES = pytest.mark.parametrize("TILE", range(9), ids=["plan", "16", "32", "48", "64", "80", "128", "256x128", "256"])
 
