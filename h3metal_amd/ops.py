@@ -23,6 +23,7 @@ specialisations.
 
 from __future__ import annotations
 
+import struct
 from dataclasses import dataclass, replace
 
 from .gpu import Gpu, Tensor, pack
@@ -32,6 +33,8 @@ FMT_ID = {"q8": 1, "q4": 2, "q4g": 3, "f16": 4, "bf16": 5, "h8": 6, "h4": 7, "h4
           "f8": 9}
 GEMM_ACT = {"q8": "i8", "h8": "f16", "f16": "f16", "bf16": "bf16", "f8": "f8"}  # the formats built here and their activations
 LOG2E = 1.4426950408889634
+# parameter blocks of calls whose time is their host work
+_PACK_8I, _PACK_6IFI, _PACK_4I = struct.Struct("<8i").pack, struct.Struct("<6ifi").pack, struct.Struct("<4i").pack
 
 
 def pad_rows(m: int, tile: int = 128) -> int:
@@ -161,7 +164,7 @@ def rms_norm_q8(gpu: Gpu, x: Tensor, w: Tensor | None, out: Tensor, scale: Tenso
                          + (f", {res.dtype}" if res is not None else ""))
     k = gpu.kernel("ops", "rms_norm_q8", IN_T=OUT_DT[x.dtype], RES_T="none" if res is None else OUT_DT[res.dtype],
                    OUT_T=out.dtype)
-    params = pack("6ifi", M, D, x_stride or D, res_stride or D, res_out_stride or D, o_stride or D, eps, int(norm))
+    params = _PACK_6IFI(M, D, x_stride or D, res_stride or D, res_out_stride or D, o_stride or D, eps, 1 if norm else 0)
     gpu.launch(k, None, None, [x, res, w, out, scale, res_out], params, no_alloc=no_alloc)
 
 
@@ -175,7 +178,7 @@ def swiglu_f8(gpu: Gpu, x: Tensor, out: Tensor, scale: Tensor, M: int, D: int, *
         raise ValueError(f"swiglu_f8: x must be f16, bf16 or f32, out f8 and scale f32, got {x.dtype}, {out.dtype}, "
                          f"{scale.dtype}")
     k = gpu.kernel("ops", "swiglu_f8", IN_T=OUT_DT[x.dtype])
-    gpu.launch(k, None, None, [x, out, scale], pack("4i", M, D, x_stride or 2 * D, o_stride or D), no_alloc=no_alloc)
+    gpu.launch(k, None, None, [x, out, scale], _PACK_4I(M, D, x_stride or 2 * D, o_stride or D), no_alloc=no_alloc)
 
 
 @dataclass
@@ -220,6 +223,9 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
     cover any N). variant: TILE names those tiles (csrc/gemm.hip: make_gemm; csrc/gemm_f8.hip: make_gemm_f8).
     no_alloc: dispatch through the allocation-free entry point (h3_dispatch_static); the h8 format's widened
     weights then live in its fixed scratch array."""
+    if wt.fmt == "f8":
+        return _gemm_f8(gpu, a, wt, out, M, sa, epi, rtype, gate, g_stride, c_stride, a_stride, ksplit, no_alloc, _low,
+                        variant)
     if wt.fmt not in GEMM_ACT:
         raise NotImplementedError(f"gemm: weight format {wt.fmt!r} is not built (q8, h8, f16, bf16, f8)")
     if a.dtype != GEMM_ACT[wt.fmt]:
@@ -238,25 +244,36 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
                  no_alloc=no_alloc, **variant)
         return
     tm, tn, nsg = tile
-    f8 = wt.fmt == "f8"
-    if wt.N % tn and not f8:
+    if wt.N % tn:
         raise ValueError(f"gemm tile {tile}: {tn} columns do not divide the product's {wt.N}")
     if wt.fmt == "q8" and sa is None:
         raise ValueError("gemm: int8 activations need their row scales sa")
-    if f8:
-        if sa is None or wt.sw is None or wt.G != 128 or (sa.dtype, wt.sw.dtype, wt.w.dtype) != ("f32", "f32", "f8"):
-            raise ValueError("gemm: e4m3 operands need their f32 scales sa and sw, for blocks of 128")
-        if epi and out.dtype != "f32":
-            raise ValueError(f"gemm: the residual must be f32, got {out.dtype}")
-        tm = 1
     out_t = OUT_DT[out.dtype] if epi == 0 else "float"
-    k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=out_t, HAS_BIAS=int(wt.bias is not None), **variant) if f8 else \
-        gpu.kernel("gemm", "gemm", WFMT=FMT_ID[wt.fmt], EPI=epi, OUT_T=out_t, TM=tm, TN=tn, NSG=nsg, G=wt.G,
+    k = gpu.kernel("gemm", "gemm", WFMT=FMT_ID[wt.fmt], EPI=epi, OUT_T=out_t, TM=tm, TN=tn, NSG=nsg, G=wt.G,
                    HAS_BIAS=int(wt.bias is not None), SWZ=swz, **variant)
     if wt.fmt == "h8":
         gpu.reserve_workspace(wt.N * wt.K * 2)  # the widened weights; grows (and waits) only the first time
     m_pad = (M + tm - 1) // tm * tm
-    params = pack("8i", m_pad, wt.N, wt.K, a_stride or wt.K, c_stride or wt.N, wt.w_stride,
-                  (wt.K + 127) // 128 if f8 else wt.K // wt.G, g_stride or wt.N)
+    params = pack("8i", m_pad, wt.N, wt.K, a_stride or wt.K, c_stride or wt.N, wt.w_stride, wt.K // wt.G,
+                  g_stride or wt.N)
     gpu.launch(k, None, None, [a, wt.w, wt.sw, sa, out, wt.bias, rtype, gate], params, params_index=8,
+               no_alloc=no_alloc)
+
+
+def _gemm_f8(gpu, a, wt, out, M, sa, epi, rtype, gate, g_stride, c_stride, a_stride, ksplit, no_alloc, low, variant):
+    """gemm with format f8. A call of few rows takes as long as its host work, so a right one meets few branches."""
+    w, sw, N, K = wt.w, wt.sw, wt.N, wt.K
+    if a.dtype != "f8" or w.dtype != "f8":
+        raise ValueError(f"gemm: format f8 takes f8 activations and codes, got {a.dtype}, {w.dtype}")
+    if sa is None or sw is None or sa.dtype != "f32" or sw.dtype != "f32" or wt.G != 128:
+        raise ValueError("gemm: e4m3 operands need their f32 scales sa and sw, for blocks of 128")
+    if wt.low is not None or low is not None:
+        raise NotImplementedError("gemm: low-rank (LoRA) terms are not built")
+    if ksplit > 1:
+        raise ValueError(f"cannot split K of a f8 product (epi {epi}, K {K}) {ksplit} ways")
+    if epi and out.dtype != "f32":
+        raise ValueError(f"gemm: the residual must be f32, got {out.dtype}")
+    k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=OUT_DT[out.dtype], HAS_BIAS=0 if wt.bias is None else 1, **variant)
+    gpu.launch(k, None, None, [a, w, sw, sa, out, wt.bias, rtype, gate],
+               _PACK_8I(M, N, K, a_stride or K, c_stride or N, wt.ws or K, (K + 127) // 128, g_stride or N), 8,
                no_alloc=no_alloc)
