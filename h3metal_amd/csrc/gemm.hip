@@ -561,23 +561,24 @@ LaunchFn pick(int epi, int ot, bool bias) {
 // gemm_f8.hip), EPI (0 or 1), OUT_T (half | bfloat | float; float for EPI 1), HAS_BIAS. The reference's tile and layout choices TM, TN, NSG, G, SWZ, FAST_LAYOUT
 // are accepted and unused (this kernel's tiles are its own); LORA must be 0. TILE (this build's, default 0: what is
 // estimated fastest) names the tiles at every size: 1 to 4 the 32 x 32, 64 x 64, 96 x 64 and (16-bit activations)
-// 96 x 128 tiles whose waves split K, 5 128 x 128, 6 256 x 256 and their tail launch.
+// 96 x 128 tiles whose waves split K, 5 128 x 128, 6 256 x 256 and their tail launch (format f8: see make_gemm_f8, which
+// also takes EXACT).
 bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err) {
   if (fn != "gemm") {
     *err = "unknown function (have: gemm)";
     return false;
   }
-  int wfmt, epi, hb, lora, tile, dummy;
+  int wfmt, epi, hb, lora, tile, exact, dummy;
   if (!macro_int(m, "WFMT", 1, &wfmt, err) || !macro_int(m, "EPI", 0, &epi, err) ||
       !macro_int(m, "HAS_BIAS", 0, &hb, err) || !macro_int(m, "LORA", 0, &lora, err) ||
-      !macro_int(m, "TILE", 0, &tile, err))
+      !macro_int(m, "TILE", 0, &tile, err) || !macro_int(m, "EXACT", 0, &exact, err))
     return false;
   for (const char *k : {"TM", "TN", "NSG", "G", "SWZ", "FAST_LAYOUT"})
     if (!macro_int(m, k, 0, &dummy, err)) return false;
   for (auto &kv : m) {
     static const char *known[] = {"WFMT", "EPI", "OUT_T", "HAS_BIAS", "LORA", "TM", "TN", "NSG", "G", "SWZ",
                                   "FAST_LAYOUT", "TILE"};
-    bool ok = false;
+    bool ok = wfmt == 9 && kv.first == "EXACT";
     for (const char *k : known) ok = ok || kv.first == k;
     if (!ok) {
       *err = "unknown macro " + kv.first;
@@ -602,7 +603,7 @@ bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string
     *err = "OUT_T must be half|bfloat|float (float with EPI 1)";
     return false;
   }
-  if (wfmt == 9) return make_gemm_f8(epi, ot, hb != 0, tile, pl, err);
+  if (wfmt == 9) return make_gemm_f8(epi, ot, hb != 0, tile, exact, pl, err);
   if (tile < 0 || tile > TILE_256 || (wfmt == 1 && tile == TILE_KSPLIT + KSPLIT_96x128)) {
     *err = "TILE must be 0 to 6, and not 4 (96 x 128) with int8 activations";
     return false;

@@ -9,7 +9,10 @@
 // bits below its exponent; sums of such groups are float. Random sums of 128 products are then 1.5e-5 off (2-norm), where
 // codes widened to half (exact: a half holds every e4m3 value) and the half instruction give 1.5e-8. 16-bit outputs, whose own
 // rounding is 1.7e-3 (bf16) or 2.1e-4 (f16), take the 8-bit instruction; float outputs, the residual's among them, the half
-// one, at half its rate.
+// one, at half its rate. A single product's 16-bit output hides the difference (1.66e-3 off in bf16 both ways), but 1.5% of its
+// bf16 values are the other neighbour, and where they are rounded to 8 bits again some fall to another code: 4608 rows through
+// 4096 -> 2 x 10240 -> 4096 (norm, product, gated unit, product) are 2.4e-3 from the same run with its sums in 64 bits, 1.7e-3
+// with exact sums in the first product (697 us and 987 us). The macro EXACT gives 16-bit outputs the half instruction.
 //
 // What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 750 to 790 us by card, 2.2 PFLOP/s at
 // 1.6 to 1.8 GHz with the matrix unit busy 55% of the time; all-zero operands 604 us; the instruction loop alone, operands in
@@ -37,7 +40,7 @@ __device__ __forceinline__ f16x8 widen(int lo, int hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// What a block's products are multiplied as (16-bit outputs, float outputs)
+// What a block's products are multiplied as (16-bit outputs; float outputs, and 16-bit ones with EXACT)
 enum { E4M3 = 0, HALF = 1 };
 
 // 16 x 16 sums of a block: lane l holds row l % 16's pieces 2 (l / 16) and 2 (l / 16) + 1; element e is that of W row
@@ -821,7 +824,7 @@ Plan make_plan(const GemmParams &p, bool half) {
 }
 
 // One launch on the product's rows from row0
-int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, int rows, int ot, int epi, hipStream_t stream,
+int run_tiles(int tile, bool half, const GemmArgs &all, const GemmParams &whole, int row0, int rows, int ot, int epi, hipStream_t stream,
               std::string *err) {
   GemmArgs g = all;
   GemmParams p = whole;
@@ -830,7 +833,7 @@ int run_tiles(int tile, const GemmArgs &all, const GemmParams &whole, int row0, 
   g.out += (size_t)row0 * p.c_stride * (ot == T_F32 ? 4 : 2);
   if (epi) g.rtype += row0;
   p.M = rows;
-  if (ot == T_F32) switch (tile) {
+  if (half) switch (tile) {
       case TILE_16: return run_ksplit<KTile<HALF, 16, 16, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
@@ -922,23 +925,29 @@ int launch_f8(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const
   const GemmArgs g{a[0].ptr, a[1].ptr, (const float *)a[2].ptr, (const float *)a[3].ptr, a[4].ptr,
                    has_bias ? (const float *)a[5].ptr : nullptr, epi ? (const unsigned char *)a[6].ptr : nullptr,
                    epi ? (const float *)a[7].ptr : nullptr, ntypes, vec};
-  const Plan plan = pl.ival[0] ? Plan{pl.ival[0], p.M, 0} : make_plan(p, ot == T_F32);
-  const Cost *cost = ot == T_F32 ? HALF_COST : E4M3_COST;
+  const bool half = ot == T_F32 || pl.ival[4];
+  const Plan plan = pl.ival[0] ? Plan{pl.ival[0], p.M, 0} : make_plan(p, half);
+  const Cost *cost = half ? HALF_COST : E4M3_COST;
   if (!grid_fits(cost[plan.tile], plan.rows, p.N)) {
     *err = "too many tiles: M " + std::to_string(p.M) + " N " + std::to_string(p.N);
     return -1;
   }
-  if (run_tiles(plan.tile, g, p, 0, plan.rows, ot, epi, ex.stream, err)) return -1;
-  return plan.tail ? run_tiles(plan.tail, g, p, plan.rows, p.M - plan.rows, ot, epi, ex.stream, err) : 0;
+  if (run_tiles(plan.tile, half, g, p, 0, plan.rows, ot, epi, ex.stream, err)) return -1;
+  return plan.tail ? run_tiles(plan.tail, half, g, p, plan.rows, p.M - plan.rows, ot, epi, ex.stream, err) : 0;
 }
 
 }  // namespace
 
 // TILE (0: the plan's choice) names the tiles: 1 to 5 the 16 x 16, 32 x 32, 48 x 64, 64 x 64 and 80 x 64 ones whose waves split
-// K, 6 to 8 128 x 128, 256 x 128 and 256 x 256 (256 x 128 again for float outputs).
-bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err) {
+// K, 6 to 8 128 x 128, 256 x 128 and 256 x 256 (256 x 128 again for float outputs and EXACT). EXACT 1: 16-bit outputs are
+// float sums of exact products, rounded once.
+bool make_gemm_f8(int epi, int out_t, bool bias, int tile, int exact, Pipeline *pl, std::string *err) {
   if (tile < 0 || tile > TILE_LAST) {
     *err = "TILE must be 0 to 8 with format f8";
+    return false;
+  }
+  if (exact != 0 && exact != 1) {
+    *err = "EXACT must be 0 or 1";
     return false;
   }
   pl->launch = launch_f8;
@@ -947,6 +956,7 @@ bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::st
   pl->ival[1] = epi;
   pl->ival[2] = out_t;
   pl->ival[3] = bias;
+  pl->ival[4] = exact;
   return true;
 }
 

@@ -113,7 +113,7 @@ bool make_ops(const std::string &fn, const Macros &m, Pipeline *pl, std::string 
 bool make_rot_q8(const Macros &m, Pipeline *pl, std::string *err);  // module "ops", function "rot_q8"
 bool make_rows_q8(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);  // rms_norm_q8, swiglu_f8
 bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
-bool make_gemm_f8(int epi, int out_t, bool bias, int tile, Pipeline *pl, std::string *err);  // weight format f8
+bool make_gemm_f8(int epi, int out_t, bool bias, int tile, int exact, Pipeline *pl, std::string *err);  // weight format f8
 
 // Wave64 lane exchanges inside a 32-lane half wave, shared by the row kernels: the value of lane (lane ^ S).
 // DPP for S = 1, 2 (quad_perm) and 8 (row_ror:8, a 16-lane rotation by 8), ds_swizzle's xor mode (no LDS

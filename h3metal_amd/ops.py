@@ -215,7 +215,9 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
            sa[m][b] * sw[n / 128][b] * (a_m . w_n over b). K a multiple of 16, any N; exactly M rows of A are read and
            of out written (the other formats take rows padded to tile[0]), and out shares memory with no input.
            Float outputs are float sums of exact products; 16-bit ones take the 8-bit matrix instruction, whose sums of
-           128 products are off by about 1.5e-5
+           128 products are off by about 1.5e-5: under their own rounding, but 16-bit values that are rounded to 8 bits
+           again (a feed-forward's first product) then take another code now and then. With EXACT=1 (a variant) they are
+           sums of exact products too, rounded once, at half the rate
 
     ksplit: accumulate over that many consecutive slices of K in separate dispatches (epi 1 only), as the
     reference does. tile / swz are the Metal kernel's tile choices: checked as the reference checks them (the

@@ -1,0 +1,79 @@
+"""ops.gemm with weight format f8 and EXACT=1: 16-bit outputs as float sums of exact products, rounded once, like the float
+outputs. The same tiles give the float output and the 16-bit one from the same sums, so these agree bit for bit."""
+
+import numpy as np
+import pytest
+
+from h3metal_amd import ops
+from h3metal_amd.gpu import GpuError
+from oracle import rows_q8 as orq
+from oracle.bf16 import from_bf16, to_bf16
+from test_gpu_gemm_f8 import operands, weight
+
+pytestmark = pytest.mark.gpu
+
+
+def product(gpu, a, sa, w, sw, out, bias=None, pads=(0, 0, 0), **variant):
+    """The bits of out [M][N]; A's, W's and the output's rows pads[0], pads[1], pads[2] columns apart; what lies behind
+    the output's rows stays."""
+    (M, K), N = a.shape, w.shape[0]
+    print(f"[gemm f8] M={M} N={N} K={K} out={out} bias={bias is not None} pads={pads} {variant}", flush=True)
+    rows = np.full((M, K + pads[0]), 0x7F, np.uint8)
+    rows[:, :K] = a
+    cs = N + pads[2]
+    raw = np.full((M + 2, cs), 3, {"f32": np.float32, "f16": np.float16, "bf16": np.uint16}[out])
+    O = gpu.upload(raw, out)
+    ops.gemm(gpu, gpu.upload(rows, "f8"), weight(gpu, w, sw, bias, K + pads[1] if pads[1] else None), O, M, sa=gpu.upload(sa),
+             a_stride=K + pads[0], c_stride=cs, **variant)
+    gpu.wait()
+    got = O.numpy()
+    res = got[:M, :N].copy()
+    got[:M, :N] = raw[:M, :N]
+    assert np.array_equal(got.view(np.uint8), raw.view(np.uint8)), "written past the rows"
+    return res
+
+
+def rounded(x, out):
+    return to_bf16(x) if out == "bf16" else x.astype(np.float16)
+
+
+@pytest.mark.parametrize("TILE", range(9), ids=["plan", "16", "32", "48", "64", "80", "128", "256x128", "256"])
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,bias,pads", [(1, 1, 16, False, (0, 0, 0)), (9, 1001, 400, True, (0, 0, 0)),
+                                             (70, 261, 336, True, (16, 48, 3)), (300, 512, 1040, False, (0, 0, 8)),
+                                             (520, 640, 128, True, (0, 0, 0))])
+def test_16_bit_outputs_are_rounded_float_outputs(gpu, M, N, K, bias, pads, out, TILE):
+    rng = np.random.default_rng(M + 7 * K)
+    ops4 = operands(rng, M, N, K)
+    b = rng.standard_normal(N).astype(np.float32) if bias else None
+    want = rounded(product(gpu, *ops4, "f32", b, pads, TILE=TILE), out)
+    got = product(gpu, *ops4, out, b, pads, TILE=TILE, EXACT=1)
+    assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+
+
+@pytest.mark.parametrize("TILE", [0, 6, 7], ids=["plan", "128", "256x128"])
+@pytest.mark.parametrize("M,N,K", [(4607, 4096, 640), (5000, 2056, 128), (4400, 2304, 272)])
+def test_large_products(gpu, M, N, K, TILE):
+    """Workgroups that take several tiles, and a last, partly filled round's rows on smaller ones."""
+    rng = np.random.default_rng(M)
+    ops4 = operands(rng, M, N, K)
+    want = rounded(product(gpu, *ops4, "f32", TILE=TILE), "bf16")
+    assert np.array_equal(product(gpu, *ops4, "bf16", TILE=TILE, EXACT=1), want)
+
+
+def test_sums_are_those_of_exact_products(gpu):
+    """Of 256 K outputs, those that are not the rounded float64 product. An error e of a row's values, in units of their
+    2-norm's mean, moves a normal value v over a tie of bf16 (2^-8 |v| apart at least) with probability min(1, c / |v|),
+    c = 2^8 e, which is 0.8 c (1 + ln(1 / c)) over all v. Float sums of about 20 additions are 2.5e-7 off or less
+    (20^0.5 steps of 2^-24): 5.5e-4 of the values; the 8-bit instruction's 1.5e-5 is more than ten times as many."""
+    rng = np.random.default_rng(21)
+    a, sa, w, sw = operands(rng, 256, 1024, 1024)
+    want = to_bf16(orq.product(a, sa, w, sw)[0].astype(np.float32))
+    off = np.mean(product(gpu, a, sa, w, sw, "bf16", EXACT=1) != want)
+    assert off <= 1e-3, off
+
+
+def test_refusals(gpu):
+    for macros in (dict(WFMT=9, EXACT=2), dict(WFMT=9, EXACT=-1), dict(WFMT=4, EXACT=1), dict(WFMT=1, EXACT=0)):
+        with pytest.raises(GpuError, match="EXACT"):
+            gpu.kernel("gemm", "gemm", **macros)
