@@ -228,7 +228,9 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
         }
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) dm = fmax(dm, __shfl_xor(dm, k));
-        if (dm > 0.0 && dm < (double)INFINITY)  // (float quotients of NaN and infinities are as they should be)
+        // The scale is made of the float mx: codes of a block whose products no float holds stay those of its floats, whatever
+        // the blocks beside it are. (Float quotients of NaN and infinities are as they should be.)
+        if (mx > 0.0f && mx < INFINITY)
 #pragma unroll
           for (int i = 0; i < PL; i++) y[i] = to_odd(d[i] * (double)F8_MAX / dm);
       }
