@@ -9,7 +9,11 @@
 //    rot_q8's mode 1).
 //
 // amax passes over NaN; the code of NaN is NaN (e4m3) or 0 (int8). A block that holds an infinity has an infinite scale
-// and NaN at the infinity; with the norm, whose root is then infinite, its scale is NaN and the row's other scales are 0. Sums, maxima and products are float.
+// and NaN at the infinity; with the norm, whose root is then infinite, its scale is NaN and the row's other scales are 0.
+//
+// Range. Sums, maxima and products are float. A row of rms_norm_q8 whose squares' sum or whose largest products (a block's,
+// for int8 the row's) pass out of 2^-100 .. the largest float is taken again in double, so any finite row and gain have the
+// codes and scales of the formula; an amax below the smallest float counts as 0. An int8 row of zeros takes that path too.
 //
 // The row's root mean square R scales every value of a block and its amax alike, so v / s = (h w) 448 / amax|h w| does
 // not need it: the codes of a block are written at once and only the scales wait for the row's sum. So a row takes one
@@ -139,6 +143,24 @@ __device__ __forceinline__ void store_codes(unsigned char *p, uint2 c, int n) {
   }
 }
 
+// The sum, or with MOST the largest, of LPR neighbouring lanes' values (LPR 256: of the workgroup's, through red), in each
+template <int LPR, bool MOST>
+__device__ __forceinline__ double over_row(double v, double *red) {
+  auto join = [](double a, double b) { return MOST ? fmax(a, b) : a + b; };
+#pragma unroll
+  for (int k = (LPR < 64 ? LPR : 64) / 2; k > 0; k >>= 1) v = join(v, __shfl_xor(v, k));
+  if constexpr (LPR > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = join(join(red[0], red[1]), join(red[2], red[3]));
+  }
+  return v;
+}
+
+// Floats from here on keep their products' and squares' sums exact to a float's steps: the square of what is lost below is
+// nothing beside it.
+constexpr float LOW = 0x1p-100f;
+
 struct NormArgs {
   const char *x, *res;
   const float *w;
@@ -156,6 +178,7 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
   constexpr int STEP = LPR * PL, HELD = I8 ? 4 : 1;  // int8: this many steps of a row stay in registers until its amax is known
   extern __shared__ float tops[];  // e4m3: the blocks' largest magnitudes
   __shared__ float red[8];
+  __shared__ double red2[8];
   const int tid = threadIdx.x, lane = tid % LPR, wave = tid >> 6;
   const int nb = (p.D + FB - 1) / FB, end = nb * FB;
   size_t m = (size_t)blockIdx.x * (256 / LPR) + tid / LPR;
@@ -213,7 +236,8 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
       mx = max16(mx);
       const Scale v = scale_of<448>(mx);
       float y[PL];
-      bool tie = v.up != 1.0f;
+      const bool out_of_range = !(mx >= LOW && mx < INFINITY);
+      bool tie = out_of_range;
 #pragma unroll
       for (int i = 0; i < PL; i++) {
         y[i] = t[i] * v.inv;
@@ -228,9 +252,10 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
         }
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) dm = fmax(dm, __shfl_xor(dm, k));
-        // The scale is made of the float mx: codes of a block whose products no float holds stay those of its floats, whatever
-        // the blocks beside it are. (Float quotients of NaN and infinities are as they should be.)
-        if (mx > 0.0f && mx < INFINITY)
+        // (float quotients of zeros, NaN and infinities are as they should be)
+        if (out_of_range) {
+          if (dm > 0.0 && dm < (double)INFINITY) sq = INFINITY;  // the row again
+        } else
 #pragma unroll
           for (int i = 0; i < PL; i++) y[i] = to_odd(d[i] * (double)F8_MAX / dm);
       }
@@ -260,16 +285,68 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
   } else {
     __syncthreads();  // the blocks' largest magnitudes are there
   }
-  const float r = p.norm ? 1.0f / sqrtf(sq / (float)p.D + p.eps) : 1.0f;
+  const float ms = sq / (float)p.D + p.eps;
+  if (!(sq < INFINITY) || (p.norm && ms < LOW) || (I8 && !(rowmax >= LOW && rowmax < INFINITY))) {
+    double s2 = 0.0, t2 = 0.0;
+    for (c = lane * PL; c < end; c += STEP) {
+      float h[PL], g[PL];
+      reload(c, h);
+      gain(c, g);
+#pragma unroll
+      for (int i = 0; i < PL; i++) {
+        s2 = __builtin_fma((double)h[i], (double)h[i], s2);
+        if constexpr (I8) t2 = fmax(t2, fabs((double)h[i] * g[i]));
+      }
+    }
+    s2 = over_row<LPR, false>(s2, red2);
+    if constexpr (I8) t2 = over_row<LPR, true>(t2, red2 + 4);
+    constexpr double CODES = I8 ? 127.0 : (double)F8_MAX;
+    const double r = p.norm ? 1.0 / sqrt(s2 / p.D + p.eps) : 1.0;
+    for (c = lane * PL; c < end; c += STEP) {
+      float h[PL], g[PL];
+      double d[PL], most = t2;
+      reload(c, h);
+      gain(c, g);
+#pragma unroll
+      for (int i = 0; i < PL; i++) {
+        d[i] = (double)h[i] * g[i];
+        if constexpr (!I8) most = fmax(most, fabs(d[i]));
+      }
+      if constexpr (!I8)
+#pragma unroll
+        for (int k = 8; k > 0; k >>= 1) most = fmax(most, __shfl_xor(most, k));
+      // a largest value below the smallest float is 0 (unless an infinite root made it so)
+      const bool none = !(most > 0.0) || (r > 0.0 && most * r < 0x1p-149), some = !none && most < (double)INFINITY;
+#pragma unroll
+      for (int i = 0; i < PL; i++) d[i] = some ? d[i] * CODES / most : d[i] * 0.0;  // NaN and infinities: NaN
+      if constexpr (I8) {
+        unsigned char q[PL];
+#pragma unroll
+        for (int i = 0; i < PL; i++) q[i] = d[i] == d[i] ? (unsigned char)(int)rint(d[i]) : 0;
+        if (there) store8(out + c, q, p.D - c);
+      } else {
+        float y[PL];
+#pragma unroll
+        for (int i = 0; i < PL; i++) y[i] = to_odd(d[i]);
+        if (there) store_codes(out + c, pack_f8(y), p.D - c);
+      }
+      if (there && (I8 ? c == 0 : (lane & 15) == 0)) a.scale[I8 ? m : m * nb + c / FB] = none ? 1.0f : (float)(most * r / CODES);
+    }
+    return;
+  }
+  const float r = p.norm ? 1.0f / sqrtf(ms) : 1.0f;
+  auto scaled = [&](float most, float codes) {  // (most * r alone may pass the largest float)
+    return most * r < INFINITY ? most * r / codes : most * (r / codes);
+  };
   if constexpr (!I8) {
     if (there)
-      for (int b = lane; b < nb; b += LPR) a.scale[m * nb + b] = top[b] > 0.0f ? top[b] * r / F8_MAX : 1.0f;
+      for (int b = lane; b < nb; b += LPR) a.scale[m * nb + b] = top[b] > 0.0f ? scaled(top[b], F8_MAX) : 1.0f;
   } else {
     const Scale v = scale_of<127>(rowmax);
     auto codes = [&](int c, const float (&t)[PL]) __attribute__((always_inline)) {
       unsigned char q[PL];
 #pragma unroll
-      for (int i = 0; i < PL; i++) q[i] = (unsigned char)(int)rintf(t[i] * v.up * v.inv);
+      for (int i = 0; i < PL; i++) q[i] = (unsigned char)(int)rintf(t[i] * v.inv);
       if (there) store8(out + c, q, p.D - c);
     };
     c = lane * PL;
@@ -284,7 +361,7 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
       for (int i = 0; i < PL; i++) h[i] *= g[i];
       codes(c, h);
     }
-    if (lane == 0 && there) a.scale[m] = rowmax > 0.0f ? rowmax * r / 127.0f : 1.0f;
+    if (lane == 0 && there) a.scale[m] = scaled(rowmax, 127.0f);
   }
 }
 

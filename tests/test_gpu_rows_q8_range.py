@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 
 from h3metal_amd import ops
+from oracle import rows_q8 as orq
+from test_gpu_rows_q8 import EXACT, U, check_codes, norm_case
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,59 @@ def test_a_block_does_not_depend_on_its_neighbours(gpu, h, g, D, norm):
         assert np.array_equal(s0[:, 0], s1[:, 0])
     if abs(h) * g < 1e-45:  # a float holds none of these values: zeros
         assert not (c1[:, :128] & 0x7F).any() and np.all(s1[:, 0] == 1)
+
+
+# Bounds of the checks: test_gpu_rows_q8.py's. A scale is off by its roundings and its sum's, and by 2^-149 where it is
+# subnormal; e4m3 codes are exactly rounded, int8 ones rounded from within 5 * 2^-24.
+CASES = [(h, 1.0, 0.0, True) for h in (1e-44, 1e-41, 3e-38, 1e-30, 3e-23, 1e-20, 1e-16, 1e-12, 1e15, 1e18, 3e19, 1e25, 3e38)] + [
+    (1e25, 1.0, 1e-6, True), (1e-30, 1e-20, 0.0, True), (1e-30, 1e20, 0.0, True), (1e25, 1e25, 1e-6, True),
+    (1e25, 1e-25, 1e-6, True), (1e-3, 1e-38, 1e-6, True), (1e-3, 3e38, 1e-6, True), (1e-20, 1e-20, 1e-6, False),
+    (3e25, 3e14, 1e-6, False), (1e15, 1e15, 1e-6, False), (1e-10, 1e-10, 1e-30, True)]
+
+
+@pytest.mark.parametrize("out", ["f8", "i8"])
+@pytest.mark.parametrize("D", [1, 200, 300, 4096, 16385])
+@pytest.mark.parametrize("hm,wm,eps,norm", CASES)
+def test_magnitudes(gpu, hm, wm, eps, norm, D, out):
+    """Rows and gains from the smallest floats to the largest, whose squares, their sum, products or largest quotient no
+    float holds."""
+    rng = np.random.default_rng(19)
+    M = 3
+    x = (rng.uniform(0.3, 1, (M, D)) * rng.choice([-1, 1], (M, D)) * hm).astype(np.float32)
+    w = (rng.uniform(0.3, 1, D) * wm).astype(np.float32)
+    h, c, s = norm_case(gpu, x, "f32", None, None, w, D, out=out, eps=eps, norm=norm)
+    check_range(h, c, s, w, D, out, eps, norm)
+
+
+def check_range(h, c, s, w, D, out, eps, norm):
+    v = orq.rms_norm(h, w, eps, norm)
+    top = orq.per_column(np.abs(orq.blocks(v)).max(-1), D) if out == "f8" else np.abs(v).max(-1, keepdims=True)
+    v = np.where(top < 2.0 ** -149, 0.0, v)  # an amax below the smallest float counts as 0
+    ws = orq.block_scales(v) if out == "f8" else orq.row_scales(v)[:, None]
+    tol = (6 + 0.5 * (D / 16 + 12)) * U
+    assert np.all(np.abs(s - ws) <= tol * ws + 2.0 ** -149), np.max(np.abs(s - ws) / ws)
+    if out == "f8":
+        check_codes(c, v / orq.per_column(ws, D), EXACT)
+    else:
+        q = v / ws
+        assert np.all((c >= np.rint(q - np.abs(q) * 5 * U)) & (c <= np.rint(q + np.abs(q) * 5 * U)))
+
+
+@pytest.mark.parametrize("out", ["f8", "i8"])
+@pytest.mark.parametrize("D", [256, 640, 4096])
+def test_magnitudes_side_by_side(gpu, D, out):
+    """Rows of every magnitude in one call, in bf16 with a residual, blocks of every magnitude in one row, and rows of zeros
+    between them."""
+    rng = np.random.default_rng(20)
+    mags = np.float32([1, 1e-30, 1e30, 0, 3e-23, 1e19, 1e-3, 0, 3e38, 1e-37])
+    M = len(mags)
+    x = rng.uniform(0.3, 1, (M, D)).astype(np.float32) * mags[:, None] / 2
+    w = np.ones(D, np.float32)
+    h, c, s = norm_case(gpu, x, "bf16", x / 2, "bf16", w, D, out=out, eps=0.0 if D == 640 else 1e-30, inplace=True)
+    live = mags > 0
+    check_range(h[live], c[live], s[live], w, D, out, 0.0 if D == 640 else 1e-30, True)
+    assert not (c[~live] & 0x7F).any() and np.all(s[~live] == 1)
+    w *= np.repeat(np.float32([1, 1e-30, 1e30, 1e-38, 3e38]), 128)[np.arange(D) % 640]
+    for norm in (True, False):
+        h, c, s = norm_case(gpu, rng.uniform(0.3, 1, (2, D)) * 1e-9, "f32", None, None, w, D, out=out, norm=norm)
+        check_range(h, c, s, w, D, out, 1e-6, norm)
