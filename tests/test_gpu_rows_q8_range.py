@@ -6,7 +6,8 @@ import pytest
 
 from h3metal_amd import ops
 from oracle import rows_q8 as orq
-from test_gpu_rows_q8 import EXACT, U, check_codes, norm_case
+from oracle.bf16 import from_bf16
+from test_gpu_rows_q8 import EXACT, U, as_type, check_codes, norm_case
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,54 @@ def test_magnitudes_side_by_side(gpu, D, out):
     for norm in (True, False):
         h, c, s = norm_case(gpu, rng.uniform(0.3, 1, (2, D)) * 1e-9, "f32", None, None, w, D, out=out, norm=norm)
         check_range(h, c, s, w, D, out, 1e-6, norm)
+
+
+def rounded_once(v, t):
+    """float64 rounded to bf16's 8 bits (values well inside its range) or to half; half to even."""
+    if t == "f16":
+        return v.astype(np.float16).astype(np.float64)
+    m, e = np.frexp(v)
+    return np.ldexp(np.rint(m * 256) / 256, e)
+
+
+@pytest.mark.parametrize("out", ["f8", "i8"])
+@pytest.mark.parametrize("rt,bits", [("bf16", 8), ("f16", 11)])
+def test_the_residuals_sum_is_rounded_once(gpu, rt, bits, out):
+    """A float x that takes a 16-bit residual beside the middle of two 16-bit values, by less than a float's step of the sum;
+    and sums of ordinary values."""
+    rng = np.random.default_rng(22)
+    M, D = 4, 600
+    rh, r = as_type(rng.uniform(1, 2, (M, D)) * rng.choice([-1, 1], (M, D)) * 2.0 ** rng.integers(-3, 4, (M, D)), rt)
+    ulp = 2.0 ** (np.floor(np.log2(np.abs(r))) - (bits - 1))  # a step of the residual
+    x = (ulp * (rng.choice([-1.5, -0.5, 0.5, 1.5], (M, D)) + rng.choice([-1, 0, 1], (M, D)) * 2.0 ** -20.0)).astype(np.float32)
+    x[3] = rng.standard_normal(D)
+    want = rounded_once(r.astype(np.float64) + x.astype(np.float64), rt)
+    twice = as_type(r + x, rt)[1].astype(np.float64)
+    assert np.mean(twice[:3] != want[:3]) > 0.1
+    print(f"[rms_norm_q8] {rt} residual of a float x, {out}", flush=True)
+    R, O, S = gpu.upload(rh, rt), gpu.empty((M, D), out), gpu.empty((M, 5 if out == "f8" else 1), "f32")
+    ops.rms_norm_q8(gpu, gpu.upload(x), None, O, S, M, D, eps=1e-6, res=R)
+    gpu.wait()
+    got = R.numpy()
+    got = (from_bf16(got) if rt == "bf16" else got).astype(np.float64)
+    assert np.array_equal(got, want), np.mean(got != want)
+    check_range(want, O.numpy(), S.numpy(), None, D, out, 1e-6, True)
+
+
+def test_sums_of_zeros_infinities_and_the_largest_values(gpu):
+    """Signs of zero, infinities, NaN, and sums that no float or no 16-bit value holds, as the float sum rounds them."""
+    big = np.float32(3.4028235e38)
+    r = np.float32([0.0, -0.0, 1.0, np.inf, -np.inf, np.inf, 3.3e38, -3.3e38, 65504, -65504, 65504, 1.0])
+    x = np.float32([-0.0, -0.0, -1.0, 1.0, np.inf, 2.0, big, -big, 16, -16, 8, np.nan])
+    for rt in ("bf16", "f16"):
+        rh, rf = as_type(r[None], rt)
+        with np.errstate(over="ignore", invalid="ignore"):
+            sh, want = as_type(rf + x[None], rt)
+        print(f"[rms_norm_q8] special sums {rt}", flush=True)
+        R = gpu.upload(rh, rt)
+        ops.rms_norm_q8(gpu, gpu.upload(x[None]), None, gpu.empty((1, 12), "f8"), gpu.empty((1, 1), "f32"), 1, 12, eps=1e-6, res=R)
+        gpu.wait()
+        got = R.numpy()
+        got = (from_bf16(got) if rt == "bf16" else got).astype(np.float32)
+        number = ~np.isnan(want)  # (a NaN's sign means nothing)
+        assert np.array_equal(got, want, equal_nan=True) and np.array_equal(np.signbit(got[number]), np.signbit(want[number]))
