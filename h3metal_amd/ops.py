@@ -273,9 +273,17 @@ def _gemm_f8(gpu, a, wt, out, M, sa, epi, rtype, gate, g_stride, c_stride, a_str
         raise NotImplementedError("gemm: low-rank (LoRA) terms are not built")
     if ksplit > 1:
         raise ValueError(f"cannot split K of a f8 product (epi {epi}, K {K}) {ksplit} ways")
-    if epi and out.dtype != "f32":
-        raise ValueError(f"gemm: the residual must be f32, got {out.dtype}")
-    k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=OUT_DT[out.dtype], HAS_BIAS=0 if wt.bias is None else 1, **variant)
-    gpu.launch(k, None, None, [a, w, sw, sa, out, wt.bias, rtype, gate],
+    bias = wt.bias
+    if bias is not None and bias.dtype != "f32":
+        raise ValueError(f"gemm: the bias must be f32, got {bias.dtype}")
+    if epi:
+        if out.dtype != "f32":
+            raise ValueError(f"gemm: the residual must be f32, got {out.dtype}")
+        if rtype is not None and rtype.dtype != "u8" or gate is not None and gate.dtype != "f32":
+            raise ValueError(f"gemm: rtype must be u8 and gate f32, got {rtype and rtype.dtype}, {gate and gate.dtype}")
+    elif out.dtype not in OUT_DT:
+        raise ValueError(f"gemm: out must be f16, bf16 or f32, got {out.dtype}")
+    k = gpu.kernel("gemm", "gemm", WFMT=9, EPI=epi, OUT_T=OUT_DT[out.dtype], HAS_BIAS=0 if bias is None else 1, **variant)
+    gpu.launch(k, None, None, [a, w, sw, sa, out, bias, rtype, gate],
                _PACK_8I(M, N, K, a_stride or K, c_stride or N, wt.ws or K, (K + 127) // 128, g_stride or N), 8,
                no_alloc=no_alloc)

@@ -136,3 +136,24 @@ def test_gemm_launcher_f8():
         with pytest.raises(ValueError, match="gemm|split"):
             ops.gemm(g, k["a"], k["wt"], k["out"], 9, sa=k["sa"], ksplit=k["ksplit"], epi=k["epi"])
     assert len(g.launches) == 1
+
+
+@pytest.mark.parametrize("bad", [dict(bias=T((1001,), "bf16")), dict(out=T((9, 1001), "f8")), dict(out=T((9, 1001), "i32")),
+                                 dict(epi=1, rtype=T((9,), "i32")), dict(epi=1, rtype=T((9,), "f32")),
+                                 dict(epi=1, gate=T((2, 1001), "bf16")), dict(epi=1, gate=T((2, 1001), "f16"))])
+def test_gemm_launcher_f8_refuses_other_types(bad):
+    """Buffers that the kernel would read or write as another type than theirs."""
+    g = FakeGpu()
+    k = dict(bias=T((1001,), "f32"), out=T((9, 1001), "f32"), epi=0, rtype=T((9,), "u8"), gate=T((2, 1001), "f32"))
+
+    def call(bias, out, **kw):
+        wt = ops.QWeight("f8", T((1001, 2000), "f8"), T((8, 16), "f32"), 1001, 2000, bias=bias)
+        ops.gemm(g, T((9, 2000), "f8"), wt, out, 9, sa=T((9, 16), "f32"), **kw)
+
+    call(**k)
+    call(**k | dict(epi=1))
+    call(**k | dict(out=T((9, 1001), "bf16")))
+    assert len(g.launches) == 3
+    with pytest.raises(ValueError, match="gemm"):
+        call(**k | bad)
+    assert len(g.launches) == 3
