@@ -77,3 +77,44 @@ def test_refusals(gpu):
     for macros in (dict(WFMT=9, EXACT=2), dict(WFMT=9, EXACT=-1), dict(WFMT=4, EXACT=1), dict(WFMT=1, EXACT=0)):
         with pytest.raises(GpuError, match="EXACT"):
             gpu.kernel("gemm", "gemm", **macros)
+
+
+def off(got, want):
+    return np.linalg.norm(got - want), np.linalg.norm(want)
+
+
+TILES = pytest.mark.parametrize("TILE", range(9), ids=["plan", "16", "32", "48", "64", "80", "128", "256x128", "256"])
+
+
+@TILES
+@pytest.mark.parametrize("M,N,K,bias", [(9, 130, 160, False), (77, 256, 1024, True), (300, 515, 256, False), (520, 640, 2064, True),
+                                        (4607, 1024, 640, False)])
+def test_residual_takes_exact_products(gpu, M, N, K, bias, TILE):
+    """X += gate[rtype] * (v + bias) in the 2-norm: 4e-6 of the added values (float sums are 1e-6 off or less, the 8-bit
+    instruction's 1.5e-5) and the roundings of gate * v and of the sum, half a float step each."""
+    rng = np.random.default_rng(M + K)
+    a, sa, w, sw = operands(rng, M, N, K)
+    b = rng.standard_normal(N).astype(np.float32) if bias else None
+    x, gate = rng.standard_normal((M, N)).astype(np.float32), rng.standard_normal((3, N)).astype(np.float32)
+    rt = rng.integers(0, 3, M).astype(np.uint8)
+    X = gpu.upload(x)
+    print(f"[gemm f8] residual M={M} N={N} K={K} bias={bias} TILE={TILE}", flush=True)
+    ops.gemm(gpu, gpu.upload(a, "f8"), weight(gpu, w, sw, b), X, M, sa=gpu.upload(sa), epi=1, rtype=gpu.upload(rt),
+             gate=gpu.upload(gate), TILE=TILE)
+    gpu.wait()
+    v = orq.product(a, sa, w, sw)[0]
+    added = gate[rt].astype(np.float64) * (v if b is None else v + b)
+    err, size = off(X.numpy(), x + added)
+    assert err <= 4e-6 * np.linalg.norm(gate[rt] * v) + 2.0 ** -24 * (2 * np.linalg.norm(added) + size), err / np.linalg.norm(added)
+
+
+@TILES
+@pytest.mark.parametrize("M,N,K", [(9, 1001, 400), (300, 512, 1040), (520, 640, 256)])
+def test_half_outputs_are_off_by_their_rounding(gpu, M, N, K, TILE):
+    """A half's rounding is 2^-11 / 3^0.5 of the values in the 2-norm at most; 1.5e-5 of the 8-bit instruction's sums and
+    2^-25 of subnormal halves beside it are under a twentieth of that."""
+    rng = np.random.default_rng(N)
+    ops4 = operands(rng, M, N, K)
+    for kw in ({}, dict(EXACT=1)):
+        err, size = off(product(gpu, *ops4, "f16", TILE=TILE, **kw).astype(np.float64), orq.product(*ops4)[0])
+        assert err <= 0.6 * 2.0 ** -11 * size, err / size
