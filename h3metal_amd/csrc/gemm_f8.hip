@@ -778,7 +778,7 @@ constexpr Cost E4M3_COST[] = {{}, {16, 16, 3.0, 0.6, 0.0625, 0, 1e9}, {32, 32, 0
                               {128, 128, 2.7, 1.35, 0.8, 1.3, 1540}, {256, 128, 1.4, 3.48, 0.936, 0, 1800}, {256, 256, 0.0, 6.6, 1.33, 0, 2200}};
 constexpr Cost HALF_COST[] = {{}, {16, 16, 2.9, 0.4, 0.069, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
                               {48, 64, 0.6, 3.2, 0.195, 0, 1e9}, {64, 64, 0.4, 4.04, 0.25, 0, 1e9}, {80, 64, 0.4, 4.7, 0.3, 0, 1e9},
-                              {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
+                              {128, 128, 1.4, 4.88, 1.074, 0, 870}, {256, 128, 0.0, 7.3, 1.6, 0, 1070}};
 
 // the tiles that cover a product of `rows` rows and N columns
 long tiles_of(const Cost &c, long rows, long N) { return ((rows + c.tm - 1) / c.tm) * ((N + c.tn - 1) / c.tn); }
@@ -794,6 +794,7 @@ struct Plan {
 Plan make_plan(const GemmParams &p, bool half) {
   const int cus = cu_count() > 0 ? cu_count() : 256;
   const Cost *cost = half ? HALF_COST : E4M3_COST;
+  const int last = half ? TILE_256x128 : TILE_256;
   const double nb = (p.K + KB - 1) / KB;
   auto time = [&](int t, long rows) {
     const Cost &c = cost[t];
@@ -805,13 +806,13 @@ Plan make_plan(const GemmParams &p, bool half) {
   };
   Plan best{TILE_16, p.M, 0};
   double least = time(TILE_16, p.M);
-  for (int t = TILE_32; t <= TILE_LAST; t++) {
+  for (int t = TILE_32; t <= last; t++) {
     const double us = time(t, p.M);
     if (us < least) least = us, best = {t, p.M, 0};
   }
   // whole rounds of large tiles, and the rows of what is left of a round on smaller ones, where that gains over 3%
   least *= 0.97;
-  for (int t = TILE_128; t <= TILE_LAST; t++) {
+  for (int t = TILE_128; t <= last; t++) {
     const long ntn = ((long)p.N + cost[t].tn - 1) / cost[t].tn;
     const long rows = tiles_of(cost[t], p.M, p.N) / cus * cus / ntn * cost[t].tm;
     if (rows <= 0 || rows >= p.M) continue;
@@ -950,6 +951,7 @@ bool make_gemm_f8(int epi, int out_t, bool bias, int tile, int exact, Pipeline *
     *err = "EXACT must be 0 or 1";
     return false;
   }
+  if ((out_t == T_F32 || exact) && tile == TILE_256) tile = TILE_256x128;  // the largest with the half instruction
   pl->launch = launch_f8;
   pl->threads = 512;
   pl->ival[0] = tile;
