@@ -213,7 +213,10 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
       f16 / bf16: A and W half / bfloat, v = a_m . w_n
       f8:  A e4m3 [M][K] with scales sa[M][ceil(K / 128)], W e4m3, v = the sum over blocks b of 128 of K of
            sa[m][b] * sw[n / 128][b] * (a_m . w_n over b). K a multiple of 16, any N; exactly M rows of A are read and
-           of out written (the other formats take rows padded to tile[0]), and out shares memory with no input.
+           of out written (the other formats take rows padded to tile[0]), and out shares memory with no input. Another
+           width D is a product of K = D rounded up to 16: the weight's codes padded with zero columns, A's rows K
+           apart (o_stride=K of rms_norm_q8 and swiglu_f8) in a buffer whose codes behind column D are zeros, as
+           Gpu.empty's are; the scales are those of D, which has as many blocks.
            Float outputs are float sums of exact products; 16-bit ones take the 8-bit matrix instruction, whose sums of
            128 products are off by about 1.5e-5: under their own rounding, but 16-bit values that are rounded to 8 bits
            again (a feed-forward's first product) then take another code now and then. With EXACT=1 (a variant) they are

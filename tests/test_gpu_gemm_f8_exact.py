@@ -4,11 +4,11 @@ outputs. The same tiles give the float output and the 16-bit one from the same s
 import numpy as np
 import pytest
 
-from h3metal_amd import ops
+from h3metal_amd import f8, ops
 from h3metal_amd.gpu import GpuError
 from oracle import rows_q8 as orq
 from oracle.bf16 import from_bf16, to_bf16
-from test_gpu_gemm_f8 import operands, weight
+from test_gpu_gemm_f8 import check, operands, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,32 @@ def test_half_outputs_are_off_by_their_rounding(gpu, M, N, K, TILE):
     for kw in ({}, dict(EXACT=1)):
         err, size = off(product(gpu, *ops4, "f16", TILE=TILE, **kw).astype(np.float64), orq.product(*ops4)[0])
         assert err <= 0.6 * 2.0 ** -11 * size, err / size
+
+
+@pytest.mark.parametrize("M,D,F", [(1, 200, 72), (37, 2632, 1001), (300, 517, 329)])
+def test_widths_that_are_no_multiple_of_16(gpu, M, D, F):
+    """Norm, product, gated unit, product, with K rounded up to 16: zero columns behind the weights' codes, rows K apart in
+    buffers that start as zeros. Each product against float64 of what it read; the zeros stay."""
+    rng = np.random.default_rng(D)
+    KD, KF = -(-D // 16) * 16, -(-F // 16) * 16
+    print(f"[feed-forward] widths M={M} D={D} F={F}", flush=True)
+
+    def codes(N, K, k):
+        c, s = f8.block_codes((rng.standard_normal((N, K)) / np.sqrt(K)).astype(np.float32))
+        return np.pad(c, ((0, 0), (0, k - K))), s
+
+    w1, s1 = codes(2 * F, D, KD)
+    w2, s2 = codes(D, F, KF)
+    x = to_bf16(rng.standard_normal((M, D)).astype(np.float32))
+    A, SA = gpu.empty((M, KD), "f8"), gpu.empty((M, -(-D // 128)), "f32")
+    H, B, SB = gpu.empty((M, 2 * F), "bf16"), gpu.empty((M, KF), "f8"), gpu.empty((M, -(-F // 128)), "f32")
+    O = gpu.empty((M, D), "f32")
+    ops.rms_norm_q8(gpu, gpu.upload(x, "bf16"), None, A, SA, M, D, eps=1e-6, o_stride=KD)
+    ops.gemm(gpu, A, weight(gpu, w1, s1), H, M, sa=SA)
+    ops.swiglu_f8(gpu, H, B, SB, M, F, o_stride=KF)
+    ops.gemm(gpu, B, weight(gpu, w2, s2), O, M, sa=SB)
+    gpu.wait()
+    a, b = A.numpy(), B.numpy()
+    assert not a[:, D:].any() and not b[:, F:].any()
+    check(from_bf16(H.numpy()).astype(np.float64), a[:, :D], SA.numpy(), w1[:, :D], s1, "bf16")
+    check(O.numpy().astype(np.float64), b[:, :F], SB.numpy(), w2[:, :F], s2, "f32")
