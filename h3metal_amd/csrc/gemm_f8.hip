@@ -12,7 +12,9 @@
 // one, at half its rate. A single product's 16-bit output hides the difference (1.66e-3 off in bf16 both ways), but 1.5% of its
 // bf16 values are the other neighbour, and where they are rounded to 8 bits again some fall to another code: 4608 rows through
 // 4096 -> 2 x 10240 -> 4096 (norm, product, gated unit, product) are 2.4e-3 from the same run with its sums in 64 bits, 1.7e-3
-// with exact sums in the first product (697 us and 987 us). The macro EXACT gives 16-bit outputs the half instruction.
+// with exact sums in the first product (697 us and 987 us). So the 8-bit instruction is taken only where it saves time: the
+// 16 x 16 tiles, bound by the weight's loads, take the half one for every output (1 x 12288 x 4096 to bf16 10.55 us both ways,
+// 1 x 20480 x 4096 15.9 and 15.7), and the macro EXACT gives it to all 16-bit outputs.
 //
 // What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 750 to 790 us by card, 2.2 PFLOP/s at
 // 1.6 to 1.8 GHz with the matrix unit busy 55% of the time; all-zero operands 604 us; the instruction loop alone, operands in
@@ -40,7 +42,7 @@ __device__ __forceinline__ f16x8 widen(int lo, int hi) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// What a block's products are multiplied as (16-bit outputs; float outputs, and 16-bit ones with EXACT)
+// What a block's products are multiplied as (16-bit outputs; float outputs, 16-bit ones of the smallest tiles and with EXACT)
 enum { E4M3 = 0, HALF = 1 };
 
 // 16 x 16 sums of a block: lane l holds row l % 16's pieces 2 (l / 16) and 2 (l / 16) + 1; element e is that of W row
@@ -773,7 +775,7 @@ struct Cost {
   int tm, tn;
   double launch, fixed, per_block, pair, rate;
 };
-constexpr Cost E4M3_COST[] = {{}, {16, 16, 3.0, 0.6, 0.0625, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
+constexpr Cost E4M3_COST[] = {{}, {16, 16, 2.7, 0.4, 0.069, 0, 1e9}, {32, 32, 0.6, 2.29, 0.0865, 0, 1e9},
                               {48, 64, 0.3, 3.1, 0.157, 0, 1e9}, {64, 64, 0.0, 3.8, 0.186, 0, 1e9}, {80, 64, 0.0, 4.3, 0.22, 0, 1e9},
                               {128, 128, 2.7, 1.35, 0.8, 1.3, 1540}, {256, 128, 1.4, 3.48, 0.936, 0, 1800}, {256, 256, 0.0, 6.6, 1.33, 0, 2200}};
 constexpr Cost HALF_COST[] = {{}, {16, 16, 2.9, 0.4, 0.069, 0, 1e9}, {32, 32, 1.1, 2.33, 0.0967, 0, 1e9},
@@ -834,7 +836,7 @@ int run_tiles(int tile, bool half, const GemmArgs &all, const GemmParams &whole,
   g.out += (size_t)row0 * p.c_stride * (ot == T_F32 ? 4 : 2);
   if (epi) g.rtype += row0;
   p.M = rows;
-  if (half) switch (tile) {
+  if (half || tile == TILE_16) switch (tile) {
       case TILE_16: return run_ksplit<KTile<HALF, 16, 16, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_32: return run_ksplit<KTile<HALF, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
       case TILE_48: return run_ksplit<KTile<HALF, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
@@ -844,7 +846,6 @@ int run_tiles(int tile, bool half, const GemmArgs &all, const GemmParams &whole,
       default: return run_tile<Tile<HALF, 256, 128>>(g, p, ot, epi, stream, err);
     }
   switch (tile) {
-    case TILE_16: return run_ksplit<KTile<E4M3, 16, 16, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_32: return run_ksplit<KTile<E4M3, 32, 32, 8, 2>>(g, p, ot, epi, stream, err);
     case TILE_48: return run_ksplit<KTile<E4M3, 48, 64, 8, 1>>(g, p, ot, epi, stream, err);
     case TILE_64: return run_ksplit<KTile<E4M3, 64, 64, 8, 1>>(g, p, ot, epi, stream, err);

@@ -73,6 +73,16 @@ def test_sums_are_those_of_exact_products(gpu):
     assert off <= 1e-3, off
 
 
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (9, 1001, 2000), (16, 512, 640)])
+def test_the_smallest_tiles_take_exact_products(gpu, M, N, K, out):
+    """They are bound by the weight's loads, so 16-bit outputs need no choice."""
+    rng = np.random.default_rng(K)
+    ops4 = operands(rng, M, N, K)
+    want = rounded(product(gpu, *ops4, "f32", TILE=1), out)
+    assert np.array_equal(product(gpu, *ops4, out, TILE=1).view(np.uint16), want.view(np.uint16))
+
+
 def test_refusals(gpu):
     for macros in (dict(WFMT=9, EXACT=2), dict(WFMT=9, EXACT=-1), dict(WFMT=4, EXACT=1), dict(WFMT=1, EXACT=0)):
         with pytest.raises(GpuError, match="EXACT"):
