@@ -18,8 +18,9 @@
 //
 // What bounds it. Large products: the card's power (16896 x 12288 x 4096 to bf16: 750 to 790 us by card, 2.2 PFLOP/s at
 // 1.6 to 1.8 GHz with the matrix unit busy 55% of the time; all-zero operands 604 us; the instruction loop alone, operands in
-// registers, 3.5 PFLOP/s), for float outputs the vector instructions as well (2 conversions and an add for each matrix
-// instruction). Few tiles: the L2 -> LDS stream of the operands and the start and end of the launch.
+// registers, 3.5 PFLOP/s). For float outputs neither unit alone: matrix units 47% and vector units 56% busy, 4096 x 4096 x
+// 10240 370 us; with all-zero operands 302 (power), and of these the adds' being left out saves 25, the widening's nothing.
+// Few tiles: the L2 -> LDS stream of the operands and the start and end of the launch.
 #include "gemm_common.h"
 
 #include <algorithm>
@@ -770,7 +771,7 @@ int run_tile(const GemmArgs &g, const GemmParams &p, int ot, int epi, hipStream_
 // per_block * blocks of K; or, where the card's power bounds it, the operations over `rate` (in 10^6 a microsecond) if that is
 // longer. pair: per block for two tiles at a time on a compute unit, where it holds two. Fitted to 13 row counts (1 to 4608) x
 // 4 N (128 to 12288) x 4 K (256 to 10240) for 16-bit and for float outputs; the plan's tiles were the fastest ones or within
-// 10% of them there, split rounds up to 30% faster than any one kind (4608 x 4096 x 10240 254 -> 188 us).
+// 10% of them there, split rounds up to 18% faster than any one kind (4608 x 4096 x 10240 236 -> 193 us, to float 430 -> 354).
 struct Cost {
   int tm, tn;
   double launch, fixed, per_block, pair, rate;

@@ -191,7 +191,8 @@ struct NormArgs {
 };
 
 // LPR lanes a row: 256 / LPR rows a workgroup. The e4m3 codes are the exactly rounded ones: where a float quotient is near a
-// tie (about one in a hundred of the waves' steps), its products and the largest of them are taken again in double.
+// tie or a subnormal code's (5% of the waves' steps on normal rows, 12% where every 64th column is 8 times larger), its
+// products and the largest of them are taken again in double.
 template <int XT, int RT, bool I8, int LPR>
 __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Params p) {
   using XE = typename Elem<XT>::type;

@@ -220,7 +220,8 @@ def gemm(gpu: Gpu, a: Tensor, wt: QWeight, out: Tensor, M: int, *, sa: Tensor | 
            Float outputs are float sums of exact products; 16-bit ones take the 8-bit matrix instruction, whose sums of
            128 products are off by about 1.5e-5: under their own rounding, but 16-bit values that are rounded to 8 bits
            again (a feed-forward's first product) then take another code now and then. With EXACT=1 (a variant) they are
-           sums of exact products too, rounded once, at half the rate; those of about 16 rows always are
+           sums of exact products too, rounded once, at half the rate; those of the smallest tiles (TILE=1), which most
+           products of up to 16 rows take, always are. sa * sw is a float: below 2^-126 it loses bits
 
     ksplit: accumulate over that many consecutive slices of K in separate dispatches (epi 1 only), as the
     reference does. tile / swz are the Metal kernel's tile choices: checked as the reference checks them (the
