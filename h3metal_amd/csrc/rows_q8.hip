@@ -14,6 +14,7 @@
 // Range. Sums, maxima and products are float. A row of rms_norm_q8 whose squares' sum or whose largest products (a block's,
 // for int8 the row's) pass out of 2^-100 .. the largest float is taken again in double, so any finite row and gain have the
 // codes and scales of the formula; an amax below the smallest float counts as 0. An int8 row of zeros takes that path too.
+// swiglu_f8's products stay floats: one past the largest is infinite, and of a gate below 2^-126 bits are lost.
 //
 // The row's root mean square R scales every value of a block and its amax alike, so v / s = (h w) 448 / amax|h w| does
 // not need it: the codes of a block are written at once and only the scales wait for the row's sum. So a row takes one
@@ -157,9 +158,9 @@ __device__ __forceinline__ double over_row(double v, double *red) {
   return v;
 }
 
-// a + b in float, rounded to odd. The float sum of a 16-bit residual and a float has up to 24 bits more than it keeps, and
-// its own rounding may make a tie of what the residual's type would round up or down (1 + (2^-8 + 2^-30) to bf16). Two 16-bit
-// values do not need it: no bit of theirs lies below a float's next to one that is half a step of the 16-bit sum.
+// a + b in float, rounded to odd. The sum of a 16-bit residual and a float has more bits than a float, whose rounding may make a
+// tie of what the residual's type would round up or down (1 + (2^-8 + 2^-30) to bf16). So may a half's sum with bf16, which has
+// fewer bits. Other pairs do not need it: neither value has a bit that is half a step of their sum next to values that far below.
 __device__ __forceinline__ float sum_to_odd(float a, float b) {
   const float s = a + b, t = s - a, e = (a - (s - t)) + (b - t);  // s + e is the sum, exactly
   unsigned u = __builtin_bit_cast(unsigned, s);
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(256) void rms_norm_q8_kernel(NormArgs a, NormQ8Para
       RE s[PL];
 #pragma unroll
       for (int i = 0; i < PL; i++) t[i] = r[i] + h[i];
-      if constexpr (XT == T_F32 && RT != T_F32) {
+      if constexpr ((XT == T_F32 && RT != T_F32) || (XT == T_F16 && RT == T_BF16)) {
         bool tie = false;
 #pragma unroll
         for (int i = 0; i < PL; i++) tie |= maybe_tie<RT>(t[i]);

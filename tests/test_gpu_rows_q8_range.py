@@ -133,6 +133,24 @@ def test_the_residuals_sum_is_rounded_once(gpu, rt, bits, out):
     check_range(want, O.numpy(), S.numpy(), None, D, out, 1e-6, True)
 
 
+def test_a_half_is_added_to_a_bf16_residual_with_one_rounding(gpu):
+    """Halves that are the middle of two bf16 values, beside residuals far below a float's step of the sum."""
+    rng = np.random.default_rng(23)
+    M, D = 3, 700
+    x = (rng.integers(128, 256, (M, D)) + 0.5) * 2.0 ** rng.integers(-12, 6, (M, D)) * rng.choice([-1, 1], (M, D))
+    xh, xf = as_type(x, "f16")
+    assert np.array_equal(xf, x)
+    rh, r = as_type(x * rng.choice([-1, 0, 1], (M, D)) * 2.0 ** rng.integers(-40, -26, (M, D)), "bf16")
+    want = rounded_once(r.astype(np.float64) + xf.astype(np.float64), "bf16")
+    assert np.mean(as_type(r + xf, "bf16")[1] != want) > 0.2
+    print("[rms_norm_q8] bf16 residual of a half x", flush=True)
+    R, O, S = gpu.upload(rh, "bf16"), gpu.empty((M, D), "f8"), gpu.empty((M, 6), "f32")
+    ops.rms_norm_q8(gpu, gpu.upload(xh), None, O, S, M, D, eps=1e-6, res=R)
+    gpu.wait()
+    assert np.array_equal(from_bf16(R.numpy()), want)
+    check_range(want, O.numpy(), S.numpy(), None, D, "f8", 1e-6, True)
+
+
 def test_sums_of_zeros_infinities_and_the_largest_values(gpu):
     """Signs of zero, infinities, NaN, and sums that no float or no 16-bit value holds, as the float sum rounds them."""
     big = np.float32(3.4028235e38)
