@@ -828,8 +828,8 @@ Plan make_plan(const GemmParams &p, bool half) {
 }
 
 // One launch on the product's rows from row0
-int run_tiles(int tile, bool half, const GemmArgs &all, const GemmParams &whole, int row0, int rows, int ot, int epi, hipStream_t stream,
-              std::string *err) {
+int run_tiles(int tile, bool half, const GemmArgs &all, const GemmParams &whole, int row0, int rows, int ot, int epi,
+              hipStream_t stream, std::string *err) {
   GemmArgs g = all;
   GemmParams p = whole;
   g.a += (size_t)row0 * p.a_stride;
