@@ -807,9 +807,10 @@ int type_of(const std::string &s) {
 // refused). SMALL (this build's) names the small tiles at every size, whichever
 // is faster: their 32-row query tiles per workgroup, 1, or 2 with HD 96.
 bool make_attention(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err) {
+  if (fn == "attention_paged") return make_attention_paged(m, pl, err);
   const bool dump = fn == "attention_scores";
   if (fn != "attention" && !dump) {
-    *err = "unknown function (have: attention, attention_scores)";
+    *err = "unknown function (have: attention, attention_scores, attention_paged)";
     return false;
   }
   int hd, qk8, causal, dummy;

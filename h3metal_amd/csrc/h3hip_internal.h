@@ -6,7 +6,8 @@
 //   QkRopeParams <- kernels/ops.metal:344-349, packed by h3metal/ops.py:237 ("8ifi")
 //   RotQParams   <- kernels/params.h:25-29, packed by h3metal/ops.py:221 ("4i")
 //   GemmParams   <- kernels/params.h:7-16, packed by h3metal/ops.py:165-166 ("8i")
-// NormQ8Params ("6ifi") and SwigluF8Params ("4i") have no counterpart there.
+// NormQ8Params ("6ifi"), SwigluF8Params ("4i"), PagedRopeParams ("11i2f") and PagedAttnParams ("11if") have no counterpart
+// there.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -74,6 +75,27 @@ struct SwigluF8Params {
 };
 static_assert(sizeof(SwigluF8Params) == 16, "SwigluF8Params must match struct.pack('<4i')");
 
+struct PagedRopeParams {
+  int M, B;                 // rows, sequences
+  int Hq, Hk;               // query heads; key heads, and as many value heads
+  int in_stride, q_stride;  // elements between rows of the input, of the queries
+  int rot;                  // channels of a head that are rotated
+  int norm;                 // 0: without the norm
+  int pages, page, width;   // pages of the cache, rows of a page, pages a sequence's row of the table names
+  float eps, rope_scale;    // of the norm; on rotated channels
+};
+static_assert(sizeof(PagedRopeParams) == 52, "PagedRopeParams must match struct.pack('<11i2f')");
+
+struct PagedAttnParams {
+  int M, B;                 // rows of queries, sequences
+  int H, KVH;               // query heads, key/value heads
+  int q_stride, o_stride;   // elements between rows of the queries, of the output
+  int pages, page, width;   // as above
+  int max_q, max_kv;        // the most new tokens, keys of a sequence as far as the caller knows (they choose tiles only)
+  float scale;              // softmax scale times log2(e)
+};
+static_assert(sizeof(PagedAttnParams) == 48, "PagedAttnParams must match struct.pack('<11if')");
+
 using Macros = std::map<std::string, std::string>;
 
 // One bound buffer argument as the launchers see it: a device address and the
@@ -112,6 +134,8 @@ bool make_attention(const std::string &fn, const Macros &m, Pipeline *pl, std::s
 bool make_ops(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
 bool make_rot_q8(const Macros &m, Pipeline *pl, std::string *err);  // module "ops", function "rot_q8"
 bool make_rows_q8(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);  // rms_norm_q8, swiglu_f8
+bool make_qk_norm_rope_paged(const Macros &m, Pipeline *pl, std::string *err);  // module "ops"
+bool make_attention_paged(const Macros &m, Pipeline *pl, std::string *err);     // module "attention"
 bool make_gemm(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err);
 bool make_gemm_f8(int epi, int out_t, bool bias, int tile, int exact, Pipeline *pl, std::string *err);  // weight format f8
 

@@ -538,8 +538,9 @@ int type_of(const std::string &s) {
 bool make_ops(const std::string &fn, const Macros &m, Pipeline *pl, std::string *err) {
   if (fn == "rot_q8") return make_rot_q8(m, pl, err);
   if (fn == "rms_norm_q8" || fn == "swiglu_f8") return make_rows_q8(fn, m, pl, err);
+  if (fn == "qk_norm_rope_paged") return make_qk_norm_rope_paged(m, pl, err);
   if (fn != "qk_norm_rope") {
-    *err = "unknown function (have: qk_norm_rope, rot_q8, rms_norm_q8, swiglu_f8)";
+    *err = "unknown function (have: qk_norm_rope, rot_q8, rms_norm_q8, swiglu_f8, qk_norm_rope_paged)";
     return false;
   }
   int hd, q8, rot, nsg;

@@ -35,6 +35,7 @@ GEMM_ACT = {"q8": "i8", "h8": "f16", "f16": "f16", "bf16": "bf16", "f8": "f8"}  
 LOG2E = 1.4426950408889634
 # parameter blocks of calls whose time is their host work
 _PACK_8I, _PACK_6IFI, _PACK_4I = struct.Struct("<8i").pack, struct.Struct("<6ifi").pack, struct.Struct("<4i").pack
+_PACK_11I2F, _PACK_11IF = struct.Struct("<11i2f").pack, struct.Struct("<11if").pack
 
 
 def pad_rows(m: int, tile: int = 128) -> int:
@@ -179,6 +180,93 @@ def swiglu_f8(gpu: Gpu, x: Tensor, out: Tensor, scale: Tensor, M: int, D: int, *
                          f"{scale.dtype}")
     k = gpu.kernel("ops", "swiglu_f8", IN_T=OUT_DT[x.dtype])
     gpu.launch(k, None, None, [x, out, scale], _PACK_4I(M, D, x_stride or 2 * D, o_stride or D), no_alloc=no_alloc)
+
+
+def _paged(name: str, kc: Tensor, vc: Tensor, table: Tensor, q_start: Tensor, kv_len: Tensor, heads: int, hd: int):
+    """(pages, rows of a page, pages a row of the table names) of a cache and its page table."""
+    if kc.dtype not in ("f16", "bf16") or vc.dtype != kc.dtype:
+        raise ValueError(f"{name}: kc and vc must both be f16 or both bf16, got {kc.dtype}, {vc.dtype}")
+    shape = kc.shape
+    if len(shape) != 4 or vc.shape != shape or shape[1] != heads or shape[3] != hd:
+        raise ValueError(f"{name}: kc and vc must be [pages][{heads}][page][{hd}], got {shape}, {vc.shape}")
+    if table.dtype != "i32" or q_start.dtype != "i32" or kv_len.dtype != "i32" or len(table.shape) != 2:
+        raise ValueError(f"{name}: table must be [B][pages] i32, q_start and kv_len i32, got {table.shape} {table.dtype}, "
+                         f"{q_start.dtype}, {kv_len.dtype}")
+    return shape[0], shape[2], table.shape[1]
+
+
+def qk_norm_rope_paged(gpu: Gpu, qkv: Tensor, wq: Tensor | None, wk: Tensor | None, turns: Tensor | None, Q: Tensor | None,
+                       kc: Tensor | None, vc: Tensor | None, table: Tensor | None, q_start: Tensor, kv_len: Tensor, *, M: int,
+                       B: int, Hq: int, Hk: int, hd: int, rot: int, eps: float, norm: bool = True, interleaved: bool = False,
+                       rope_scale: float = 1.0, pos: Tensor | None = None, in_stride: int | None = None,
+                       q_stride: int | None = None, no_alloc: bool = False):
+    """Per-head RMS norm and rotary embedding of a batch's new queries and keys; queries go to rows, keys and values to their
+    places in a paged cache (what attention_paged reads).
+
+      qkv [M][in_stride] f16 / bf16 / f32: Hq query heads, Hk key heads, Hk value heads of hd (64, 96 or 128) channels a row
+      rows q_start[b] .. q_start[b + 1] - 1 are the new tokens of sequence b, the last of its kv_len[b] tokens; rows before
+        q_start[0] and from q_start[B] on (a padded batch) are left as they are, in Q and in the cache
+      queries and keys: v = x / sqrt(mean(x^2) + eps) * w (norm; wq, wk [hd] f32), then pair j of the first `rot` channels,
+        (j, j + rot / 2) or, interleaved, (2 j, 2 j + 1), turns by position * frequency j, times rope_scale; rounded once
+      turns [rot / 2][2] u32: the frequencies' codes (rope.turns(rope.frequencies(...))); the position is pos[m] (pos [M]
+        i32) or the token's place in its sequence
+      Q [M][q_stride], kc and vc [pages][Hk][page][hd] f16 / bf16 (all of one type), page a power of two from 16 to 256;
+        table [B][..] i32: token c of sequence b goes to row c % page of page table[b][c / page]
+
+    q_start [B + 1] (not falling), kv_len [B] and table are read on the device. A token without a place (before 0, past the
+    table, a page number outside the cache) is not stored; two tokens with the same place leave either. Hq = 0 (Q None) and
+    Hk = 0 (kc, vc, table None) leave that side out. Q, kc and vc share memory with nothing else. no_alloc: as rms_norm_q8's."""
+    side = Q if Q is not None else kc
+    if side is None or (Q is None) != (Hq == 0) or (kc is None or vc is None or table is None) != (Hk == 0):
+        raise ValueError(f"qk_norm_rope_paged: Q goes with Hq > 0, kc, vc and table with Hk > 0, got Hq {Hq}, Hk {Hk}")
+    if side.dtype not in ("f16", "bf16") or qkv.dtype not in OUT_DT or (Hk and kc.dtype != side.dtype):
+        raise ValueError(f"qk_norm_rope_paged: qkv must be f16, bf16 or f32, Q and the cache both f16 or both bf16, got "
+                         f"{qkv.dtype}, {side.dtype}" + (f", {kc.dtype}" if Hk else ""))
+    if norm and any(w is None or w.dtype != "f32" for w, n in ((wq, Hq), (wk, Hk)) if n):
+        raise ValueError("qk_norm_rope_paged: the norm needs its f32 weights wq and wk")
+    if rot and (turns is None or turns.dtype != "u32") or pos is not None and pos.dtype != "i32":
+        raise ValueError("qk_norm_rope_paged: turns must be u32 (rope.turns) and pos i32")
+    if Hk:
+        pages, page, width = _paged("qk_norm_rope_paged", kc, vc, table, q_start, kv_len, Hk, hd)
+    else:
+        pages = page = width = 0
+        if q_start.dtype != "i32" or kv_len.dtype != "i32":
+            raise ValueError(f"qk_norm_rope_paged: q_start and kv_len must be i32, got {q_start.dtype}, {kv_len.dtype}")
+    k = gpu.kernel("ops", "qk_norm_rope_paged", HDIM=hd, IN_T=OUT_DT[qkv.dtype], OUT_T=OUT_DT[side.dtype],
+                   INTER=1 if interleaved else 0)
+    params = _PACK_11I2F(M, B, Hq, Hk, in_stride or (Hq + 2 * Hk) * hd, q_stride or Hq * hd, rot, 1 if norm else 0, pages,
+                         page, width, eps, rope_scale)
+    gpu.launch(k, None, None, [qkv, wq, wk, turns, Q, kc, vc, table, q_start, kv_len, pos], params, no_alloc=no_alloc)
+
+
+def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, table: Tensor, q_start: Tensor, kv_len: Tensor, *,
+                    M: int, B: int, H: int, KVH: int, D: int, scale: float, causal: bool = True, q_stride: int | None = None,
+                    o_stride: int | None = None, max_q: int | None = None, max_kv: int | None = None, no_alloc: bool = False):
+    """Attention of a batch's new tokens, one or many a sequence, over a paged cache: per query head h the softmax over the
+    visible keys of (scale * q_i . k_j), the weights applied to the values; 0 where no key is visible.
+
+      q [M][q_stride], out [M][o_stride]: rows of H heads of D (64, 96 or 128) channels, query head h reads key/value head
+        h / (H / KVH); rows q_start[b] .. q_start[b + 1] - 1 are the last tokens of sequence b, rows before q_start[0] and from
+        q_start[B] on are not written
+      kc, vc [pages][KVH][page][D], table [B][..], q_start [B + 1], kv_len [B] i32: as qk_norm_rope_paged leaves them; the
+        new tokens' keys are among the kv_len[b]
+      causal: token i of n sees the keys up to kv_len[b] - n + i, else all kv_len[b]
+
+    q, kc, vc and out are of one type, f16 or bf16; scores, softmax and sums are float, the weights are rounded to that type
+    for their product with the values. q, kc and vc are 16-byte aligned and q_stride a multiple of 8, out and o_stride of 4
+    elements. What the cache holds behind a sequence's end, and NaN or infinities in keys and values that a query does not see, do
+    not reach its output. A page number outside the cache makes the scores of its keys NaN; kv_len past the table's
+    pages counts up to them. max_q and max_kv, the most new tokens and keys of a sequence as far as the caller knows, choose
+    the kernel and how far it splits the keys (default: M, and the table's pages); results hold whatever they say. no_alloc: the
+    allocation-free entry point; its scratch array may split the keys less far."""
+    if q.dtype != kc.dtype or out.dtype != q.dtype:
+        raise ValueError(f"attention_paged: q, kc, vc and out must all be f16 or all bf16, got {q.dtype}, {kc.dtype}, "
+                         f"{vc.dtype}, {out.dtype}")
+    pages, page, width = _paged("attention_paged", kc, vc, table, q_start, kv_len, KVH, D)
+    k = gpu.kernel("attention", "attention_paged", HD=D, IN_T=OUT_DT[q.dtype], CAUSAL=1 if causal else 0)
+    params = _PACK_11IF(M, B, H, KVH, q_stride or H * D, o_stride or H * D, pages, page, width, M if max_q is None else max_q,
+                        min(width * page, 0x7FFFFFFF) if max_kv is None else max_kv, scale * LOG2E)
+    gpu.launch(k, None, None, [q, kc, vc, out, table, q_start, kv_len], params, no_alloc=no_alloc)
 
 
 @dataclass

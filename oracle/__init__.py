@@ -14,6 +14,7 @@ missing.
                     weight format q8): exact integer product, float32 epilogue
   oracle.attention  float64 softmax attention (reference tests/test_attention.py:9-21)
                     and exact integer scores
+  oracle.paged      float64 rows and attention over a paged cache
   oracle.bf16       bf16 <-> float32 conversions (round to nearest even)
 
 How each function is pinned (checks that do not retype its formula) is in
