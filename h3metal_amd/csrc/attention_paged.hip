@@ -2,7 +2,18 @@
 // the keys j < L_b, with a causal mask those up to L_b - n_b + i;
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j, 0 where no key is visible
 // Query head h reads key/value head h / (H / KVH). A key whose page number lies outside the cache has the score NaN.
+//
+// A tile's 32 rows are (token, head) pairs that share a key/value head, so that a single token of grouped heads reads its
+// keys once. The work is cut as paged_plan.h says; lengths are known on the device only, so every workgroup finds its slice by
+// itself. Within a workgroup the waves split the keys: wave w takes the 32-key blocks w, w + NW, ... of its part of a tile,
+// with a running maximum, sum and output of its own, staged through LDS of its own by LDS-direct loads that its own vmcnt
+// orders, with no barrier; the waves' states meet in LDS at the end. Scores are S^T = K Q^T and outputs O^T = V^T P^T on the 32 x
+// 32 MFMA, in attention_small.hip's layouts (a lane holds one query's keys, so the softmax is per lane; V's operands are
+// transposing LDS reads). The loads of a block's two 16-key halves go through descriptors that end at the sequence's last
+// key: what a page holds behind it reads as zero.
+#include "attention_common.h"
 #include "paged.h"
+#include "paged_plan.h"
 
 #include <algorithm>
 #include <cmath>
@@ -11,55 +22,503 @@
 namespace h3 {
 namespace {
 
-// One wave per query row and head: a lane scores one of 64 keys, then every lane sums its channels of the values.
-template <int D, int T>
-__global__ __launch_bounds__(256) void attention_paged_simple(const char *q, const char *kc, const char *vc, char *out,
-                                                              Batch bt, PagedAttnParams p, int causal) {
-  using E = typename PElem<T>::type;
-  const int lane = threadIdx.x & 63, m = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (h >= p.H) return;
-  int b = 0;
-  for (int k = 0; k < bt.B; k += 64) b += __popcll(__ballot(k + lane < bt.B && bt.q_start[k + lane + 1] <= m));
-  if (b >= bt.B || bt.q_start[b] > m) return;
-  const long long most = (long long)bt.width << bt.lg, L = min(max((long long)bt.kv_len[b], 0ll), most);
-  const long long end = causal ? min(L, (long long)bt.kv_len[b] - bt.q_start[b + 1] + m + 1) : L;
-  const int kvh = h / (p.H / p.KVH);
-  const E *qr = (const E *)q + (size_t)m * p.q_stride + h * D;
-  float top = -INFINITY, sum = 0.0f, o[2] = {0.0f, 0.0f};
-  for (long long j0 = 0; j0 < end; j0 += 64) {
-    const long long j = j0 + lane;
-    float s = -INFINITY;
-    long long row = -1;
-    if (j < end) {
-      const int pg = bt.table[(long long)b * bt.width + (j >> bt.lg)];
-      s = NAN;
-      if (pg >= 0 && pg < bt.pages) {
-        row = (((long long)pg * p.KVH + kvh) << bt.lg) + (j & ((1 << bt.lg) - 1));
-        s = 0.0f;
-        for (int d = 0; d < D; d++) s = fmaf((float)qr[d], (float)((const E *)kc)[row * D + d], s);
-        s *= p.scale;
+using plan::i64;
+
+constexpr int RT = 32;             // rows of a tile
+constexpr int KB = 32;             // keys of a block
+constexpr float SLACK_P = 8.0f;    // log2 units the running maximum may lag behind a score
+
+// Query heads of a tile: a key/value head's G heads in HS groups of GP (the last may have fewer).
+struct Heads {
+  int G, HS, GP;
+};
+
+struct AttnArgs {
+  const char *q, *kc, *vc;
+  char *out;
+  float *ws;  // partial states: O [RT][D], then m and l of each row
+};
+
+// -- finding the work -------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ i64 wave_sum_to(i64 v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const i64 u = __shfl_up(v, d);
+    v += lane >= d ? u : 0;
+  }
+  return v;
+}
+__device__ __forceinline__ i64 lane_value(i64 v, int l) {
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)v, l), hi = __builtin_amdgcn_readlane((int)(v >> 32), l);
+  return (i64)(((unsigned long long)hi << 32) | lo);
+}
+
+// The batch's weight, and the sequence at a weight of it; 64 sequences at a time, one a lane.
+struct Order {
+  const plan::Shape &sh;
+  const Batch &bt;
+  i64 own, upto, first;  // of the first 64 sequences: this lane's weight, the sum up to it, their sum
+
+  __device__ Order(const plan::Shape &s, const Batch &b) : sh(s), bt(b) {
+    own = weight(threadIdx.x & 63);
+    upto = wave_sum_to(own);
+    first = lane_value(upto, 63);
+  }
+  __device__ i64 weight(int b) const {
+    if (b >= bt.B) return 0;
+    return plan::head_weight(plan::seq_of(sh, bt.q_start[b], bt.q_start[b + 1], bt.kv_len[b])) * sh.VH;
+  }
+  __device__ i64 total() const {
+    i64 t = first;
+    for (int k = 64; k < bt.B; k += 64) t += lane_value(wave_sum_to(weight(k + (threadIdx.x & 63))), 63);
+    return t;
+  }
+  // the sequence at weight x, and the weight before it
+  __device__ int find(i64 x, i64 *before) const {
+    i64 base = 0, w = own, s = upto, all = first;
+    for (int k = 0;; k += 64) {
+      const unsigned long long m = __ballot(base + s > x);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        *before = base + lane_value(s - w, l);
+        return __builtin_amdgcn_readfirstlane(k + l);
       }
-    }
-    float mx = s;
-    for (int i = 32; i; i /= 2) mx = fmaxf(mx, __shfl_xor(mx, i));
-    mx = fmaxf(mx, top);
-    const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - mx);
-    const float w = j < end ? (mx == -INFINITY ? s - s : __builtin_amdgcn_exp2f(s - mx)) : 0.0f;
-    top = mx;
-    sum = sum * f + w;
-    o[0] *= f;
-    o[1] *= f;
-    for (int k = 0; k < 64 && j0 + k < end; k++) {
-      const long long r = __shfl(row, k);
-      const float wk = __shfl(w, k);
-      for (int e = 0; e < 2; e++)
-        if (e * 64 + lane < D) o[e] += wk * (r < 0 ? 0.0f : (float)((const E *)vc)[r * D + e * 64 + lane]);
+      if (k + 64 >= bt.B) return -1;
+      base += all;
+      w = weight(k + 64 + (threadIdx.x & 63));
+      s = wave_sum_to(w);
+      all = lane_value(s, 63);
     }
   }
-  for (int i = 32; i; i /= 2) sum += __shfl_xor(sum, i);
-  const float inv = end > 0 ? 1.0f / sum : 0.0f;
-  for (int e = 0; e < 2; e++)
-    if (e * 64 + lane < D) ((E *)out)[(size_t)m * p.o_stride + h * D + e * 64 + lane] = (E)(o[e] * inv);
+  __device__ plan::Seq seq(int b) const { return plan::seq_of(sh, bt.q_start[b], bt.q_start[b + 1], bt.kv_len[b]); }
+};
+
+// A tile: sequence, head group, place in the group, the weight before it and its own.
+struct Tile {
+  int b, v, t;
+  i64 p, w;
+  plan::Seq q;
+};
+__device__ __forceinline__ bool tile_at(const Order &o, i64 x, Tile *c) {
+  i64 before;
+  c->b = o.find(x, &before);
+  if (c->b < 0) return false;
+  c->q = o.seq(c->b);
+  const i64 w = plan::head_weight(c->q), y = x - before;
+  c->v = (int)(y / w);
+  c->t = plan::tile_at(c->q, y - w * c->v);
+  c->p = before + w * c->v + plan::before_tile(c->q, c->t);
+  c->w = plan::tile_weight(c->q, c->t);
+  return true;
+}
+__device__ __forceinline__ bool next_tile(const Order &o, Tile *c) {
+  c->p += c->w;
+  if (++c->t == c->q.K) {
+    c->t = 0;
+    if (++c->v == o.sh.VH) {
+      c->v = 0;
+      do {
+        if (++c->b >= o.bt.B) return false;
+        c->q = o.seq(c->b);
+      } while (!c->q.K);
+    }
+  }
+  c->w = plan::tile_weight(c->q, c->t);
+  return true;
+}
+
+// The slice of a workgroup: workgroup b runs on XCD b % 8; each XCD takes a contiguous run of the slices, so that tiles that share
+// keys share an L2.
+__device__ __forceinline__ int slice_of(int b, int n) {
+  const int per = n >> 3, rem = n & 7, xcd = b & 7;
+  return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (b >> 3);
+}
+
+// -- tiles of 32 rows -------------------------------------------------------------------------------------------------
+
+template <int DG, int NW>
+struct Rows {
+  static constexpr int D = DG == 96 ? 128 : DG;        // channels of an LDS row
+  static constexpr int RB = D * 2, RBG = DG * 2;       // bytes of a row: in LDS, in memory
+  static constexpr int NP = RB / 16;                   // 16-byte pieces of a row
+  static constexpr int NCH = DG / 16;                  // score MFMAs per 32 x 32 tile
+  static constexpr int NDB = DG / 32;                  // 32-channel blocks of O
+  static constexpr int BYTES = KB * RB;                // a block of K or V
+  static constexpr int NDMA = BYTES / 1024;            // 1 KB loads of it
+  static constexpr int ORS = (DG + 4) * 4;             // bytes of a row of a wave's state
+  static constexpr int MERGE = NW * RT * (ORS + 8);    // the waves' states: O, then (m, l)
+  static constexpr int LDS = NW * 2 * BYTES > MERGE ? NW * 2 * BYTES : MERGE;
+};
+
+// A 16-bit value that is infinite or NaN in either half
+template <int T>
+__device__ __forceinline__ bool odd16(unsigned v) {
+  constexpr unsigned E = T == T_BF16 ? 0x7F80u : 0x7C00u;
+  return (v & E) == E || (v & (E << 16)) == E << 16;
+}
+
+template <int DG, int T, int NW, bool CAUSAL>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh, Heads hd, int least) {
+  using C = Rows<DG, NW>;
+  constexpr int NDB = C::NDB, NCH = C::NCH;
+  using VT8 = typename Vec8<T>::type;
+  using VE = typename Vec8<T>::elem;
+  using VP2 = typename Vec8<T>::pair;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const Order order(sh, bt);
+  const i64 total = order.total();
+  if (total <= 0) return;
+  const int nsl = sh.each ? (int)(total < (i64)gridDim.x ? total : (i64)gridDim.x) : plan::slices(total, gridDim.x, least);
+  if ((int)blockIdx.x >= nsl) return;
+  int sl = slice_of(blockIdx.x, nsl);
+  if (sh.each) sl = nsl - 1 - sl;  // with a causal mask the longest tiles go first
+  i64 x0 = sl, x1 = sl + 1;
+  if (!sh.each) {
+    x0 = plan::slice_start(total, nsl, sl);
+    x1 = plan::slice_start(total, nsl, sl + 1);
+  }
+
+  // this lane's 16 bytes of each 1 KB load: row and swizzled piece (attention_common.h: kswz, voff); pieces past a row in
+  // memory (head dim 96) are sent out of the descriptor's range
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char *)smem + w * 2 * C::BYTES;
+  const char *Ks = smem + w * 2 * C::BYTES, *Vs = Ks + C::BYTES;
+  unsigned kgo[C::NDMA], vgo[C::NDMA];
+#pragma unroll
+  for (int r = 0; r < C::NDMA; r++) {
+    constexpr int R = 256 / C::RB > 0 ? 256 / C::RB : 1;
+    const int o = r * 1024 + 16 * lane, row = o / C::RB, in = o % C::RB;
+    const int kp = (in / 16) ^ kswz<C::RB, C::NP>(row), vp = 2 * ((in >> 5) ^ (2 * ((row & 3) / R))) + ((in >> 4) & 1);
+    kgo[r] = kp * 16 < C::RBG ? (row & 15) * C::RBG + kp * 16 : 0x80000000u;
+    vgo[r] = vp * 16 < C::RBG ? (row & 15) * C::RBG + vp * 16 : 0x80000000u;
+  }
+  const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
+  const int l16 = lane & 15, tr_row = l16 >> 2, tr_col = (l16 & 3) * 8;
+
+  Tile tile;
+  bool more = tile_at(order, x0, &tile);
+  for (; more && tile.p < x1; more = next_tile(order, &tile)) {
+    const plan::Seq &q = tile.q;
+    const int nblk = plan::tile_blocks(sh, q, tile.t, KB);
+    int blk0 = 0, blk1 = nblk;
+    bool begun = false, whole = true;
+    if (!sh.each) {
+      blk0 = plan::block_at(x0, tile.p, tile.w, nblk);
+      blk1 = plan::block_at(x1, tile.p, tile.w, nblk);
+      begun = tile.p < x0;
+      whole = !begun && tile.p + tile.w <= x1;
+      if (blk0 == blk1) continue;  // (a whole tile has a block)
+    }
+    const int kvh = tile.v / hd.HS, g0 = (tile.v - kvh * hd.HS) * hd.GP;
+    const int m0 = q.lo + tile.t * sh.TT, R = min(sh.TT, q.hi - m0) * hd.GP;
+    const int L = (int)q.L;
+    // this lane's query row: its token, head and last visible key
+    const int ti = (int)((unsigned)l32 / (unsigned)hd.GP), gi = l32 - ti * hd.GP;
+    const bool ok = l32 < R && g0 + gi < hd.G;
+    const int last = !ok ? -1 : CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
+    const i64 first_last = CAUSAL ? plan::clamp(q.off + m0, -1, q.L - 1) : q.L - 1;  // of the tile's first token
+    i32x4 qreg[NCH];
+    {
+      const char *qrow = a.q + ((size_t)(m0 + (ok ? ti : 0)) * p.q_stride + (size_t)(kvh * hd.G + (ok ? g0 + gi : 0)) * DG) * 2;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) {
+        const i32x4 v = *(const i32x4 *)(qrow + (2 * c + hl) * 16);
+        qreg[c] = ok ? v : i32x4{0, 0, 0, 0};
+      }
+    }
+
+    // Page numbers of this wave's next 32 blocks: lane 2 i + h holds that of half h of the i-th; -1: outside the cache.
+    int ids = 0;
+    auto fetch_ids = [&](int blk) __attribute__((always_inline)) {
+      const i64 key = (i64)(blk + (lane >> 1) * NW) * KB + 16 * (lane & 1), pi = key >> bt.lg;
+      ids = 0;
+      if (key < L) {
+        ids = bt.table[(size_t)tile.b * bt.width + pi];
+        if (ids < 0 || ids >= bt.pages) ids = -1;
+      }
+    };
+    auto page_of = [&](int it, int h) __attribute__((always_inline)) {
+      return __builtin_amdgcn_readlane(ids, 2 * (it & 31) + h);
+    };
+    auto half_rsrc = [&](const char *base, int pg, i64 key) __attribute__((always_inline)) {
+      const size_t row = ((((size_t)max(pg, 0) * p.KVH + kvh) << bt.lg) + (size_t)(key & ((1 << bt.lg) - 1)));
+      const int n = pg < 0 ? 0 : (int)plan::clamp(L - key, 0, 16);
+      return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row * C::RBG), (short)0, n * C::RBG, 0x00020000);
+    };
+    auto load = [&](const char *base, unsigned lds, const unsigned (&go)[C::NDMA], int blk, int pg0, int pg1)
+        __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const __amdgpu_buffer_rsrc_t r = half_rsrc(base, h ? pg1 : pg0, (i64)blk * KB + 16 * h);
+#pragma unroll
+        for (int i = 0; i < C::NDMA / 2; i++) dma16(lds + (h * (C::NDMA / 2) + i) * 1024, go[h * (C::NDMA / 2) + i], r);
+      }
+    };
+
+    f32x16 o[NDB];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int db = 0; db < NDB; db++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[db][i] = 0.0f;
+
+    int blk = blk0 + w, it = 0;
+    if (blk < blk1) {
+      fetch_ids(blk);
+      int pg0 = page_of(0, 0), pg1 = page_of(0, 1);
+      load(a.kc, lds0, kgo, blk, pg0, pg1);
+      load(a.vc, lds0 + C::BYTES, vgo, blk, pg0, pg1);
+      for (;; blk += NW) {
+        const bool next = blk + NW < blk1;
+        const bool lost0 = pg0 < 0, lost1 = pg1 < 0;
+        if (next) {
+          if ((++it & 31) == 0) fetch_ids(blk + NW);
+          pg0 = page_of(it, 0);
+          pg1 = page_of(it, 1);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::NDMA) : "memory");  // the block's K has landed (V may be in flight)
+        i32x4 ka[NCH];
+#pragma unroll
+        for (int c = 0; c < NCH; c++)
+          ka[c] = *(const i32x4 *)(Ks + krow * C::RB + (((2 * c + hl) ^ kswz<C::RB, C::NP>(krow)) * 16));
+        f32x16 x;
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; c++) x = mma_qk<T>(ka[c], qreg[c], x);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the K slot's reads are done
+        if (next) load(a.kc, lds0, kgo, blk + NW, pg0, pg1);
+        if (__builtin_expect(lost0 || lost1, 0)) {
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (i < 8 ? lost0 : lost1) x[i] = NAN;
+        }
+        const bool edge = (i64)blk * KB + KB - 1 > first_last;  // some row does not see some key
+        if (edge) {
+          // element i of lane half hl holds key KB blk + 16 (i / 8) + 8 hl + i % 8
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (blk * KB + 16 * (i >> 3) + 8 * hl + (i & 7) > last) x[i] = -INFINITY;
+        }
+        float am[2] = {x[0], x[1]};
+#pragma unroll
+        for (int i = 2; i < 16; i++) am[i & 1] = fmaxf(am[i & 1], x[i]);
+        const float amax = fmaxf(am[0], am[1]);
+        // lazy running maximum (wave-uniform branch); partner lanes (the same query) always update together
+        if (__any(amax * p.scale > m + SLACK_P)) {
+          const float ap = fmaxf(amax, __shfl_xor(amax, 32));
+          const float mn = fmaxf(m, ap * p.scale);
+          const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= f;
+#pragma unroll
+          for (int db = 0; db < NDB; db++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[db][i] *= f;
+        }
+        const float nm = m == -INFINITY ? 0.0f : -m;
+        float ls[2] = {0.0f, 0.0f};  // of the rounded weights, which the product with V takes
+        i32x4 pb[2];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(x[i], p.scale, nm));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(x[i + 1], p.scale, nm));
+          const VP2 pr = {(VE)p0, (VE)p1};
+          pb[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, pr);
+          ls[(i >> 1) & 1] = sum2<T>(pr, ls[(i >> 1) & 1]);
+        }
+        l += ls[0] + ls[1];
+        if (next) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C::NDMA) : "memory");  // the block's V has landed
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int s2 = 0; s2 < 2; s2++) {
+          const int k0 = 16 * s2 + 8 * hl + tr_row;
+          i16x8 va[NDB];
+#pragma unroll
+          for (int db = 0; db < NDB; db++) {
+            const int pc = (db * 32 + (l32 & 16)) / 8;
+            const i16x4 lo = lds_tr16(Vs + voff<C::D>(k0, pc) + tr_col);
+            const i16x4 hi = lds_tr16(Vs + voff<C::D>(k0 + 4, pc) + tr_col);
+            va[db] = i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          }
+          if (CAUSAL && edge) {
+            // A weight of 0 does not keep a value that is infinite or NaN out of a sum: rows that do not see it take the
+            // product with the values they see alone, one count of visible keys after the other.
+            bool odd = false;
+#pragma unroll
+            for (int db = 0; db < NDB; db++) {
+              const i32x4 d = __builtin_bit_cast(i32x4, va[db]);
+#pragma unroll
+              for (int i = 0; i < 4; i++) odd = odd || odd16<T>((unsigned)d[i]);
+            }
+            if (__builtin_expect(__any(odd), 0)) {
+              const int seen = min(max(last + 1 - (blk * KB + 16 * s2), 0), 16);
+              for (unsigned long long left = __ballot(seen > 0); left;) {
+                const int n = __builtin_amdgcn_readlane(seen, __builtin_ctzll(left));
+#pragma unroll
+                for (int db = 0; db < NDB; db++) {
+                  i16x8 vz = va[db];
+#pragma unroll
+                  for (int e = 0; e < 8; e++)
+                    if (8 * hl + e >= n) vz[e] = 0;
+                  const f32x16 u = mma_pv<T>(vz, __builtin_bit_cast(VT8, pb[s2]), o[db]);
+#pragma unroll
+                  for (int i = 0; i < 16; i++) o[db][i] = seen == n ? u[i] : o[db][i];
+                }
+                left &= ~__ballot(seen == n);
+              }
+              continue;
+            }
+          }
+#pragma unroll
+          for (int db = 0; db < NDB; db++) o[db] = mma_pv<T>(va[db], __builtin_bit_cast(VT8, pb[s2]), o[db]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the V slot's reads are done
+        if (!next) break;
+        load(a.vc, lds0 + C::BYTES, vgo, blk + NW, pg0, pg1);
+      }
+    }
+
+    // the waves' states meet: each leaves O, m and l, then a thread takes 8 channels of a row
+    const float lt = l + __shfl_xor(l, 32);
+    __syncthreads();
+    char *orow = smem + (w * RT + l32) * C::ORS;
+#pragma unroll
+    for (int db = 0; db < NDB; db++)
+#pragma unroll
+      for (int g = 0; g < 4; g++)
+        store4<T_F32>(orow + (db * 32 + 8 * g + 4 * hl) * 4, o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2],
+                      o[db][4 * g + 3]);
+    float *ml = (float *)(smem + NW * RT * C::ORS);
+    if (hl == 0) *(float2 *)(ml + (w * RT + l32) * 2) = make_float2(m, lt);
+    __syncthreads();
+    constexpr int PPR = DG / 8;
+    for (int c = tid; c < R * PPR; c += NW * 64) {
+      const int r = c / PPR, d0 = 8 * (c - r * PPR);
+      const int rt = (int)((unsigned)r / (unsigned)hd.GP), rg = r - rt * hd.GP;
+      if (g0 + rg >= hd.G) continue;
+      float2 s[NW];
+      float mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NW; k++) {
+        s[k] = *(const float2 *)(ml + (k * RT + r) * 2);
+        mx = fmaxf(mx, s[k].x);
+      }
+      float v[8] = {};
+#pragma unroll
+      for (int k = 0; k < NW; k++) {
+        // a sum of 0: nothing was seen (a sum of NaN counts, whatever its maximum)
+        const float wt = s[k].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s[k].x - mx);
+        sum += wt * s[k].y;
+        const char *pr = smem + (k * RT + r) * C::ORS + d0 * 4;
+        const f32x4 lo = *(const f32x4 *)pr, hi = *(const f32x4 *)(pr + 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          v[e] += wt * lo[e];
+          v[4 + e] += wt * hi[e];
+        }
+      }
+      if (whole) {
+        // no sum although a key is visible: all scores are -infinity, and 0 / 0
+        const bool any = CAUSAL ? q.L > 0 && q.off + m0 + rt >= 0 : q.L > 0;
+        const float inv = sum != 0.0f ? 1.0f / sum : any ? NAN : 0.0f;
+        char *dst = a.out + ((size_t)(m0 + rt) * p.o_stride + (size_t)(kvh * hd.G + g0 + rg) * DG + d0) * 2;
+        store4<T>(dst, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+        store4<T>(dst + 8, v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+      } else {
+        float *st = a.ws + (size_t)plan::state_of(sl, begun) * (RT * (DG + 2));
+        store4<T_F32>((char *)(st + r * DG + d0), v[0], v[1], v[2], v[3]);
+        store4<T_F32>((char *)(st + r * DG + d0 + 4), v[4], v[5], v[6], v[7]);
+        if (d0 == 0) *(float2 *)(st + RT * DG + 2 * r) = make_float2(mx, sum);
+      }
+    }
+    __syncthreads();  // before the next tile's loads
+  }
+}
+
+// Joins the parts of cut tiles: workgroup j, the tile that slice j leaves unfinished if it begins in it. One wave per row.
+template <int DG, int T, bool CAUSAL>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh,
+                                                             Heads hd, int least, int most) {
+  const int j = blockIdx.x, lane = threadIdx.x & 63;
+  const Order order(sh, bt);
+  const i64 total = order.total();
+  if (total <= 0) return;
+  const int nsl = plan::slices(total, most, least);
+  if (j + 1 >= nsl) return;
+  const i64 x = plan::slice_start(total, nsl, j + 1);
+  Tile c;
+  if (!tile_at(order, x, &c) || c.p >= x || c.p < plan::slice_start(total, nsl, j)) return;
+  const int nblk = plan::tile_blocks(sh, c.q, c.t, KB);
+  const int kvh = c.v / hd.HS, g0 = (c.v - kvh * hd.HS) * hd.GP;
+  const int m0 = c.q.lo + c.t * sh.TT, R = min(sh.TT, c.q.hi - m0) * hd.GP;
+  int n = j + 1;  // the slice behind the tile's last part
+  while (n < nsl && plan::slice_start(total, nsl, n) < c.p + c.w) n++;
+  for (int r = threadIdx.x >> 6; r < R; r += 4) {
+    const int rt = (int)((unsigned)r / (unsigned)hd.GP), rg = r - rt * hd.GP;
+    if (g0 + rg >= hd.G) continue;
+    constexpr int PER = DG > 64 ? 2 : 1;
+    const int d0 = PER * lane;
+    float mx = -INFINITY, sum = 0.0f, v[2] = {0.0f, 0.0f};
+    for (int i = j; i < n; i++) {
+      const i64 s0 = plan::slice_start(total, nsl, i), s1 = plan::slice_start(total, nsl, i + 1);
+      if (plan::block_at(s0, c.p, c.w, nblk) == plan::block_at(s1, c.p, c.w, nblk)) continue;  // nothing was written
+      const float *st = a.ws + (size_t)plan::state_of(i, c.p < s0) * (RT * (DG + 2));
+      const float2 s = *(const float2 *)(st + RT * DG + 2 * r);
+      const float m = fmaxf(mx, s.x);
+      const float f0 = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mx - m);
+      const float f1 = s.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s.x - m);
+      mx = m;
+      sum = sum * f0 + s.y * f1;
+      if (d0 < DG)
+#pragma unroll
+        for (int e = 0; e < PER; e++) v[e] = v[e] * f0 + st[r * DG + d0 + e] * f1;
+    }
+    const bool any = CAUSAL ? c.q.L > 0 && c.q.off + m0 + rt >= 0 : c.q.L > 0;
+    const float inv = sum != 0.0f ? 1.0f / sum : any ? NAN : 0.0f;
+    using E = typename Vec8<T>::elem;
+    E *dst = (E *)a.out + (size_t)(m0 + rt) * p.o_stride + (size_t)(kvh * hd.G + g0 + rg) * DG + d0;
+    if (d0 < DG)
+#pragma unroll
+      for (int e = 0; e < PER; e++) dst[e] = (E)(v[e] * inv);
+  }
+}
+
+template <int DG, int T, bool CAUSAL>
+int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
+  constexpr int NW = 4;
+  using C = Rows<DG, NW>;
+  auto kern = attention_rows_kernel<DG, T, NW, CAUSAL>;
+  static bool attr_set = false;
+  if (!attr_set) {
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
+    if (e != hipSuccess) {
+      *err = std::string("hipFuncSetAttribute: ") + hipGetErrorString(e);
+      return -1;
+    }
+    attr_set = true;
+  }
+  const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
+  const Heads hd{G, HS, GP};
+  const int cus = std::max(1, cu_count());
+  const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
+  const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float);
+  const int least = 256, most = (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state));
+  const bool each = tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= 8 * most);
+  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 128, (i64)bt.width << bt.lg};
+  AttnArgs g = a;
+  g.ws = (float *)ex.ws;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(each ? tiles : std::max(most, 1))), dim3(NW * 64), C::LDS, ex.stream, g, bt, p, sh,
+                     hd, least);
+  if (!each && most > 1)
+    hipLaunchKernelGGL((attention_join_kernel<DG, T, CAUSAL>), dim3((unsigned)(most - 1)), dim3(256), 0, ex.stream, g, bt, p,
+                       sh, hd, least, most);
+  return 0;
 }
 
 template <int D, int T>
@@ -79,9 +538,10 @@ int launch(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const vo
            " o_stride " + std::to_string(p.o_stride);
     return -1;
   }
-  if (lg < 0 || p.pages < 0 || p.width < 0) {
+  if (lg < 0 || p.pages < 0 || p.width < 0 || (i64)p.width << lg > 0x7fffffffll) {
     *err = "bad cache: " + std::to_string(p.pages) + " pages of " + std::to_string(p.page) +
-           " rows (a power of two from 16 to 256), " + std::to_string(p.width) + " in a row of the table";
+           " rows (a power of two from 16 to 256), " + std::to_string(p.width) +
+           " in a row of the table (below 2^31 rows in all)";
     return -1;
   }
   if (!(p.scale > 0.0f) || !std::isfinite(p.scale)) {
@@ -110,15 +570,14 @@ int launch(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const vo
       *err = std::string("out shares memory with ") + what[i];
       return -1;
     }
+  const AttnArgs g{a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, nullptr};
   const Batch bt{(const int *)a[4].ptr, (const int *)a[5].ptr, (const int *)a[6].ptr, p.B, p.width, p.pages, lg};
-  hipLaunchKernelGGL((attention_paged_simple<D, T>), dim3((unsigned)p.M, (unsigned)((p.H + 3) / 4)), dim3(256), 0, ex.stream,
-                     a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, bt, p, pl.ival[0]);
-  return 0;
+  return pl.ival[0] ? run<D, T, true>(ex, g, bt, p, err) : run<D, T, false>(ex, g, bt, p, err);
 }
 
 template <int D>
 LaunchFn pick(int t) {
-  return t == P_BF16 ? launch<D, P_BF16> : launch<D, P_F16>;
+  return t == P_BF16 ? launch<D, T_BF16> : launch<D, T_F16>;
 }
 
 }  // namespace
