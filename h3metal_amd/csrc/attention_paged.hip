@@ -59,25 +59,42 @@ __device__ __forceinline__ i64 lane_value(i64 v, int l) {
 struct Order {
   const plan::Shape &sh;
   const Batch &bt;
-  i64 own, upto, first;  // of the first 64 sequences: this lane's weight, the sum up to it, their sum
+  int q0, q1, kv;        // of the first 64 sequences: this lane's
+  i64 own, upto, first;  // its weight, the sum up to it, their sum
+  i64 all, tiles;        // the batch's weight and tiles
 
   __device__ Order(const plan::Shape &s, const Batch &b) : sh(s), bt(b) {
-    own = weight(threadIdx.x & 63);
+    int K;
+    own = weight(threadIdx.x & 63, &q0, &q1, &kv, &K);
+    if (bt.B == 1) {
+      upto = own = all = first = lane_value(own, 0);
+      tiles = (i64)__builtin_amdgcn_readfirstlane(K) * sh.VH;
+      return;
+    }
     upto = wave_sum_to(own);
-    first = lane_value(upto, 63);
+    all = first = lane_value(upto, 63);
+    i64 mine = K;
+    for (int k = 64; k < bt.B; k += 64) {
+      int x, y, z;
+      all += lane_value(wave_sum_to(weight(k + (threadIdx.x & 63), &x, &y, &z, &K)), 63);
+      mine += K;
+    }
+    tiles = lane_value(wave_sum_to(mine), 63) * sh.VH;
   }
-  __device__ i64 weight(int b) const {
-    if (b >= bt.B) return 0;
-    return plan::head_weight(plan::seq_of(sh, bt.q_start[b], bt.q_start[b + 1], bt.kv_len[b])) * sh.VH;
-  }
-  __device__ i64 total() const {
-    i64 t = first;
-    for (int k = 64; k < bt.B; k += 64) t += lane_value(wave_sum_to(weight(k + (threadIdx.x & 63))), 63);
-    return t;
+  __device__ i64 weight(int b, int *s0, int *s1, int *n, int *K) const {
+    *s0 = *s1 = *n = 0;
+    if (b < bt.B) {
+      *s0 = bt.q_start[b];
+      *s1 = bt.q_start[b + 1];
+      *n = bt.kv_len[b];
+    }
+    const plan::Seq q = plan::seq_of(sh, *s0, *s1, *n);
+    *K = q.K;
+    return plan::head_weight(q) * sh.VH;
   }
   // the sequence at weight x, and the weight before it
   __device__ int find(i64 x, i64 *before) const {
-    i64 base = 0, w = own, s = upto, all = first;
+    i64 base = 0, w = own, s = upto, sum = first;
     for (int k = 0;; k += 64) {
       const unsigned long long m = __ballot(base + s > x);
       if (m) {
@@ -86,13 +103,19 @@ struct Order {
         return __builtin_amdgcn_readfirstlane(k + l);
       }
       if (k + 64 >= bt.B) return -1;
-      base += all;
-      w = weight(k + 64 + (threadIdx.x & 63));
+      base += sum;
+      int t0, t1, t2, t3;
+      w = weight(k + 64 + (threadIdx.x & 63), &t0, &t1, &t2, &t3);
       s = wave_sum_to(w);
-      all = lane_value(s, 63);
+      sum = lane_value(s, 63);
     }
   }
-  __device__ plan::Seq seq(int b) const { return plan::seq_of(sh, bt.q_start[b], bt.q_start[b + 1], bt.kv_len[b]); }
+  __device__ plan::Seq seq(int b) const {  // one sequence for the wave: scalar values
+    if (b < 64)
+      return plan::seq_of(sh, __builtin_amdgcn_readlane(q0, b), __builtin_amdgcn_readlane(q1, b), __builtin_amdgcn_readlane(kv, b));
+    return plan::seq_of(sh, __builtin_amdgcn_readfirstlane(bt.q_start[b]), __builtin_amdgcn_readfirstlane(bt.q_start[b + 1]),
+                        __builtin_amdgcn_readfirstlane(bt.kv_len[b]));
+  }
 };
 
 // A tile: sequence, head group, place in the group, the weight before it and its own.
@@ -107,8 +130,8 @@ __device__ __forceinline__ bool tile_at(const Order &o, i64 x, Tile *c) {
   if (c->b < 0) return false;
   c->q = o.seq(c->b);
   const i64 w = plan::head_weight(c->q), y = x - before;
-  c->v = (int)(y / w);
-  c->t = plan::tile_at(c->q, y - w * c->v);
+  c->v = __builtin_amdgcn_readfirstlane((int)plan::div(y, w));
+  c->t = __builtin_amdgcn_readfirstlane(plan::tile_at(c->q, y - w * c->v));
   c->p = before + w * c->v + plan::before_tile(c->q, c->t);
   c->w = plan::tile_weight(c->q, c->t);
   return true;
@@ -152,11 +175,11 @@ struct Rows {
   static constexpr int LDS = NW * 2 * BYTES > MERGE ? NW * 2 * BYTES : MERGE;
 };
 
-// A 16-bit value that is infinite or NaN in either half
+// Whether the 16-bit value in the high half is infinite or NaN
 template <int T>
 __device__ __forceinline__ bool odd16(unsigned v) {
-  constexpr unsigned E = T == T_BF16 ? 0x7F80u : 0x7C00u;
-  return (v & E) == E || (v & (E << 16)) == E << 16;
+  constexpr unsigned E = T == T_BF16 ? 0x7F800000u : 0x7C000000u;
+  return (v & E) == E;
 }
 
 template <int DG, int T, int NW, bool CAUSAL>
@@ -172,17 +195,13 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const Order order(sh, bt);
-  const i64 total = order.total();
-  if (total <= 0) return;
-  const int nsl = sh.each ? (int)(total < (i64)gridDim.x ? total : (i64)gridDim.x) : plan::slices(total, gridDim.x, least);
-  if ((int)blockIdx.x >= nsl) return;
-  int sl = slice_of(blockIdx.x, nsl);
-  if (sh.each) sl = nsl - 1 - sl;  // with a causal mask the longest tiles go first
-  i64 x0 = sl, x1 = sl + 1;
-  if (!sh.each) {
-    x0 = plan::slice_start(total, nsl, sl);
-    x1 = plan::slice_start(total, nsl, sl + 1);
-  }
+  if (order.all <= 0) return;
+  plan::Cut cut{1, (int)(order.all < (i64)gridDim.x ? order.all : (i64)gridDim.x), 0};
+  if (!sh.each) cut = plan::cut(order.all, order.tiles, gridDim.x, least);
+  if ((int)blockIdx.x >= cut.n) return;
+  int sl = slice_of(blockIdx.x, cut.n);
+  if (sh.each) sl = cut.n - 1 - sl;  // with a causal mask the longest tiles go first
+  const i64 x0 = plan::slice_start(cut, sl), x1 = plan::slice_start(cut, sl + 1);
 
   // this lane's 16 bytes of each 1 KB load: row and swizzled piece (attention_common.h: kswz, voff); pieces past a row in
   // memory (head dim 96) are sent out of the descriptor's range
@@ -262,6 +281,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
 
     f32x16 o[NDB];
     float m = -INFINITY, l = 0.0f;
+    bool odd = false;
 #pragma unroll
     for (int db = 0; db < NDB; db++)
 #pragma unroll
@@ -347,32 +367,22 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
             va[db] = i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           }
           if (CAUSAL && edge) {
-            // A weight of 0 does not keep a value that is infinite or NaN out of a sum: rows that do not see it take the
-            // product with the values they see alone, one count of visible keys after the other.
-            bool odd = false;
+            // A weight of 0 does not keep a value that is infinite or NaN out of a sum: such values are taken as 0 here, and
+            // the rows that see them get them at the end.
+            bool some = false;
 #pragma unroll
             for (int db = 0; db < NDB; db++) {
               const i32x4 d = __builtin_bit_cast(i32x4, va[db]);
 #pragma unroll
-              for (int i = 0; i < 4; i++) odd = odd || odd16<T>((unsigned)d[i]);
+              for (int i = 0; i < 4; i++) some |= odd16<T>((unsigned)d[i]) | odd16<T>((unsigned)d[i] << 16);
             }
-            if (__builtin_expect(__any(odd), 0)) {
-              const int seen = min(max(last + 1 - (blk * KB + 16 * s2), 0), 16);
-              for (unsigned long long left = __ballot(seen > 0); left;) {
-                const int n = __builtin_amdgcn_readlane(seen, __builtin_ctzll(left));
+            if (__builtin_expect(__any(some), 0)) {
+              odd = true;
 #pragma unroll
-                for (int db = 0; db < NDB; db++) {
-                  i16x8 vz = va[db];
+              for (int db = 0; db < NDB; db++)
 #pragma unroll
-                  for (int e = 0; e < 8; e++)
-                    if (8 * hl + e >= n) vz[e] = 0;
-                  const f32x16 u = mma_pv<T>(vz, __builtin_bit_cast(VT8, pb[s2]), o[db]);
-#pragma unroll
-                  for (int i = 0; i < 16; i++) o[db][i] = seen == n ? u[i] : o[db][i];
-                }
-                left &= ~__ballot(seen == n);
-              }
-              continue;
+                for (int e = 0; e < 8; e++)
+                  if (odd16<T>((unsigned)va[db][e] << 16)) va[db][e] = 0;
             }
           }
 #pragma unroll
@@ -396,7 +406,8 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
                       o[db][4 * g + 3]);
     float *ml = (float *)(smem + NW * RT * C::ORS);
     if (hl == 0) *(float2 *)(ml + (w * RT + l32) * 2) = make_float2(m, lt);
-    __syncthreads();
+    if (CAUSAL) odd = __syncthreads_or(odd);
+    else __syncthreads();
     constexpr int PPR = DG / 8;
     for (int c = tid; c < R * PPR; c += NW * 64) {
       const int r = c / PPR, d0 = 8 * (c - r * PPR);
@@ -423,6 +434,20 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
           v[4 + e] += wt * hi[e];
         }
       }
+      if (CAUSAL && __builtin_expect(odd, 0)) {  // the values left out above, from the first key that some row does not see
+        const i64 seen = plan::clamp(q.off + m0 + rt + 1, 0, min(q.L, (i64)blk1 * KB));
+        for (i64 key = max((i64)blk0 * KB, (first_last + 1) / KB * KB); key < seen; key++) {
+          const int pg = bt.table[(size_t)tile.b * bt.width + (key >> bt.lg)];
+          if (pg < 0 || pg >= bt.pages) continue;
+          const size_t row = (((size_t)pg * p.KVH + kvh) << bt.lg) + (size_t)(key & ((1 << bt.lg) - 1));
+          const i32x4 vv = *(const i32x4 *)(a.vc + row * C::RBG + d0 * 2);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const unsigned u = (unsigned)vv[e / 2] << (e & 1 ? 0 : 16);
+            if (odd16<T>(u)) v[e] += (u & (T == T_BF16 ? 0x007F0000u : 0x03FF0000u)) ? NAN : (int)u < 0 ? -INFINITY : INFINITY;
+          }
+        }
+      }
       if (whole) {
         // no sum although a key is visible: all scores are -infinity, and 0 / 0
         const bool any = CAUSAL ? q.L > 0 && q.off + m0 + rt >= 0 : q.L > 0;
@@ -447,51 +472,77 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, Batch b
                                                              Heads hd, int least, int most) {
   const int j = blockIdx.x, lane = threadIdx.x & 63;
   const Order order(sh, bt);
-  const i64 total = order.total();
-  if (total <= 0) return;
-  const int nsl = plan::slices(total, most, least);
-  if (j + 1 >= nsl) return;
-  const i64 x = plan::slice_start(total, nsl, j + 1);
+  if (order.all <= 0) return;
+  const plan::Cut cut = plan::cut(order.all, order.tiles, most, least);
+  if (j + 1 >= cut.n) return;
+  const i64 x = plan::slice_start(cut, j + 1);
   Tile c;
-  if (!tile_at(order, x, &c) || c.p >= x || c.p < plan::slice_start(total, nsl, j)) return;
+  if (!tile_at(order, x, &c) || c.p >= x || c.p < plan::slice_start(cut, j)) return;
   const int nblk = plan::tile_blocks(sh, c.q, c.t, KB);
   const int kvh = c.v / hd.HS, g0 = (c.v - kvh * hd.HS) * hd.GP;
   const int m0 = c.q.lo + c.t * sh.TT, R = min(sh.TT, c.q.hi - m0) * hd.GP;
   int n = j + 1;  // the slice behind the tile's last part
-  while (n < nsl && plan::slice_start(total, nsl, n) < c.p + c.w) n++;
+  for (int in = 64; in == 64; n += in)
+    in = __popcll(__ballot(n + lane < cut.n && plan::slice_start(cut, n + lane) < c.p + c.w));
+  // a wave takes a row: its lower and upper half every other part, 4 channels a lane
+  const int half = lane >> 5, d0 = 4 * (lane & 31), d = min(d0, DG - 4);
   for (int r = threadIdx.x >> 6; r < R; r += 4) {
     const int rt = (int)((unsigned)r / (unsigned)hd.GP), rg = r - rt * hd.GP;
     if (g0 + rg >= hd.G) continue;
-    constexpr int PER = DG > 64 ? 2 : 1;
-    const int d0 = PER * lane;
-    float mx = -INFINITY, sum = 0.0f, v[2] = {0.0f, 0.0f};
-    for (int i = j; i < n; i++) {
-      const i64 s0 = plan::slice_start(total, nsl, i), s1 = plan::slice_start(total, nsl, i + 1);
-      if (plan::block_at(s0, c.p, c.w, nblk) == plan::block_at(s1, c.p, c.w, nblk)) continue;  // nothing was written
-      const float *st = a.ws + (size_t)plan::state_of(i, c.p < s0) * (RT * (DG + 2));
-      const float2 s = *(const float2 *)(st + RT * DG + 2 * r);
-      const float m = fmaxf(mx, s.x);
-      const float f0 = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mx - m);
-      const float f1 = s.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s.x - m);
-      mx = m;
-      sum = sum * f0 + s.y * f1;
-      if (d0 < DG)
+    float mx = -INFINITY, sum = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = j; i0 < n; i0 += 64) {  // 64 parts at a time, one a lane: their places and weights
+      const int i = i0 + lane;
+      int place = -1;
+      float2 s = make_float2(-INFINITY, 0.0f);
+      if (i < n) {
+        const i64 s0 = plan::slice_start(cut, i), s1 = plan::slice_start(cut, i + 1);
+        if (plan::block_at(s0, c.p, c.w, nblk) != plan::block_at(s1, c.p, c.w, nblk)) {  // else nothing was written
+          place = plan::state_of(i, c.p < s0);
+          s = *(const float2 *)(a.ws + (size_t)place * (RT * (DG + 2)) + RT * DG + 2 * r);
+        }
+      }
+      float top = s.x;
 #pragma unroll
-        for (int e = 0; e < PER; e++) v[e] = v[e] * f0 + st[r * DG + d0 + e] * f1;
+      for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+      top = fmaxf(top, mx);
+      const float f0 = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mx - top);
+      const float f = s.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s.x - top);
+      float add = f * s.y;
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) add += __shfl_xor(add, k);
+      mx = top;
+      sum = sum * f0 + add;
+      v *= f0;
+      const int parts = min(64, n - i0);
+      constexpr int AHEAD = 16;  // loads of a lane in flight
+      for (int k0 = 0; k0 < parts; k0 += 2 * AHEAD) {
+        f32x4 u[AHEAD];
+        float fk[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+          const int from = k0 + 2 * k + half, at = __shfl(place, from);
+          fk[k] = __shfl(f, from);
+          u[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (at >= 0) u[k] = *(const f32x4 *)(a.ws + (size_t)at * (RT * (DG + 2)) + r * DG + d);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) v += fk[k] * u[k];
+      }
     }
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], 32);
     const bool any = CAUSAL ? c.q.L > 0 && c.q.off + m0 + rt >= 0 : c.q.L > 0;
     const float inv = sum != 0.0f ? 1.0f / sum : any ? NAN : 0.0f;
-    using E = typename Vec8<T>::elem;
-    E *dst = (E *)a.out + (size_t)(m0 + rt) * p.o_stride + (size_t)(kvh * hd.G + g0 + rg) * DG + d0;
-    if (d0 < DG)
-#pragma unroll
-      for (int e = 0; e < PER; e++) dst[e] = (E)(v[e] * inv);
+    if (lane < DG / 4)
+      store4<T>(a.out + ((size_t)(m0 + rt) * p.o_stride + (size_t)(kvh * hd.G + g0 + rg) * DG + d0) * 2, v[0] * inv,
+                v[1] * inv, v[2] * inv, v[3] * inv);
   }
 }
 
-template <int DG, int T, bool CAUSAL>
-int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
-  constexpr int NW = 4;
+template <int DG, int T, bool CAUSAL, int NW>
+int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Shape &sh,
+             const Heads &hd, unsigned grid, int least, std::string *err) {
   using C = Rows<DG, NW>;
   auto kern = attention_rows_kernel<DG, T, NW, CAUSAL>;
   static bool attr_set = false;
@@ -503,18 +554,25 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
     }
     attr_set = true;
   }
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(NW * 64), C::LDS, ex.stream, a, bt, p, sh, hd, least);
+  return 0;
+}
+
+template <int DG, int T, bool CAUSAL>
+int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
   const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
   const Heads hd{G, HS, GP};
   const int cus = std::max(1, cu_count());
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
   const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float);
-  const int least = 256, most = (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state));
-  const bool each = tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= 8 * most);
+  const int least = 256, most = std::max(1, (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state)));
+  const bool few = tiles <= cus && p.max_kv <= 2048;
+  const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= 8 * most));
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(each ? tiles : std::max(most, 1))), dim3(NW * 64), C::LDS, ex.stream, g, bt, p, sh,
-                     hd, least);
+  if (few) return run_rows<DG, T, CAUSAL, 8>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
+  if (run_rows<DG, T, CAUSAL, 4>(ex, g, bt, p, sh, hd, (unsigned)(each ? tiles : most), least, err)) return -1;
   if (!each && most > 1)
     hipLaunchKernelGGL((attention_join_kernel<DG, T, CAUSAL>), dim3((unsigned)(most - 1)), dim3(256), 0, ex.stream, g, bt, p,
                        sh, hd, least, most);

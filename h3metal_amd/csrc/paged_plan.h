@@ -31,6 +31,14 @@ struct Shape {
   i64 most;     // keys the page table can name
 };
 
+// a / b rounded down for 0 <= a, 1 <= b and a quotient below 2^50, by way of doubles (off by one at most): a 64-bit integer
+// division is some 150 instructions
+H3_HD i64 div(i64 a, i64 b) {
+  i64 q = (i64)((double)a / (double)b);
+  const i64 r = a - q * b;
+  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
+}
+
 // A sequence's part of the batch: rows lo .. hi - 1, L keys, row m sees keys up to off + m (with a causal mask); K tiles a head
 // group, tile t weighs a + s t.
 struct Seq {
@@ -69,7 +77,7 @@ H3_HD i64 tile_weight(const Seq &q, int t) { return q.a + q.s * t; }
 H3_HD int tile_at(const Seq &q, i64 z) {
   i64 t;
   if (q.s == 0) {
-    t = z / q.a;
+    t = div(z, q.a);
   } else {
     const double p = (double)q.a - 0.5 * (double)q.s;
     t = (i64)((sqrt(p * p + 2.0 * (double)q.s * (double)z) - p) / (double)q.s);
@@ -91,18 +99,29 @@ H3_HD int tile_blocks(const Shape &sh, const Seq &q, int t, int kb) {
   return n < 1 ? 1 : (int)n;
 }
 
-// Slice i of n begins at this weight of `total`.
-H3_HD i64 slice_start(i64 total, int n, int i) { return total / n * i + total % n * i / n; }
-
-// Slices worth making: one for each `least` of the weight, at most n.
-H3_HD int slices(i64 total, int n, int least) {
-  const i64 k = total / (least < 1 ? 1 : least);
-  return k < 1 ? 1 : k < n ? (int)k : n;
+// The cut of a weight into n slices, n below 2^16.
+struct Cut {
+  i64 each;  // weight of a slice, and what is left over all of them
+  int n, left;
+};
+H3_HD Cut cut_into(i64 total, int n) {
+  const i64 e = total / n;
+  return Cut{e, n, (int)(total - e * n)};
+}
+// At most n slices, of `least` each; as many for each tile if there are more slices than tiles, so that tiles of equal weight
+// (one token of one sequence: as many tiles as head groups) are cut alike and no slice has pieces of two.
+H3_HD Cut cut(i64 total, i64 tiles, int n, int least) {
+  const i64 k = clamp(total / (least < 1 ? 1 : least), 1, n);
+  return cut_into(total, (int)(tiles > 0 && k > tiles ? k / tiles * tiles : k));
+}
+// The weight before slice i.
+H3_HD i64 slice_start(const Cut &c, int i) {
+  return c.each * i + (int)((unsigned)c.left * (unsigned)i / (unsigned)c.n);
 }
 
 // The first key block behind weight x of a tile that starts at p, weighs w and has n blocks: where a slice that ends or
-// begins at x cuts it.
-H3_HD int block_at(i64 x, i64 p, i64 w, int n) { return x <= p ? 0 : x >= p + w ? n : (int)((x - p) * n / w); }
+// begins at x cuts it (w n below 2^63).
+H3_HD int block_at(i64 x, i64 p, i64 w, int n) { return x <= p ? 0 : x >= p + w ? n : (int)div((x - p) * n, w); }
 
 // A partial state's place: 2 i for the tile that slice i found begun, 2 i + 1 for the one it leaves unfinished.
 H3_HD int state_of(int i, bool begun) { return 2 * i + (begun ? 0 : 1); }

@@ -57,13 +57,15 @@ extern "C" int check(int M, int B, int TT, int VH, int causal, int each, int cos
     total += w * VH;
   }
   if (tiles.empty()) return 0;
-  const int n = each ? (int)total : slices(total, most_slices, least);
+  const Cut cut_ = each ? Cut{1, (int)total, 0} : cut(total, (i64)tiles.size(), most_slices, least);
+  const int n = cut_.n;
+  if (slice_start(cut_, 0) != 0 || slice_start(cut_, n) != total) return 13;
   std::map<int, std::pair<size_t, int>> state;  // place -> tile, blocks
   std::vector<std::vector<int>> done(tiles.size());
   for (size_t k = 0; k < tiles.size(); k++) done[k].assign(tiles[k].nb, 0);
   size_t first = 0;
   for (int i = 0; i < n; i++) {
-    const i64 x0 = slice_start(total, n, i), x1 = slice_start(total, n, i + 1);
+    const i64 x0 = slice_start(cut_, i), x1 = slice_start(cut_, i + 1);
     while (first < tiles.size() && tiles[first].p + tiles[first].w <= x0) first++;
     for (size_t k = first; k < tiles.size() && tiles[k].p < x1; k++) {
       const Tile &c = tiles[k];
@@ -85,18 +87,18 @@ extern "C" int check(int M, int B, int TT, int VH, int causal, int each, int cos
   std::map<size_t, int> merged;
   size_t used = 0;
   for (int j = 0; j + 1 < n; j++) {
-    const i64 x = slice_start(total, n, j + 1);
+    const i64 x = slice_start(cut_, j + 1);
     size_t k = 0;
     while (k + 1 < tiles.size() && tiles[k + 1].p <= x) k++;
     const Tile &c = tiles[k];
-    if (c.p >= x || c.p < slice_start(total, n, j)) continue;
+    if (c.p >= x || c.p < slice_start(cut_, j)) continue;
     merged[k]++;
     int blocks = 0;
-    for (int i = j; i < n && slice_start(total, n, i) < c.p + c.w; i++) {
-      const auto s = state.find(state_of(i, c.p < slice_start(total, n, i)));
+    for (int i = j; i < n && slice_start(cut_, i) < c.p + c.w; i++) {
+      const auto s = state.find(state_of(i, c.p < slice_start(cut_, i)));
       if (s == state.end() || s->second.first != k) return 8;
-      if (s->second.second != block_at(slice_start(total, n, i + 1), c.p, c.w, c.nb) -
-                                  block_at(slice_start(total, n, i), c.p, c.w, c.nb)) return 9;
+      if (s->second.second != block_at(slice_start(cut_, i + 1), c.p, c.w, c.nb) -
+                                  block_at(slice_start(cut_, i), c.p, c.w, c.nb)) return 9;
       blocks += s->second.second;
       used++;
     }
