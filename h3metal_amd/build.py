@@ -38,11 +38,13 @@ PER_FILE = {
     "rows_q8.hip": ["-ffp-contract=off"],
     # score MFMAs with VGPR results (the softmax reads them), P V accumulators in AGPRs (inline assembly)
     "attention_wave.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "attention_paged_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 # sources whose inline assembly (MFMAs, DPP fmacs) is checked for hazards in the generated code (isa_check.py)
-ISA_CHECKED = ["attention_wave.hip", "qk_prepass.hip", "rot_q8.hip"]
+ISA_CHECKED = ["attention_wave.hip", "attention_paged.hip", "attention_paged_chunk.hip", "qk_prepass.hip", "rot_q8.hip"]
 SOURCES = ["attention_wave.hip", "attention.hip", "attention_small.hip", "capi.hip", "qk_prepass.hip", "rot_q8.hip",
-           "gemm.hip", "gemm_ksplit.hip", "gemm_f8.hip", "rows_q8.hip", "rope_paged.hip", "attention_paged.hip"]
+           "gemm.hip", "gemm_ksplit.hip", "gemm_f8.hip", "rows_q8.hip", "rope_paged.hip", "attention_paged.hip",
+           "attention_paged_chunk.hip"]
 
 
 def hipcc() -> str:

@@ -12,8 +12,7 @@
 // transposing LDS reads). The loads of a block's two 16-key halves go through descriptors that end at the sequence's last
 // key: what a page holds behind it reads as zero.
 #include "attention_common.h"
-#include "paged.h"
-#include "paged_plan.h"
+#include "paged_attn.h"
 
 #include <algorithm>
 #include <cmath>
@@ -22,142 +21,9 @@
 namespace h3 {
 namespace {
 
-using plan::i64;
-
 constexpr int RT = 32;             // rows of a tile
 constexpr int KB = 32;             // keys of a block
 constexpr float SLACK_P = 8.0f;    // log2 units the running maximum may lag behind a score
-
-// Query heads of a tile: a key/value head's G heads in HS groups of GP (the last may have fewer).
-struct Heads {
-  int G, HS, GP;
-};
-
-struct AttnArgs {
-  const char *q, *kc, *vc;
-  char *out;
-  float *ws;  // partial states: O [RT][D], then m and l of each row
-};
-
-// -- finding the work -------------------------------------------------------------------------------------------------
-
-__device__ __forceinline__ i64 wave_sum_to(i64 v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const i64 u = __shfl_up(v, d);
-    v += lane >= d ? u : 0;
-  }
-  return v;
-}
-__device__ __forceinline__ i64 lane_value(i64 v, int l) {
-  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)v, l), hi = __builtin_amdgcn_readlane((int)(v >> 32), l);
-  return (i64)(((unsigned long long)hi << 32) | lo);
-}
-
-// The batch's weight, and the sequence at a weight of it; 64 sequences at a time, one a lane.
-struct Order {
-  const plan::Shape &sh;
-  const Batch &bt;
-  int q0, q1, kv;        // of the first 64 sequences: this lane's
-  i64 own, upto, first;  // its weight, the sum up to it, their sum
-  i64 all, tiles;        // the batch's weight and tiles
-
-  __device__ Order(const plan::Shape &s, const Batch &b) : sh(s), bt(b) {
-    int K;
-    own = weight(threadIdx.x & 63, &q0, &q1, &kv, &K);
-    if (bt.B == 1) {
-      upto = own = all = first = lane_value(own, 0);
-      tiles = (i64)__builtin_amdgcn_readfirstlane(K) * sh.VH;
-      return;
-    }
-    upto = wave_sum_to(own);
-    all = first = lane_value(upto, 63);
-    i64 mine = K;
-    for (int k = 64; k < bt.B; k += 64) {
-      int x, y, z;
-      all += lane_value(wave_sum_to(weight(k + (threadIdx.x & 63), &x, &y, &z, &K)), 63);
-      mine += K;
-    }
-    tiles = lane_value(wave_sum_to(mine), 63) * sh.VH;
-  }
-  __device__ i64 weight(int b, int *s0, int *s1, int *n, int *K) const {
-    *s0 = *s1 = *n = 0;
-    if (b < bt.B) {
-      *s0 = bt.q_start[b];
-      *s1 = bt.q_start[b + 1];
-      *n = bt.kv_len[b];
-    }
-    const plan::Seq q = plan::seq_of(sh, *s0, *s1, *n);
-    *K = q.K;
-    return plan::head_weight(q) * sh.VH;
-  }
-  // the sequence at weight x, and the weight before it
-  __device__ int find(i64 x, i64 *before) const {
-    i64 base = 0, w = own, s = upto, sum = first;
-    for (int k = 0;; k += 64) {
-      const unsigned long long m = __ballot(base + s > x);
-      if (m) {
-        const int l = __builtin_ctzll(m);
-        *before = base + lane_value(s - w, l);
-        return __builtin_amdgcn_readfirstlane(k + l);
-      }
-      if (k + 64 >= bt.B) return -1;
-      base += sum;
-      int t0, t1, t2, t3;
-      w = weight(k + 64 + (threadIdx.x & 63), &t0, &t1, &t2, &t3);
-      s = wave_sum_to(w);
-      sum = lane_value(s, 63);
-    }
-  }
-  __device__ plan::Seq seq(int b) const {  // one sequence for the wave: scalar values
-    if (b < 64)
-      return plan::seq_of(sh, __builtin_amdgcn_readlane(q0, b), __builtin_amdgcn_readlane(q1, b), __builtin_amdgcn_readlane(kv, b));
-    return plan::seq_of(sh, __builtin_amdgcn_readfirstlane(bt.q_start[b]), __builtin_amdgcn_readfirstlane(bt.q_start[b + 1]),
-                        __builtin_amdgcn_readfirstlane(bt.kv_len[b]));
-  }
-};
-
-// A tile: sequence, head group, place in the group, the weight before it and its own.
-struct Tile {
-  int b, v, t;
-  i64 p, w;
-  plan::Seq q;
-};
-__device__ __forceinline__ bool tile_at(const Order &o, i64 x, Tile *c) {
-  i64 before;
-  c->b = o.find(x, &before);
-  if (c->b < 0) return false;
-  c->q = o.seq(c->b);
-  const i64 w = plan::head_weight(c->q), y = x - before;
-  c->v = __builtin_amdgcn_readfirstlane((int)plan::div(y, w));
-  c->t = __builtin_amdgcn_readfirstlane(plan::tile_at(c->q, y - w * c->v));
-  c->p = before + w * c->v + plan::before_tile(c->q, c->t);
-  c->w = plan::tile_weight(c->q, c->t);
-  return true;
-}
-__device__ __forceinline__ bool next_tile(const Order &o, Tile *c) {
-  c->p += c->w;
-  if (++c->t == c->q.K) {
-    c->t = 0;
-    if (++c->v == o.sh.VH) {
-      c->v = 0;
-      do {
-        if (++c->b >= o.bt.B) return false;
-        c->q = o.seq(c->b);
-      } while (!c->q.K);
-    }
-  }
-  c->w = plan::tile_weight(c->q, c->t);
-  return true;
-}
-
-// The slice of a workgroup: workgroup b runs on XCD b % 8; each XCD takes a contiguous run of the slices, so that tiles that share
-// keys share an L2.
-__device__ __forceinline__ int slice_of(int b, int n) {
-  const int per = n >> 3, rem = n & 7, xcd = b & 7;
-  return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (b >> 3);
-}
 
 // -- tiles of 32 rows -------------------------------------------------------------------------------------------------
 
@@ -195,10 +61,12 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const Order order(sh, bt);
-  if (order.all <= 0) return;
   plan::Cut cut{1, (int)(order.all < (i64)gridDim.x ? order.all : (i64)gridDim.x), 0};
   if (!sh.each) cut = plan::cut(order.all, order.tiles, gridDim.x, least);
-  if ((int)blockIdx.x >= cut.n) return;
+  if (order.all <= 0 || (int)blockIdx.x >= cut.n) {
+    if (!sh.each && tid == 0) left_of(a, blockIdx.x)->R = 0;
+    return;
+  }
   int sl = slice_of(blockIdx.x, cut.n);
   if (sh.each) sl = cut.n - 1 - sl;  // with a causal mask the longest tiles go first
   const i64 x0 = plan::slice_start(cut, sl), x1 = plan::slice_start(cut, sl + 1);
@@ -220,6 +88,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
   const int l16 = lane & 15, tr_row = l16 >> 2, tr_col = (l16 & 3) * 8;
 
   Tile tile;
+  bool unfinished = false;
   bool more = tile_at(order, x0, &tile);
   for (; more && tile.p < x1; more = next_tile(order, &tile)) {
     const plan::Seq &q = tile.q;
@@ -231,16 +100,28 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
       blk1 = plan::block_at(x1, tile.p, tile.w, nblk);
       begun = tile.p < x0;
       whole = !begun && tile.p + tile.w <= x1;
-      if (blk0 == blk1) continue;  // (a whole tile has a block)
     }
     const int kvh = tile.v / hd.HS, g0 = (tile.v - kvh * hd.HS) * hd.GP;
     const int m0 = q.lo + tile.t * sh.TT, R = min(sh.TT, q.hi - m0) * hd.GP;
     const int L = (int)q.L;
+    const i64 first_last = CAUSAL ? plan::clamp(q.off + m0, -M_MOST, q.L - 1) : q.L - 1;  // of the tile's first token
+    float *st = a.ws + (size_t)plan::state_of(sl, begun) * (RT * (DG + 2));
+    if (!whole && !begun) {
+      const int end = last_slice(cut, sl, tile.p + tile.w);
+      // (rows of a causal tile that see no key begin before the sequence; without keys none sees any)
+      if (tid == 0)
+        *left_of(a, sl) = Left{R, m0, kvh * hd.G + g0, hd.GP, min(hd.GP, hd.G - g0),
+                               q.L > 0 ? CAUSAL ? (int)first_last : 0 : -M_MOST, end, 0};
+      unfinished = true;
+    }
+    if (blk0 == blk1) {  // a part without blocks (a whole tile has one)
+      if (tid < R) *(float2 *)(st + RT * DG + 2 * tid) = make_float2(-INFINITY, 0.0f);
+      continue;
+    }
     // this lane's query row: its token, head and last visible key
     const int ti = (int)((unsigned)l32 / (unsigned)hd.GP), gi = l32 - ti * hd.GP;
     const bool ok = l32 < R && g0 + gi < hd.G;
     const int last = !ok ? -1 : CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
-    const i64 first_last = CAUSAL ? plan::clamp(q.off + m0, -1, q.L - 1) : q.L - 1;  // of the tile's first token
     i32x4 qreg[NCH];
     {
       const char *qrow = a.q + ((size_t)(m0 + (ok ? ti : 0)) * p.q_stride + (size_t)(kvh * hd.G + (ok ? g0 + gi : 0)) * DG) * 2;
@@ -436,7 +317,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
       }
       if (CAUSAL && __builtin_expect(odd, 0)) {  // the values left out above, from the first key that some row does not see
         const i64 seen = plan::clamp(q.off + m0 + rt + 1, 0, min(q.L, (i64)blk1 * KB));
-        for (i64 key = max((i64)blk0 * KB, (first_last + 1) / KB * KB); key < seen; key++) {
+        for (i64 key = max((i64)blk0 * KB, max(first_last + 1, (i64)0) / KB * KB); key < seen; key++) {
           const int pg = bt.table[(size_t)tile.b * bt.width + (key >> bt.lg)];
           if (pg < 0 || pg >= bt.pages) continue;
           const size_t row = (((size_t)pg * p.KVH + kvh) << bt.lg) + (size_t)(key & ((1 << bt.lg) - 1));
@@ -456,7 +337,6 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
         store4<T>(dst, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
         store4<T>(dst + 8, v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
       } else {
-        float *st = a.ws + (size_t)plan::state_of(sl, begun) * (RT * (DG + 2));
         store4<T_F32>((char *)(st + r * DG + d0), v[0], v[1], v[2], v[3]);
         store4<T_F32>((char *)(st + r * DG + d0 + 4), v[4], v[5], v[6], v[7]);
         if (d0 == 0) *(float2 *)(st + RT * DG + 2 * r) = make_float2(mx, sum);
@@ -464,81 +344,17 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
     }
     __syncthreads();  // before the next tile's loads
   }
+  if (!sh.each && !unfinished && tid == 0) left_of(a, sl)->R = 0;
 }
 
-// Joins the parts of cut tiles: workgroup j, the tile that slice j leaves unfinished if it begins in it. One wave per row.
-template <int DG, int T, bool CAUSAL>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh,
-                                                             Heads hd, int least, int most) {
-  const int j = blockIdx.x, lane = threadIdx.x & 63;
-  const Order order(sh, bt);
-  if (order.all <= 0) return;
-  const plan::Cut cut = plan::cut(order.all, order.tiles, most, least);
-  if (j + 1 >= cut.n) return;
-  const i64 x = plan::slice_start(cut, j + 1);
-  Tile c;
-  if (!tile_at(order, x, &c) || c.p >= x || c.p < plan::slice_start(cut, j)) return;
-  const int nblk = plan::tile_blocks(sh, c.q, c.t, KB);
-  const int kvh = c.v / hd.HS, g0 = (c.v - kvh * hd.HS) * hd.GP;
-  const int m0 = c.q.lo + c.t * sh.TT, R = min(sh.TT, c.q.hi - m0) * hd.GP;
-  int n = j + 1;  // the slice behind the tile's last part
-  for (int in = 64; in == 64; n += in)
-    in = __popcll(__ballot(n + lane < cut.n && plan::slice_start(cut, n + lane) < c.p + c.w));
-  // a wave takes a row: its lower and upper half every other part, 4 channels a lane
-  const int half = lane >> 5, d0 = 4 * (lane & 31), d = min(d0, DG - 4);
-  for (int r = threadIdx.x >> 6; r < R; r += 4) {
-    const int rt = (int)((unsigned)r / (unsigned)hd.GP), rg = r - rt * hd.GP;
-    if (g0 + rg >= hd.G) continue;
-    float mx = -INFINITY, sum = 0.0f;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i0 = j; i0 < n; i0 += 64) {  // 64 parts at a time, one a lane: their places and weights
-      const int i = i0 + lane;
-      int place = -1;
-      float2 s = make_float2(-INFINITY, 0.0f);
-      if (i < n) {
-        const i64 s0 = plan::slice_start(cut, i), s1 = plan::slice_start(cut, i + 1);
-        if (plan::block_at(s0, c.p, c.w, nblk) != plan::block_at(s1, c.p, c.w, nblk)) {  // else nothing was written
-          place = plan::state_of(i, c.p < s0);
-          s = *(const float2 *)(a.ws + (size_t)place * (RT * (DG + 2)) + RT * DG + 2 * r);
-        }
-      }
-      float top = s.x;
-#pragma unroll
-      for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
-      top = fmaxf(top, mx);
-      const float f0 = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mx - top);
-      const float f = s.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s.x - top);
-      float add = f * s.y;
-#pragma unroll
-      for (int k = 1; k < 64; k *= 2) add += __shfl_xor(add, k);
-      mx = top;
-      sum = sum * f0 + add;
-      v *= f0;
-      const int parts = min(64, n - i0);
-      constexpr int AHEAD = 16;  // loads of a lane in flight
-      for (int k0 = 0; k0 < parts; k0 += 2 * AHEAD) {
-        f32x4 u[AHEAD];
-        float fk[AHEAD];
-#pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-          const int from = k0 + 2 * k + half, at = __shfl(place, from);
-          fk[k] = __shfl(f, from);
-          u[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          if (at >= 0) u[k] = *(const f32x4 *)(a.ws + (size_t)at * (RT * (DG + 2)) + r * DG + d);
-        }
-#pragma unroll
-        for (int k = 0; k < AHEAD; k++) v += fk[k] * u[k];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] += __shfl_xor(v[e], 32);
-    const bool any = CAUSAL ? c.q.L > 0 && c.q.off + m0 + rt >= 0 : c.q.L > 0;
-    const float inv = sum != 0.0f ? 1.0f / sum : any ? NAN : 0.0f;
-    if (lane < DG / 4)
-      store4<T>(a.out + ((size_t)(m0 + rt) * p.o_stride + (size_t)(kvh * hd.G + g0 + rg) * DG + d0) * 2, v[0] * inv,
-                v[1] * inv, v[2] * inv, v[3] * inv);
-  }
+}  // namespace
+
+// Two states for each slice of the tiles of 256 rows, one a compute unit.
+size_t attention_paged_workspace_max(int cus) {
+  return (size_t)std::max(cus, 1) * (2 * CHUNK_ROWS * (128 + 2) * sizeof(float) + sizeof(Left));
 }
+
+namespace {
 
 template <int DG, int T, bool CAUSAL, int NW>
 int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Shape &sh,
@@ -559,23 +375,26 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
 }
 
 template <int DG, int T, bool CAUSAL>
-int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
+int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
+  if (DG == 128 && (rows ? rows == CHUNK_ROWS : (i64)p.max_q * (p.H / p.KVH) >= 192))
+    return launch_attention_chunk(T, CAUSAL, ex, a, bt, p, err);
   const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
   const Heads hd{G, HS, GP};
   const int cus = std::max(1, cu_count());
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
-  const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float);
+  const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float) + sizeof(Left);  // of a slice
   const int least = 256, most = std::max(1, (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state)));
   const bool few = tiles <= cus && p.max_kv <= 2048;
   const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= 8 * most));
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
+  g.left = (char *)ex.ws + most * (state - sizeof(Left));
   if (few) return run_rows<DG, T, CAUSAL, 8>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
   if (run_rows<DG, T, CAUSAL, 4>(ex, g, bt, p, sh, hd, (unsigned)(each ? tiles : most), least, err)) return -1;
   if (!each && most > 1)
-    hipLaunchKernelGGL((attention_join_kernel<DG, T, CAUSAL>), dim3((unsigned)(most - 1)), dim3(256), 0, ex.stream, g, bt, p,
-                       sh, hd, least, most);
+    hipLaunchKernelGGL((attention_join_kernel<DG, T, RT, 1>), dim3((unsigned)(most - 1), RT / 4), dim3(256), 0, ex.stream, g,
+                       p.o_stride);
   return 0;
 }
 
@@ -628,9 +447,9 @@ int launch(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const vo
       *err = std::string("out shares memory with ") + what[i];
       return -1;
     }
-  const AttnArgs g{a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, nullptr};
+  const AttnArgs g{a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, nullptr, nullptr};
   const Batch bt{(const int *)a[4].ptr, (const int *)a[5].ptr, (const int *)a[6].ptr, p.B, p.width, p.pages, lg};
-  return pl.ival[0] ? run<D, T, true>(ex, g, bt, p, err) : run<D, T, false>(ex, g, bt, p, err);
+  return pl.ival[0] ? run<D, T, true>(pl.ival[1], ex, g, bt, p, err) : run<D, T, false>(pl.ival[1], ex, g, bt, p, err);
 }
 
 template <int D>
@@ -640,12 +459,14 @@ LaunchFn pick(int t) {
 
 }  // namespace
 
-// Macros: HD (64, 96 or 128), IN_T (half | bfloat: queries, cache and output), CAUSAL.
+// Macros: HD (64, 96 or 128), IN_T (half | bfloat: queries, cache and output), CAUSAL, and ROWS, which names the rows of a
+// tile: 32, or with HD 128 256; 0 (the default) chooses them by the size.
 bool make_attention_paged(const Macros &m, Pipeline *pl, std::string *err) {
-  int hd, causal;
-  if (!macro_int(m, "HD", 128, &hd, err) || !macro_int(m, "CAUSAL", 1, &causal, err)) return false;
+  int hd, causal, rows;
+  if (!macro_int(m, "HD", 128, &hd, err) || !macro_int(m, "CAUSAL", 1, &causal, err) || !macro_int(m, "ROWS", 0, &rows, err))
+    return false;
   for (auto &kv : m)
-    if (kv.first != "HD" && kv.first != "CAUSAL" && kv.first != "IN_T") {
+    if (kv.first != "HD" && kv.first != "CAUSAL" && kv.first != "IN_T" && kv.first != "ROWS") {
       *err = "unknown macro " + kv.first;
       return false;
     }
@@ -658,8 +479,13 @@ bool make_attention_paged(const Macros &m, Pipeline *pl, std::string *err) {
     *err = "HD " + std::to_string(hd) + " not supported (64, 96 or 128)";
     return false;
   }
+  if (rows != 0 && rows != RT && !(rows == CHUNK_ROWS && hd == 128)) {
+    *err = "ROWS must be 0, 32, or 256 with HD 128";
+    return false;
+  }
   pl->launch = hd == 128 ? pick<128>(t) : hd == 96 ? pick<96>(t) : pick<64>(t);
   pl->ival[0] = causal != 0;
+  pl->ival[1] = rows;
   pl->threads = 256;
   return true;
 }

@@ -201,7 +201,8 @@ h3_ctx *h3_open(const char *kernel_dir) {
     delete ctx;
     return nullptr;
   }
-  const size_t ws = h3::attention_workspace_max(h3::cu_count());
+  const int cus = h3::cu_count();
+  const size_t ws = std::max(h3::attention_workspace_max(cus), h3::attention_paged_workspace_max(cus));
   if (!hip_ok(hipMalloc(&ctx->ws, ws), "cannot allocate the dispatch scratch memory")) {
     h3_close(ctx);
     return nullptr;

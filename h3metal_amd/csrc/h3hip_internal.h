@@ -216,6 +216,8 @@ int cu_count();
 // Scratch bytes the attention launcher's tail split can use at most on a device with `cus` compute units
 // (what h3_open reserves, so that ordinary dispatches never wait for memory).
 size_t attention_workspace_max(int cus);
+// The same of the paged attention's partial states.
+size_t attention_paged_workspace_max(int cus);
 
 // Helpers for macro parsing in the factories.
 bool macro_int(const Macros &m, const char *key, int def, int *out, std::string *err);

@@ -10,6 +10,13 @@
 #include <string>
 
 namespace h3 {
+
+// Where the batch's rows are.
+struct Batch {
+  const int *table, *q_start, *kv_len;
+  int B, width, pages, lg;  // sequences, pages a row of the table names, pages of the cache, log2 of a page's rows
+};
+
 namespace {
 
 enum { P_BF16 = 0, P_F16 = 1, P_F32 = 2 };
@@ -17,12 +24,6 @@ template <int T> struct PElem;
 template <> struct PElem<P_BF16> { using type = __bf16; };
 template <> struct PElem<P_F16> { using type = _Float16; };
 template <> struct PElem<P_F32> { using type = float; };
-
-// Where the batch's rows are.
-struct Batch {
-  const int *table, *q_start, *kv_len;
-  int B, width, pages, lg;  // sequences, pages a row of the table names, pages of the cache, log2 of a page's rows
-};
 
 // Host side: the checks both operators make of an argument and of the page table's shape.
 inline bool paged_fits(const Arg *a, int i, uint64_t bytes, int align, const char *what, std::string *err) {

@@ -7,7 +7,9 @@ cannot see there (its own builtin MFMAs it protects itself):
   destination (back-to-back accumulation, which the matrix unit forwards without wait states);
 * a VALU write of a register that an MFMA reads, within 2 wait states before that MFMA;
 * a VALU write of a register that a DPP instruction reads through its DPP operand (src0), within 2 wait states
-  before it (the cross-lane butterflies of the row kernels are DPP fmacs written as assembly).
+  before it (the cross-lane butterflies of the row kernels are DPP fmacs written as assembly);
+* a VALU write of a scalar register (v_readlane, v_readfirstlane, a comparison) that a memory access in inline assembly reads,
+  within 5 wait states before it (the descriptors of the paged attention's loads are made of lane values).
 
 The scan is straight-line over each function (a conservative approximation across branches: pending results
 are carried into the next block in layout order). Used by build.py on the sources it lists in ISA_CHECKED; also runnable as
@@ -22,6 +24,7 @@ import sys
 XDL_WAIT = 18
 VALU_TO_MFMA = 2
 VALU_TO_DPP = 2
+VALU_TO_VMEM = 5  # through a scalar register
 
 
 def _regs(tok: str) -> set:
@@ -32,11 +35,20 @@ def _regs(tok: str) -> set:
     return {(m.group(1), int(m.group(2)))} if m else set()
 
 
+def _scalars(tok: str) -> set:
+    m = re.match(r"s\[(\d+):(\d+)\]", tok)
+    if m:
+        return set(range(int(m.group(1)), int(m.group(2)) + 1))
+    m = re.match(r"s(\d+)$", tok)
+    return {int(m.group(1))} if m else set()
+
+
 def scan(text: str, name: str = "<asm>") -> list[str]:
     problems = []
     pending: dict = {}  # register -> wait states still to go after an inline-assembly MFMA wrote it
     recent: dict = {}   # register -> wait states since a VALU wrote it
     asm_dst: dict = {}  # register -> (opcode, destination operand) of the inline-assembly MFMA that wrote it
+    scalar: dict = {}   # scalar register -> wait states since a VALU wrote it
     in_asm = False
     for ln, line in enumerate(text.split("\n"), 1):
         s = line.strip()
@@ -50,12 +62,22 @@ def scan(text: str, name: str = "<asm>") -> list[str]:
             pending.clear()
             recent.clear()
             asm_dst.clear()
+            scalar.clear()
             continue
         if not s or s.startswith((".", ";", "//")):
             continue
         op = s.split()[0]
         args = [a.strip() for a in s[len(op):].split(",")] if len(s) > len(op) else []
         ws = int(s.split()[1], 0) + 1 if op == "s_nop" else 1
+        if in_asm and op.startswith(("buffer_", "global_", "flat_")):
+            hit = sorted(r for r in set().union(*[_scalars(a.split()[0]) for a in args if a])
+                         if scalar.get(r, VALU_TO_VMEM + 1) - 1 < VALU_TO_VMEM)
+            if hit:
+                problems.append(f"{name}:{ln}: VALU write of s{hit[0]} {scalar[hit[0]] - 1} wait states before: {s}")
+        for r in _scalars(args[0]) if args else ():
+            scalar.pop(r, None)
+            if op.startswith("v_"):
+                scalar[r] = 0
         if op.startswith("v_mfma"):
             dst = _regs(args[0])
             for r in set().union(*[_regs(a) for a in args[1:]]):
@@ -98,6 +120,10 @@ def scan(text: str, name: str = "<asm>") -> list[str]:
             pending[r] -= ws
             if pending[r] <= 0:
                 del pending[r]
+        for r in list(scalar):
+            scalar[r] += ws
+            if scalar[r] > VALU_TO_VMEM + 1:
+                del scalar[r]
         for r in list(recent):
             recent[r] += ws
             if recent[r] > max(VALU_TO_MFMA, VALU_TO_DPP) + 1:

@@ -241,7 +241,8 @@ def qk_norm_rope_paged(gpu: Gpu, qkv: Tensor, wq: Tensor | None, wk: Tensor | No
 
 def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, table: Tensor, q_start: Tensor, kv_len: Tensor, *,
                     M: int, B: int, H: int, KVH: int, D: int, scale: float, causal: bool = True, q_stride: int | None = None,
-                    o_stride: int | None = None, max_q: int | None = None, max_kv: int | None = None, no_alloc: bool = False):
+                    o_stride: int | None = None, max_q: int | None = None, max_kv: int | None = None, no_alloc: bool = False,
+                    **variant):
     """Attention of a batch's new tokens, one or many a sequence, over a paged cache: per query head h the softmax over the
     visible keys of (scale * q_i . k_j), the weights applied to the values; 0 where no key is visible.
 
@@ -258,12 +259,13 @@ def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, ta
     not reach its output. A page number outside the cache makes the scores of its keys NaN; kv_len past the table's
     pages counts up to them. max_q and max_kv, the most new tokens and keys of a sequence as far as the caller knows, choose
     the kernel and how far it splits the keys (default: M, and the table's pages); results hold whatever they say. no_alloc: the
-    allocation-free entry point; its scratch array may split the keys less far."""
+    allocation-free entry point; its scratch array may split the keys less far. variant: ROWS names the rows of a tile (32, or
+    256 with head dim 128), which is chosen by the size otherwise."""
     if q.dtype != kc.dtype or out.dtype != q.dtype:
         raise ValueError(f"attention_paged: q, kc, vc and out must all be f16 or all bf16, got {q.dtype}, {kc.dtype}, "
                          f"{vc.dtype}, {out.dtype}")
     pages, page, width = _paged("attention_paged", kc, vc, table, q_start, kv_len, KVH, D)
-    k = gpu.kernel("attention", "attention_paged", HD=D, IN_T=OUT_DT[q.dtype], CAUSAL=1 if causal else 0)
+    k = gpu.kernel("attention", "attention_paged", HD=D, IN_T=OUT_DT[q.dtype], CAUSAL=1 if causal else 0, **variant)
     params = _PACK_11IF(M, B, H, KVH, q_stride or H * D, o_stride or H * D, pages, page, width, M if max_q is None else max_q,
                         min(width * page, 0x7FFFFFFF) if max_kv is None else max_kv, scale * LOG2E)
     gpu.launch(k, None, None, [q, kc, vc, out, table, q_start, kv_len], params, no_alloc=no_alloc)
