@@ -447,7 +447,7 @@ int launch(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const vo
       *err = std::string("out shares memory with ") + what[i];
       return -1;
     }
-  const AttnArgs g{a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, nullptr, nullptr};
+  const AttnArgs g{a[0].ptr, a[1].ptr, a[2].ptr, a[3].ptr, nullptr, nullptr, nullptr};
   const Batch bt{(const int *)a[4].ptr, (const int *)a[5].ptr, (const int *)a[6].ptr, p.B, p.width, p.pages, lg};
   return pl.ival[0] ? run<D, T, true>(pl.ival[1], ex, g, bt, p, err) : run<D, T, false>(pl.ival[1], ex, g, bt, p, err);
 }

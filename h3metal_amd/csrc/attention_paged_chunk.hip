@@ -11,7 +11,7 @@
 //    lane, from page numbers loaded 16 blocks before, and read lane by lane into the descriptors of the loads.
 //  * Rows see keys up to one of their own: the blocks that some row does not see whole run in a loop of their own, which masks.
 //  * V of those blocks is searched in LDS for infinities and NaN, which a weight of 0 would not keep out of a sum: they are taken
-//    as 0, and the rows that see them get them at the end.
+//    as 0, and the rows that see them get them at the end. So is what a page holds behind the sequence's end.
 #include "paged_attn.h"
 
 #include <algorithm>
@@ -42,7 +42,7 @@ constexpr int NCH = RB / 32;              // score MFMAs per 32 x 32 tile
 constexpr int NR = 4;                     // blocks of a ring
 constexpr int KBYTES = BK * RB;           // a block of K or V
 constexpr int VOFF = NR * KBYTES;
-constexpr int LDSC = 2 * NR * KBYTES;
+constexpr int LDSC = RTC * (D * 4 + 16) > 2 * NR * KBYTES ? RTC * (D * 4 + 16) : 2 * NR * KBYTES;  // rings, then outputs
 constexpr int GPB = BK / 16;              // 16-key groups of a block, one 1 KB load of a wave each
 static_assert(KBYTES == GPB * NWC * 1024, "a wave loads 4 rows of each group");
 
@@ -55,6 +55,10 @@ __device__ __forceinline__ bool odd_high(unsigned v) {  // the 16-bit value in t
   constexpr unsigned E = VT == T_BF16 ? 0x7F800000u : 0x7C000000u;
   return (v & E) == E;
 }
+
+struct __attribute__((packed, aligned(8))) Piece {  // 16 bytes of an output row, whose rows are aligned to 8
+  float v[4];
+};
 
 template <int VT, bool CAUSAL>
 __global__ __launch_bounds__(NWC * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
@@ -89,6 +93,9 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
   for (int db = 0; db < D / 32; db++) vbase[db] = voff<D>(8 * hl + tr_row, (db * 32 + (l32 & 16)) / 8) + tr_col;
 #pragma unroll
   for (int c = 0; c < NCH; c++) kbase[c] = krow * RB + (((2 * c + hl) ^ kswz<RB, RB / 16>(krow)) * 16);
+
+  const float per_token = 1.0f / (float)hd.GP;
+  auto row_token = [&](int r) __attribute__((always_inline)) { return (int)(((float)r + 0.5f) * per_token); };  // r / GP
 
   Tile tile;
   bool unfinished = false;
@@ -125,27 +132,24 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     // blocks (from blk0 on) that every row sees whole
     const int clear = __builtin_amdgcn_readfirstlane((int)plan::clamp(max(first_last + 1, (i64)0) / BK - blk0, 0, nblk));
 
-    // Q operands (B of S^T = K Q^T) and the last visible key of this lane's rows
+    // Q operands (B of S^T = K Q^T), and the last visible key of this lane's rows
     i32x4 qreg[NU][NCH];
     int last[NU];
+    const char *qrow[NU];
+    bool ok[NU];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       const int r = w * (32 * NU) + 32 * u + l32;
-      const int ti = (int)((unsigned)r / (unsigned)hd.GP), gi = r - ti * hd.GP;
-      const bool ok = r < R && g0 + gi < hd.G;
-      last[u] = !ok ? -1 : CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
-      const char *qrow = a.q + ((size_t)(m0 + (ok ? ti : 0)) * p.q_stride + (size_t)(kvh * hd.G + (ok ? g0 + gi : 0)) * D) * 2;
-#pragma unroll
-      for (int c = 0; c < NCH; c++) {
-        i32x4 v = *(const i32x4 *)(qrow + (2 * c + hl) * 16);
-        qreg[u][c] = ok ? v : i32x4{0, 0, 0, 0};
-        asm volatile("" : "+a"(qreg[u][c]));  // from here on Q lives in AGPRs only
-      }
+      const int ti = row_token(r), gi = r - ti * hd.GP;
+      ok[u] = r < R && g0 + gi < hd.G;
+      last[u] = !ok[u] ? -1 : CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
+      qrow[u] = a.q + ((size_t)(m0 + (ok[u] ? ti : 0)) * p.q_stride + (size_t)(kvh * hd.G + (ok[u] ? g0 + gi : 0)) * D) * 2;
     }
 
-    // -- staging. 64 groups of 16 keys (16 blocks from a multiple of 16 on, counted from blk0), one a lane: the offset of their rows
-    // in either cache and the rows that are there; those of K (blocks up to j + 3) and those of V (up to j + 1)
-    unsigned koff_lo, koff_hi, krows, voff_lo, voff_hi, vrows;
+    // -- staging. The addresses of 64 groups of 16 keys (16 blocks from a multiple of 16 on, counted from blk0), one a lane: those
+    // of K (blocks up to j + 3), those of V beside them, and those of V still in use (up to j + 1). Groups past the sequence and
+    // those whose page number lies outside the cache take other memory, which their rows' masks or `lost` keep out.
+    unsigned k_lo, k_hi, v_lo, v_hi, vnext_lo, vnext_hi;
     i64 lost = 0x7fffffffffffffffll;  // the first key whose page number lies outside the cache
     auto group_key = [&](int win) __attribute__((always_inline)) { return ((i64)blk0 * GPB + win * 64 + lane) * 16; };
     auto fetch = [&](int win) __attribute__((always_inline)) {
@@ -158,38 +162,50 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       const unsigned long long bad = __ballot(there && !in);
       if (__builtin_expect(bad != 0, 0)) lost = min(lost, ((i64)blk0 * GPB + win * 64 + __builtin_ctzll(bad)) * 16);
       const unsigned long long off =
-          ((((unsigned long long)(there && in ? id : 0) * p.KVH + kvh) << bt.lg) + (key & ((1 << bt.lg) - 1))) * RB;
-      koff_lo = (unsigned)off;
-      koff_hi = (unsigned)(off >> 32);
-      krows = there && in ? (unsigned)plan::clamp(L - key, 0, 16) : 0;
+          ((((unsigned long long)id * p.KVH + kvh) << bt.lg) + (key & ((1 << bt.lg) - 1))) * RB;
+      const unsigned long long ka = (unsigned long long)(there && in ? a.kc + off : a.spare);
+      const unsigned long long va = (unsigned long long)(there && in ? a.vc + off : a.spare);
+      k_lo = (unsigned)ka;
+      k_hi = (unsigned)(ka >> 32);
+      vnext_lo = (unsigned)va;
+      vnext_hi = (unsigned)(va >> 32);
     };
     int ahead;  // page numbers of the window behind K's
     auto windows = [&](int j) __attribute__((always_inline)) {  // before the loads of step j
       if (((j + 1) & 15) == 0) {
-        voff_lo = koff_lo;
-        voff_hi = koff_hi;
-        vrows = krows;
+        v_lo = vnext_lo;
+        v_hi = vnext_hi;
       }
       if (((j + 3) & 15) == 0) {
         addresses(ahead, (j + 3) >> 4);
         ahead = fetch(((j + 3) >> 4) + 1);
       }
     };
-    auto rsrc = [&](const char *base, unsigned lo, unsigned hi, unsigned rows, int at) __attribute__((always_inline)) {
-      const unsigned long long off = (unsigned)__builtin_amdgcn_readlane((int)lo, at) |
-                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, at) << 32;
-      return __builtin_amdgcn_make_buffer_rsrc((void *)(base + off), (short)0,
-                                               __builtin_amdgcn_readlane((int)rows, at) * RB, 0x00020000);
+    auto stage = [&](unsigned lds, int add, unsigned go, unsigned lo, unsigned hi, int at) __attribute__((always_inline)) {
+      const unsigned long long base = (unsigned)__builtin_amdgcn_readlane((int)lo, at) |
+                                      (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, at) << 32;
+      // a lane value takes 5 wait states to reach a memory access as a scalar
+      asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %2, %3" ::"s"(lds), "i"(add), "v"(go), "s"(base)
+                   : "memory", "m0", "scc");
     };
+    const unsigned lds_w = lds0 + w * 1024;
     // load i < 4: group i of K of block kb; from 4 on: of V of block vb
-    auto stage_one = [&](int i, int kb, int vb) __attribute__((always_inline)) {
-      if (i < GPB) {
-        dma16(lds0 + (kb & (NR - 1)) * KBYTES + (i * NWC + w) * 1024, kgo,
-              rsrc(a.kc, koff_lo, koff_hi, krows, (kb & 15) * GPB + i));
-      } else {
-        const int r = i - GPB;
-        dma16(lds0 + VOFF + (vb & (NR - 1)) * KBYTES + (r * NWC + w) * 1024, vgo,
-              rsrc(a.vc, voff_lo, voff_hi, vrows, (vb & 15) * GPB + r));
+    auto stage_one = [&](auto ic, int kb, int vb) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, r = i & (GPB - 1);
+      if (i < GPB) stage(lds_w + (kb & (NR - 1)) * KBYTES, r * NWC * 1024, kgo, k_lo, k_hi, (kb & 15) * GPB + r);
+      else stage(lds_w + (vb & (NR - 1)) * KBYTES, VOFF + r * NWC * 1024, vgo, v_lo, v_hi, (vb & 15) * GPB + r);
+    };
+
+    auto stage_k = [&](int k, int kb, int vb) __attribute__((always_inline)) {  // (k is known where this is inlined)
+      switch (k) {
+        case 0: stage_one(std::integral_constant<int, 0>{}, kb, vb); break;
+        case 1: stage_one(std::integral_constant<int, 1>{}, kb, vb); break;
+        case 2: stage_one(std::integral_constant<int, 2>{}, kb, vb); break;
+        case 3: stage_one(std::integral_constant<int, 3>{}, kb, vb); break;
+        case 4: stage_one(std::integral_constant<int, 4>{}, kb, vb); break;
+        case 5: stage_one(std::integral_constant<int, 5>{}, kb, vb); break;
+        case 6: stage_one(std::integral_constant<int, 6>{}, kb, vb); break;
+        default: stage_one(std::integral_constant<int, 7>{}, kb, vb);
       }
     };
 
@@ -243,7 +259,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #pragma unroll
         for (int e = 0; e < 4; e++) some |= odd_high<VT>((unsigned)v[e]) | odd_high<VT>((unsigned)v[e] << 16);
         if (__builtin_expect(__any(some), 0)) {
-          odd = true;
+          odd = odd || (some && ((i64)blk0 + j) * BK + 16 * r + lrow < L);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             unsigned d = (unsigned)v[e];
@@ -258,24 +274,24 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 
     // One (key tile t, row tile u) of step j, in issue order: P V of block j - 1 and scores of block j + 1 spread between runs of
     // independent VALU work on block j. With `refresh` each operand is replaced by the next tile's (jn, tn) after its last use.
-    auto sub_tile = [&](Ops &op, int j, int t, int u, bool has_pv, bool has_next, bool mask, bool refresh, int jn, int tn,
-                        int nst) __attribute__((always_inline)) {
+    auto sub_tile = [&](Ops &op, int j, int t, int u, bool mask, bool refresh, int jn, int tn, int nst)
+        __attribute__((always_inline)) {
       const float nm = nmv[u];
       const int see = mask ? beyond(j, u) : 0;
       float xv[16];
       int npv = 0, ns = 0;
       auto pv = [&]() __attribute__((always_inline)) {
         const int k = npv++;
-        if (has_pv) mma_pv_acc<VT>(o[u][k & 3], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k >> 2]));
+        mma_pv_acc<VT>(o[u][k & 3], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k >> 2]));
         if (refresh) op.va[k] = vread(jn - 1, tn, k);
-        if (k < nst) stage_one(k, j + 3, j + 1);
+        if (nst) stage_k(k, j + 3, j + 1);
       };
       auto sm = [&]() __attribute__((always_inline)) {
         const int c = ns++;
         f32x16 zero;
 #pragma unroll
         for (int i = 0; i < 16; i++) zero[i] = 0.0f;
-        if (has_next) s[t][u] = mma_qk<VT>(op.ka[c], qreg[u][c], c == 0 ? zero : s[t][u]);
+        s[t][u] = mma_qk<VT>(op.ka[c], qreg[u][c], c == 0 ? zero : s[t][u]);
         if (refresh) op.ka[c] = kread(jn + 1, tn, c);
       };
       auto cv = [&](int g) __attribute__((always_inline)) {
@@ -310,96 +326,121 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #undef SB
     };
 
-    // Step j: P V of block j - 1, softmax of block j, scores of block j + 1. The barrier sits before the last sub-tile: the loads
-    // behind it (K of block j + 3, V of block j + 1) land during the next step, and the last sub-tile reads the next step's
-    // first operands. Ring slots: K(j + 3) replaces K(j - 1), V(j + 1) V(j - 3).
-    auto step = [&](Ops &op, int j, bool has_pv, bool has_next, bool mask) __attribute__((always_inline)) {
+    // Row tile u's weights of block j with the block's own maximum, its sum so far in la[u][0]; returns the factor of what was
+    // summed before. (A row that sees no key of the first block sees none of the later ones either.)
+    auto exact = [&](int j, int u, bool mask) __attribute__((always_inline)) {
+      f32x16 xs[2];
+      float bmax = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) xs[t][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NCH; c++) xs[t] = mma_qk<VT>(kread(j, t, c), qreg[u][c], xs[t]);
+        if (mask) {
+          const int see = beyond(j, u);
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (32 * t + 16 * (i >> 3) + (i & 7) > see) xs[t][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) bmax = fmaxf(bmax, xs[t][i]);
+      }
+      const float mn = fmaxf(m[u], fmaxf(bmax, __shfl_xor(bmax, 32)) * p.scale);
+      const float f = (m[u] == -INFINITY || mn == -INFINITY) ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+      m[u] = mn;
+      const float nm = mn == -INFINITY ? 0.0f : -mn;
+      nmv[u] = nm;
+      float add[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const VP2 pp = {(VE)__builtin_amdgcn_exp2f(fmaf(xs[t][i], p.scale, nm)),
+                          (VE)__builtin_amdgcn_exp2f(fmaf(xs[t][i + 1], p.scale, nm))};
+          pb[t][u][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, pp);
+          add[t] = sum2<VT>(pp, add[t]);
+        }
+      la[u][0] = l[u] * f + (add[0] + add[1]);
+      la[u][1] = la[u][2] = la[u][3] = 0.0f;
+      return f;
+    };
+
+    // Step j from 1 on: P V of block j - 1, softmax of block j, scores of block j + 1 (behind the last one: of zeros).
+    // The barrier sits before the last sub-tile: the loads behind it (K of block j + 3, V of block j + 1) land during the next
+    // step, and the last sub-tile reads the next step's first operands. Ring slots: K(j + 3) replaces K(j - 1), V(j + 1) V(j - 3).
+    // The masking steps and the others are the only two copies of this code: a tile of few blocks is bound by fetching it.
+    static_assert(NU == 2, "two row tiles");
+    auto step = [&](Ops &op, int j, bool mask) __attribute__((always_inline)) {
       float tot[NU];
       bool bad = false;
+      auto sums = [&](int u) __attribute__((always_inline)) {
+        tot[u] = (la[u][0] + la[u][1]) + (la[u][2] + la[u][3]);
+        bad = bad | !(tot[u] - l[u] <= sum_limit<VT>());
+      };
       windows(j);
-#pragma unroll
-      for (int idx = 0; idx < 2 * NU - 1; idx++) {
-        const int t = idx / NU, u = idx % NU;
-        sub_tile(op, j, t, u, has_pv, has_next, mask, u == NU - 1, t == 0 ? j : j + 1, t == 0 ? 1 : 0, 0);
-        if (t == 1) {
-          tot[u] = (la[u][0] + la[u][1]) + (la[u][2] + la[u][3]);
-          bad = bad | !(tot[u] - l[u] <= sum_limit<VT>());
-        }
-      }
+      sub_tile(op, j, 0, 0, mask, false, j, 1, 0);
+      sub_tile(op, j, 0, 1, mask, true, j, 1, 0);
+      sub_tile(op, j, 1, 0, mask, false, j + 1, 0, 0);
+      sums(0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the previous step
-      if (CAUSAL && mask) clean(j);
+      if (mask) clean(j);
       __syncthreads();
-      sub_tile(op, j, 1, NU - 1, has_pv, has_next, mask, true, j + 1, 0, 2 * GPB);
-      tot[NU - 1] = (la[NU - 1][0] + la[NU - 1][1]) + (la[NU - 1][2] + la[NU - 1][3]);
-      bad = bad | !(tot[NU - 1] - l[NU - 1] <= sum_limit<VT>());
-      // rare: a score far above the running maximum, or the first block: block j's weights again with the exact maximum (its K is
-      // still in its ring slot). A row that sees no key of the first block sees none of the later ones either.
-      if (__builtin_expect(j == 0 || __builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
+      sub_tile(op, j, 1, 1, mask, true, j + 1, 0, 2 * GPB);
+      sums(1);
+      // rare: a score far above the running maximum: block j's weights again with the exact one (its K is still in its slot)
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
         o_fence(o);  // P V MFMAs of this step may still be writing O
 #pragma unroll
         for (int u = 0; u < NU; u++) {
-          f32x16 xs[2];
-          float bmax = -INFINITY;
-#pragma unroll
-          for (int t = 0; t < 2; t++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) xs[t][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NCH; c++) xs[t] = mma_qk<VT>(kread(j, t, c), qreg[u][c], xs[t]);
-            if (mask) {
-              const int see = beyond(j, u);
-#pragma unroll
-              for (int i = 0; i < 16; i++)
-                if (32 * t + 16 * (i >> 3) + (i & 7) > see) xs[t][i] = -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) bmax = fmaxf(bmax, xs[t][i]);
-          }
-          const float mn = fmaxf(m[u], fmaxf(bmax, __shfl_xor(bmax, 32)) * p.scale);
-          const float f = (m[u] == -INFINITY || mn == -INFINITY) ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
-          m[u] = mn;
-          l[u] *= f;
+          const float f = exact(j, u, mask);
 #pragma unroll
           for (int db = 0; db < D / 32; db++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[u][db][i] *= f;
-          const float nm = mn == -INFINITY ? 0.0f : -mn;
-          nmv[u] = nm;
-          float add[2] = {0.0f, 0.0f};
-#pragma unroll
-          for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const VP2 pp = {(VE)__builtin_amdgcn_exp2f(fmaf(xs[t][i], p.scale, nm)),
-                              (VE)__builtin_amdgcn_exp2f(fmaf(xs[t][i + 1], p.scale, nm))};
-              pb[t][u][i >> 3][(i & 7) >> 1] = __builtin_bit_cast(int, pp);
-              add[t] = sum2<VT>(pp, add[t]);
-            }
-          tot[u] = l[u] + (add[0] + add[1]);
-          la[u][0] = tot[u];
-          la[u][1] = la[u][2] = la[u][3] = 0.0f;
+          tot[u] = la[u][0];
         }
-        asm volatile("s_nop 2" ::: "memory");  // VALU writes of O before the next MFMA reads it
+        o_fence(o);  // VALU writes of O before the next MFMA reads it
       }
 #pragma unroll
       for (int u = 0; u < NU; u++) l[u] = tot[u];
     };
 
-    ahead = fetch(0);
-    addresses(ahead, 0);
-    voff_lo = koff_lo;
-    voff_hi = koff_hi;
-    vrows = krows;
+    // the first loads: page numbers, Q operands (B of S^T = K Q^T) under way while K and V of the first blocks are asked for
+    const int id0 = fetch(0);
     ahead = fetch(1);
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int c = 0; c < NCH; c++) qreg[u][c] = *(const i32x4 *)(qrow[u] + (2 * c + hl) * 16);
+    __builtin_amdgcn_sched_barrier(0);
+    addresses(id0, 0);
+    v_lo = vnext_lo;
+    v_hi = vnext_hi;
 #pragma unroll
     for (int b = 0; b < 3; b++)
 #pragma unroll
-      for (int i = 0; i < GPB; i++) stage_one(i, b, 0);
+      for (int i = 0; i < GPB; i++) stage_k(i, b, 0);
 #pragma unroll
-    for (int i = 0; i < GPB; i++) stage_one(GPB + i, 0, 0);
+    for (int i = 0; i < GPB; i++) stage_k(GPB + i, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int c = 0; c < NCH; c++) {
+        qreg[u][c] = ok[u] ? qreg[u][c] : i32x4{0, 0, 0, 0};
+        asm volatile("" : "+a"(qreg[u][c]));  // from here on Q lives in AGPRs only
+      }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (CAUSAL && clear == 0) clean(0);
+    if (clear == 0) clean(0);
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * GPB; i++) stage_k(i, 3, 1);
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      exact(0, u, true);
+      l[u] = la[u][0];
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -407,22 +448,21 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #pragma unroll
         for (int i = 0; i < 16; i++) s[t][u][i] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NCH; c++) s[t][u] = mma_qk<VT>(kread(0, t, c), qreg[u][c], s[t][u]);
+        for (int c = 0; c < NCH; c++) s[t][u] = mma_qk<VT>(kread(1, t, c), qreg[u][c], s[t][u]);
       }
     Ops op;
 #pragma unroll
-    for (int k = 0; k < 8; k++) op.va[k] = vread(-1, 0, k);  // (not used: there is no P V yet)
+    for (int k = 0; k < 8; k++) op.va[k] = vread(0, 0, k);
 #pragma unroll
-    for (int c = 0; c < NCH; c++) op.ka[c] = kread(1, 0, c);
-    if (nblk == 1) {
-      step(op, 0, false, false, true);
-    } else {
-      step(op, 0, false, true, true);
-      int j = 1;
-      for (; j < min(clear, nblk - 1); j++) step(op, j, true, true, false);
-      for (; j < nblk - 1; j++) step(op, j, true, true, true);
-      step(op, nblk - 1, true, false, true);
-    }
+    for (int c = 0; c < NCH; c++) op.ka[c] = kread(2, 0, c);
+    // from here on O lives in AGPRs only
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int db = 0; db < D / 32; db++) asm volatile("" : "+a"(o[u][db]));
+    int j = 1;
+    for (; j < clear; j++) step(op, j, false);
+    for (; j < nblk; j++) step(op, j, true);
     // P V of the last block (its tile-0 V operands were read by the last step)
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -438,42 +478,82 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the last block land before the slots are used again
     o_fence(o);
 
+    // Outputs go through LDS (each wave its own rows, a few bytes apart, so that neither side meets bank conflicts): a lane holds
+    // 4 channels of a row here and there, and stores 16 bytes of whole rows.
+    __syncthreads();
+    constexpr int S16 = D * 2 + 8, S32 = D * 4 + 16;  // bytes between rows in LDS
+    const unsigned mine = w * (32 * NU) * S32;
+    float sum[NU];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-      const int r = w * (32 * NU) + 32 * u + l32;
-      const int ti = (int)((unsigned)r / (unsigned)hd.GP), gi = r - ti * hd.GP;
-      float sum = l[u] + __shfl_xor(l[u], 32);
-      if (last[u] >= lost) sum = NAN;
-      if (r >= R || g0 + gi >= hd.G) continue;
-      if (whole) {
+      sum[u] = l[u] + __shfl_xor(l[u], 32);
+      if (last[u] >= lost) sum[u] = NAN;
+    }
+    if (whole) {
+      unsigned to = mine + l32 * S16 + 8 * hl, from = mine + (lane >> 4) * S16 + (lane & 15) * 16;
+      asm volatile("" : "+v"(to), "+v"(from));  // (the addresses of all pieces would be kept over the tiles' loop otherwise)
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
         // no sum although a key is visible: all scores are -infinity, and 0 / 0
-        const float inv = sum != 0.0f ? 1.0f / sum : last[u] >= 0 ? NAN : 0.0f;
-        char *dst = a.out + ((size_t)(m0 + ti) * p.o_stride + (size_t)(kvh * hd.G + g0 + gi) * D) * 2;
+        const float inv = sum[u] != 0.0f ? __builtin_amdgcn_rcpf(sum[u]) : last[u] >= 0 ? NAN : 0.0f;
 #pragma unroll
         for (int db = 0; db < D / 32; db++)
 #pragma unroll
           for (int g = 0; g < 4; g++)
-            store4<VT>(dst + (db * 32 + 8 * g + 4 * hl) * 2, o[u][db][4 * g] * inv, o[u][db][4 * g + 1] * inv,
+            store4<VT>(smem + to + 32 * u * S16 + (db * 32 + 8 * g) * 2, o[u][db][4 * g] * inv, o[u][db][4 * g + 1] * inv,
                        o[u][db][4 * g + 2] * inv, o[u][db][4 * g + 3] * inv);
-      } else {
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      char *base = a.out + ((size_t)m0 * p.o_stride + (size_t)(kvh * hd.G + g0) * D) * 2 + (lane & 15) * 16;
+#pragma unroll 1
+      for (int i = 0; i < 32 * NU / 4; i += 4) {
+        float2 lo[4], hi[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          lo[k] = *(const float2 *)(smem + from + 4 * k * S16);
+          hi[k] = *(const float2 *)(smem + from + 4 * k * S16 + 8);
+        }
+        from += 16 * S16;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int row = w * (32 * NU) + 4 * (i + k) + (lane >> 4), ti = row_token(row), gi = row - ti * hd.GP;
+          if (row < R && g0 + gi < hd.G)
+            *(Piece *)(base + ((size_t)ti * p.o_stride + gi * D) * 2) = Piece{{lo[k].x, lo[k].y, hi[k].x, hi[k].y}};
+        }
+      }
+    } else {
+      unsigned to = mine + l32 * S32 + 16 * hl, from = mine + hl * S32 + l32 * 16;
+      asm volatile("" : "+v"(to), "+v"(from));
+#pragma unroll
+      for (int u = 0; u < NU; u++) {
 #pragma unroll
         for (int db = 0; db < D / 32; db++)
 #pragma unroll
           for (int g = 0; g < 4; g++)
-            store4<T_F32>((char *)(st + r * D + db * 32 + 8 * g + 4 * hl), o[u][db][4 * g], o[u][db][4 * g + 1],
+            store4<T_F32>(smem + to + 32 * u * S32 + (db * 32 + 8 * g) * 4, o[u][db][4 * g], o[u][db][4 * g + 1],
                           o[u][db][4 * g + 2], o[u][db][4 * g + 3]);
-        if (hl == 0) *(float2 *)(st + RTC * D + 2 * r) = make_float2(m[u], sum);
+        if (hl == 0) *(float2 *)(st + RTC * D + 2 * (w * (32 * NU) + 32 * u + l32)) = make_float2(m[u], sum[u]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      float *base = st + (w * (32 * NU) + hl) * D + 4 * l32;
+#pragma unroll 1
+      for (int i = 0; i < 32 * NU / 2; i += 8) {
+        f32x4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = *(const f32x4 *)(smem + from + 2 * k * S32);
+        from += 16 * S32;
+#pragma unroll
+        for (int k = 0; k < 8; k++) *(f32x4 *)(base + 2 * (i + k) * D) = v[k];
       }
     }
-    if (CAUSAL) odd = __syncthreads_or(odd);
-    else __syncthreads();
-    if (CAUSAL && __builtin_expect(odd, 0)) {  // the values left out above, for the rows that see them
+    odd = __syncthreads_or(odd);
+    if (__builtin_expect(odd, 0)) {  // the values left out above, for the rows that see them
       __threadfence_block();
       for (int c = tid; c < R * (D / 8); c += NWC * 64) {
         const int r = c / (D / 8), d0 = 8 * (c - r * (D / 8));
-        const int ti = (int)((unsigned)r / (unsigned)hd.GP), gi = r - ti * hd.GP;
+        const int ti = row_token(r), gi = r - ti * hd.GP;
         if (g0 + gi >= hd.G) continue;
-        const i64 seen = plan::clamp(q.off + m0 + ti + 1, 0, min(q.L, (i64)blk1 * BK));
+        const i64 seen = plan::clamp(CAUSAL ? q.off + m0 + ti + 1 : q.L, 0, min(q.L, (i64)blk1 * BK));
         float v[8] = {};
         bool some = false;
         for (i64 key = (i64)(blk0 + clear) * BK; key < seen; key++) {
@@ -527,6 +607,7 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 256, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
+  g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 4 KB that can be read
   g.left = (char *)ex.ws + most * (state - sizeof(Left));
   hipLaunchKernelGGL(kern, dim3((unsigned)(each ? tiles : most)), dim3(NWC * 64), LDSC, ex.stream, g, bt, p, sh, hd, least);
   if (!each && most > 1)

@@ -20,6 +20,7 @@ struct AttnArgs {
   char *out;
   float *ws;   // partial states: O [rows][D], then m and l of each row
   void *left;  // a Left for each slice
+  const char *spare;  // memory that loads without a place of their own may read
 };
 
 // Tiles of 256 rows for long chunks (attention_paged_chunk.hip), head dim 128; t: T_BF16 or T_F16.
