@@ -374,18 +374,35 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
   return 0;
 }
 
+// Whether a call of head dim 128 runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile,
+// its blocks (of 32 keys, of 64), and what cutting costs 256-row tiles; fitted to 60 calls of 1 to 64 sequences of 16 to 4096 new
+// tokens over 128 to 32 768 keys with 4 and 16 heads a key/value head and with 1, which it has within 1.3x. Measured, 32 rows -> 256:
+// a prompt of 4096 tokens 313 -> 167 us, of 1024 37 (256: 66), a chunk of 512 over 16 384 keys 243 -> 173, of 64 over 4096 33 (38).
+bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
+  const i64 n = std::max(1, std::min(p.max_q, p.M)), seqs = (p.M + n - 1) / n, G = p.H / p.KVH;
+  const double keys = causal ? std::max(p.max_kv - 0.5 * n, 0.5 * n) : p.max_kv;
+  auto tiles = [&](int rows) {
+    const i64 HS = (G + rows - 1) / rows, TT = rows / ((G + HS - 1) / HS);
+    return (double)(p.KVH * HS * seqs * ((n + TT - 1) / TT));
+  };
+  const double few = tiles(RT), many = tiles(CHUNK_ROWS);
+  const double cut = chunk_each((i64)many, cus, p) ? 0 : 2ll * p.max_q >= p.max_kv ? 30 : 13;
+  return 20 + many * (0.048 + 0.0085 / 64 * keys) + cut < 10 + few * (0.015 + 0.001 / 32 * keys);
+}
+
 template <int DG, int T, bool CAUSAL>
 int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
-  if (DG == 128 && (rows ? rows == CHUNK_ROWS : (i64)p.max_q * (p.H / p.KVH) >= 192))
+  const int cus = std::max(1, cu_count());
+  if (DG == 128 && (rows ? rows == CHUNK_ROWS : long_chunks(p, cus, CAUSAL)))
     return launch_attention_chunk(T, CAUSAL, ex, a, bt, p, err);
   const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
   const Heads hd{G, HS, GP};
-  const int cus = std::max(1, cu_count());
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
   const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float) + sizeof(Left);  // of a slice
   const int least = 256, most = std::max(1, (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state)));
   const bool few = tiles <= cus && p.max_kv <= 2048;
-  const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= 8 * most));
+  const bool shared = p.max_q > TT;  // several tiles read the same keys
+  const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;

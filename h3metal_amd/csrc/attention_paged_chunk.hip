@@ -603,7 +603,7 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
   const size_t state = (size_t)2 * RTC * (D + 2) * sizeof(float) + sizeof(Left);  // of a slice
   const int least = 512, most = std::max(1, (int)std::min<i64>(cus, (i64)(ex.ws_bytes / state)));
-  const bool each = tiles <= 1 << 22 && tiles >= 3 * most;
+  const bool each = chunk_each(tiles, most, p);
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 256, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
