@@ -48,7 +48,7 @@ __device__ __forceinline__ bool odd16(unsigned v) {
   return (v & E) == E;
 }
 
-template <int DG, int T, int NW, bool CAUSAL>
+template <int DG, int T, int NW, bool CAUSAL, bool EACH>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh, Heads hd, int least) {
   using C = Rows<DG, NW>;
@@ -60,16 +60,28 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Order order(sh, bt);
-  plan::Cut cut{1, (int)(order.all < (i64)gridDim.x ? order.all : (i64)gridDim.x), 0};
-  if (!sh.each) cut = plan::cut(order.all, order.tiles, gridDim.x, least);
-  if (order.all <= 0 || (int)blockIdx.x >= cut.n) {
-    if (!sh.each && tid == 0) left_of(a, blockIdx.x)->R = 0;
-    return;
+  // a whole tile, or a slice of the batch's weight
+  Tile tile;
+  int sl = 0;
+  plan::Cut cut{};
+  i64 x0 = 0, x1 = 1;
+  bool more;
+  std::conditional_t<EACH, Tiles, Order> order(sh, bt);
+  if constexpr (EACH) {
+    const int n = min(order.all, (int)gridDim.x);
+    if ((int)blockIdx.x >= n) return;
+    more = order.tile(n - 1 - slice_of(blockIdx.x, n), &tile);  // with a causal mask the longest tiles go first
+  } else {
+    cut = plan::cut(order.all, order.tiles, gridDim.x, least);
+    if (order.all <= 0 || (int)blockIdx.x >= cut.n) {
+      if (tid == 0) left_of(a, blockIdx.x)->R = 0;
+      return;
+    }
+    sl = slice_of(blockIdx.x, cut.n);
+    x0 = plan::slice_start(cut, sl);
+    x1 = plan::slice_start(cut, sl + 1);
+    more = tile_at(order, x0, &tile);
   }
-  int sl = slice_of(blockIdx.x, cut.n);
-  if (sh.each) sl = cut.n - 1 - sl;  // with a causal mask the longest tiles go first
-  const i64 x0 = plan::slice_start(cut, sl), x1 = plan::slice_start(cut, sl + 1);
 
   // this lane's 16 bytes of each 1 KB load: row and swizzled piece (attention_common.h: kswz, voff); pieces past a row in
   // memory (head dim 96) are sent out of the descriptor's range
@@ -87,15 +99,18 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
   const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
   const int l16 = lane & 15, tr_row = l16 >> 2, tr_col = (l16 & 3) * 8;
 
-  Tile tile;
   bool unfinished = false;
-  bool more = tile_at(order, x0, &tile);
-  for (; more && tile.p < x1; more = next_tile(order, &tile)) {
+  auto next = [&]() {
+    if constexpr (EACH) return false;
+    else return next_tile(order, &tile) && tile.p < x1;
+  };
+  if (!EACH) more = more && tile.p < x1;
+  for (; more; more = next()) {
     const plan::Seq &q = tile.q;
     const int nblk = plan::tile_blocks(sh, q, tile.t, KB);
     int blk0 = 0, blk1 = nblk;
     bool begun = false, whole = true;
-    if (!sh.each) {
+    if constexpr (!EACH) {
       blk0 = plan::block_at(x0, tile.p, tile.w, nblk);
       blk1 = plan::block_at(x1, tile.p, tile.w, nblk);
       begun = tile.p < x0;
@@ -106,7 +121,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
     const int L = (int)q.L;
     const i64 first_last = CAUSAL ? plan::clamp(q.off + m0, -M_MOST, q.L - 1) : q.L - 1;  // of the tile's first token
     float *st = a.ws + (size_t)plan::state_of(sl, begun) * (RT * (DG + 2));
-    if (!whole && !begun) {
+    if (!EACH && !whole && !begun) {
       const int end = last_slice(cut, sl, tile.p + tile.w);
       // (rows of a causal tile that see no key begin before the sequence; without keys none sees any)
       if (tid == 0)
@@ -114,7 +129,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
                                q.L > 0 ? CAUSAL ? (int)first_last : 0 : -M_MOST, end, 0};
       unfinished = true;
     }
-    if (blk0 == blk1) {  // a part without blocks (a whole tile has one)
+    if (!EACH && blk0 == blk1) {  // a part without blocks (a whole tile has one)
       if (tid < R) *(float2 *)(st + RT * DG + 2 * tid) = make_float2(-INFINITY, 0.0f);
       continue;
     }
@@ -329,7 +344,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
           }
         }
       }
-      if (whole) {
+      if (EACH || whole) {
         // no sum although a key is visible: all scores are -infinity, and 0 / 0
         const bool any = CAUSAL ? q.L > 0 && q.off + m0 + rt >= 0 : q.L > 0;
         const float inv = sum != 0.0f ? 1.0f / sum : any ? NAN : 0.0f;
@@ -344,7 +359,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
     }
     __syncthreads();  // before the next tile's loads
   }
-  if (!sh.each && !unfinished && tid == 0) left_of(a, sl)->R = 0;
+  if (!EACH && !unfinished && tid == 0) left_of(a, sl)->R = 0;
 }
 
 }  // namespace
@@ -356,11 +371,11 @@ size_t attention_paged_workspace_max(int cus) {
 
 namespace {
 
-template <int DG, int T, bool CAUSAL, int NW>
+template <int DG, int T, bool CAUSAL, int NW, bool EACH>
 int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Shape &sh,
              const Heads &hd, unsigned grid, int least, std::string *err) {
   using C = Rows<DG, NW>;
-  auto kern = attention_rows_kernel<DG, T, NW, CAUSAL>;
+  auto kern = attention_rows_kernel<DG, T, NW, CAUSAL, EACH>;
   static bool attr_set = false;
   if (!attr_set) {
     hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS);
@@ -377,7 +392,7 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
 // Whether a call of head dim 128 runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile,
 // its blocks (of 32 keys, of 64), and what cutting costs 256-row tiles; fitted to 60 calls of 1 to 64 sequences of 16 to 4096 new
 // tokens over 128 to 32 768 keys with 4 and 16 heads a key/value head and with 1, which it has within 1.3x. Measured, 32 rows -> 256:
-// a prompt of 4096 tokens 313 -> 167 us, of 1024 37 (256: 66), a chunk of 512 over 16 384 keys 243 -> 173, of 64 over 4096 33 (38).
+// a prompt of 4096 tokens 266 -> 170 us, of 1024 33 (256: 67), a chunk of 512 over 16 384 keys 226 -> 150, of 64 over 4096 33 (38).
 bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
   const i64 n = std::max(1, std::min(p.max_q, p.M)), seqs = (p.M + n - 1) / n, G = p.H / p.KVH;
   const double keys = causal ? std::max(p.max_kv - 0.5 * n, 0.5 * n) : p.max_kv;
@@ -387,7 +402,7 @@ bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
   };
   const double few = tiles(RT), many = tiles(CHUNK_ROWS);
   const double cut = chunk_each((i64)many, cus, p) ? 0 : 2ll * p.max_q >= p.max_kv ? 30 : 13;
-  return 20 + many * (0.048 + 0.0085 / 64 * keys) + cut < 10 + few * (0.015 + 0.001 / 32 * keys);
+  return 18 + many * (0.036 + 0.0085 / 64 * keys) + cut < 10 + few * (0.012 + 0.001 / 32 * keys);
 }
 
 template <int DG, int T, bool CAUSAL>
@@ -403,13 +418,14 @@ int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const Page
   const bool few = tiles <= cus && p.max_kv <= 2048;
   const bool shared = p.max_q > TT;  // several tiles read the same keys
   const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));
-  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 128, (i64)bt.width << bt.lg};
+  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
   g.left = (char *)ex.ws + most * (state - sizeof(Left));
-  if (few) return run_rows<DG, T, CAUSAL, 8>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
-  if (run_rows<DG, T, CAUSAL, 4>(ex, g, bt, p, sh, hd, (unsigned)(each ? tiles : most), least, err)) return -1;
-  if (!each && most > 1)
+  if (few) return run_rows<DG, T, CAUSAL, 8, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
+  if (each) return run_rows<DG, T, CAUSAL, 4, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
+  if (run_rows<DG, T, CAUSAL, 4, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
+  if (most > 1)
     hipLaunchKernelGGL((attention_join_kernel<DG, T, RT, 1>), dim3((unsigned)(most - 1), RT / 4), dim3(256), 0, ex.stream, g,
                        p.o_stride);
   return 0;

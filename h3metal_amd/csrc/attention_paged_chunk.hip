@@ -60,7 +60,7 @@ struct __attribute__((packed, aligned(8))) Piece {  // 16 bytes of an output row
   float v[4];
 };
 
-template <int VT, bool CAUSAL>
+template <int VT, bool CAUSAL, bool EACH>
 __global__ __launch_bounds__(NWC * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh, Heads hd, int least) {
   using VT8 = typename Vec8<VT>::type;
@@ -71,16 +71,28 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
   const int tid = threadIdx.x, lane = tid & 63, hl = lane >> 5, l32 = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const Order order(sh, bt);
-  plan::Cut cut{1, (int)(order.all < (i64)gridDim.x ? order.all : (i64)gridDim.x), 0};
-  if (!sh.each) cut = plan::cut(order.all, order.tiles, gridDim.x, least);
-  if (order.all <= 0 || (int)blockIdx.x >= cut.n) {
-    if (!sh.each && tid == 0) left_of(a, blockIdx.x)->R = 0;
-    return;
+  // a whole tile, or a slice of the batch's weight
+  Tile tile;
+  int sl = 0;
+  plan::Cut cut{};
+  i64 x0 = 0, x1 = 1;
+  bool more;
+  std::conditional_t<EACH, Tiles, Order> order(sh, bt);
+  if constexpr (EACH) {
+    const int n = min(order.all, (int)gridDim.x);
+    if ((int)blockIdx.x >= n) return;
+    more = order.tile(n - 1 - slice_of(blockIdx.x, n), &tile);  // with a causal mask the longest tiles go first
+  } else {
+    cut = plan::cut(order.all, order.tiles, gridDim.x, least);
+    if (order.all <= 0 || (int)blockIdx.x >= cut.n) {
+      if (tid == 0) left_of(a, blockIdx.x)->R = 0;
+      return;
+    }
+    sl = slice_of(blockIdx.x, cut.n);
+    x0 = plan::slice_start(cut, sl);
+    x1 = plan::slice_start(cut, sl + 1);
+    more = tile_at(order, x0, &tile);
   }
-  int sl = slice_of(blockIdx.x, cut.n);
-  if (sh.each) sl = cut.n - 1 - sl;  // with a causal mask the longest tiles go first
-  const i64 x0 = plan::slice_start(cut, sl), x1 = plan::slice_start(cut, sl + 1);
 
   // this lane's 16 bytes of each 1 KB load, within a group of 16 rows: row and swizzled piece (attention_common.h: kswz, voff)
   const int lrow = w * 4 + (lane >> 4);
@@ -97,15 +109,18 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
   const float per_token = 1.0f / (float)hd.GP;
   auto row_token = [&](int r) __attribute__((always_inline)) { return (int)(((float)r + 0.5f) * per_token); };  // r / GP
 
-  Tile tile;
   bool unfinished = false;
-  bool more = tile_at(order, x0, &tile);
-  for (; more && tile.p < x1; more = next_tile(order, &tile)) {
+  auto next = [&]() {
+    if constexpr (EACH) return false;
+    else return next_tile(order, &tile) && tile.p < x1;
+  };
+  if (!EACH) more = more && tile.p < x1;
+  for (; more; more = next()) {
     const plan::Seq &q = tile.q;
     const int all = plan::tile_blocks(sh, q, tile.t, BK);
     int blk0 = 0, blk1 = all;
     bool begun = false, whole = true;
-    if (!sh.each) {
+    if constexpr (!EACH) {
       blk0 = plan::block_at(x0, tile.p, tile.w, all);
       blk1 = plan::block_at(x1, tile.p, tile.w, all);
       begun = tile.p < x0;
@@ -118,14 +133,14 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     const int L = (int)q.L;
     const i64 first_last = CAUSAL ? plan::clamp(q.off + m0, -M_MOST, q.L - 1) : q.L - 1;  // last key of the tile's first token
     float *st = a.ws + (size_t)plan::state_of(sl, begun) * (RTC * (D + 2));
-    if (!whole && !begun) {
+    if (!EACH && !whole && !begun) {
       const int end = last_slice(cut, sl, tile.p + tile.w);
       if (tid == 0)
         *left_of(a, sl) = Left{R, m0, kvh * hd.G + g0, hd.GP, min(hd.GP, hd.G - g0),
                                q.L > 0 ? CAUSAL ? (int)first_last : 0 : -M_MOST, end, 0};
       unfinished = true;
     }
-    if (blk0 == blk1) {  // a part without blocks (a whole tile has one)
+    if (!EACH && blk0 == blk1) {  // a part without blocks (a whole tile has one)
       if (tid < R) *(float2 *)(st + RTC * D + 2 * tid) = make_float2(-INFINITY, 0.0f);
       continue;
     }
@@ -489,7 +504,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       sum[u] = l[u] + __shfl_xor(l[u], 32);
       if (last[u] >= lost) sum[u] = NAN;
     }
-    if (whole) {
+    if (EACH || whole) {
       unsigned to = mine + l32 * S16 + 8 * hl, from = mine + (lane >> 4) * S16 + (lane & 15) * 16;
       asm volatile("" : "+v"(to), "+v"(from));  // (the addresses of all pieces would be kept over the tiles' loop otherwise)
 #pragma unroll
@@ -571,7 +586,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
           }
         }
         if (!some) continue;
-        if (whole) {
+        if (EACH || whole) {
           VE *dst = (VE *)a.out + (size_t)(m0 + ti) * p.o_stride + (size_t)(kvh * hd.G + g0 + gi) * D + d0;
 #pragma unroll
           for (int e = 0; e < 8; e++) dst[e] = (VE)((float)dst[e] + v[e]);
@@ -582,12 +597,13 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       }
     }
   }
-  if (!sh.each && !unfinished && tid == 0) left_of(a, sl)->R = 0;
+  if (!EACH && !unfinished && tid == 0) left_of(a, sl)->R = 0;
 }
 
-template <int VT, bool CAUSAL>
-int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
-  auto kern = attention_chunk_kernel<VT, CAUSAL>;
+template <int VT, bool CAUSAL, bool EACH>
+int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Shape &sh, const Heads &hd,
+        unsigned grid, int least, std::string *err) {
+  auto kern = attention_chunk_kernel<VT, CAUSAL, EACH>;
   static bool attr_set = false;
   if (!attr_set) {
     hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDSC);
@@ -597,20 +613,26 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
     }
     attr_set = true;
   }
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(NWC * 64), LDSC, ex.stream, a, bt, p, sh, hd, least);
+  return 0;
+}
+
+template <int VT, bool CAUSAL>
+int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
   const int G = p.H / p.KVH, HS = (G + RTC - 1) / RTC, GP = (G + HS - 1) / HS, TT = RTC / GP;
   const Heads hd{G, HS, GP};
   const int cus = std::max(1, cu_count());
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
   const size_t state = (size_t)2 * RTC * (D + 2) * sizeof(float) + sizeof(Left);  // of a slice
   const int least = 512, most = std::max(1, (int)std::min<i64>(cus, (i64)(ex.ws_bytes / state)));
-  const bool each = chunk_each(tiles, most, p);
-  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, each, 256, (i64)bt.width << bt.lg};
+  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, 256, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
-  g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 4 KB that can be read
   g.left = (char *)ex.ws + most * (state - sizeof(Left));
-  hipLaunchKernelGGL(kern, dim3((unsigned)(each ? tiles : most)), dim3(NWC * 64), LDSC, ex.stream, g, bt, p, sh, hd, least);
-  if (!each && most > 1)
+  g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 4 KB that can be read
+  if (chunk_each(tiles, most, p)) return run<VT, CAUSAL, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
+  if (run<VT, CAUSAL, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
+  if (most > 1)
     hipLaunchKernelGGL((attention_join_kernel<D, VT, RTC, 4>), dim3((unsigned)(most - 1), RTC / 16), dim3(256), 0, ex.stream, g,
                        p.o_stride);
   return 0;

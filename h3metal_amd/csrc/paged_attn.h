@@ -128,7 +128,7 @@ __device__ __forceinline__ bool tile_at(const Order &o, i64 x, Tile *c) {
   if (c->b < 0) return false;
   c->q = o.seq(c->b);
   const i64 w = plan::head_weight(c->q), y = x - before;
-  c->v = __builtin_amdgcn_readfirstlane((int)plan::div(y, w));
+  c->v = __builtin_amdgcn_readfirstlane((int)plan::clamp(plan::div(y, w), 0, o.sh.VH - 1));
   c->t = __builtin_amdgcn_readfirstlane(plan::tile_at(c->q, y - w * c->v));
   c->p = before + w * c->v + plan::before_tile(c->q, c->t);
   c->w = plan::tile_weight(c->q, c->t);
@@ -149,6 +149,65 @@ __device__ __forceinline__ bool next_tile(const Order &o, Tile *c) {
   c->w = plan::tile_weight(c->q, c->t);
   return true;
 }
+
+// The same where a workgroup takes a whole tile, in 32 bits: tile x of the batch, *n of them in all (a grid holds no more than
+// 2^22; what garbage lengths add up to is clamped).
+__device__ __forceinline__ int wave_sum_to(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int u = __shfl_up(v, d);
+    v += lane >= d ? u : 0;
+  }
+  return v;
+}
+struct Tiles {
+  const plan::Shape &sh;
+  const Batch &bt;
+  int q0, q1, kv, K, upto, all;  // of the first 64 sequences: this lane's, its tiles a head group, the tiles up to it; all tiles
+
+  __device__ Tiles(const plan::Shape &s, const Batch &b) : sh(s), bt(b) {
+    load(threadIdx.x & 63, &q0, &q1, &kv, &K);
+    upto = bt.B == 1 ? __builtin_amdgcn_readfirstlane(K * sh.VH) : wave_sum_to(K * sh.VH);
+    all = __builtin_amdgcn_readlane(upto, 63);
+    int a, c, d, k;
+    for (int i = 64; i < bt.B; i += 64) {
+      load(i + (threadIdx.x & 63), &a, &c, &d, &k);
+      all += __builtin_amdgcn_readlane(wave_sum_to(k * sh.VH), 63);
+    }
+  }
+  __device__ void load(int b, int *a, int *c, int *n, int *k) const {
+    *a = *c = *n = 0;
+    if (b < bt.B) {
+      *a = bt.q_start[b];
+      *c = bt.q_start[b + 1];
+      *n = bt.kv_len[b];
+    }
+    const int lo = min(max(*a, 0), sh.M), hi = min(max(*c, lo), sh.M);
+    *k = (hi - lo + sh.TT - 1) / sh.TT;
+  }
+  __device__ bool tile(int x, Tile *t) const {
+    int a = q0, c = q1, n = kv, k = K, s = upto, base = 0;
+    for (int i = 0;; i += 64) {
+      const unsigned long long m = __ballot(base + s > x);
+      if (m) {
+        const int l = __builtin_ctzll(m);
+        const int kt = __builtin_amdgcn_readlane(k, l);
+        const unsigned y = (unsigned)(x - base - (__builtin_amdgcn_readlane(s, l) - kt * sh.VH));
+        t->b = i + l;
+        t->q = plan::seq_of(sh, __builtin_amdgcn_readlane(a, l), __builtin_amdgcn_readlane(c, l), __builtin_amdgcn_readlane(n, l));
+        if (kt < 1) return false;
+        t->v = min((int)(y / (unsigned)kt), sh.VH - 1);
+        t->t = min((int)(y % (unsigned)kt), kt - 1);
+        return true;
+      }
+      if (i + 64 >= bt.B) return false;
+      base += __builtin_amdgcn_readlane(s, 63);
+      load(i + 64 + (threadIdx.x & 63), &a, &c, &n, &k);
+      s = wave_sum_to(k * sh.VH);
+    }
+  }
+};
 
 // The slice of a workgroup: workgroup b runs on XCD b % 8; each XCD takes a contiguous run of the slices, so that tiles that share
 // keys share an L2.

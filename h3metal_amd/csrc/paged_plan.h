@@ -26,7 +26,6 @@ struct Shape {
   int M, B;     // rows, sequences
   int TT, VH;   // tokens of a tile, head groups
   int causal;
-  int each;     // every tile weighs 1 (a workgroup takes whole tiles)
   int cost;     // what a tile costs besides its keys, in keys
   i64 most;     // keys the page table can name
 };
@@ -56,10 +55,7 @@ H3_HD Seq seq_of(const Shape &sh, int q0, int q1, int kv) {
   q.K = (q.hi - q.lo + sh.TT - 1) / sh.TT;
   q.L = clamp(kv, 0, sh.most);
   q.off = (i64)kv - q1;
-  if (sh.each) {
-    q.a = 1;
-    q.s = 0;
-  } else if (sh.causal) {
+  if (sh.causal) {
     q.a = clamp(q.off + q.lo, 0, q.L) + sh.TT + sh.cost;
     q.s = sh.TT;
   } else {

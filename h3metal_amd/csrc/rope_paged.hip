@@ -17,11 +17,14 @@
 
 #include <cmath>
 #include <cstring>
+#include <type_traits>
+
 
 namespace h3 {
 namespace {
 
-enum { PAIR_LANE = 0, PAIR_NEXT = 1, PAIR_ANY = 2 };  // rotary partners: whole lanes apart, side by side, anywhere
+// rotary partners: whole lanes apart, side by side, anywhere, the lanes of the other half (all of a head of 64 or 128)
+enum { PAIR_LANE = 0, PAIR_NEXT = 1, PAIR_ANY = 2, PAIR_ALL = 3 };
 
 constexpr int PL = 8;  // channels per lane
 
@@ -38,13 +41,39 @@ struct RopeArgs {
   const int *pos;
 };
 
-// Where a row goes: its place in the cache (-1: nowhere), its rotary position, and whether it belongs to a sequence at all.
-struct RowAt {
-  long long page;  // page of the cache, -1: not stored
-  int row, turn, live;
-};
+// 16 bytes of a row, whose rows are aligned to their elements only
+typedef unsigned Piece __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename E, int N> struct __attribute__((packed, aligned(sizeof(E)))) Packed { E v[N]; };
+template <int T>
+__device__ __forceinline__ void load8(float (&v)[PL], const Piece (&x)[T == P_F32 ? 2 : 1]) {
+  if constexpr (T == P_F32) {
+#pragma unroll
+    for (int i = 0; i < PL; i++) v[i] = __builtin_bit_cast(float, (unsigned)x[i / 4][i & 3]);
+  } else if constexpr (T == P_BF16) {
+#pragma unroll
+    for (int i = 0; i < PL; i += 2) {
+      v[i] = __builtin_bit_cast(float, (unsigned)x[0][i / 2] << 16);
+      v[i + 1] = __builtin_bit_cast(float, (unsigned)x[0][i / 2] & 0xFFFF0000u);
+    }
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < PL; i += 2) {
+      const f16x2 h = __builtin_bit_cast(f16x2, (unsigned)x[0][i / 2]);
+      v[i] = (float)h[0];
+      v[i + 1] = (float)h[1];
+    }
+  }
+}
+template <int T>
+__device__ __forceinline__ Piece pack8(const float (&v)[PL]) {
+  using E = typename PElem<T>::type;
+  typedef E E2 __attribute__((ext_vector_type(2)));
+  Piece o;
+#pragma unroll
+  for (int i = 0; i < PL; i += 2) o[i / 2] = __builtin_bit_cast(unsigned, E2{(E)v[i], (E)v[i + 1]});
+  return o;
+}
 
 // cos and sin of a fraction of a turn in 2^-32: the nearest quarter turn, and an angle within +-pi/4 of it
 __device__ __forceinline__ float2 cos_sin(unsigned t) {
@@ -73,32 +102,47 @@ __device__ __forceinline__ float slot_max(float v) {
   return v;
 }
 
-// The sequence of row m and its place, by one wave: sequences that end at or before m are counted 64 at a time.
-__device__ __forceinline__ RowAt find_row(int m, const Batch &bt, const int *pos, bool keys) {
-  const int lane = threadIdx.x & 63;
-  int b = 0;
-  for (int k = 0; k < bt.B; k += 64)
-    b += __popcll(__ballot(k + lane < bt.B && bt.q_start[k + lane + 1] <= m));
-  RowAt r{-1, 0, 0, 0};
-  if (b >= bt.B || bt.q_start[b] > m) return r;
-  const long long c = (long long)bt.kv_len[b] - bt.q_start[b + 1] + m, pi = c >> bt.lg;
-  r.live = 1;
-  r.turn = pos ? pos[m] : (int)c;
+// Where rows go, by one wave, a row a lane: the rotary position, and the row of the cache, pages counted through (-1: not
+// stored; -2: the row is of no sequence).
+struct RowsAt {
+  long long to;
+  int turn;
+};
+template <int ROWS>
+__device__ __forceinline__ RowsAt find_rows(int m0, int M, const Batch &bt, const int *pos, bool keys) {
+  const int lane = threadIdx.x & 63, m = m0 + lane;
+  int b = 0;  // sequences that end at or before the row, counted 64 at a time
+  if (bt.B == 1) {
+    b = bt.q_start[1] <= m;
+  } else {
+    for (int k = 0; k < bt.B; k += 64) {
+      const int end = k + lane < bt.B ? bt.q_start[k + lane + 1] : 0x7fffffff;
+#pragma unroll
+      for (int r = 0; r < ROWS; r++) {
+        const int n = __popcll(__ballot(end <= m0 + r));
+        b += lane == r ? n : 0;
+      }
+    }
+  }
+  RowsAt at{-2, 0};
+  if (lane >= ROWS || m >= M || b >= bt.B) return at;
+  const int first = bt.q_start[b], end = bt.q_start[b + 1], n = bt.kv_len[b], given = pos ? pos[m] : 0;
+  if (first > m || end <= m) return at;
+  const long long c = (long long)n - end + m, pi = c >> bt.lg;
+  at.to = -1;
+  at.turn = pos ? given : (int)c;
   if (keys && c >= 0 && pi < bt.width) {
     const int pg = bt.table[(long long)b * bt.width + pi];
-    if (pg >= 0 && pg < bt.pages) r.page = pg;
-    r.row = (int)(c & ((1 << bt.lg) - 1));
+    if (pg >= 0 && pg < bt.pages) at.to = ((long long)pg << bt.lg) + (c & ((1 << bt.lg) - 1));
   }
-  return r;
+  return at;
 }
 
 template <int HDIM, int IT, int OT, int PAIR, int ROWS>
 __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, PagedRopeParams p) {
   using S = Slots<HDIM>;
-  using IE = typename PElem<IT>::type;
-  using OE = typename PElem<OT>::type;
-  __shared__ RowAt at[ROWS];
-  __shared__ float2 cs[ROWS][HDIM / 2];
+  constexpr int IB = IT == P_F32 ? 4 : 2, NP = IB / 2;  // bytes of an element, pieces of a lane's channels
+  __shared__ __attribute__((aligned(16))) float2 cs[ROWS][HDIM / 2];
   __shared__ float mix[PAIR == PAIR_ANY ? 256 * PL : 1];
   const int tid = threadIdx.x, l = tid % S::LPS, c0 = l * PL;
   const int slot = blockIdx.y * S::SPG + tid / S::LPS, m0 = blockIdx.x * ROWS;
@@ -106,38 +150,47 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
   const bool on = slot < slots && c0 < HDIM, turned = slot < p.Hq + p.Hk;
   const int half = p.rot / 2;
 
-  Packed<IE, PL> x[ROWS];
+  Piece x[ROWS][NP];  // (rows and slots past the last ones read the last again)
+  {
+    const char *from = a.qkv + ((size_t)min(slot, slots - 1) * HDIM + min(c0, HDIM - PL)) * IB;
 #pragma unroll
-  for (int r = 0; r < ROWS; r++)
-    if (on && m0 + r < p.M)
-      x[r] = *(const Packed<IE, PL> *)((const IE *)a.qkv + (size_t)(m0 + r) * p.in_stride + slot * HDIM + c0);
-    else
-      for (int i = 0; i < PL; i++) x[r].v[i] = (IE)0.0f;
+    for (int r = 0; r < ROWS; r++)
+#pragma unroll
+      for (int k = 0; k < NP; k++)
+        x[r][k] = *(const Piece *)(from + (size_t)min(m0 + r, p.M - 1) * p.in_stride * IB + 16 * k);
+  }
   float w[PL];
 #pragma unroll
-  for (int i = 0; i < PL; i++) w[i] = on && turned && p.norm ? (slot < p.Hq ? a.wq : a.wk)[c0 + i] : 1.0f;
-
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  for (int r = wave; r < ROWS; r += 4) {
-    RowAt f{-1, 0, 0, 0};
-    if (m0 + r < p.M) f = find_row(m0 + r, bt, a.pos, p.Hk > 0);
-    if ((tid & 63) == 0) at[r] = f;
+  for (int i = 0; i < PL; i++) w[i] = 1.0f;
+  if (p.norm && turned && c0 < HDIM) {
+    const float *from = (slot < p.Hq ? a.wq : a.wk) + c0;
+#pragma unroll
+    for (int i = 0; i < PL; i++) w[i] = from[i];
   }
-  __syncthreads();
-  for (int i = tid; i < ROWS * half; i += 256) {
-    const int r = i / half, j = i - r * half;
-    const unsigned long long t = (unsigned long long)(long long)at[r].turn * a.turns[j];
-    const float2 f = cos_sin((unsigned)((t + 0x80000000ull) >> 32));
-    cs[r][j] = make_float2(f.x * p.rope_scale, f.y * p.rope_scale);
+
+  const RowsAt at = find_rows<ROWS>(m0, p.M, bt, a.pos, p.Hk > 0);
+  for (int i = tid; i < ROWS * HDIM / 2; i += 256) {
+    const int r = i / (HDIM / 2), j = i - r * (HDIM / 2);
+    const int turn = __shfl(at.turn, r);
+    if (j < half) {
+      const unsigned long long t = (unsigned long long)(long long)turn * a.turns[j];
+      const float2 f = cos_sin((unsigned)((t + 0x80000000ull) >> 32));
+      cs[r][j] = make_float2(f.x * p.rope_scale, f.y * p.rope_scale);
+    }
   }
   __syncthreads();
 
 #pragma unroll
   for (int r = 0; r < ROWS; r++) {
-    if (m0 + r >= p.M || !at[r].live) continue;  // the same for the whole workgroup
+    const long long to = (long long)((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)at.to, r) |
+                                     (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(at.to >> 32), r) << 32);
+    if (to == -2) continue;  // the same for the whole workgroup
     float v[PL];
+    load8<IT>(v, x[r]);
+    if (HDIM == 96 && c0 >= HDIM) {  // idle lanes of a slot
 #pragma unroll
-    for (int i = 0; i < PL; i++) v[i] = (float)x[r].v[i];
+      for (int i = 0; i < PL; i++) v[i] = 0.0f;
+    }
     if (p.norm) {
       float ss = 0.0f;
 #pragma unroll
@@ -180,6 +233,19 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
           }
         }
       }
+    } else if (PAIR == PAIR_ALL) {
+      if (turned) {
+        const bool low = l < S::LPS / 2;
+        float2 f[PL];
+#pragma unroll
+        for (int i = 0; i < PL; i += 2)
+          *(float4 *)&f[i] = *(const float4 *)&cs[r][(low ? c0 : c0 - HDIM / 2) + i];
+#pragma unroll
+        for (int i = 0; i < PL; i++) {
+          const float u = xshfl<S::LPS / 2>(v[i]);
+          v[i] = v[i] * f[i].x + (low ? -u : u) * f[i].y;
+        }
+      }
     } else if (PAIR == PAIR_LANE) {
       // half is a multiple of 8: a lane's channels are all in the first or the second half, its partner half / 8 lanes off
       const int hl = half / PL, low = l < hl, pl = low ? l + hl : l - hl;
@@ -213,26 +279,32 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
       }
       __syncthreads();
     }
-    Packed<OE, PL> o;
-#pragma unroll
-    for (int i = 0; i < PL; i++) o.v[i] = (OE)v[i];
     if (!on) continue;
+    char *dst;
     if (slot < p.Hq) {
-      *(Packed<OE, PL> *)((OE *)a.q + (size_t)(m0 + r) * p.q_stride + slot * HDIM + c0) = o;
-    } else if (at[r].page >= 0) {
+      dst = a.q + ((size_t)(m0 + r) * p.q_stride + slot * HDIM + c0) * 2;
+    } else {
+      if (to < 0) continue;
       const int h = slot - p.Hq - (turned ? 0 : p.Hk);
-      const size_t to = (((size_t)at[r].page * p.Hk + h) * p.page + at[r].row) * HDIM + c0;
-      *(Packed<OE, PL> *)((OE *)(turned ? a.kc : a.vc) + to) = o;
+      const size_t row = ((((size_t)to >> bt.lg) * p.Hk + h) << bt.lg) + ((size_t)to & ((1 << bt.lg) - 1));
+      dst = (turned ? a.kc : a.vc) + (row * HDIM + c0) * 2;
     }
+    *(Piece *)dst = pack8<OT>(v);
   }
 }
 
 template <int HDIM, int IT, int OT, int PAIR>
 void run(const Exec &ex, const RopeArgs &a, const Batch &bt, const PagedRopeParams &p) {
   const int slots = p.Hq + 2 * p.Hk, ny = (slots + Slots<HDIM>::SPG - 1) / Slots<HDIM>::SPG;
-  constexpr int ROWS = 8;
-  hipLaunchKernelGGL((rope_paged_kernel<HDIM, IT, OT, PAIR, ROWS>), dim3((unsigned)((p.M + ROWS - 1) / ROWS), (unsigned)ny),
-                     dim3(256), 0, ex.stream, a, bt, p);
+  auto go = [&](auto rows) {
+    constexpr int ROWS = decltype(rows)::value;
+    hipLaunchKernelGGL((rope_paged_kernel<HDIM, IT, OT, PAIR, ROWS>), dim3((unsigned)((p.M + ROWS - 1) / ROWS), (unsigned)ny),
+                       dim3(256), 0, ex.stream, a, bt, p);
+  };
+  // Few rows are bound by the chain of a workgroup's loads and take 2 rows each, many share a workgroup's angles (heads 32 + 8 + 8:
+  // 64 single tokens 5.3 us with 2 rows, 9.9 with 8; 512 rows 8.4, 10.6; 2048 rows 22, 19).
+  if ((long)p.M * ny < 4000) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 8>{});
 }
 
 template <int HDIM, int IT, int OT>
@@ -298,6 +370,7 @@ int launch(const Pipeline &pl, const Exec &ex, const Arg *a, int nargs, const vo
   const Batch bt{(const int *)a[7].ptr, (const int *)a[8].ptr, (const int *)a[9].ptr, p.B, (int)width, p.Hk ? p.pages : 0,
                  p.Hk ? lg : 4};
   if (inter) run<HDIM, IT, OT, PAIR_NEXT>(ex, g, bt, p);
+  else if (HDIM != 96 && p.rot == HDIM) run<HDIM, IT, OT, PAIR_ALL>(ex, g, bt, p);
   else if (p.rot / 2 % PL == 0) run<HDIM, IT, OT, PAIR_LANE>(ex, g, bt, p);
   else run<HDIM, IT, OT, PAIR_ANY>(ex, g, bt, p);
   return 0;

@@ -33,9 +33,9 @@ static std::vector<Tile> walk(const Shape &sh, const int *qs, const int *kv, int
   }
   return out;
 }
-extern "C" int check(int M, int B, int TT, int VH, int causal, int each, int cost, long long most, const int *qs, const int *kv,
+extern "C" int check(int M, int B, int TT, int VH, int causal, int cost, long long most, const int *qs, const int *kv,
                      int kb, int most_slices, int least) {
-  const Shape sh{M, B, TT, VH, causal, each, cost, most};
+  const Shape sh{M, B, TT, VH, causal, cost, most};
   const std::vector<Tile> tiles = walk(sh, qs, kv, kb);
   i64 total = 0;
   size_t at = 0;
@@ -57,7 +57,7 @@ extern "C" int check(int M, int B, int TT, int VH, int causal, int each, int cos
     total += w * VH;
   }
   if (tiles.empty()) return 0;
-  const Cut cut_ = each ? Cut{1, (int)total, 0} : cut(total, (i64)tiles.size(), most_slices, least);
+  const Cut cut_ = cut(total, (i64)tiles.size(), most_slices, least);
   const int n = cut_.n;
   if (slice_start(cut_, 0) != 0 || slice_start(cut_, n) != total) return 13;
   std::map<int, std::pair<size_t, int>> state;  // place -> tile, blocks
@@ -120,12 +120,12 @@ def check(tmp_path_factory):
     subprocess.run([cxx, "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-shared", "-fPIC", "-I",
                     os.path.join(ROOT, "h3metal_amd", "csrc"), str(d / "plan.cpp"), "-o", str(d / "plan.so")], check=True)
     fn = ctypes.CDLL(str(d / "plan.so")).check
-    fn.argtypes = [ctypes.c_int] * 7 + [ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int] * 3
+    fn.argtypes = [ctypes.c_int] * 6 + [ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int] * 3
 
-    def run(q_start, kv_len, *, TT, VH, causal, each=0, cost=64, most=1 << 20, kb=32, slices=512, least=256, M=None):
+    def run(q_start, kv_len, *, TT, VH, causal, cost=64, most=1 << 20, kb=32, slices=512, least=256, M=None):
         qs, kv = np.asarray(q_start, np.int32), np.asarray(kv_len, np.int32)
         M = int(qs[-1]) if M is None else M
-        return fn(M, len(kv), TT, VH, causal, each, cost, most, qs.ctypes.data, kv.ctypes.data, kb, slices, least)
+        return fn(M, len(kv), TT, VH, causal, cost, most, qs.ctypes.data, kv.ctypes.data, kb, slices, least)
     return run
 
 
@@ -141,7 +141,6 @@ def test_every_block_is_done_once(check, seed):
             for slices, least in ((1, 1), (7, 1), (512, 64), (512, 1024), (2048, 1)):
                 assert check(starts, keys, TT=TT, VH=int(rng.integers(1, 9)), causal=causal, slices=slices, least=least,
                              kb=int(rng.choice([32, 64, 128]))) == 0
-            assert check(starts, keys, TT=TT, VH=2, causal=causal, each=1) == 0
 
 
 def test_long_and_short_ones(check):
