@@ -296,15 +296,11 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
 template <int HDIM, int IT, int OT, int PAIR>
 void run(const Exec &ex, const RopeArgs &a, const Batch &bt, const PagedRopeParams &p) {
   const int slots = p.Hq + 2 * p.Hk, ny = (slots + Slots<HDIM>::SPG - 1) / Slots<HDIM>::SPG;
-  auto go = [&](auto rows) {
-    constexpr int ROWS = decltype(rows)::value;
-    hipLaunchKernelGGL((rope_paged_kernel<HDIM, IT, OT, PAIR, ROWS>), dim3((unsigned)((p.M + ROWS - 1) / ROWS), (unsigned)ny),
-                       dim3(256), 0, ex.stream, a, bt, p);
-  };
-  // Few rows are bound by the chain of a workgroup's loads and take 2 rows each, many share a workgroup's angles (heads 32 + 8 + 8:
-  // 64 single tokens 5.3 us with 2 rows, 9.9 with 8; 512 rows 8.4, 10.6; 2048 rows 22, 19).
-  if ((long)p.M * ny < 4000) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 8>{});
+  // Rows a workgroup: more share its angles, fewer share the chain of its loads (heads 32 + 8 + 8, us with 1, 2, 4 and 8 rows: 64
+  // single tokens 3.6, 4.2, 5.4, 7.3; 2048 rows 12.9, 12.0, 12.0, 12.1; 8192 rows 37.7, 32.7, 33.8, 37.9).
+  constexpr int ROWS = 2;
+  hipLaunchKernelGGL((rope_paged_kernel<HDIM, IT, OT, PAIR, ROWS>), dim3((unsigned)((p.M + ROWS - 1) / ROWS), (unsigned)ny),
+                     dim3(256), 0, ex.stream, a, bt, p);
 }
 
 template <int HDIM, int IT, int OT>

@@ -7,11 +7,13 @@ off by (D + 4) 2^-24 sum|q k| scale at most, an exponential by 2^-22, a sum over
 (32 lanes and tiles of keys side by side): as parts of sum|w v|, doubled for numerator and denominator. In half precision a
 weight below 2^-14 is off by 2^-25 instead: L 2^-25 max|v| (the largest weight is 1 or more)."""
 
+import itertools
+
 import numpy as np
 import pytest
 
 from h3metal_amd import ops, rope
-from h3metal_amd.gpu import GpuError
+from h3metal_amd.gpu import Gpu, GpuError
 from oracle import paged as op
 from paged_util import HALF, as_type, ints, page_table, q_starts, value
 
@@ -64,8 +66,14 @@ def check(got, c, *, causal=True, scale=None):
     return want
 
 
+def variants(c):
+    """The choices of tiles: the call's own, and at head dim 128 both heights by name."""
+    return [{}] + [dict(ROWS=r) for r in (32, 256)] * (c["D"] == 128)
+
+
 def both(gpu, c, causal=True, **kw):
-    check(launch(gpu, c, causal=causal, **kw), c, causal=causal, scale=kw.get("scale"))
+    for v in variants(c):
+        check(launch(gpu, c, causal=causal, **kw, **v), c, causal=causal, scale=kw.get("scale"))
 
 
 @pytest.mark.parametrize("t", ["bf16", "f16"])
@@ -179,11 +187,12 @@ def test_not_numbers_where_nothing_looks(gpu, D, t):
             c[n].transpose(0, 2, 1, 3)[~used] = bits
         both(gpu, c)
         both(gpu, c, False)
-        clean = launch(gpu, c)
-        for token, name in ((55, "vc"), (69, "vc"), (61, "kc")):  # tokens of sequence 0 that its rows up to token - 1 miss
+        for (token, name), v in itertools.product(((55, "vc"), (69, "vc"), (61, "kc")), variants(c)):
+            # tokens of sequence 0 that its rows up to token - 1 miss
+            clean = launch(gpu, c, **v)
             d = dict(c, **{name: c[name].copy()})
             d[name][c["table"][0, token // 16], 1, token % 16, 5:9] = bits
-            got = launch(gpu, d)
+            got = launch(gpu, d, **v)
             assert np.array_equal(got[:token - 30], clean[:token - 30]) and np.array_equal(got[40:], clean[40:])
             rows = got[token - 30:40, 2:]  # heads 2 and 3 read key/value head 1
             if name == "vc":
@@ -191,27 +200,57 @@ def test_not_numbers_where_nothing_looks(gpu, D, t):
                 assert np.isfinite(rows[:, :, :5]).all() and np.isfinite(rows[:, :, 9:]).all()
 
 
-def test_not_numbers_in_a_query(gpu):
+@pytest.mark.parametrize("ROWS", [0, 32, 256])
+def test_not_numbers_in_a_query(gpu, ROWS):
     c = batch([20, 2], [40, 9], seed=9)
     c["q"][3, 1, 7] = as_type(np.array([np.nan]), "bf16")[0][0]
-    got = launch(gpu, c)
+    got = launch(gpu, c, ROWS=ROWS)
     assert np.isnan(got[3, 1]).all()
     c["q"][3, 1, 7] = 0
-    again = launch(gpu, c)
+    again = launch(gpu, c, ROWS=ROWS)
     got[3, 1] = again[3, 1]
     assert np.array_equal(got, again)
+
+
+@pytest.mark.parametrize("ROWS", [32, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_not_numbers_that_are_seen(gpu, ROWS, causal):
+    """Infinities of both signs in values that every row, or some rows of a tile, or of a cut tile, see."""
+    for seed, (new, keys, at) in enumerate([([100], [400], (3, 250, 330, 399)), ([1], [3000], (5, 2999)),
+                                            ([300], [1300], (20, 1000, 1200))]):
+        c = batch(new, keys, H=2, KVH=1, D=128, seed=seed)
+        for i, token in enumerate(at):
+            c["vc"][c["table"][0, token // 16], 0, token % 16, 10 * i] = as_type(np.array([(-1) ** i * np.inf]), "bf16")[0][0]
+        got = launch(gpu, c, causal=causal, ROWS=ROWS)
+        want = check(got, c, causal=causal)
+        assert np.isinf(want).any()
+
+
+@pytest.mark.parametrize("ROWS", [32, 256])
+def test_scores_that_jump(gpu, ROWS):
+    """Keys whose scores outgrow those before by far, in any block: the running maximum follows."""
+    c = batch([70, 1], [900, 700], H=4, KVH=1, D=128, seed=21)
+    q = np.ones((c["M"], 4, 128)) * 0.5
+    c["q"] = as_type(q, "bf16")[0]
+    for b, tokens in ((0, (1, 70, 300, 301, 640, 899)), (1, (699,))):
+        for i, token in enumerate(tokens):
+            c["kc"][c["table"][b, token // 16], 0, token % 16] = as_type(np.full(128, 3.0 * (i + 1)), "bf16")[0]
+    check(launch(gpu, c, ROWS=ROWS), c)
+    c["q"] = as_type(-q, "bf16")[0]
+    check(launch(gpu, c, ROWS=ROWS), c)
 
 
 def test_page_numbers_outside_the_cache(gpu):
     """Their keys score NaN: the rows that see them are NaN, the others as always."""
     c = batch([50, 3, 1], [80, 40, 300], seed=10)
     c["table"][0, 3], c["table"][1, 2], c["table"][2, 9] = len(c["kc"]), -1, 2 ** 31 - 1
-    got = launch(gpu, c)
-    want = check(got, c)
-    assert np.isnan(want[18:50]).all() and not np.isnan(want[:18]).any() and np.isnan(want[53]).all()
-    check(launch(gpu, c, causal=False), c, causal=False)
+    for v in variants(c):
+        want = check(launch(gpu, c, **v), c)
+        assert np.isnan(want[18:50]).all() and not np.isnan(want[:18]).any() and np.isnan(want[53]).all()
+        check(launch(gpu, c, causal=False, **v), c, causal=False)
     c["kc"], c["vc"] = c["kc"][:0], c["vc"][:0]  # a cache of no pages
-    assert np.isnan(launch(gpu, c, causal=False)).all()
+    for v in variants(c):
+        assert np.isnan(launch(gpu, c, causal=False, **v)).all()
 
 
 def test_starts_that_fall_are_harmless(gpu):
@@ -219,22 +258,66 @@ def test_starts_that_fall_are_harmless(gpu):
     for q_start in ([0, 5, 2, 8], [-3, 4, 9, 2], [8, 8, 100, 2 ** 31 - 1], [-2 ** 31, -5, 2 ** 31 - 1, -1]):
         c = batch([3, 3, 2], [30, 40, 9], seed=11)
         c["q_start"] = np.array(q_start, np.int32)
-        launch(gpu, c)
-        launch(gpu, c, causal=False, max_q=1)
+        for v in variants(c):
+            launch(gpu, c, **v)
+            launch(gpu, c, causal=False, max_q=1, **v)
 
 
 def test_no_alloc_and_repeats(gpu):
     """Both entry points, twice each on the same context with other work between: bit for bit the same."""
     c = batch([1, 200, 1], [3000, 700, 90], H=8, KVH=2, page=32, seed=12)
-    first = launch(gpu, c)
-    check(first, c)
     other = batch([1], [5000], H=8, KVH=1, seed=13)
-    check(launch(gpu, other, no_alloc=True), other)
-    assert np.array_equal(launch(gpu, c), first)
-    static = launch(gpu, c, no_alloc=True)
-    check(static, c)
-    both(gpu, other)
-    assert np.array_equal(launch(gpu, c, no_alloc=True), static)
+    for v in variants(c):
+        first = launch(gpu, c, **v)
+        check(first, c)
+        check(launch(gpu, other, no_alloc=True, **v), other)
+        assert np.array_equal(launch(gpu, c, **v), first)
+        static = launch(gpu, c, no_alloc=True, **v)
+        check(static, c)
+        both(gpu, other)
+        assert np.array_equal(launch(gpu, c, no_alloc=True, **v), static)
+
+
+def test_two_contexts_at_once(gpu):
+    """Calls queued on two contexts, each with its scratch memory, before either is waited for."""
+    other = Gpu()
+    try:
+        a, b = batch([1, 90], [4000, 2000], H=8, KVH=2, seed=15), batch([3, 400], [900, 1700], H=8, KVH=2, seed=16)
+        for v in variants(a):
+            tensors, outs = [], []
+            for g, c in ((gpu, a), (other, b)):
+                M, H, D = c["M"], c["H"], c["D"]
+                t = dict(q=g.upload(c["q"].reshape(M, H * D), "bf16"), kc=g.upload(c["kc"], "bf16"), vc=g.upload(c["vc"], "bf16"),
+                         out=g.empty((M, H * D), "bf16"), table=ints(g, c["table"]), q_start=ints(g, c["q_start"]),
+                         kv_len=ints(g, c["kv_len"]))
+                tensors.append(t)
+            for _ in range(5):
+                for g, c, t in ((gpu, a, tensors[0]), (other, b, tensors[1])):
+                    ops.attention_paged(g, t["q"], t["kc"], t["vc"], t["out"], t["table"], t["q_start"], t["kv_len"], M=c["M"],
+                                        B=c["B"], H=c["H"], KVH=c["KVH"], D=c["D"], scale=c["D"] ** -0.5, **v)
+            for g, c, t in ((gpu, a, tensors[0]), (other, b, tensors[1])):
+                g.wait()
+                outs.append(t["out"].numpy())
+                check(value(outs[-1], "bf16").reshape(c["M"], c["H"], c["D"]), c)
+            del tensors, t
+    finally:
+        other.close()
+
+
+def test_lengths_that_change_between_calls(gpu):
+    """The same buffers with other lengths and pages in them: the next call follows what they hold."""
+    c = batch([40, 1, 1], [500, 900, 20], H=8, KVH=2, seed=17, width=64)
+    bufs = dict(q=gpu.upload(c["q"].reshape(c["M"], -1), "bf16"), kc=gpu.upload(c["kc"], "bf16"), vc=gpu.upload(c["vc"], "bf16"),
+                out=gpu.empty((c["M"], 1024), "bf16"), table=ints(gpu, c["table"]), q_start=ints(gpu, c["q_start"]),
+                kv_len=ints(gpu, c["kv_len"]))
+    for q_start, kv_len in (([0, 40, 41, 42], [500, 900, 20]), ([0, 1, 41, 42], [3, 900, 17]), ([0, 0, 2, 42], [500, 2, 20])):
+        c["q_start"], c["kv_len"] = np.array(q_start, np.int32), np.array(kv_len, np.int32)
+        bufs["q_start"].write(c["q_start"])
+        bufs["kv_len"].write(c["kv_len"])
+        for v in variants(c):
+            ops.attention_paged(gpu, *bufs.values(), M=c["M"], B=3, H=8, KVH=2, D=128, scale=128 ** -0.5, **v)
+            gpu.wait()
+            check(value(bufs["out"].numpy(), "bf16").reshape(c["M"], 8, 128), c)
 
 
 def test_layer_grows_its_cache(gpu):
@@ -310,3 +393,6 @@ def test_refuses_shared_memory_alignment_and_other_heads(gpu):
                                         kc=gpu.empty((3, 2, 16, 32), "bf16"), vc=gpu.empty((3, 2, 16, 32), "bf16")))
     with pytest.raises(GpuError, match="unknown macro"):
         gpu.kernel("attention", "attention_paged", QK8=1)
+    for bad in (dict(ROWS=64), dict(ROWS=-1), dict(ROWS=256, HD=64), dict(ROWS="x")):
+        with pytest.raises(GpuError, match="ROWS"):
+            gpu.kernel("attention", "attention_paged", **bad)
