@@ -7,10 +7,12 @@
 // keys once. The work is cut as paged_plan.h says; lengths are known on the device only, so every workgroup finds its slice by
 // itself. Within a workgroup the waves split the keys: wave w takes the 32-key blocks w, w + NW, ... of its part of a tile,
 // with a running maximum, sum and output of its own, staged through LDS of its own by LDS-direct loads that its own vmcnt
-// orders, with no barrier; the waves' states meet in LDS at the end. Scores are S^T = K Q^T and outputs O^T = V^T P^T on the 32 x
-// 32 MFMA, in attention_small.hip's layouts (a lane holds one query's keys, so the softmax is per lane; V's operands are
+// orders, with no barrier; the waves' states meet in LDS at the end. Scores are S^T = K Q^T and outputs O^T = V^T P^T on the
+// 32 x 32 MFMA, in attention_small.hip's layouts (a lane holds one query's keys, so the softmax is per lane; V's operands are
 // transposing LDS reads). The loads of a block's two 16-key halves go through descriptors that end at the sequence's last
-// key: what a page holds behind it reads as zero.
+// key: what a page holds behind it reads as zero. Two workgroups a compute unit have up to 128 KB of loads under way, and single
+// tokens are bound by HBM: 64 sequences with 275 181 keys (32 + 8 heads of 128) 214 us, 5.3 TB/s; one of 131 072 104 us.
+// A few short tiles are bound by the chain of a wave's blocks (1.1 us each, alone): 8 waves instead of 4, 512 keys 13 -> 10 us.
 #include "attention_common.h"
 #include "paged_attn.h"
 
@@ -389,10 +391,10 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
   return 0;
 }
 
-// Whether a call of head dim 128 runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile,
-// its blocks (of 32 keys, of 64), and what cutting costs 256-row tiles; fitted to 60 calls of 1 to 64 sequences of 16 to 4096 new
-// tokens over 128 to 32 768 keys with 4 and 16 heads a key/value head and with 1, which it has within 1.3x. Measured, 32 rows -> 256:
-// a prompt of 4096 tokens 266 -> 170 us, of 1024 33 (256: 67), a chunk of 512 over 16 384 keys 226 -> 150, of 64 over 4096 33 (38).
+// Whether a call of head dim 128 runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a
+// tile, its blocks (of 32 keys, of 64), and what cutting costs 256-row tiles; fitted to 60 calls of 1 to 64 sequences of 16 to
+// 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head. Measured, 32 rows -> 256: a prompt of 4096
+// tokens 266 -> 170 us, of 1024 33 (256: 67), a chunk of 512 over 16 384 keys 226 -> 150, of 64 over 4096 33 (38).
 bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
   const i64 n = std::max(1, std::min(p.max_q, p.M)), seqs = (p.M + n - 1) / n, G = p.H / p.KVH;
   const double keys = causal ? std::max(p.max_kv - 0.5 * n, 0.5 * n) : p.max_kv;
@@ -415,8 +417,11 @@ int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const Page
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
   const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float) + sizeof(Left);  // of a slice
   const int least = 256, most = std::max(1, (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state)));
+  // Whole tiles or slices. Few tiles of few keys are not worth a second kernel (one token, us whole with 8 waves and sliced: 512
+  // keys 13, 19; 2048 21, 19). Tiles that share keys stay whole, side by side, from one a compute unit on (24 chunks of 48 tokens
+  // over 2000 keys 86, 178 sliced); others are sliced until there are many, so that uneven lengths cost nothing.
   const bool few = tiles <= cus && p.max_kv <= 2048;
-  const bool shared = p.max_q > TT;  // several tiles read the same keys
+  const bool shared = p.max_q > TT;
   const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));
   const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;

@@ -12,6 +12,9 @@
 //  * Rows see keys up to one of their own: the blocks that some row does not see whole run in a loop of their own, which masks.
 //  * V of those blocks is searched in LDS for infinities and NaN, which a weight of 0 would not keep out of a sum: they are taken
 //    as 0, and the rows that see them get them at the end. So is what a page holds behind the sequence's end.
+// A prompt of 8192 tokens (32 + 8 heads) takes 500 us, 1.1 PFLOP/s, a large library product's rate on the same card; a step of
+// 64 keys 2.1 us, of which its 64 matrix instructions would take 0.9: the softmax's instructions beside them bound it. A tile
+// starts and ends in about 15 us, so code is kept in two copies only and everything of a start is asked for at once.
 #include "paged_attn.h"
 
 #include <algorithm>
@@ -563,7 +566,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     }
     odd = __syncthreads_or(odd);
     if (__builtin_expect(odd, 0)) {  // the values left out above, for the rows that see them
-      __threadfence_block();
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's outputs are written before another adds to them
+      __syncthreads();
       for (int c = tid; c < R * (D / 8); c += NWC * 64) {
         const int r = c / (D / 8), d0 = 8 * (c - r * (D / 8));
         const int ti = row_token(r), gi = r - ti * hd.GP;

@@ -27,7 +27,7 @@ struct AttnArgs {
 constexpr int CHUNK_ROWS = 256;
 // Whether its workgroups take whole tiles, in the order of their length: from 2 tiles a compute unit on where tiles differ in
 // length (a prompt from its start: 4096 tokens 220 -> 167 us), from 4 on where they do not and a last round would be short of
-// tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost their partial states.
+// tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost their states.
 inline bool chunk_each(i64 tiles, int most, const PagedAttnParams &p) {
   return tiles <= 1 << 22 && tiles >= (2ll * p.max_q >= p.max_kv ? 2 : 4) * (i64)most;
 }
@@ -110,7 +110,8 @@ struct Order {
   }
   __device__ plan::Seq seq(int b) const {  // one sequence for the wave: scalar values
     if (b < 64)
-      return plan::seq_of(sh, __builtin_amdgcn_readlane(q0, b), __builtin_amdgcn_readlane(q1, b), __builtin_amdgcn_readlane(kv, b));
+      return plan::seq_of(sh, __builtin_amdgcn_readlane(q0, b), __builtin_amdgcn_readlane(q1, b),
+                          __builtin_amdgcn_readlane(kv, b));
     return plan::seq_of(sh, __builtin_amdgcn_readfirstlane(bt.q_start[b]), __builtin_amdgcn_readfirstlane(bt.q_start[b + 1]),
                         __builtin_amdgcn_readfirstlane(bt.kv_len[b]));
   }
@@ -138,13 +139,7 @@ __device__ __forceinline__ bool next_tile(const Order &o, Tile *c) {
   c->p += c->w;
   if (++c->t == c->q.K) {
     c->t = 0;
-    if (++c->v == o.sh.VH) {
-      c->v = 0;
-      do {
-        if (++c->b >= o.bt.B) return false;
-        c->q = o.seq(c->b);
-      } while (!c->q.K);
-    }
+    if (++c->v == o.sh.VH) return c->p < o.all && tile_at(o, c->p, c);  // (past any number of sequences without new tokens)
   }
   c->w = plan::tile_weight(c->q, c->t);
   return true;
@@ -164,7 +159,7 @@ __device__ __forceinline__ int wave_sum_to(int v) {
 struct Tiles {
   const plan::Shape &sh;
   const Batch &bt;
-  int q0, q1, kv, K, upto, all;  // of the first 64 sequences: this lane's, its tiles a head group, the tiles up to it; all tiles
+  int q0, q1, kv, K, upto, all;  // of the first 64 sequences: this lane's, its tiles a head group, tiles up to it; all tiles
 
   __device__ Tiles(const plan::Shape &s, const Batch &b) : sh(s), bt(b) {
     load(threadIdx.x & 63, &q0, &q1, &kv, &K);
@@ -195,7 +190,8 @@ struct Tiles {
         const int kt = __builtin_amdgcn_readlane(k, l);
         const unsigned y = (unsigned)(x - base - (__builtin_amdgcn_readlane(s, l) - kt * sh.VH));
         t->b = i + l;
-        t->q = plan::seq_of(sh, __builtin_amdgcn_readlane(a, l), __builtin_amdgcn_readlane(c, l), __builtin_amdgcn_readlane(n, l));
+        t->q = plan::seq_of(sh, __builtin_amdgcn_readlane(a, l), __builtin_amdgcn_readlane(c, l),
+                            __builtin_amdgcn_readlane(n, l));
         if (kt < 1) return false;
         t->v = min((int)(y / (unsigned)kt), sh.VH - 1);
         t->t = min((int)(y % (unsigned)kt), kt - 1);
@@ -209,8 +205,8 @@ struct Tiles {
   }
 };
 
-// The slice of a workgroup: workgroup b runs on XCD b % 8; each XCD takes a contiguous run of the slices, so that tiles that share
-// keys share an L2.
+// The slice of a workgroup: workgroup b runs on XCD b % 8; each XCD takes a contiguous run of the slices, so that tiles that
+// share keys share an L2.
 __device__ __forceinline__ int slice_of(int b, int n) {
   const int per = n >> 3, rem = n & 7, xcd = b & 7;
   return (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + (b >> 3);

@@ -13,7 +13,8 @@ return value (None; results are valid after `gpu.wait()`):
 
 and, without a counterpart there, the 8-bit feed-forward path: rms_norm_q8 (RMS norm with the residual's addition and an
 8-bit output), swiglu_f8 (the gated unit with an 8-bit output) and gemm's weight format f8 (e4m3 operands with a scale for
-each block of 128).
+each block of 128); and a text model's paged cache: qk_norm_rope_paged (per-head norm, rotary embedding and the cache's update) and
+attention_paged (a batch's new tokens over the cache).
 
 Element types come from the tensors, as in the reference (`OUT_DT`,
 ops.py:17). The gfx950 kernels additionally accept bf16 Q/K/V (the reference's
@@ -266,8 +267,9 @@ def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, ta
                          f"{vc.dtype}, {out.dtype}")
     pages, page, width = _paged("attention_paged", kc, vc, table, q_start, kv_len, KVH, D)
     k = gpu.kernel("attention", "attention_paged", HD=D, IN_T=OUT_DT[q.dtype], CAUSAL=1 if causal else 0, **variant)
-    params = _PACK_11IF(M, B, H, KVH, q_stride or H * D, o_stride or H * D, pages, page, width, M if max_q is None else max_q,
-                        min(width * page, 0x7FFFFFFF) if max_kv is None else max_kv, scale * LOG2E)
+    params = _PACK_11IF(M, B, H, KVH, q_stride or H * D, o_stride or H * D, pages, page, width,
+                        M if max_q is None else max(0, min(max_q, M)),
+                        min(width * page if max_kv is None else max(0, max_kv), 0x7FFFFFFF), scale * LOG2E)
     gpu.launch(k, None, None, [q, kc, vc, out, table, q_start, kv_len], params, no_alloc=no_alloc)
 
 

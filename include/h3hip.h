@@ -70,8 +70,9 @@ void *h3_buffer_device(void *buf);
 int h3_buffer_copy(h3_ctx *ctx, void *dst, uint64_t dst_offset, void *src, uint64_t src_offset, uint64_t bytes);
 
 // Looks up kernel `fn` of module `file` specialised by macros "NAME=value;...".
-// Modules: "attention" (fn "attention", "attention_scores") and "ops" (fn
-// "qk_norm_rope", "rot_q8", and without a counterpart "rms_norm_q8", "swiglu_f8") and
+// Modules: "attention" (fn "attention", "attention_scores", and without a counterpart
+// "attention_paged") and "ops" (fn "qk_norm_rope", "rot_q8", and without a counterpart
+// "rms_norm_q8", "swiglu_f8", "qk_norm_rope_paged") and
 // "gemm" (fn "gemm"; macro WFMT selects the weight format as in
 // kernels/gemm.metal:1-40: 1 q8, 4 f16, 5 bf16, 6 h8, and without a counterpart 9 f8;
 // other formats return NULL); the reference's "attention.metal"/"ops.metal"/"gemm.metal" names are
@@ -92,10 +93,11 @@ int h3_dispatch(h3_ctx *ctx, void *pso, const uint32_t grid[3], const uint32_t t
 // h3_dispatch without any allocation (no reference counterpart: for callers that cannot allocate device
 // memory, such as code under HIP graph capture or a serving loop that forbids it). Same arguments, checks and
 // kernels as h3_dispatch, but the scratch memory the kernels use (the attention tail split's partial states,
-// the h8 GEMM's widened weights) is a fixed 32 MiB array compiled into the library, one per GPU and held until
-// the process ends, instead of the context's workspace; it calls no hipMalloc, hipFree, event creation or other
-// allocating routine (per-dispatch profiling is skipped). Work that needs more scratch than 32 MiB: the
-// attention split shrinks to fit (down to none), an h8 GEMM with N * K * 2 > 32 MiB fails with a message.
+// those of the paged attention, the h8 GEMM's widened weights) is a fixed 32 MiB array compiled into the library,
+// one per GPU and held until the process ends, instead of the context's workspace; it calls no hipMalloc, hipFree,
+// event creation or other allocating routine (per-dispatch profiling is skipped). Work that needs more scratch than
+// 32 MiB: the attention split and the paged attention's slices shrink to fit (down to none), an h8 GEMM with
+// N * K * 2 > 32 MiB fails with a message.
 // Calls on one GPU share the array: dispatches through this entry point that may run at the same time on one
 // GPU (different contexts or streams) race; on one context's stream they are ordered. Nothing in the array
 // needs to start at zero (every kernel writes what it later reads).
@@ -104,7 +106,7 @@ int h3_dispatch_static(h3_ctx *ctx, void *pso, const uint32_t grid[3], const uin
 
 // Scratch memory of the dispatches (addition, no reference counterpart: Metal
 // kernels there keep no scratch). h3_open reserves what the attention's tail
-// split needs at most, so h3_dispatch never allocates or synchronises; the h8
+// split and the paged attention's slices need at most, so h3_dispatch never allocates or synchronises; the h8
 // GEMM's widened weights (N * K * 2 bytes) need an explicit h3_reserve_workspace
 // first when they exceed it. h3_reserve_workspace drains the stream, then grows
 // the buffer (never shrinks it); 0 or -1. h3_workspace_bytes: the current size.

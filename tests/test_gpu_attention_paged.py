@@ -116,6 +116,15 @@ def test_many_sequences(gpu, B):
     both(gpu, batch([1] * B, rng.integers(1, 200, B).tolist(), H=4, KVH=1, D=64, seed=B), max_q=1)
 
 
+def test_mostly_idle_sequences(gpu):
+    """Sequences without new tokens around and between those that have some."""
+    new, keys = np.zeros(500, int), np.full(500, 40)
+    new[[3, 70, 71, 200, 330, 498]] = [1, 100, 1, 30, 1, 7]
+    keys[[3, 70, 71, 200, 330, 498]] = [900, 1500, 1, 30, 3000, 700]
+    both(gpu, batch(new.tolist(), keys.tolist(), H=4, KVH=1, D=128, seed=22))
+    both(gpu, batch(new.tolist(), keys.tolist(), H=4, KVH=1, D=64, seed=22))
+
+
 @pytest.mark.parametrize("D,t", [(128, "bf16"), (64, "f16")])
 def test_long(gpu, D, t):
     both(gpu, batch([1], [20000], H=4, KVH=1, D=D, t=t, page=64, seed=1))

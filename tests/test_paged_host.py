@@ -64,6 +64,10 @@ def test_attention_packs_its_parameters():
     assert vals[:11] == (5, 2, 32, 8, 4096, 4096, 9, 16, 4, 5, 64)
     assert abs(vals[11] - 128 ** -0.5 * 1.4426950408889634) < 1e-7
     assert struct.unpack("<11if", second)[4:11] == (4104, 4100, 9, 16, 4, 1, 33)
+    ops.attention_paged(g, **attn_args(max_q=10 ** 12, max_kv=10 ** 12))  # hints of any size
+    ops.attention_paged(g, **attn_args(max_q=-1, max_kv=-10 ** 12))
+    assert struct.unpack("<11if", g.launches[2][2])[9:11] == (5, 2 ** 31 - 1)
+    assert struct.unpack("<11if", g.launches[3][2])[9:11] == (0, 0)
 
 
 @pytest.mark.parametrize("bad", [
