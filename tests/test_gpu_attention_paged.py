@@ -262,6 +262,51 @@ def test_page_numbers_outside_the_cache(gpu):
         assert np.isnan(launch(gpu, c, causal=False, **v)).all()
 
 
+def test_rows_before_the_first_sequence_and_shared_pages(gpu):
+    """A batch whose first rows belong to nobody, and sequences that share the pages of their first 48 keys."""
+    c = batch([40, 1, 9], [100, 300, 60], H=4, KVH=2, seed=18, pad=5)
+    c["q_start"] = c["q_start"] + 5
+    c["table"][1:, :3] = c["table"][0, :3]
+    both(gpu, c)
+    both(gpu, c, False)
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_a_cache_past_32_bits(gpu, t):
+    """Pages 4 GiB and more into the cache: keys and values go there and come from there."""
+    KVH, D, page, H = 2, 128, 256, 4
+    pages = (5 << 30) // (KVH * page * D * 2)
+    rng = np.random.default_rng(19)
+    new, keys = [300, 1], [300, 700]
+    used = np.array([pages - 1, pages // 5 * 4 + 3, pages - 7, 2, pages - 2], np.int32)
+    table = np.full((2, 3), -7, np.int32)
+    table[0, :2], table[1] = used[:2], used[2:]
+    kc, vc = gpu.empty((pages, KVH, page, D), t), gpu.empty((pages, KVH, page, D), t)
+    held = [as_type(rng.standard_normal((5, KVH, page, D)), t)[0] for _ in range(2)]
+    for c, rows in ((kc, held[0]), (vc, held[1])):
+        for i, pg in enumerate(used):
+            c.row(int(pg), 1).write(rows[i:i + 1])
+    q_start, M = q_starts(new), 301
+    qkv = gpu.upload(as_type(rng.standard_normal((M, (H + 2 * KVH) * D)), t)[0], t)
+    w, Q = gpu.upload(np.ones(D, np.float32)), gpu.empty((M, H * D), t)
+    turns = gpu.upload(rope.turns(rope.frequencies(D)[0]), "u32")
+    idx = (ints(gpu, table), ints(gpu, q_start), ints(gpu, keys))
+    print(f"[far cache] {pages} pages", flush=True)
+    ops.qk_norm_rope_paged(gpu, qkv, w, w, turns, Q, kc, vc, *idx, M=M, B=2, Hq=H, Hk=KVH, hd=D, rot=D, eps=1e-6)
+    gpu.wait()
+    small = [np.concatenate([c.row(int(pg), 1).numpy() for pg in used]) for c in (kc, vc)]
+    rows = as_type(qkv.numpy() if t == "f16" else value(qkv.numpy(), t), t)[0].reshape(M, -1, D)
+    for m in range(300):  # the values of the first sequence's rows
+        assert np.array_equal(small[1][m // page, :, m % page], rows[m, H + KVH:])
+    c = dict(q=Q.numpy().reshape(M, H, D), kc=small[0], vc=small[1], table=np.array([[0, 1, -7], [2, 3, 4]], np.int32),
+             q_start=q_start, kv_len=np.array(keys, np.int32), M=M, B=2, H=H, KVH=KVH, D=D, t=t, page=page)
+    for v in variants(c):
+        out = gpu.empty((M, H * D), t)
+        ops.attention_paged(gpu, Q, kc, vc, out, *idx, M=M, B=2, H=H, KVH=KVH, D=D, scale=D ** -0.5, **v)
+        gpu.wait()
+        check(value(out.numpy(), t).reshape(M, H, D), c)
+
+
 def test_starts_that_fall_are_harmless(gpu):
     """q_start out of order, negative or past M is no batch: nothing is promised but that only rows of q and out are touched."""
     for q_start in ([0, 5, 2, 8], [-3, 4, 9, 2], [8, 8, 100, 2 ** 31 - 1], [-2 ** 31, -5, 2 ** 31 - 1, -1]):

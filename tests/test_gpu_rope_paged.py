@@ -28,10 +28,10 @@ def within(got, want, size, t):
 
 def run_case(gpu, new, keys, *, Hq=4, Hk=2, hd=128, rot=128, x="bf16", t="bf16", inter=False, norm=True, page=16,
              scaling="none", factor=1.0, pos=None, pad=0, in_pad=0, q_pad=0, seed=0, width=None, table=None, data=None,
-             eps=1e-6, no_alloc=False, scale_w=1.0):
+             eps=1e-6, no_alloc=False, scale_w=1.0, skip=0):
     """Runs the operator on a batch and checks queries and the whole cache, which starts out with random bits."""
     rng = np.random.default_rng(seed)
-    q_start = q_starts(new)
+    q_start = q_starts(new) + np.int32(skip)
     M, B = int(q_start[-1]) + pad, len(new)
     slots = Hq + 2 * Hk
     tab, pages = page_table(rng, keys, page, width=width)
@@ -123,6 +123,22 @@ def test_single_tokens(gpu):
 def test_rows_of_no_sequence_stay(gpu):
     run_case(gpu, [4, 2], [4, 9], pad=21, seed=5)
     run_case(gpu, [0, 0], [4, 9], pad=5, seed=5)
+
+
+def test_rows_before_the_first_sequence_stay(gpu):
+    for new, keys in (([4, 2], [4, 9]), ([7], [20])):
+        run_case(gpu, new, keys, skip=3, pad=2, seed=15)
+
+
+def test_without_norm_weights(gpu):
+    """norm=False needs no weights, rot=0 no frequencies."""
+    x = as_type(np.random.default_rng(16).standard_normal((5, 3 * 64)), "bf16")[0]
+    Q, kc, vc = gpu.empty((5, 64), "bf16"), gpu.empty((2, 1, 16, 64), "bf16"), gpu.empty((2, 1, 16, 64), "bf16")
+    ops.qk_norm_rope_paged(gpu, gpu.upload(x, "bf16"), None, None, None, Q, kc, vc, ints(gpu, [[1]]), ints(gpu, [0, 5]),
+                           ints(gpu, [5]), M=5, B=1, Hq=1, Hk=1, hd=64, rot=0, eps=0.0, norm=False)
+    gpu.wait()
+    assert np.array_equal(Q.numpy(), x[:, :64]) and np.array_equal(kc.numpy()[1, 0, :5], x[:, 64:128])
+    assert np.array_equal(vc.numpy()[1, 0, :5], x[:, 128:]) and not kc.numpy()[0].any() and not vc.numpy()[1, 0, 5:].any()
 
 
 def test_strides(gpu):
