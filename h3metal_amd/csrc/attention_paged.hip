@@ -391,11 +391,13 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
   return 0;
 }
 
-// Whether a call of head dim 128 runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a
-// tile, its blocks (of 32 keys, of 64), and what cutting costs 256-row tiles; fitted to 60 calls of 1 to 64 sequences of 16 to
-// 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head. Measured, 32 rows -> 256: a prompt of 4096
-// tokens 266 -> 170 us, of 1024 33 (256: 67), a chunk of 512 over 16 384 keys 226 -> 150, of 64 over 4096 33 (38).
-bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
+// Whether a call runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile, its blocks (of
+// 32 keys, of 64; their time goes with the head dim), and what cutting costs 256-row tiles; fitted to 60 calls of head dim 128 of
+// 1 to 64 sequences of 16 to 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head, and tried on 64 of
+// head dims 64 and 96, where it loses 1 % on average to the better choice. Measured at head dim 128 | 96 | 64, 32 rows -> 256: a
+// prompt of 4096 tokens 266 -> 170 | 238 -> 146 | 133 -> 120 us, of 1024 33 (256: 67) | 30 (59) | 18 (52), a chunk of 512 over
+// 16 384 keys 226 -> 150 | 200 -> 155 | 161 -> 119, of 64 over 4096 33 (38) | 32 (35) | 27 (30).
+bool long_chunks(int d, const PagedAttnParams &p, int cus, bool causal) {
   const i64 n = std::max(1, std::min(p.max_q, p.M)), seqs = (p.M + n - 1) / n, G = p.H / p.KVH;
   const double keys = causal ? std::max(p.max_kv - 0.5 * n, 0.5 * n) : p.max_kv;
   auto tiles = [&](int rows) {
@@ -404,14 +406,15 @@ bool long_chunks(const PagedAttnParams &p, int cus, bool causal) {
   };
   const double few = tiles(RT), many = tiles(CHUNK_ROWS);
   const double cut = chunk_each((i64)many, cus, p) ? 0 : 2ll * p.max_q >= p.max_kv ? 30 : 13;
-  return 18 + many * (0.036 + 0.0085 / 64 * keys) + cut < 10 + few * (0.012 + 0.001 / 32 * keys);
+  const double wide = d / 128.0;
+  return 18 + many * (0.036 + 0.0085 / 64 * wide * keys) + cut < 10 + few * wide * (0.012 + 0.001 / 32 * keys);
 }
 
 template <int DG, int T, bool CAUSAL>
 int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
   const int cus = std::max(1, cu_count());
-  if (DG == 128 && (rows ? rows == CHUNK_ROWS : long_chunks(p, cus, CAUSAL)))
-    return launch_attention_chunk(T, CAUSAL, ex, a, bt, p, err);
+  if (rows ? rows == CHUNK_ROWS : long_chunks(DG, p, cus, CAUSAL))
+    return launch_attention_chunk(DG, T, CAUSAL, ex, a, bt, p, err);
   const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
   const Heads hd{G, HS, GP};
   const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
@@ -498,7 +501,7 @@ LaunchFn pick(int t) {
 }  // namespace
 
 // Macros: HD (64, 96 or 128), IN_T (half | bfloat: queries, cache and output), CAUSAL, and ROWS, which names the rows of a
-// tile: 32, or with HD 128 256; 0 (the default) chooses them by the size.
+// tile, 32 or 256; 0 (the default) chooses them by the size.
 bool make_attention_paged(const Macros &m, Pipeline *pl, std::string *err) {
   int hd, causal, rows;
   if (!macro_int(m, "HD", 128, &hd, err) || !macro_int(m, "CAUSAL", 1, &causal, err) || !macro_int(m, "ROWS", 0, &rows, err))
@@ -517,8 +520,8 @@ bool make_attention_paged(const Macros &m, Pipeline *pl, std::string *err) {
     *err = "HD " + std::to_string(hd) + " not supported (64, 96 or 128)";
     return false;
   }
-  if (rows != 0 && rows != RT && !(rows == CHUNK_ROWS && hd == 128)) {
-    *err = "ROWS must be 0, 32, or 256 with HD 128";
+  if (rows != 0 && rows != RT && rows != CHUNK_ROWS) {
+    *err = "ROWS must be 0, 32 or 256";
     return false;
   }
   pl->launch = hd == 128 ? pick<128>(t) : hd == 96 ? pick<96>(t) : pick<64>(t);

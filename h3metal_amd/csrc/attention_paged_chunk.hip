@@ -1,5 +1,5 @@
-// The paged attention of long chunks for gfx950 (head dim 128): tiles of 256 (token, head) rows. Semantics and the cut of the
-// work: attention_paged.hip.
+// The paged attention of long chunks for gfx950: tiles of 256 (token, head) rows. Semantics and the cut of the work:
+// attention_paged.hip.
 //
 // 4 waves per workgroup, one per SIMD, 64 rows each (two 32-row MFMA tiles that share every K and V operand), so that a tile
 // reads its keys 8 times less often than 32-row tiles do. The pipeline is attention_wave.hip's: a wave runs the softmax of
@@ -12,9 +12,13 @@
 //  * Rows see keys up to one of their own: the blocks that some row does not see whole run in a loop of their own, which masks.
 //  * V of those blocks is searched in LDS for infinities and NaN, which a weight of 0 would not keep out of a sum: they are taken
 //    as 0, and the rows that see them get them at the end. So is what a page holds behind the sequence's end.
+// LDS rows of head dim 96 are as wide as those of 128 (what is behind its channels is never read); a step has as many slots for
+// instructions and loads at every head dim, some of them empty.
 // A prompt of 8192 tokens (32 + 8 heads) takes 500 us, 1.1 PFLOP/s, a large library product's rate on the same card; a step of
 // 64 keys 2.1 us, of which its 64 matrix instructions would take 0.9: the softmax's instructions beside them bound it. A tile
-// starts and ends in about 15 us, so code is kept in two copies only and everything of a start is asked for at once.
+// starts and ends in about 15 us, so code is kept in two copies only and everything of a start is asked for at once. A
+// prompt of 4096 tokens takes 170 us at head dim 128 (0.82 PFLOP/s), 146 at 96 (0.70) and 120 at 64 (0.57), where as many
+// exponentials stand beside half the matrix instructions.
 #include "paged_attn.h"
 
 #include <algorithm>
@@ -30,24 +34,37 @@ __device__ __forceinline__ void mma_pv_acc(f32x16 &acc, i16x8 a, typename Vec8<V
   if constexpr (VT == T_BF16) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
   else asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
-__device__ __forceinline__ void o_fence(f32x16 (&o)[2][4]) {  // a 16-pass result needs 18 wait states
-  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 4"
-               : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[0][2]), "+a"(o[0][3]), "+a"(o[1][0]), "+a"(o[1][1]),
-                 "+a"(o[1][2]), "+a"(o[1][3]));
+template <int NDB>
+__device__ __forceinline__ void o_fence(f32x16 (&o)[2][NDB]) {  // a 16-pass result needs 18 wait states
+  if constexpr (NDB == 4)
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 4"
+                 : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[0][2]), "+a"(o[0][3]), "+a"(o[1][0]), "+a"(o[1][1]),
+                   "+a"(o[1][2]), "+a"(o[1][3]));
+  else if constexpr (NDB == 3)
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 4"
+                 : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[0][2]), "+a"(o[1][0]), "+a"(o[1][1]), "+a"(o[1][2]));
+  else
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 4" : "+a"(o[0][0]), "+a"(o[0][1]), "+a"(o[1][0]), "+a"(o[1][1]));
 }
 
 constexpr int NWC = 4;                    // waves per workgroup
 constexpr int NU = 2;                     // 32-row tiles per wave
 constexpr int RTC = NWC * 32 * NU;        // rows of a tile
 static_assert(RTC == CHUNK_ROWS, "rows of a tile");
-constexpr int D = 128, RB = D * 2;        // channels, bytes of a row
-constexpr int NCH = RB / 32;              // score MFMAs per 32 x 32 tile
 constexpr int NR = 4;                     // blocks of a ring
-constexpr int KBYTES = BK * RB;           // a block of K or V
-constexpr int VOFF = NR * KBYTES;
-constexpr int LDSC = RTC * (D * 4 + 16) > 2 * NR * KBYTES ? RTC * (D * 4 + 16) : 2 * NR * KBYTES;  // rings, then outputs
-constexpr int GPB = BK / 16;              // 16-key groups of a block, one 1 KB load of a wave each
-static_assert(KBYTES == GPB * NWC * 1024, "a wave loads 4 rows of each group");
+constexpr int GPB = BK / 16;              // 16-key groups of a block
+
+template <int DG>
+struct Chunk {
+  static constexpr int D = DG == 96 ? 128 : DG;              // channels of an LDS row
+  static constexpr int RB = D * 2, RBG = DG * 2;             // bytes of a row: in LDS, in memory
+  static constexpr int NCH = DG / 16, NDB = DG / 32;         // score MFMAs per 32 x 32 tile, 32-channel blocks of O
+  static constexpr int KBYTES = BK * RB, VOFF = NR * KBYTES;  // a block of K or V; the V ring
+  static constexpr int LPB = KBYTES / (NWC * 1024);          // 1 KB loads of a wave and block
+  static constexpr int S16 = DG * 2 + 8, S32 = DG * 4 + 16;  // bytes between output rows in LDS
+  static constexpr int LDS = RTC * S32 > 2 * VOFF ? RTC * S32 : 2 * VOFF;  // rings, then outputs
+  static_assert(LPB == 4 || LPB == 2, "a load holds 4 or 8 rows of a group");
+};
 
 // accepted growth of a row sum per key block: bf16 P (float's exponent range) and f16 P (largest finite 65504)
 template <int VT>
@@ -63,9 +80,11 @@ struct __attribute__((packed, aligned(8))) Piece {  // 16 bytes of an output row
   float v[4];
 };
 
-template <int VT, bool CAUSAL, bool EACH>
+template <int D, int VT, bool CAUSAL, bool EACH>
 __global__ __launch_bounds__(NWC * 64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh, Heads hd, int least) {
+  using C = Chunk<D>;
+  constexpr int RB = C::RB, NCH = C::NCH, NDB = C::NDB, KBYTES = C::KBYTES, VOFF = C::VOFF, LPB = C::LPB;
   using VT8 = typename Vec8<VT>::type;
   using VE = typename Vec8<VT>::elem;
   using VP2 = typename Vec8<VT>::pair;
@@ -97,15 +116,19 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     more = tile_at(order, x0, &tile);
   }
 
-  // this lane's 16 bytes of each 1 KB load, within a group of 16 rows: row and swizzled piece (attention_common.h: kswz, voff)
-  const int lrow = w * 4 + (lane >> 4);
-  const unsigned kgo = lrow * RB + ((lane & 15) ^ lrow) * 16;
-  const unsigned vgo = lrow * RB + (2 * (((lane & 15) >> 1) ^ (2 * (lrow & 3))) + (lane & 1)) * 16;
+  // this lane's 16 bytes of each 1 KB load, within a group of 16 rows: row and swizzled piece (attention_common.h: kswz, voff);
+  // what lies past a row in memory (head dim 96) is never read and takes another piece of it
+  constexpr int NP = RB / 16, R1 = 64 / NP, RW = 256 / RB;  // pieces of a row, rows of a load, of 256 bytes
+  const int lrow = (w * R1 + lane / NP) & 15, lpc = lane % NP;
+  const int kp = lpc ^ kswz<RB, NP>(lrow), vp = 2 * ((lpc >> 1) ^ (2 * ((lrow & 3) / RW))) + (lpc & 1);
+  const unsigned kgo = lrow * C::RBG + (kp * 16 < C::RBG ? kp : kp - NP / 2) * 16;
+  const unsigned vgo = lrow * C::RBG + (vp * 16 < C::RBG ? vp : vp - NP / 2) * 16;
+  auto group_of = [&](int r) __attribute__((always_inline)) { return (r * NWC + w) * R1 / 16; };  // of load r of a block
   const int krow = 16 * (l32 >> 4) + 8 * ((l32 >> 2) & 1) + 4 * ((l32 >> 3) & 1) + (l32 & 3);
   const int l16 = lane & 15, tr_row = l16 >> 2, tr_col = (l16 & 3) * 8;
-  unsigned vbase[D / 32], kbase[NCH];
+  unsigned vbase[NDB], kbase[NCH];
 #pragma unroll
-  for (int db = 0; db < D / 32; db++) vbase[db] = voff<D>(8 * hl + tr_row, (db * 32 + (l32 & 16)) / 8) + tr_col;
+  for (int db = 0; db < NDB; db++) vbase[db] = voff<C::D>(8 * hl + tr_row, (db * 32 + (l32 & 16)) / 8) + tr_col;
 #pragma unroll
   for (int c = 0; c < NCH; c++) kbase[c] = krow * RB + (((2 * c + hl) ^ kswz<RB, RB / 16>(krow)) * 16);
 
@@ -180,7 +203,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       const unsigned long long bad = __ballot(there && !in);
       if (__builtin_expect(bad != 0, 0)) lost = min(lost, ((i64)blk0 * GPB + win * 64 + __builtin_ctzll(bad)) * 16);
       const unsigned long long off =
-          ((((unsigned long long)id * p.KVH + kvh) << bt.lg) + (key & ((1 << bt.lg) - 1))) * RB;
+          ((((unsigned long long)id * p.KVH + kvh) << bt.lg) + (key & ((1 << bt.lg) - 1))) * C::RBG;
       const unsigned long long ka = (unsigned long long)(there && in ? a.kc + off : a.spare);
       const unsigned long long va = (unsigned long long)(there && in ? a.vc + off : a.spare);
       k_lo = (unsigned)ka;
@@ -207,11 +230,13 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
                    : "memory", "m0", "scc");
     };
     const unsigned lds_w = lds0 + w * 1024;
-    // load i < 4: group i of K of block kb; from 4 on: of V of block vb
+    // load i < LPB: of K of block kb; from there on: of V of block vb
     auto stage_one = [&](auto ic, int kb, int vb) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value, r = i & (GPB - 1);
-      if (i < GPB) stage(lds_w + (kb & (NR - 1)) * KBYTES, r * NWC * 1024, kgo, k_lo, k_hi, (kb & 15) * GPB + r);
-      else stage(lds_w + (vb & (NR - 1)) * KBYTES, VOFF + r * NWC * 1024, vgo, v_lo, v_hi, (vb & 15) * GPB + r);
+      constexpr int i = decltype(ic)::value, r = i % LPB;
+      if constexpr (i < LPB)
+        stage(lds_w + (kb & (NR - 1)) * KBYTES, r * NWC * 1024, kgo, k_lo, k_hi, (kb & 15) * GPB + group_of(r));
+      else if constexpr (i < 2 * LPB)
+        stage(lds_w + (vb & (NR - 1)) * KBYTES, VOFF + r * NWC * 1024, vgo, v_lo, v_hi, (vb & 15) * GPB + group_of(r));
     };
 
     auto stage_k = [&](int k, int kb, int vb) __attribute__((always_inline)) {  // (k is known where this is inlined)
@@ -227,12 +252,12 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       }
     };
 
-    f32x16 o[NU][D / 32];
+    f32x16 o[NU][NDB];
     float m[NU], l[NU], nmv[NU], la[NU][4];  // maximum, sum, -maximum (0 at -inf), running partial sums
 #pragma unroll
     for (int u = 0; u < NU; u++) {
 #pragma unroll
-      for (int db = 0; db < D / 32; db++)
+      for (int db = 0; db < NDB; db++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[u][db][i] = 0.0f;
       m[u] = -INFINITY;
@@ -252,12 +277,12 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       }
     bool odd = false;
 
-    struct Ops {  // operands of one key tile of a step: V of block j - 1 (index 4 * s2 + db), K of block j + 1
-      i16x8 va[8];
+    struct Ops {  // operands of one key tile of a step: V of block j - 1 (index NDB * s2 + db), K of block j + 1
+      i16x8 va[2 * NDB];
       i32x4 ka[NCH];
     };
     auto vread = [&](int j, int t, int k) __attribute__((always_inline)) {
-      const char *Vs = smem + VOFF + (j & (NR - 1)) * KBYTES + (32 * t + 16 * (k >> 2)) * RB + vbase[k & 3];
+      const char *Vs = smem + VOFF + (j & (NR - 1)) * KBYTES + (32 * t + 16 * (k / NDB)) * RB + vbase[k % NDB];
       const i16x4 lo = lds_tr16(Vs);
       const i16x4 hi = lds_tr16(Vs + 4 * RB);
       return i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -270,14 +295,14 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     // this wave's own loads of V of block j, landed: infinities and NaN out
     auto clean = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < GPB; r++) {
+      for (int r = 0; r < LPB; r++) {
         i32x4 *at = (i32x4 *)(smem + VOFF + (j & (NR - 1)) * KBYTES + (r * NWC + w) * 1024 + 16 * lane);
         i32x4 v = *at;
         bool some = false;
 #pragma unroll
         for (int e = 0; e < 4; e++) some |= odd_high<VT>((unsigned)v[e]) | odd_high<VT>((unsigned)v[e] << 16);
         if (__builtin_expect(__any(some), 0)) {
-          odd = odd || (some && ((i64)blk0 + j) * BK + 16 * r + lrow < L);
+          odd = odd || (some && ((i64)blk0 + j) * BK + 16 * group_of(r) + lrow < L);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             unsigned d = (unsigned)v[e];
@@ -297,14 +322,20 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       const float nm = nmv[u];
       const int see = mask ? beyond(j, u) : 0;
       float xv[16];
-      int npv = 0, ns = 0;
+      int npv = 0, ns = 0, pslot = 0, sslot = 0;
+      // 8 slots for either product's instructions, some of them empty at smaller head dims
+      auto taken = [](int slot) { return D == 128 || (D == 96 ? (slot & 3) != 3 : (slot & 1) == 0); };
       auto pv = [&]() __attribute__((always_inline)) {
-        const int k = npv++;
-        mma_pv_acc<VT>(o[u][k & 3], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k >> 2]));
-        if (refresh) op.va[k] = vread(jn - 1, tn, k);
-        if (nst) stage_k(k, j + 3, j + 1);
+        const int slot = pslot++;
+        if (taken(slot)) {
+          const int k = npv++;
+          mma_pv_acc<VT>(o[u][k % NDB], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k / NDB]));
+          if (refresh) op.va[k] = vread(jn - 1, tn, k);
+        }
+        if (nst) stage_k(slot, j + 3, j + 1);
       };
       auto sm = [&]() __attribute__((always_inline)) {
+        if (!taken(sslot++)) return;
         const int c = ns++;
         f32x16 zero;
 #pragma unroll
@@ -404,7 +435,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of the previous step
       if (mask) clean(j);
       __syncthreads();
-      sub_tile(op, j, 1, 1, mask, true, j + 1, 0, 2 * GPB);
+      sub_tile(op, j, 1, 1, mask, true, j + 1, 0, 1);
       sums(1);
       // rare: a score far above the running maximum: block j's weights again with the exact one (its K is still in its slot)
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
@@ -413,7 +444,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
         for (int u = 0; u < NU; u++) {
           const float f = exact(j, u, mask);
 #pragma unroll
-          for (int db = 0; db < D / 32; db++)
+          for (int db = 0; db < NDB; db++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[u][db][i] *= f;
           tot[u] = la[u][0];
@@ -438,9 +469,9 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #pragma unroll
     for (int b = 0; b < 3; b++)
 #pragma unroll
-      for (int i = 0; i < GPB; i++) stage_k(i, b, 0);
+      for (int i = 0; i < LPB; i++) stage_k(i, b, 0);
 #pragma unroll
-    for (int i = 0; i < GPB; i++) stage_k(GPB + i, 0, 0);
+    for (int i = 0; i < LPB; i++) stage_k(LPB + i, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < NU; u++)
@@ -453,7 +484,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     if (clear == 0) clean(0);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2 * GPB; i++) stage_k(i, 3, 1);
+    for (int i = 0; i < 2 * LPB; i++) stage_k(i, 3, 1);
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       exact(0, u, true);
@@ -470,14 +501,14 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       }
     Ops op;
 #pragma unroll
-    for (int k = 0; k < 8; k++) op.va[k] = vread(0, 0, k);
+    for (int k = 0; k < 2 * NDB; k++) op.va[k] = vread(0, 0, k);
 #pragma unroll
     for (int c = 0; c < NCH; c++) op.ka[c] = kread(2, 0, c);
     // from here on O lives in AGPRs only
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
-      for (int db = 0; db < D / 32; db++) asm volatile("" : "+a"(o[u][db]));
+      for (int db = 0; db < NDB; db++) asm volatile("" : "+a"(o[u][db]));
     int j = 1;
     for (; j < clear; j++) step(op, j, false);
     for (; j < nblk; j++) step(op, j, true);
@@ -486,12 +517,13 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     for (int t = 0; t < 2; t++) {
       if (t == 1) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) op.va[k] = vread(nblk - 1, 1, k);
+        for (int k = 0; k < 2 * NDB; k++) op.va[k] = vread(nblk - 1, 1, k);
       }
 #pragma unroll
       for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) mma_pv_acc<VT>(o[u][k & 3], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k >> 2]));
+        for (int k = 0; k < 2 * NDB; k++)
+          mma_pv_acc<VT>(o[u][k % NDB], op.va[k], __builtin_bit_cast(VT8, pb[t][u][k / NDB]));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads past the last block land before the slots are used again
     o_fence(o);
@@ -499,7 +531,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     // Outputs go through LDS (each wave its own rows, a few bytes apart, so that neither side meets bank conflicts): a lane holds
     // 4 channels of a row here and there, and stores 16 bytes of whole rows.
     __syncthreads();
-    constexpr int S16 = D * 2 + 8, S32 = D * 4 + 16;  // bytes between rows in LDS
+    constexpr int S16 = C::S16, S32 = C::S32;
     const unsigned mine = w * (32 * NU) * S32;
     float sum[NU];
 #pragma unroll
@@ -508,44 +540,48 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       if (last[u] >= lost) sum[u] = NAN;
     }
     if (EACH || whole) {
-      unsigned to = mine + l32 * S16 + 8 * hl, from = mine + (lane >> 4) * S16 + (lane & 15) * 16;
+      constexpr int LR = D == 64 ? 8 : 16, RI = 64 / LR;  // lanes a row (12 of 16 at head dim 96), rows at a time
+      const int piece = lane % LR;
+      unsigned to = mine + l32 * S16 + 8 * hl, from = mine + lane / LR * S16 + min(piece, D / 8 - 1) * 16;
       asm volatile("" : "+v"(to), "+v"(from));  // (the addresses of all pieces would be kept over the tiles' loop otherwise)
 #pragma unroll
       for (int u = 0; u < NU; u++) {
         // no sum although a key is visible: all scores are -infinity, and 0 / 0
         const float inv = sum[u] != 0.0f ? __builtin_amdgcn_rcpf(sum[u]) : last[u] >= 0 ? NAN : 0.0f;
 #pragma unroll
-        for (int db = 0; db < D / 32; db++)
+        for (int db = 0; db < NDB; db++)
 #pragma unroll
           for (int g = 0; g < 4; g++)
             store4<VT>(smem + to + 32 * u * S16 + (db * 32 + 8 * g) * 2, o[u][db][4 * g] * inv, o[u][db][4 * g + 1] * inv,
                        o[u][db][4 * g + 2] * inv, o[u][db][4 * g + 3] * inv);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      char *base = a.out + ((size_t)m0 * p.o_stride + (size_t)(kvh * hd.G + g0) * D) * 2 + (lane & 15) * 16;
+      char *base = a.out + ((size_t)m0 * p.o_stride + (size_t)(kvh * hd.G + g0) * D) * 2 + piece * 16;
 #pragma unroll 1
-      for (int i = 0; i < 32 * NU / 4; i += 4) {
+      for (int i = 0; i < 32 * NU / RI; i += 4) {
         float2 lo[4], hi[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          lo[k] = *(const float2 *)(smem + from + 4 * k * S16);
-          hi[k] = *(const float2 *)(smem + from + 4 * k * S16 + 8);
+          lo[k] = *(const float2 *)(smem + from + RI * k * S16);
+          hi[k] = *(const float2 *)(smem + from + RI * k * S16 + 8);
         }
-        from += 16 * S16;
+        from += 4 * RI * S16;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const int row = w * (32 * NU) + 4 * (i + k) + (lane >> 4), ti = row_token(row), gi = row - ti * hd.GP;
-          if (row < R && g0 + gi < hd.G)
+          const int row = w * (32 * NU) + RI * (i + k) + lane / LR, ti = row_token(row), gi = row - ti * hd.GP;
+          if (row < R && g0 + gi < hd.G && piece < D / 8)
             *(Piece *)(base + ((size_t)ti * p.o_stride + gi * D) * 2) = Piece{{lo[k].x, lo[k].y, hi[k].x, hi[k].y}};
         }
       }
     } else {
-      unsigned to = mine + l32 * S32 + 16 * hl, from = mine + hl * S32 + l32 * 16;
+      constexpr int LR = D == 64 ? 16 : 32, RI = 64 / LR;  // (24 of 32 at head dim 96)
+      const int piece = lane % LR;
+      unsigned to = mine + l32 * S32 + 16 * hl, from = mine + lane / LR * S32 + min(piece, D / 4 - 1) * 16;
       asm volatile("" : "+v"(to), "+v"(from));
 #pragma unroll
       for (int u = 0; u < NU; u++) {
 #pragma unroll
-        for (int db = 0; db < D / 32; db++)
+        for (int db = 0; db < NDB; db++)
 #pragma unroll
           for (int g = 0; g < 4; g++)
             store4<T_F32>(smem + to + 32 * u * S32 + (db * 32 + 8 * g) * 4, o[u][db][4 * g], o[u][db][4 * g + 1],
@@ -553,15 +589,16 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
         if (hl == 0) *(float2 *)(st + RTC * D + 2 * (w * (32 * NU) + 32 * u + l32)) = make_float2(m[u], sum[u]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      float *base = st + (w * (32 * NU) + hl) * D + 4 * l32;
+      float *base = st + (w * (32 * NU) + lane / LR) * D + 4 * piece;
 #pragma unroll 1
-      for (int i = 0; i < 32 * NU / 2; i += 8) {
+      for (int i = 0; i < 32 * NU / RI; i += 8) {
         f32x4 v[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = *(const f32x4 *)(smem + from + 2 * k * S32);
-        from += 16 * S32;
+        for (int k = 0; k < 8; k++) v[k] = *(const f32x4 *)(smem + from + RI * k * S32);
+        from += 8 * RI * S32;
 #pragma unroll
-        for (int k = 0; k < 8; k++) *(f32x4 *)(base + 2 * (i + k) * D) = v[k];
+        for (int k = 0; k < 8; k++)
+          if (piece < D / 4) *(f32x4 *)(base + RI * (i + k) * D) = v[k];
       }
     }
     odd = __syncthreads_or(odd);
@@ -579,7 +616,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
           const int pg = bt.table[(size_t)tile.b * bt.width + (key >> bt.lg)];
           if (pg < 0 || pg >= bt.pages) continue;
           const size_t row = (((size_t)pg * p.KVH + kvh) << bt.lg) + (size_t)(key & ((1 << bt.lg) - 1));
-          const i32x4 vv = *(const i32x4 *)(a.vc + row * RB + d0 * 2);
+          const i32x4 vv = *(const i32x4 *)(a.vc + row * C::RBG + d0 * 2);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             const unsigned x = (unsigned)vv[e / 2] << (e & 1 ? 0 : 16);
@@ -604,24 +641,24 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
   if (!EACH && !unfinished && tid == 0) left_of(a, sl)->R = 0;
 }
 
-template <int VT, bool CAUSAL, bool EACH>
+template <int D, int VT, bool CAUSAL, bool EACH>
 int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Shape &sh, const Heads &hd,
         unsigned grid, int least, std::string *err) {
-  auto kern = attention_chunk_kernel<VT, CAUSAL, EACH>;
+  auto kern = attention_chunk_kernel<D, VT, CAUSAL, EACH>;
   static bool attr_set = false;
   if (!attr_set) {
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDSC);
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Chunk<D>::LDS);
     if (e != hipSuccess) {
       *err = std::string("hipFuncSetAttribute: ") + hipGetErrorString(e);
       return -1;
     }
     attr_set = true;
   }
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(NWC * 64), LDSC, ex.stream, a, bt, p, sh, hd, least);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(NWC * 64), Chunk<D>::LDS, ex.stream, a, bt, p, sh, hd, least);
   return 0;
 }
 
-template <int VT, bool CAUSAL>
+template <int D, int VT, bool CAUSAL>
 int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
   const int G = p.H / p.KVH, HS = (G + RTC - 1) / RTC, GP = (G + HS - 1) / HS, TT = RTC / GP;
   const Heads hd{G, HS, GP};
@@ -633,9 +670,9 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
   g.left = (char *)ex.ws + most * (state - sizeof(Left));
-  g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 4 KB that can be read
-  if (chunk_each(tiles, most, p)) return run<VT, CAUSAL, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
-  if (run<VT, CAUSAL, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
+  g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 16 rows that can be read (no page has fewer)
+  if (chunk_each(tiles, most, p)) return run<D, VT, CAUSAL, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
+  if (run<D, VT, CAUSAL, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
   if (most > 1)
     hipLaunchKernelGGL((attention_join_kernel<D, VT, RTC, 4>), dim3((unsigned)(most - 1), RTC / 16), dim3(256), 0, ex.stream, g,
                        p.o_stride);
@@ -644,10 +681,16 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
 
 }  // namespace
 
-int launch_attention_chunk(int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p,
-                           std::string *err) {
-  if (t == T_BF16) return causal ? run<T_BF16, true>(ex, a, bt, p, err) : run<T_BF16, false>(ex, a, bt, p, err);
-  return causal ? run<T_F16, true>(ex, a, bt, p, err) : run<T_F16, false>(ex, a, bt, p, err);
+int launch_attention_chunk(int d, int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt,
+                           const PagedAttnParams &p, std::string *err) {
+  auto go = [&](auto dc) {
+    constexpr int D = decltype(dc)::value;
+    if (t == T_BF16) return causal ? run<D, T_BF16, true>(ex, a, bt, p, err) : run<D, T_BF16, false>(ex, a, bt, p, err);
+    return causal ? run<D, T_F16, true>(ex, a, bt, p, err) : run<D, T_F16, false>(ex, a, bt, p, err);
+  };
+  if (d == 64) return go(std::integral_constant<int, 64>{});
+  if (d == 96) return go(std::integral_constant<int, 96>{});
+  return go(std::integral_constant<int, 128>{});
 }
 
 }  // namespace h3

@@ -23,7 +23,7 @@ struct AttnArgs {
   const char *spare;  // memory that loads without a place of their own may read
 };
 
-// Tiles of 256 rows for long chunks (attention_paged_chunk.hip), head dim 128; t: T_BF16 or T_F16.
+// Tiles of 256 rows for long chunks (attention_paged_chunk.hip); t: T_BF16 or T_F16.
 constexpr int CHUNK_ROWS = 256;
 // Whether its workgroups take whole tiles, in the order of their length: from 2 tiles a compute unit on where tiles differ in
 // length (a prompt from its start: 4096 tokens 220 -> 167 us), from 4 on where they do not and a last round would be short of
@@ -32,8 +32,8 @@ inline bool chunk_each(i64 tiles, int most, const PagedAttnParams &p) {
   return tiles <= 1 << 22 && tiles >= (2ll * p.max_q >= p.max_kv ? 2 : 4) * (i64)most;
 }
 constexpr int M_MOST = 1 << 24;  // rows of a call are fewer
-int launch_attention_chunk(int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p,
-                           std::string *err);
+int launch_attention_chunk(int d, int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt,
+                           const PagedAttnParams &p, std::string *err);
 
 namespace {
 

@@ -260,8 +260,8 @@ def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, ta
     not reach its output. A page number outside the cache makes the scores of its keys NaN; kv_len past the table's
     pages counts up to them. max_q and max_kv, the most new tokens and keys of a sequence as far as the caller knows, choose
     the kernel and how far it splits the keys (default: M, and the table's pages); results hold whatever they say. no_alloc: the
-    allocation-free entry point; its scratch array may split the keys less far. variant: ROWS names the rows of a tile (32, or
-    256 with head dim 128), which is chosen by the size otherwise."""
+    allocation-free entry point; its scratch array may split the keys less far. variant: ROWS names the rows of a tile (32 or
+    256), which is chosen by the size otherwise."""
     if q.dtype != kc.dtype or out.dtype != q.dtype:
         raise ValueError(f"attention_paged: q, kc, vc and out must all be f16 or all bf16, got {q.dtype}, {kc.dtype}, "
                          f"{vc.dtype}, {out.dtype}")
