@@ -22,6 +22,7 @@
 #include "paged_attn.h"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace h3 {
 namespace {
@@ -183,7 +184,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       const int r = w * (32 * NU) + 32 * u + l32;
       const int ti = row_token(r), gi = r - ti * hd.GP;
       ok[u] = r < R && g0 + gi < hd.G;
-      last[u] = !ok[u] ? -1 : CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
+      // (a lane without a row looks at every key with a query of zeros, so that it never asks for a block to be done again)
+      last[u] = ok[u] && CAUSAL ? (int)plan::clamp(q.off + m0 + ti, -1, q.L - 1) : L - 1;
       qrow[u] = a.q + ((size_t)(m0 + (ok[u] ? ti : 0)) * p.q_stride + (size_t)(kvh * hd.G + (ok[u] ? g0 + gi : 0)) * D) * 2;
     }
 
@@ -253,7 +255,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     };
 
     f32x16 o[NU][NDB];
-    float m[NU], l[NU], nmv[NU], la[NU][4];  // maximum, sum, -maximum (0 at -inf), running partial sums
+    float m[NU], l[NU], nmv[NU], la[NU][4];  // maximum, sum, -maximum (FLT_MAX at -inf), running partial sums
 #pragma unroll
     for (int u = 0; u < NU; u++) {
 #pragma unroll
@@ -261,7 +263,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #pragma unroll
         for (int i = 0; i < 16; i++) o[u][db][i] = 0.0f;
       m[u] = -INFINITY;
-      l[u] = nmv[u] = 0.0f;
+      l[u] = 0.0f;
+      nmv[u] = FLT_MAX;
 #pragma unroll
       for (int c = 0; c < 4; c++) la[u][c] = 0.0f;
     }
@@ -376,7 +379,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
     };
 
     // Row tile u's weights of block j with the block's own maximum, its sum so far in la[u][0]; returns the factor of what was
-    // summed before. (A row that sees no key of the first block sees none of the later ones either.)
+    // summed before. A row whose scores are all -infinity so far, or that sees no key, keeps the weights 0: its offset of FLT_MAX
+    // takes -infinity to 0 and any finite score to an infinite weight, so that the first block with one comes here.
     auto exact = [&](int j, int u, bool mask) __attribute__((always_inline)) {
       f32x16 xs[2];
       float bmax = -INFINITY;
@@ -398,7 +402,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       const float mn = fmaxf(m[u], fmaxf(bmax, __shfl_xor(bmax, 32)) * p.scale);
       const float f = (m[u] == -INFINITY || mn == -INFINITY) ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
       m[u] = mn;
-      const float nm = mn == -INFINITY ? 0.0f : -mn;
+      const float nm = mn == -INFINITY ? FLT_MAX : -mn;
       nmv[u] = nm;
       float add[2] = {0.0f, 0.0f};
 #pragma unroll
