@@ -5,6 +5,7 @@
 #include "attention_common.h"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace h3 {
 namespace {
@@ -245,12 +246,15 @@ void attention_wave_kernel(const char *__restrict__ Q, const char *__restrict__ 
       for (int i = 0; i < 16; i++) o[u][db][i] = 0.0f;
   // l: row sums up to the previous block; la: running partial row sums (four chains per query tile)
   float m[NU], l[NU];
-  float nmv[NU];  // -m (0 while m = -inf): the exponent offset, changed only where m changes
+  // -m: the exponent offset, changed only where m changes. While m = -inf it is FLT_MAX: scores of -infinity keep the weight 0,
+  // and a finite one gets an infinite weight, which sends its block to the exact path below.
+  float nmv[NU];
   float la[NU][4];  // running partial row sums (four chains per query tile)
 #pragma unroll
   for (int u = 0; u < NU; u++) {
     m[u] = -INFINITY;
-    l[u] = nmv[u] = 0.0f;
+    l[u] = 0.0f;
+    nmv[u] = FLT_MAX;
 #pragma unroll
     for (int c = 0; c < 4; c++) la[u][c] = 0.0f;
   }
@@ -575,8 +579,8 @@ void attention_wave_kernel(const char *__restrict__ Q, const char *__restrict__ 
 #ifdef WAVE_NO_CHECK
     bad = false;
 #endif
-    // rare: a score far above the reference maximum, or the first block (no maximum yet; it always holds
-    // valid keys, so m is finite after it): recompute block j's P with the exact maximum
+    // rare: a score far above the reference maximum, or the first block (no maximum yet): recompute block j's P with
+    // the exact maximum
     if (__builtin_expect(j == 0 || __builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
       o_fence(o);  // P V MFMAs of this step may still be writing O
 #pragma unroll
@@ -605,7 +609,7 @@ void attention_wave_kernel(const char *__restrict__ Q, const char *__restrict__ 
         for (int db = 0; db < D / 32; db++)
 #pragma unroll
           for (int i = 0; i < 16; i++) o[u][db][i] *= f;
-        const float nm = mn == -INFINITY ? 0.0f : -mn;
+        const float nm = mn == -INFINITY ? FLT_MAX : -mn;
         nmv[u] = nm;
         tot[u] = l[u] + (exps(xs[0], qsc[u], nm, pb[0][u]) + exps(xs[1], qsc[u], nm, pb[1][u]));
         la[u][0] = tot[u];
