@@ -132,7 +132,7 @@ void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape 
       unfinished = true;
     }
     if (!EACH && blk0 == blk1) {  // a part without blocks (a whole tile has one)
-      if (tid < R) *(float2 *)(st + RT * DG + 2 * tid) = make_float2(-INFINITY, 0.0f);
+      if (tid < R) *(float2 *)(st + RT * DG + 2 * tid) = make_float2(-INFINITY, NO_PART);
       continue;
     }
     // this lane's query row: its token, head and last visible key

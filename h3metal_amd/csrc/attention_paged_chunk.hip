@@ -168,7 +168,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       unfinished = true;
     }
     if (!EACH && blk0 == blk1) {  // a part without blocks (a whole tile has one)
-      if (tid < R) *(float2 *)(st + RTC * D + 2 * tid) = make_float2(-INFINITY, 0.0f);
+      if (tid < R) *(float2 *)(st + RTC * D + 2 * tid) = make_float2(-INFINITY, NO_PART);
       continue;
     }
     // blocks (from blk0 on) that every row sees whole

@@ -230,9 +230,13 @@ __device__ __forceinline__ int last_slice(const plan::Cut &cut, int i, i64 e) {
   return n - 1;
 }
 
-// Joins the parts of cut tiles: o = sum 2^(m_k - m) o_k / sum 2^(m_k - m) l_k. Workgroup (j, y): the tile that slice j leaves
-// unfinished, rows from 4 RPW y on, RPW a wave; a wave's halves take every other part, 4 channels a lane. It is bound by the
-// chain of three loads (the tile, the weights, the outputs), so those of all rows and parts are under way at once.
+// A part without key blocks has no outputs: the sign of its sum of 0, and of its factor, says so.
+constexpr float NO_PART = -0.0f;
+
+// Joins the parts of cut tiles: o = sum 2^(m_k - m) o_k / sum 2^(m_k - m) l_k. A part whose factor vanishes counts all the
+// same: infinities and NaN of its outputs make NaN, as they would if the row had not been cut. Workgroup (j, y): the tile that
+// slice j leaves unfinished, rows from 4 RPW y on, RPW a wave; a wave's halves take every other part, 4 channels a lane. It is
+// bound by the chain of three loads (the tile, the weights, the outputs), so those of all rows and parts are under way at once.
 template <int DG, int T, int RT, int RPW>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int o_stride) {
   const int j = blockIdx.x, lane = threadIdx.x & 63, half = lane >> 5;
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int o_s
     float f[RPW];
 #pragma unroll
     for (int i = 0; i < RPW; i++) {
-      s[i] = make_float2(-INFINITY, 0.0f);
+      s[i] = make_float2(-INFINITY, NO_PART);
       if (lane < parts && r0 + i < t.R) s[i] = *(const float2 *)(state(k0 + lane) + RT * DG + 2 * (r0 + i));
     }
 #pragma unroll
@@ -266,7 +270,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int o_s
       top = fmaxf(top, mx[i]);
       // a sum of 0: nothing was seen (a sum of NaN counts, whatever its maximum)
       const float f0 = sum[i] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mx[i] - top);
-      f[i] = s[i].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(s[i].x - top);
+      f[i] = s[i].y == 0.0f ? s[i].y : __builtin_amdgcn_exp2f(s[i].x - top);
       float add = f[i] * s[i].y;
 #pragma unroll
       for (int k = 1; k < 64; k *= 2) add += __shfl_xor(add, k);
@@ -286,7 +290,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a, int o_s
             const int from = k1 + 2 * k + half;
             fk[i][k] = __shfl(f[i], from);
             u[i][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (from < parts && fk[i][k] != 0.0f) u[i][k] = *(const f32x4 *)(state(k0 + from) + (r0 + i) * DG + d);
+            if (from < parts && __builtin_bit_cast(int, fk[i][k]) >= 0)
+              u[i][k] = *(const f32x4 *)(state(k0 + from) + (r0 + i) * DG + d);
           }
 #pragma unroll
         for (int i = 0; i < RPW; i++)

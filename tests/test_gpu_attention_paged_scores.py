@@ -45,3 +45,16 @@ def test_all_keys_score_minus_infinity(gpu, ROWS):
     for new, keys in (([70], [70]), ([5], [3000])):
         c = masked(new, keys, [(0, -np.inf)])
         assert np.isnan(check(launch(gpu, c, scale=1.0, ROWS=ROWS), c, scale=1.0)).all()
+
+
+@pytest.mark.parametrize("ROWS", [32, 256])
+@pytest.mark.parametrize("D,t", [(128, "bf16"), (96, "f16"), (64, "bf16")])
+def test_seen_values_whose_weight_vanishes(gpu, D, t, ROWS):
+    """NaN, or an infinity with a weight below any float, in the value of a seen key: the channel is NaN, also where the key
+    lies in a part of a cut tile whose factor is 0."""
+    for new, keys in (([1], [3000]), ([64], [3000]), ([70], [400])):
+        for level, what in ((300.0, np.nan), (1200.0, np.inf), (1200.0, -np.inf)):
+            c = masked(new, keys, [(0, 0.0), (keys[0] // 2, level)], t=t, D=D, seed=3)
+            c["vc"][c["table"][0, 0], 0, 3, 10] = as_type(np.array([what]), t)[0][0]
+            want = check(launch(gpu, c, scale=1.0, ROWS=ROWS), c, scale=1.0)
+            assert np.isnan(want[:, :, 10]).all() and np.isfinite(want[:, :, :10]).all()
