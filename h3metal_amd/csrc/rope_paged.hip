@@ -198,9 +198,10 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
       for (int i = 0; i < PL; i++) ss = fmaf(v[i], v[i], ss);
       ss = slot_sum<S::LPS>(ss);
       float inv = __builtin_amdgcn_rsqf(ss * (1.0f / HDIM) + p.eps);
-      if (__builtin_expect(__any(turned && !(ss > 0x1p-80f && ss < 0x1p+120f)), 0)) {
-        // squares that leave a float's range: the row by a power of two that brings its largest value near 1, eps by its
-        // square (2^60 at most upwards: below that eps is all of the sum, or 0)
+      const bool out = turned && !(ss > 0x1p-80f && ss < 0x1p+120f);
+      if (__builtin_expect(__any(out), 0)) {
+        // squares that leave a float's range: the head by a power of two that brings its largest value near 1, eps by its
+        // square (2^60 at most upwards: below that eps is all of the sum, or 0). The wave's other heads keep what they have.
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < PL; i++) top = fmaxf(top, fabsf(v[i]));
@@ -210,11 +211,11 @@ __global__ __launch_bounds__(256) void rope_paged_kernel(RopeArgs a, Batch bt, P
         float s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < PL; i++) {
-          v[i] = turned ? ldexpf(v[i], -e) : v[i];
+          v[i] = out ? ldexpf(v[i], -e) : v[i];
           s2 = fmaf(v[i], v[i], s2);
         }
         s2 = slot_sum<S::LPS>(s2);
-        inv = 1.0f / sqrtf(s2 * (1.0f / HDIM) + ldexpf(p.eps, -2 * e));
+        inv = out ? 1.0f / sqrtf(s2 * (1.0f / HDIM) + ldexpf(p.eps, -2 * e)) : inv;
       }
       if (turned) {
 #pragma unroll
