@@ -18,8 +18,8 @@ def frequencies(rot: int, *, base: float = 10000.0, scaling: str = "none", facto
       linear: every frequency / factor (positions interpolated)
       ntk:    the base grows by factor^(rot / (rot - 2)): the fastest pair keeps its frequency, the slowest one is / factor
       yarn:   pairs that turn at least `fast` times over the `trained` positions keep their frequency, those that turn at most
-              `slow` times are / factor, between them the share falls linearly with j (bounds at whole pairs); rotated
-              channels times 0.1 ln(factor) + 1"""
+              `slow` times are / factor, between them the share falls linearly with j (bounds at whole pairs, the slow one
+              at rot - 1 at most: it may lie behind the last pair, rot / 2 - 1); rotated channels times 0.1 ln(factor) + 1"""
     if rot < 2 or rot % 2:
         raise ValueError(f"rope: rot must be even and positive, got {rot}")
     if not (base > 1 and math.isfinite(base)) or not (factor >= 1 and math.isfinite(factor)):
@@ -37,7 +37,7 @@ def frequencies(rot: int, *, base: float = 10000.0, scaling: str = "none", facto
     if trained < 1 or not fast > slow > 0:
         raise ValueError(f"rope: yarn needs the trained positions and fast > slow > 0, got {trained}, {fast}, {slow}")
     first, last = (rot * math.log(trained / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (fast, slow))
-    first, last = max(math.floor(first), 0), min(math.ceil(last), rot // 2 - 1)
+    first, last = max(math.floor(first), 0), min(math.ceil(last), rot - 1)
     share = 1 - np.clip((j - first) / max(last - first, 1e-3), 0, 1)
     return f * share + f / factor * (1 - share), 0.1 * math.log(factor) + 1.0
 
