@@ -38,7 +38,7 @@ def frequencies(rot: int, *, base: float = 10000.0, scaling: str = "none", facto
         raise ValueError(f"rope: yarn needs the trained positions and fast > slow > 0, got {trained}, {fast}, {slow}")
     first, last = (rot * math.log(trained / (n * 2 * math.pi)) / (2 * math.log(base)) for n in (fast, slow))
     first, last = max(math.floor(first), 0), min(math.ceil(last), rot - 1)
-    share = 1 - np.clip((j - first) / max(last - first, 1e-3), 0, 1)
+    share = 1 - np.clip((j - first) / max(last - first, 1e-3), 0, 1) if last > 0 else 0 * j  # (0: all turn too seldom)
     return f * share + f / factor * (1 - share), 0.1 * math.log(factor) + 1.0
 
 

@@ -39,3 +39,11 @@ def test_shares_of_the_pairs(rot, base, trained, factor, fast, slow):
     assert math.isclose(s, 0.1 * math.log(factor) + 1)
     laps = trained * f / (2 * math.pi)
     assert np.all(g[laps > slow * (1 + 1e-9)] > f[laps > slow * (1 + 1e-9)] / factor * (1 + 1e-9))  # not the whole factor
+
+
+@pytest.mark.parametrize("rot,trained,fast,slow", [(8, 6, 32.0, 1.0), (8, 60, 32.0, 20.0), (2, 1, 32.0, 1.0)])
+def test_trained_positions_that_no_pair_turns_often_over(rot, trained, fast, slow):
+    """Even the fastest pair turns at most `slow` times: all of them are divided."""
+    f, _ = rope.frequencies(rot, base=1e4)
+    g, _ = rope.frequencies(rot, base=1e4, scaling="yarn", factor=4.0, trained=trained, fast=fast, slow=slow)
+    assert shares(rot, 1e4, trained, fast, slow) == [1.0] * (rot // 2) and np.allclose(g, f / 4, rtol=1e-14, atol=0)
