@@ -23,7 +23,7 @@
 namespace h3 {
 namespace {
 
-constexpr int RT = 32;             // rows of a tile
+constexpr int RT = plan::SHORT_ROWS;
 constexpr int KB = 32;             // keys of a block
 constexpr float SLACK_P = 8.0f;    // log2 units the running maximum may lag behind a score
 
@@ -391,50 +391,22 @@ int run_rows(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttn
   return 0;
 }
 
-// Whether a call runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile, its blocks (of
-// 32 keys, of 64; their time goes with the head dim), and what cutting costs 256-row tiles; fitted to 60 calls of head dim 128 of
-// 1 to 64 sequences of 16 to 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head, and tried on 64 of
-// head dims 64 and 96, where it loses 1 % on average to the better choice. Measured at head dim 128 | 96 | 64, 32 rows -> 256: a
-// prompt of 4096 tokens 266 -> 170 | 238 -> 146 | 133 -> 120 us, of 1024 33 (256: 67) | 30 (59) | 18 (52), a chunk of 512 over
-// 16 384 keys 226 -> 150 | 200 -> 155 | 161 -> 119, of 64 over 4096 33 (38) | 32 (35) | 27 (30).
-bool long_chunks(int d, const PagedAttnParams &p, int cus, bool causal) {
-  const i64 n = std::max(1, std::min(p.max_q, p.M)), seqs = (p.M + n - 1) / n, G = p.H / p.KVH;
-  const double keys = causal ? std::max(p.max_kv - 0.5 * n, 0.5 * n) : p.max_kv;
-  auto tiles = [&](int rows) {
-    const i64 HS = (G + rows - 1) / rows, TT = rows / ((G + HS - 1) / HS);
-    return (double)(p.KVH * HS * seqs * ((n + TT - 1) / TT));
-  };
-  const double few = tiles(RT), many = tiles(CHUNK_ROWS);
-  const double cut = chunk_each((i64)many, cus, p) ? 0 : 2ll * p.max_q >= p.max_kv ? 30 : 13;
-  const double wide = d / 128.0;
-  return 18 + many * (0.036 + 0.0085 / 64 * wide * keys) + cut < 10 + few * wide * (0.012 + 0.001 / 32 * keys);
-}
-
 template <int DG, int T, bool CAUSAL>
 int run(int rows, const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
-  const int cus = std::max(1, cu_count());
-  if (rows ? rows == CHUNK_ROWS : long_chunks(DG, p, cus, CAUSAL))
-    return launch_attention_chunk(DG, T, CAUSAL, ex, a, bt, p, err);
-  const int G = p.H / p.KVH, HS = (G + RT - 1) / RT, GP = (G + HS - 1) / HS, TT = RT / GP;
-  const Heads hd{G, HS, GP};
-  const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
-  const size_t state = (size_t)2 * RT * (DG + 2) * sizeof(float) + sizeof(Left);  // of a slice
-  const int least = 256, most = std::max(1, (int)std::min<i64>(2 * cus, (i64)(ex.ws_bytes / state)));
-  // Whole tiles or slices. Few tiles of few keys are not worth a second kernel (one token, us whole with 8 waves and sliced: 512
-  // keys 13, 19; 2048 21, 19). Tiles that share keys stay whole, side by side, from one a compute unit on (24 chunks of 48 tokens
-  // over 2000 keys 86, 178 sliced); others are sliced until there are many, so that uneven lengths cost nothing.
-  const bool few = tiles <= cus && p.max_kv <= 2048;
-  const bool shared = p.max_q > TT;
-  const bool each = few || (tiles <= 1 << 22 && (p.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));
-  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, 128, (i64)bt.width << bt.lg};
+  const plan::Choice c = plan::choose(plan::Call{p.M, p.B, p.H, p.KVH, p.max_q, p.max_kv}, DG, CAUSAL, rows,
+                                      std::max(1, cu_count()), ex.ws_bytes);
+  if (c.rows == CHUNK_ROWS) return launch_attention_chunk(DG, T, CAUSAL, ex, a, bt, p, c, err);
+  const Heads hd = plan::heads_of(p.H, p.KVH, RT);
+  const int least = 256;  // weight of a slice
+  const plan::Shape sh{p.M, p.B, RT / hd.GP, p.KVH * hd.HS, CAUSAL, 128, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
-  g.left = (char *)ex.ws + most * (state - sizeof(Left));
-  if (few) return run_rows<DG, T, CAUSAL, 8, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
-  if (each) return run_rows<DG, T, CAUSAL, 4, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
-  if (run_rows<DG, T, CAUSAL, 4, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
-  if (most > 1)
-    hipLaunchKernelGGL((attention_join_kernel<DG, T, RT, 1>), dim3((unsigned)(most - 1), RT / 4), dim3(256), 0, ex.stream, g,
+  g.left = (char *)ex.ws + (size_t)c.most * 2 * RT * (DG + 2) * sizeof(float);
+  if (c.each && c.waves == 8) return run_rows<DG, T, CAUSAL, 8, true>(ex, g, bt, p, sh, hd, (unsigned)c.tiles, least, err);
+  if (c.each) return run_rows<DG, T, CAUSAL, 4, true>(ex, g, bt, p, sh, hd, (unsigned)c.tiles, least, err);
+  if (run_rows<DG, T, CAUSAL, 4, false>(ex, g, bt, p, sh, hd, (unsigned)c.most, least, err)) return -1;
+  if (c.most > 1)
+    hipLaunchKernelGGL((attention_join_kernel<DG, T, RT, 1>), dim3((unsigned)(c.most - 1), RT / 4), dim3(256), 0, ex.stream, g,
                        p.o_stride);
   return 0;
 }

@@ -663,34 +663,30 @@ int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParam
 }
 
 template <int D, int VT, bool CAUSAL>
-int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, std::string *err) {
-  const int G = p.H / p.KVH, HS = (G + RTC - 1) / RTC, GP = (G + HS - 1) / HS, TT = RTC / GP;
-  const Heads hd{G, HS, GP};
-  const int cus = std::max(1, cu_count());
-  const i64 tiles = (i64)p.KVH * HS * std::min<i64>(p.M, ((i64)p.M + (i64)p.B * (TT - 1)) / TT);
-  const size_t state = (size_t)2 * RTC * (D + 2) * sizeof(float) + sizeof(Left);  // of a slice
-  const int least = 512, most = std::max(1, (int)std::min<i64>(cus, (i64)(ex.ws_bytes / state)));
-  const plan::Shape sh{p.M, p.B, TT, p.KVH * HS, CAUSAL, 256, (i64)bt.width << bt.lg};
+int run(const Exec &ex, const AttnArgs &a, const Batch &bt, const PagedAttnParams &p, const plan::Choice &c, std::string *err) {
+  const Heads hd = plan::heads_of(p.H, p.KVH, RTC);
+  const int least = 512;  // weight of a slice
+  const plan::Shape sh{p.M, p.B, RTC / hd.GP, p.KVH * hd.HS, CAUSAL, 256, (i64)bt.width << bt.lg};
   AttnArgs g = a;
   g.ws = (float *)ex.ws;
-  g.left = (char *)ex.ws + most * (state - sizeof(Left));
+  g.left = (char *)ex.ws + (size_t)c.most * 2 * RTC * (D + 2) * sizeof(float);
   g.spare = p.pages ? a.kc : (const char *)ex.ws;  // 16 rows that can be read (no page has fewer)
-  if (chunk_each(tiles, most, p)) return run<D, VT, CAUSAL, true>(ex, g, bt, p, sh, hd, (unsigned)tiles, least, err);
-  if (run<D, VT, CAUSAL, false>(ex, g, bt, p, sh, hd, (unsigned)most, least, err)) return -1;
-  if (most > 1)
-    hipLaunchKernelGGL((attention_join_kernel<D, VT, RTC, 4>), dim3((unsigned)(most - 1), RTC / 16), dim3(256), 0, ex.stream, g,
-                       p.o_stride);
+  if (c.each) return run<D, VT, CAUSAL, true>(ex, g, bt, p, sh, hd, (unsigned)c.tiles, least, err);
+  if (run<D, VT, CAUSAL, false>(ex, g, bt, p, sh, hd, (unsigned)c.most, least, err)) return -1;
+  if (c.most > 1)
+    hipLaunchKernelGGL((attention_join_kernel<D, VT, RTC, 4>), dim3((unsigned)(c.most - 1), RTC / 16), dim3(256), 0, ex.stream,
+                       g, p.o_stride);
   return 0;
 }
 
 }  // namespace
 
 int launch_attention_chunk(int d, int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt,
-                           const PagedAttnParams &p, std::string *err) {
+                           const PagedAttnParams &p, const plan::Choice &c, std::string *err) {
   auto go = [&](auto dc) {
     constexpr int D = decltype(dc)::value;
-    if (t == T_BF16) return causal ? run<D, T_BF16, true>(ex, a, bt, p, err) : run<D, T_BF16, false>(ex, a, bt, p, err);
-    return causal ? run<D, T_F16, true>(ex, a, bt, p, err) : run<D, T_F16, false>(ex, a, bt, p, err);
+    if (t == T_BF16) return causal ? run<D, T_BF16, true>(ex, a, bt, p, c, err) : run<D, T_BF16, false>(ex, a, bt, p, c, err);
+    return causal ? run<D, T_F16, true>(ex, a, bt, p, c, err) : run<D, T_F16, false>(ex, a, bt, p, c, err);
   };
   if (d == 64) return go(std::integral_constant<int, 64>{});
   if (d == 96) return go(std::integral_constant<int, 96>{});

@@ -10,10 +10,7 @@ namespace h3 {
 
 using plan::i64;
 
-// Query heads of a tile: a key/value head's G heads in HS groups of GP (the last may have fewer).
-struct Heads {
-  int G, HS, GP;
-};
+using plan::Heads;
 
 struct AttnArgs {
   const char *q, *kc, *vc;
@@ -23,17 +20,11 @@ struct AttnArgs {
   const char *spare;  // memory that loads without a place of their own may read
 };
 
-// Tiles of 256 rows for long chunks (attention_paged_chunk.hip); t: T_BF16 or T_F16.
-constexpr int CHUNK_ROWS = 256;
-// Whether its workgroups take whole tiles, in the order of their length: from 2 tiles a compute unit on where tiles differ in
-// length (a prompt from its start: 4096 tokens 220 -> 167 us), from 4 on where they do not and a last round would be short of
-// tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost their states.
-inline bool chunk_each(i64 tiles, int most, const PagedAttnParams &p) {
-  return tiles <= 1 << 22 && tiles >= (2ll * p.max_q >= p.max_kv ? 2 : 4) * (i64)most;
-}
+constexpr int CHUNK_ROWS = plan::CHUNK_ROWS;
 constexpr int M_MOST = 1 << 24;  // rows of a call are fewer
+// Tiles of 256 rows for long chunks (attention_paged_chunk.hip); t: T_BF16 or T_F16.
 int launch_attention_chunk(int d, int t, bool causal, const Exec &ex, const AttnArgs &a, const Batch &bt,
-                           const PagedAttnParams &p, std::string *err);
+                           const PagedAttnParams &p, const plan::Choice &c, std::string *err);
 
 namespace {
 
@@ -219,6 +210,7 @@ __device__ __forceinline__ int slice_of(int b, int n) {
 struct Left {
   int R, m0, h0, GP, gc, first_last, end, pad;
 };
+static_assert(sizeof(Left) == plan::LEFT_BYTES, "what the host counts");
 __device__ __forceinline__ Left *left_of(const AttnArgs &a, int slice) { return (Left *)a.left + slice; }
 
 // The last slice that has a part of a tile that ends at weight e and begins in slice i.

@@ -122,5 +122,79 @@ H3_HD int block_at(i64 x, i64 p, i64 w, int n) { return x <= p ? 0 : x >= p + w 
 // A partial state's place: 2 i for the tile that slice i found begun, 2 i + 1 for the one it leaves unfinished.
 H3_HD int state_of(int i, bool begun) { return 2 * i + (begun ? 0 : 1); }
 
+// -- on the host: which kernel runs a call, and how its tiles are shared out --------------------------------------------
+
+constexpr int SHORT_ROWS = 32, CHUNK_ROWS = 256;  // rows of a tile: attention_paged.hip, attention_paged_chunk.hip
+constexpr int LEFT_BYTES = 32;                    // of what a slice leaves behind besides its two states
+
+// Query heads of a tile: a key/value head's G heads in HS groups of GP (the last may have fewer).
+struct Heads {
+  int G, HS, GP;
+};
+inline Heads heads_of(int H, int KVH, int rows) {
+  const int G = H / KVH, HS = (G + rows - 1) / rows;
+  return Heads{G, HS, (G + HS - 1) / HS};
+}
+
+// What the host knows of a call: rows, sequences, heads, and the caller's maxima of new tokens and keys.
+struct Call {
+  int M, B, H, KVH, max_q, max_kv;
+};
+// The tiles that a call has at most, whatever its sequences' lengths.
+inline i64 most_tiles(const Call &c, const Heads &h, int rows) {
+  const i64 TT = rows / h.GP, n = ((i64)c.M + (i64)c.B * (TT - 1)) / TT;
+  return (i64)c.KVH * h.HS * (n < c.M ? n : c.M);
+}
+
+// Whether workgroups take whole 256-row tiles, in the order of their length: from 2 tiles a compute unit on where tiles differ in
+// length (a prompt from its start: 4096 tokens 220 -> 167 us), from 4 on where they do not and a last round would be short of
+// tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost their states.
+inline bool chunk_each(i64 tiles, int most, const Call &c) {
+  return tiles <= 1 << 22 && tiles >= (2ll * c.max_q >= c.max_kv ? 2 : 4) * (i64)most;
+}
+
+// Whether a call runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile, its blocks (of
+// 32 keys, of 64; their time goes with the head dim), and what cutting costs 256-row tiles; fitted to 60 calls of head dim 128 of
+// 1 to 64 sequences of 16 to 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head, and tried on 64 of
+// head dims 64 and 96, where it loses 1 % on average to the better choice. Measured at head dim 128 | 96 | 64, 32 rows -> 256: a
+// prompt of 4096 tokens 266 -> 170 | 238 -> 146 | 133 -> 120 us, of 1024 33 (256: 67) | 30 (59) | 18 (52), a chunk of 512 over
+// 16 384 keys 226 -> 150 | 200 -> 155 | 161 -> 119, of 64 over 4096 33 (38) | 32 (35) | 27 (30).
+inline bool long_chunks(const Call &c, int d, bool causal, int cus) {
+  const i64 n = clamp(c.max_q < c.M ? c.max_q : c.M, 1, c.M), seqs = (c.M + n - 1) / n, G = c.H / c.KVH;
+  const double behind = c.max_kv - 0.5 * n, half = 0.5 * n;
+  const double keys = !causal ? c.max_kv : behind > half ? behind : half;
+  auto tiles = [&](int rows) {
+    const i64 HS = (G + rows - 1) / rows, TT = rows / ((G + HS - 1) / HS);
+    return (double)(c.KVH * HS * seqs * ((n + TT - 1) / TT));
+  };
+  const double few = tiles(SHORT_ROWS), many = tiles(CHUNK_ROWS);
+  const double cut = chunk_each((i64)many, cus, c) ? 0 : 2ll * c.max_q >= c.max_kv ? 30 : 13;
+  const double wide = d / 128.0;
+  return 18 + many * (0.036 + 0.0085 / 64 * wide * keys) + cut < 10 + few * wide * (0.012 + 0.001 / 32 * keys);
+}
+
+struct Choice {
+  int rows, waves;  // of a tile, of a workgroup
+  bool each;        // whole tiles, a workgroup each, else slices
+  i64 tiles;        // most_tiles
+  int most;         // slices that compute units and scratch memory allow
+};
+// rows: 32 or 256, or 0 for what is estimated faster. d: the head dim.
+inline Choice choose(const Call &c, int d, bool causal, int rows, int cus, unsigned long long ws_bytes) {
+  const bool chunk = rows ? rows == CHUNK_ROWS : long_chunks(c, d, causal, cus);
+  const int RT = chunk ? CHUNK_ROWS : SHORT_ROWS;
+  const Heads h = heads_of(c.H, c.KVH, RT);
+  const i64 tiles = most_tiles(c, h, RT), held = (i64)(ws_bytes / (2ull * RT * (d + 2) * sizeof(float) + LEFT_BYTES));
+  const int most = (int)clamp(held, 1, chunk ? cus : 2 * cus);  // one or two workgroups a compute unit
+  if (chunk) return Choice{RT, 4, chunk_each(tiles, most, c), tiles, most};
+  // Whole tiles or slices. Few tiles of few keys are not worth a second kernel (one token, us whole with 8 waves and sliced: 512
+  // keys 13, 19; 2048 21, 19). Tiles that share keys stay whole, side by side, from one a compute unit on (24 chunks of 48 tokens
+  // over 2000 keys 86, 178 sliced); others are sliced until there are many, so that uneven lengths cost nothing.
+  const bool few = tiles <= cus && c.max_kv <= 2048;
+  const bool shared = c.max_q > RT / h.GP;
+  const bool each = few || (tiles <= 1 << 22 && (c.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));
+  return Choice{RT, few ? 8 : 4, each, tiles, most};
+}
+
 }  // namespace plan
 }  // namespace h3
