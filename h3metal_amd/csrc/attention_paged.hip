@@ -12,7 +12,8 @@
 // transposing LDS reads). The loads of a block's two 16-key halves go through descriptors that end at the sequence's last
 // key: what a page holds behind it reads as zero. Two workgroups a compute unit have up to 128 KB of loads under way, and single
 // tokens are bound by HBM: 64 sequences with 275 181 keys (32 + 8 heads of 128) 214 us, 5.3 TB/s; one of 131 072 104 us.
-// A few short tiles are bound by the chain of a wave's blocks (1.1 us each, alone): 8 waves instead of 4, 512 keys 13 -> 10 us.
+// A few short tiles are bound by the chain of a wave's blocks (1.1 us each, alone): 8 waves instead of 4, 512 keys 13 -> 10 us
+// when they came, 8.8 now.
 #include "attention_common.h"
 #include "paged_attn.h"
 

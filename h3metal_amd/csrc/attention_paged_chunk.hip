@@ -17,8 +17,10 @@
 // A prompt of 8192 tokens (32 + 8 heads) takes 500 us, 1.1 PFLOP/s, a large library product's rate on the same card; a step of
 // 64 keys 2.1 us, of which its 64 matrix instructions would take 0.9: the softmax's instructions beside them bound it. A tile
 // starts and ends in about 15 us, so code is kept in two copies only and everything of a start is asked for at once. A
-// prompt of 4096 tokens takes 170 us at head dim 128 (0.82 PFLOP/s), 146 at 96 (0.70) and 120 at 64 (0.57), where as many
-// exponentials stand beside half the matrix instructions.
+// prompt of 4096 tokens takes 135 us at head dim 128 (1.02 PFLOP/s), 121 at 96 (0.85) and 93 at 64 (0.74), where as many
+// exponentials stand beside half the matrix instructions. The kernel that takes whole tiles uses no scratch memory; the one that
+// takes slices keeps the order of tiles beside them and spills at head dim 128 (61 vector registers with a causal mask, 46
+// without; scalars at every head dim), in a tile's start and end and the rare path, not in the steps themselves.
 #include "paged_attn.h"
 
 #include <algorithm>
@@ -419,7 +421,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       return f;
     };
 
-    // Step j from 1 on: P V of block j - 1, softmax of block j, scores of block j + 1 (behind the last one: of zeros).
+    // Step j from 1 on: P V of block j - 1, softmax of block j, scores of block j + 1 (behind the last one: of the spare rows
+    // that its loads took; nothing reads them).
     // The barrier sits before the last sub-tile: the loads behind it (K of block j + 3, V of block j + 1) land during the next
     // step, and the last sub-tile reads the next step's first operands. Ring slots: K(j + 3) replaces K(j - 1), V(j + 1) V(j - 3).
     // The masking steps and the others are the only two copies of this code: a tile of few blocks is bound by fetching it.
@@ -550,7 +553,8 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
       asm volatile("" : "+v"(to), "+v"(from));  // (the addresses of all pieces would be kept over the tiles' loop otherwise)
 #pragma unroll
       for (int u = 0; u < NU; u++) {
-        // no sum although a key is visible: all scores are -infinity, and 0 / 0
+        // no sum although a key is visible: all scores are -infinity, and 0 / 0 (the reciprocal is a float's last bit off at
+        // most, far below the rounding to 16 bits)
         const float inv = sum[u] != 0.0f ? __builtin_amdgcn_rcpf(sum[u]) : last[u] >= 0 ? NAN : 0.0f;
 #pragma unroll
         for (int db = 0; db < NDB; db++)

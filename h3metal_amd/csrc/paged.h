@@ -1,8 +1,8 @@
 // What the kernels over a paged cache share. A cache holds keys and values as [pages][heads][page][channels] of 16-bit
 // elements each; row c of sequence b is row c % page of page table[b][c / page]. A batch's new tokens are consecutive rows,
 // those of sequence b from q_start[b] to q_start[b + 1] - 1, and its last one is the sequence's last row, kv_len[b] - 1. All
-// three live in device memory (a captured call reads what they hold at its replay), so the host cannot check them: the
-// kernels do, and whatever they hold, no access leaves its buffer.
+// three live in device memory (a call reads what they hold when it runs), so the host cannot check them: the kernels do, and
+// whatever they hold, no access leaves its buffer.
 #pragma once
 
 #include "h3hip_internal.h"

@@ -147,8 +147,9 @@ inline i64 most_tiles(const Call &c, const Heads &h, int rows) {
 }
 
 // Whether workgroups take whole 256-row tiles, in the order of their length: from 2 tiles a compute unit on where tiles differ in
-// length (a prompt from its start: 4096 tokens 220 -> 167 us), from 4 on where they do not and a last round would be short of
-// tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost their states.
+// length (a prompt of 4096 tokens from its start: 24 % shorter than cut), from 4 on where they do not and a last round would
+// be short of tiles (24 chunks of 96 tokens over 4000 keys, 1.5 tiles a unit: 259 us cut in equal slices). Cut tiles cost
+// their states.
 inline bool chunk_each(i64 tiles, int most, const Call &c) {
   return tiles <= 1 << 22 && tiles >= (2ll * c.max_q >= c.max_kv ? 2 : 4) * (i64)most;
 }
@@ -156,9 +157,11 @@ inline bool chunk_each(i64 tiles, int most, const Call &c) {
 // Whether a call runs on tiles of 256 rows: where their estimated time (us) is the shorter one. A start, a tile, its blocks (of
 // 32 keys, of 64; their time goes with the head dim), and what cutting costs 256-row tiles; fitted to 60 calls of head dim 128 of
 // 1 to 64 sequences of 16 to 4096 new tokens over 128 to 32 768 keys with 1, 4 and 16 heads a key/value head, and tried on 64 of
-// head dims 64 and 96, where it loses 1 % on average to the better choice. Measured at head dim 128 | 96 | 64, 32 rows -> 256: a
-// prompt of 4096 tokens 266 -> 170 | 238 -> 146 | 133 -> 120 us, of 1024 33 (256: 67) | 30 (59) | 18 (52), a chunk of 512 over
-// 16 384 keys 226 -> 150 | 200 -> 155 | 161 -> 119, of 64 over 4096 33 (38) | 32 (35) | 27 (30).
+// head dims 64 and 96, where it loses 1 % on average to the better choice. Measured at head dim 128 | 96 | 64 (32 + 8 heads, calls
+// in a row), 32 rows -> 256: a prompt of 4096 tokens 218 -> 135 | 195 -> 121 | 117 -> 93 us, of 1024 29 (256: 66) | 26 (55) | 16
+// (48), a chunk of 512 over 16 384 keys 188 -> 151 | 168 -> 126 | 137 -> 99, of 64 over 4096 31 (37) | 28 (32) | 24 (27).
+// The estimate knows the maxima only: it takes M / max_q sequences of max_q tokens and max_kv keys. Without the maxima 64 single
+// tokens over a table of 32 768 keys count as one chunk and take 320 us instead of 208.
 inline bool long_chunks(const Call &c, int d, bool causal, int cus) {
   const i64 n = clamp(c.max_q < c.M ? c.max_q : c.M, 1, c.M), seqs = (c.M + n - 1) / n, G = c.H / c.KVH;
   const double behind = c.max_kv - 0.5 * n, half = 0.5 * n;
@@ -189,7 +192,9 @@ inline Choice choose(const Call &c, int d, bool causal, int rows, int cus, unsig
   if (chunk) return Choice{RT, 4, chunk_each(tiles, most, c), tiles, most};
   // Whole tiles or slices. Few tiles of few keys are not worth a second kernel (one token, us whole with 8 waves and sliced: 512
   // keys 13, 19; 2048 21, 19). Tiles that share keys stay whole, side by side, from one a compute unit on (24 chunks of 48 tokens
-  // over 2000 keys 86, 178 sliced); others are sliced until there are many, so that uneven lengths cost nothing.
+  // over 2000 keys 86, 178 sliced); others are sliced until there are many, so that uneven lengths cost nothing. The lengths
+  // themselves are not known here: 63 single tokens and a chunk of 16, one of them over 131 072 keys, stay whole and take 1160 us,
+  // 138 sliced.
   const bool few = tiles <= cus && c.max_kv <= 2048;
   const bool shared = c.max_q > RT / h.GP;
   const bool each = few || (tiles <= 1 << 22 && (c.max_kv <= 512 || tiles >= (shared ? cus : 8 * most)));

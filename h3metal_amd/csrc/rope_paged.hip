@@ -7,13 +7,14 @@
 //   one rounding, to the type of the queries and the cache; values are rounded and stored as they are
 //
 // P is pos[m] where positions are given, else the row's place in its sequence, kv_len[b] - n_b + i. The angles' fractions of a
-// turn are 64-bit integer products of P and the frequencies' codes (2^-64 turns per position), so they are exact at any
-// position; cos and sin are Taylor sums over an eighth of a turn to either side of a quarter (below 2^-24 off). Angles are
-// made once per row and workgroup, in LDS.
+// turn are 64-bit integer products of P and the frequencies' codes (2^-64 turns per position): no position adds an error to
+// the codes', which are float64 quotients (at 2^31 positions an angle is some 2^-25 turns off). cos and sin are Taylor sums
+// over an eighth of a turn to either side of a quarter: cut off below 2^-24, and with their float steps within 2 x 2^-24. Angles
+// are made once per row and workgroup, in LDS.
 //
 // A lane holds 8 consecutive channels of a slot (16-byte accesses of 16-bit rows) for ROWS rows, all loaded before the first
 // is worked on; HDIM / 8 lanes (16 at HDIM 96, 4 of them idle) form a slot, whose sums are DPP steps. Bound by HBM: 8192 rows of
-// 32 + 8 + 8 heads of 128 in 33 us from an idle card (6.1 TB/s), 43 among other calls (4.6; a plain copy reaches 4.9).
+// 32 + 8 + 8 heads of 128 in 33 us from an idle card (6.1 TB/s), 43 among other calls (4.7; a plain copy reaches 4.9).
 #include "paged.h"
 
 #include <cmath>

@@ -215,8 +215,9 @@ def qk_norm_rope_paged(gpu: Gpu, qkv: Tensor, wq: Tensor | None, wk: Tensor | No
         table [B][..] i32: token c of sequence b goes to row c % page of page table[b][c / page]
 
     q_start [B + 1] (not falling), kv_len [B] and table are read on the device. A token without a place (before 0, past the
-    table, a page number outside the cache) is not stored; two tokens with the same place leave either. Hq = 0 (Q None) and
-    Hk = 0 (kc, vc, table None) leave that side out. Q, kc and vc share memory with nothing else. no_alloc: as rms_norm_q8's."""
+    table, a page number outside the cache) is not stored; two tokens with the same place may leave 16 bytes of the one beside
+    16 bytes of the other. Hq = 0 (Q None) and Hk = 0 (kc, vc, table None) leave that side out. Q, kc and vc share memory with
+    nothing else. no_alloc: as rms_norm_q8's."""
     side = Q if Q is not None else kc
     if side is None or (Q is None) != (Hq == 0) or (kc is None or vc is None or table is None) != (Hk == 0):
         raise ValueError(f"qk_norm_rope_paged: Q goes with Hq > 0, kc, vc and table with Hk > 0, got Hq {Hq}, Hk {Hk}")
@@ -245,7 +246,8 @@ def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, ta
                     o_stride: int | None = None, max_q: int | None = None, max_kv: int | None = None, no_alloc: bool = False,
                     **variant):
     """Attention of a batch's new tokens, one or many a sequence, over a paged cache: per query head h the softmax over the
-    visible keys of (scale * q_i . k_j), the weights applied to the values; 0 where no key is visible.
+    visible keys of (scale * q_i . k_j), the weights applied to the values; 0 where no key is visible, NaN where all visible
+    ones score -infinity.
 
       q [M][q_stride], out [M][o_stride]: rows of H heads of D (64, 96 or 128) channels, query head h reads key/value head
         h / (H / KVH); rows q_start[b] .. q_start[b + 1] - 1 are the last tokens of sequence b, rows before q_start[0] and from
@@ -257,11 +259,14 @@ def attention_paged(gpu: Gpu, q: Tensor, kc: Tensor, vc: Tensor, out: Tensor, ta
     q, kc, vc and out are of one type, f16 or bf16; scores, softmax and sums are float, the weights are rounded to that type
     for their product with the values. q, kc and vc are 16-byte aligned and q_stride a multiple of 8, out and o_stride of 4
     elements. What the cache holds behind a sequence's end, and NaN or infinities in keys and values that a query does not see, do
-    not reach its output. A page number outside the cache makes the scores of its keys NaN; kv_len past the table's
-    pages counts up to them. max_q and max_kv, the most new tokens and keys of a sequence as far as the caller knows, choose
-    the kernel and how far it splits the keys (default: M, and the table's pages); results hold whatever they say. no_alloc: the
-    allocation-free entry point; its scratch array may split the keys less far. variant: ROWS names the rows of a tile (32 or
-    256), which is chosen by the size otherwise."""
+    not reach its output. A visible key that scores -infinity (an infinite channel as a mask) has the weight 0; a visible value
+    that is infinite or NaN makes its channel infinite or NaN, whatever its weight. Weights reach 2^30 before they are scaled by
+    a new maximum: bf16 values beyond 2^64 may take the sums out of a float's range. A page number outside the cache
+    makes the scores of its keys NaN; kv_len past the table's pages counts up to them. max_q and max_kv, the most new tokens and
+    keys of a sequence as far as the caller knows, choose the kernel and how far it splits the keys (default: M, and the
+    table's pages): results hold whatever they say, times only if they are the batch's (64 single tokens: 208 us, 320 without
+    them). no_alloc: the allocation-free entry point; its scratch array may split the keys less far. variant: ROWS names the
+    rows of a tile (32 or 256), which is chosen by the size otherwise."""
     if q.dtype != kc.dtype or out.dtype != q.dtype:
         raise ValueError(f"attention_paged: q, kc, vc and out must all be f16 or all bf16, got {q.dtype}, {kc.dtype}, "
                          f"{vc.dtype}, {out.dtype}")

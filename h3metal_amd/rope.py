@@ -44,8 +44,9 @@ def frequencies(rot: int, *, base: float = 10000.0, scaling: str = "none", facto
 
 def turns(freq: np.ndarray) -> np.ndarray:
     """uint32 [n][2] (low word, high word): the 2^-64 parts of a turn that each angle grows by per position. The product of
-    a code and a position keeps its fraction of a turn in 64-bit integer arithmetic, so an angle is as accurate at position
-    10^9 as at 1, where a float's product has lost the fraction at 10^6."""
+    a code and a position keeps its fraction of a turn in 64-bit integer arithmetic, where a float's product has lost it at
+    10^6. A code is a float64 quotient, off by 2^-53 of itself or so: an angle at position P by up to P 2^-56 turns for the
+    fastest pair, 2^-25 at 2^31."""
     freq = np.asarray(freq, np.float64)
     if freq.ndim != 1 or not np.isfinite(freq).all():
         raise ValueError(f"rope: frequencies must be a vector of finite numbers, got shape {freq.shape}")
