@@ -44,13 +44,6 @@ struct Rows {
   static constexpr int LDS = NW * 2 * BYTES > MERGE ? NW * 2 * BYTES : MERGE;
 };
 
-// Whether the 16-bit value in the high half is infinite or NaN
-template <int T>
-__device__ __forceinline__ bool odd16(unsigned v) {
-  constexpr unsigned E = T == T_BF16 ? 0x7F800000u : 0x7C000000u;
-  return (v & E) == E;
-}
-
 template <int DG, int T, int NW, bool CAUSAL, bool EACH>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void attention_rows_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape sh, Heads hd, int least) {

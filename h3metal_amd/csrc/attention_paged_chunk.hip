@@ -73,12 +73,6 @@ struct Chunk {
 template <int VT>
 constexpr float sum_limit() { return VT == T_F16 ? 0x1p15f : 0x1p30f; }
 
-template <int VT>
-__device__ __forceinline__ bool odd_high(unsigned v) {  // the 16-bit value in the high half is infinite or NaN
-  constexpr unsigned E = VT == T_BF16 ? 0x7F800000u : 0x7C000000u;
-  return (v & E) == E;
-}
-
 struct __attribute__((packed, aligned(8))) Piece {  // 16 bytes of an output row, whose rows are aligned to 8
   float v[4];
 };
@@ -305,14 +299,14 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
         i32x4 v = *at;
         bool some = false;
 #pragma unroll
-        for (int e = 0; e < 4; e++) some |= odd_high<VT>((unsigned)v[e]) | odd_high<VT>((unsigned)v[e] << 16);
+        for (int e = 0; e < 4; e++) some |= odd16<VT>((unsigned)v[e]) | odd16<VT>((unsigned)v[e] << 16);
         if (__builtin_expect(__any(some), 0)) {
           odd = odd || (some && ((i64)blk0 + j) * BK + 16 * group_of(r) + lrow < L);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             unsigned d = (unsigned)v[e];
-            if (odd_high<VT>(d)) d &= 0xFFFFu;
-            if (odd_high<VT>(d << 16)) d &= 0xFFFF0000u;
+            if (odd16<VT>(d)) d &= 0xFFFFu;
+            if (odd16<VT>(d << 16)) d &= 0xFFFF0000u;
             v[e] = (int)d;
           }
           *at = v;
@@ -628,7 +622,7 @@ void attention_chunk_kernel(AttnArgs a, Batch bt, PagedAttnParams p, plan::Shape
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             const unsigned x = (unsigned)vv[e / 2] << (e & 1 ? 0 : 16);
-            if (odd_high<VT>(x)) {
+            if (odd16<VT>(x)) {
               v[e] += x & (VT == T_BF16 ? 0x007F0000u : 0x03FF0000u) ? NAN : (int)x < 0 ? -INFINITY : INFINITY;
               some = true;
             }

@@ -28,6 +28,13 @@ int launch_attention_chunk(int d, int t, bool causal, const Exec &ex, const Attn
 
 namespace {
 
+// Whether the 16-bit value in the high half is infinite or NaN
+template <int T>
+__device__ __forceinline__ bool odd16(unsigned v) {
+  constexpr unsigned E = T == T_BF16 ? 0x7F800000u : 0x7C000000u;
+  return (v & E) == E;
+}
+
 // -- finding the work -------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ i64 wave_sum_to(i64 v) {  // inclusive
